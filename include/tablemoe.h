@@ -47,6 +47,7 @@ extern "C" {
 #define TM_DT_F32 0
 #define TM_DT_F16 1
 #define TM_DT_BF16 2
+#define TM_DT_E4M3 3 /* 8 bits with block scales: q of tm_fp8_quantize_rows */
 
 /* ---- hit comparators (max score vs threshold) ------------------------ */
 #define TM_CMP_GE 0 /* hit = max >= threshold */
@@ -83,6 +84,38 @@ const char *tm_last_error(void);
 int tm_topk_softmax(const float *logits, int64_t n_tokens, int32_t n_experts, int64_t ld_logits,
                     int32_t top_k, int32_t renormalize, float *out_weights, int64_t *out_ids,
                     tm_stream_t stream);
+
+/* ======================================================================
+ * Router of grouped experts with a balancing bias: the routers of the second
+ * model family's larger layers (models/deepseek_vl2 gate: softmax or sigmoid
+ * scores, groups, correction bias), beside tm_topk_softmax.
+ * For each row of logits [n_tokens, n_experts] (dtype F32, F16 or BF16, row
+ * stride ld_logits): scores s = softmax(l) or sigmoid(l); v = s + bias (fp32
+ * [n_experts], nullable: 0); order key = v, or l without a bias (the scores
+ * rise with l, so no two of them are tied that the logits tell apart).
+ * n_groups > 1: the experts form n_groups groups of n_experts / n_groups;
+ * a group's value is its largest key (TM_GROUP_MAX) or the sum of its two
+ * largest v (TM_GROUP_TOP2; one of them, where it has one); the topk_groups
+ * best groups (ties: lower group) keep their experts.  The top_k experts of
+ * largest key (ties: lower id) come out in that order with weights s,
+ * divided by their sum (clamped to 1e-20) with renormalize != 0, times scale.
+ * Keys and group values are compared in 64 bits, weights are rounded once.
+ * An expert whose logit is NaN or -inf, or whose key is NaN or -inf, is not
+ * available: it comes after every available one (lower id first), in a group
+ * without any last of all, with weight 0, and leaves the softmax.  +inf counts
+ * as the largest finite fp32 number.
+ * out_weights fp32, out_ids int64, [n_tokens, top_k] contiguous.
+ * Limits: n_experts <= 1024, n_groups divides it and is <= 64, 1 <= top_k <=
+ * min(32, topk_groups * n_experts / n_groups).
+ * ====================================================================== */
+#define TM_ROUTE_SOFTMAX 0
+#define TM_ROUTE_SIGMOID 1
+#define TM_GROUP_MAX 0
+#define TM_GROUP_TOP2 1
+int tm_route_experts(int32_t dtype, const void *logits, int64_t n_tokens, int32_t n_experts, int64_t ld_logits,
+                     const float *bias, int32_t scoring, int32_t n_groups, int32_t topk_groups, int32_t group_rule,
+                     int32_t top_k, int32_t renormalize, float scale, float *out_weights, int64_t *out_ids,
+                     tm_stream_t stream);
 
 /* ======================================================================
  * a4 -- projection of hidden states into the PCA space.
@@ -503,6 +536,83 @@ int tm_grouped_swiglu_packed(int32_t dtype, const void *x, int64_t ld_x, int32_t
                              tm_stream_t stream);
 
 /* ======================================================================
+ * 8-bit weights: quantisation, a linear layer and the expert MLPs (no
+ * counterpart in the reference, whose recompute is 16-bit).  Values are e4m3
+ * (OCP: largest 448, no infinity) with one fp32 scale per block: 128
+ * consecutive columns of a row of activations, 128 x 128 elements of a weight
+ * matrix (blocks at the ends are smaller); a value stands for q * scale.
+ *
+ * The quantisers give each block the smallest power of two s with
+ * max|v| / s <= 448 over its finite elements (1 if they are all 0, never
+ * below 2^-126): v / s is exact and q its nearest e4m3 value (ties to even);
+ * a non-finite v becomes NaN.  The products take any fp32 scales.
+ *
+ * tm_fp8_quantize_rows: x [n_rows, k] (F32, F16, BF16, row stride ld_x) -> q
+ * (bytes, row stride ld_q, a multiple of 16) and scale [n_rows, ceil(k/128)]
+ * (row stride ld_scale).  Columns k .. ceil(k/128) * 128 of q become 0.
+ * tm_fp8_quantize_weight: w [n_mats, n_rows, k] contiguous -> q [n_mats,
+ * n_rows] rows of ld_q bytes, padded as above, and scale [n_mats,
+ * ceil(n_rows/128), ceil(k/128)] contiguous.
+ * ====================================================================== */
+int tm_fp8_quantize_rows(int32_t dtype, const void *x, int64_t n_rows, int64_t k, int64_t ld_x, void *q, int64_t ld_q,
+                         float *scale, int64_t ld_scale, tm_stream_t stream);
+int tm_fp8_quantize_weight(int32_t dtype, const void *w, int64_t n_mats, int64_t n_rows, int64_t k, void *q,
+                           int64_t ld_q, float *scale, tm_stream_t stream);
+
+/* y = dtype(x^ W^T + bias): x [n_rows, k] of `dtype` (row stride ld_x),
+ * quantised in the call, or with x_scale non-NULL the q (row stride ld_x
+ * bytes, padded to whole blocks with zeros) and scale (row stride ld_xs) of
+ * tm_fp8_quantize_rows; w [n_out] rows of ceil(k/128) * 128 bytes (contiguous;
+ * what lies past k must not be NaN), w_scale [ceil(n_out/128),
+ * ceil(k/128)]; bias [n_out] of `dtype`, nullable; out [n_rows, n_out] of
+ * `dtype` (row stride ld_out).  fp32 sums; F32 outputs and the up product of
+ * the MLPs below take every product exactly, 16-bit outputs may take the
+ * 8-bit matrix instructions, which truncate products at about 2^-13 of the
+ * largest (an error of 1.5e-5 to 6e-5 of a sum's size).
+ * 16-byte aligned w and workspace (tm_fp8_linear_workspace_size); k <= 16384,
+ * n_out < 2^24. */
+size_t tm_fp8_linear_workspace_size(int64_t n_rows, int64_t k, int32_t dtype);
+int tm_fp8_linear(int32_t dtype, const void *x, const float *x_scale, int64_t n_rows, int64_t k, int64_t ld_x,
+                  int64_t ld_xs, const void *w, const float *w_scale, int64_t n_out, const void *bias, void *out,
+                  int64_t ld_out, void *workspace, size_t workspace_bytes, tm_stream_t stream);
+
+/* Expert weights in 8 bits, as nn.Linear stores them: w1, w3 [n_experts,
+ * inter, hidden], w2 [n_experts, hidden, inter] contiguous, scales s1, s3
+ * [n_experts, inter/128, hidden/128], s2 [n_experts, hidden/128, inter/128].
+ * hidden and inter: multiples of 128 up to 16384; n_experts <= 1024. */
+typedef struct tm_fp8_experts {
+  int32_t n_experts, hidden, inter, reserved;
+  const void *w1;
+  const float *s1;
+  const void *w3;
+  const float *s3;
+  const void *w2;
+  const float *s2;
+} tm_fp8_experts;
+
+/* The SwiGLU MLP of every selected (token, slot) through its expert, the
+ * selection and the outputs as in tm_group_slots + tm_grouped_swiglu: pair
+ * (b, s) is taken when mask[b*ms_b + s*ms_s] != 0 and 0 <= ids[b*ld_ids + s] <
+ * n_experts; its row of `hidden` elements goes to out + b*so_b + s*so_s
+ * (others are left as they were).  g = x^ W1^T, u = x^ W3^T in fp32, f =
+ * silu(g) * u in fp32, f^ = f quantised in blocks of 128 columns, y =
+ * dtype(f^ W2^T).  dtype F16 or BF16; x rows, out and the workspace 16-byte
+ * aligned, so_b and so_s multiples of 8 elements.  The grouping is part of
+ * the call (no host sync). */
+size_t tm_fp8_grouped_swiglu_workspace_size(const tm_fp8_experts *experts, int64_t n_tokens, int32_t top_k);
+int tm_fp8_grouped_swiglu(const tm_fp8_experts *experts, int32_t dtype, const void *x, int64_t n_tokens, int64_t ld_x,
+                          const int64_t *ids, int32_t top_k, int64_t ld_ids, const uint8_t *mask, int64_t ms_b,
+                          int64_t ms_s, void *out, int64_t so_b, int64_t so_s, void *workspace,
+                          size_t workspace_bytes, tm_stream_t stream);
+/* The same MLP of one expert (n_experts = 1) over every row (a layer's shared
+ * experts): out [n_rows, hidden] = dtype(addend + f^ W2^T), addend nullable,
+ * not overlapping out. */
+size_t tm_fp8_expert_swiglu_workspace_size(const tm_fp8_experts *experts, int64_t n_rows);
+int tm_fp8_expert_swiglu(const tm_fp8_experts *experts, int32_t dtype, const void *x, int64_t n_rows, int64_t ld_x,
+                         const void *addend, int64_t ld_add, void *out, int64_t ld_out, void *workspace,
+                         size_t workspace_bytes, tm_stream_t stream);
+
+/* ======================================================================
  * Mode G -- one MoE layer of the table path in ONE call.
  * Enqueues, back to back on `stream`: tm_topk_softmax (router) ->
  * tm_project -> tm_search_global -> tm_keep_select (n_keep =
@@ -567,8 +677,9 @@ typedef struct tm_layer_io {
  * shared experts sit between the keep selection and the combine). */
 #define TM_LAYER_NO_COMBINE 1
 
-/* sizeof(tm_table_layer) for which == 0, sizeof(tm_layer_io) for which == 1
- * (lets a binding check its mirror of the two structs). */
+/* sizeof(tm_table_layer) for which == 0, sizeof(tm_layer_io) for which == 1,
+ * sizeof(tm_fp8_experts) for which == 2 (lets a binding check its mirror of
+ * the structs). */
 size_t tm_struct_size(int32_t which);
 /* Workspace of tm_table_forward.  Its first TM_LAYER_SYNC_BYTES bytes hold
  * arrival counters and flags (batches of at most 64 tokens hand the

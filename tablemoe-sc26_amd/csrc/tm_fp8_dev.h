@@ -1,0 +1,70 @@
+// 8-bit (e4m3) values with a scale per block of 128: the quantisation rule and
+// the conversions shared by the kernels that write and read them.
+//
+// A block is 128 consecutive columns of a row (activations) or 128 x 128
+// elements (weights).  Its scale is the smallest power of two s with
+// max|v| / s <= 448 over the block's finite v (1 for a block of zeros, never
+// below 2^-126), so v / s is exact and each stored value is one rounding (half
+// to even) of it.  A non-finite v is stored as NaN.
+#pragma once
+
+#include "tm_mfma.h"
+
+constexpr int kFp8Block = 128;
+
+// max|v| of a block over its finite elements, from fp32 bit patterns: for
+// non-negative floats the integer order is the float order.
+__device__ __forceinline__ uint32_t tm_fp8_amax(uint32_t m, float v) {
+  const uint32_t a = __float_as_uint(v) & 0x7fffffffu;
+  return a < 0x7f800000u && a > m ? a : m;
+}
+
+// The block scale of max|v| (bits): a / s <= 448 = 1.75 * 2^8 with a = m 2^e,
+// 1 <= m < 2, asks for s = 2^(e - 8), or 2^(e - 7) where m > 1.75.  Subnormal
+// a gives the smallest scale.  `inv` receives 1 / s (exact).
+__device__ __forceinline__ float tm_fp8_scale(uint32_t amax, float &inv) {
+  int b = (int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);  // biased exponent of s
+  b = b < 1 ? 1 : b;
+  b = amax == 0 ? 127 : b;
+  inv = __uint_as_float((uint32_t)(254 - b) << 23);
+  return __uint_as_float((uint32_t)b << 23);
+}
+
+// The quotient to be rounded: non-finite values become NaN.
+__device__ __forceinline__ float tm_fp8_quot(float v, float inv) {
+  return (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u ? v * inv : __uint_as_float(0x7fc00000u);
+}
+
+// Four values to e4m3, packed in order.
+__device__ __forceinline__ uint32_t tm_fp8_pack4(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+
+typedef __bf16 tm_bf16x2 __attribute__((ext_vector_type(2)));
+
+// Eight e4m3 values as bf16 (exact: 4 significant bits).
+__device__ __forceinline__ uint4 tm_fp8_to_bf16x8(uint32_t lo, uint32_t hi) {
+  uint4 r;
+  r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+  r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+  r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+  r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+  return r;
+}
+
+// Two fp32 values whose low 16 bits are zero, as packed bf16.
+__device__ __forceinline__ uint32_t tm_bf16_hi2(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+
+// Four e4m3 values times a power of two as bf16 (exact, apart from values
+// under 2^-126, which blocks of max|v| < 2^-108 alone can have).
+__device__ __forceinline__ uint2 tm_fp8_scaled_bf16x4(uint32_t q, float s) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, true);
+  uint2 r;
+  r.x = tm_bf16_hi2(a.x * s, a.y * s);
+  r.y = tm_bf16_hi2(b.x * s, b.y * s);
+  return r;
+}

@@ -270,7 +270,12 @@ int scratch_for_current_device(hipStream_t s, void **out) {
 }  // namespace
 
 extern "C" size_t tm_struct_size(int32_t which) {
-  return which == 0 ? sizeof(tm_table_layer) : (which == 1 ? sizeof(tm_layer_io) : 0);
+  switch (which) {
+    case 0: return sizeof(tm_table_layer);
+    case 1: return sizeof(tm_layer_io);
+    case 2: return sizeof(tm_fp8_experts);
+    default: return 0;
+  }
 }
 
 extern "C" size_t tm_table_forward_workspace_size(const tm_table_layer *table, int64_t n_tokens, int32_t n_nearest) {

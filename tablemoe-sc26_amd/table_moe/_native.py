@@ -25,6 +25,8 @@ TM_TARGET_ONE, TM_TARGET_ORIG_SUM, TM_TARGET_GIVEN = 0, 1, 2
 TM_SCORE_MODEL, TM_SCORE_F32 = 0, 1
 TM_LAYER_NO_COMBINE = 1
 TM_PACK_GATE_UP, TM_PACK_DOWN = 0, 1
+TM_ROUTE_SOFTMAX, TM_ROUTE_SIGMOID = 0, 1
+TM_GROUP_MAX, TM_GROUP_TOP2 = 0, 1
 # tm_table_forward workspace: sync region size and the byte offset of the
 # count of bounded waits that ran out (include/tablemoe.h)
 TM_LAYER_SYNC_BYTES = 16384
@@ -54,12 +56,28 @@ class LayerIO(C.Structure):
                 ("q", vp), ("q_sqnorm", vp), ("dist", vp), ("idx", vp), ("keep", vp)]
 
 
+class Fp8Experts(C.Structure):
+    """Mirror of tm_fp8_experts (include/tablemoe.h)."""
+
+    _fields_ = [("n_experts", i32), ("hidden", i32), ("inter", i32), ("reserved", i32), ("w1", vp), ("s1", vp),
+                ("w3", vp), ("s3", vp), ("w2", vp), ("s2", vp)]
+
+
 # name -> (restype, argtypes); mirrors include/tablemoe.h
 PROTOTYPES = {
     "tm_version": (C.c_int, []),
     "tm_status_string": (C.c_char_p, [C.c_int]),
     "tm_last_error": (C.c_char_p, []),
     "tm_topk_softmax": (C.c_int, [vp, i64, i32, i64, i32, i32, vp, vp, vp]),
+    "tm_route_experts": (C.c_int, [i32, vp, i64, i32, i64, vp, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp]),
+    "tm_fp8_quantize_rows": (C.c_int, [i32, vp, i64, i64, i64, vp, i64, vp, i64, vp]),
+    "tm_fp8_quantize_weight": (C.c_int, [i32, vp, i64, i64, i64, vp, i64, vp, vp]),
+    "tm_fp8_linear_workspace_size": (sz, [i64, i64, i32]),
+    "tm_fp8_linear": (C.c_int, [i32, vp, vp, i64, i64, i64, i64, vp, vp, i64, vp, vp, i64, vp, sz, vp]),
+    "tm_fp8_grouped_swiglu_workspace_size": (sz, [vp, i64, i32]),
+    "tm_fp8_grouped_swiglu": (C.c_int, [vp, i32, vp, i64, i64, vp, i32, i64, vp, i64, i64, vp, i64, i64, vp, sz, vp]),
+    "tm_fp8_expert_swiglu_workspace_size": (sz, [vp, i64]),
+    "tm_fp8_expert_swiglu": (C.c_int, [vp, i32, vp, i64, i64, vp, i64, vp, i64, vp, sz, vp]),
     "tm_project_workspace_size": (sz, [i64, i32, i32]),
     "tm_project_packed_size": (sz, [i32, i32, i32]),
     "tm_project_pack": (C.c_int, [i32, vp, i32, i32, i64, i64, vp, sz, vp]),
@@ -141,7 +159,7 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
-        for which, struct in ((0, TableLayer), (1, LayerIO)):
+        for which, struct in ((0, TableLayer), (1, LayerIO), (2, Fp8Experts)):
             if lib.tm_struct_size(which) != C.sizeof(struct):
                 raise RuntimeError(f"{struct.__name__} mirror ({C.sizeof(struct)} bytes) does not match the library "
                                    f"({lib.tm_struct_size(which)} bytes)")
@@ -208,6 +226,23 @@ def stream(device: torch.device) -> int:
     if _raw_stream is not None and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class _SameDevice:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME_DEVICE = _SameDevice()
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one (launches go to the
+    current device): nothing to do where it is already."""
+    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def mask_bytes(mask: torch.Tensor, device: torch.device) -> torch.Tensor:
