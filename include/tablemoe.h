@@ -567,8 +567,8 @@ int tm_fp8_quantize_weight(int32_t dtype, const void *w, int64_t n_mats, int64_t
  * ceil(k/128)]; bias [n_out] of `dtype`, nullable; out [n_rows, n_out] of
  * `dtype` (row stride ld_out).  fp32 sums; F32 outputs and the up product of
  * the MLPs below take every product exactly, 16-bit outputs may take the
- * 8-bit matrix instructions, which truncate products at about 2^-13 of the
- * largest (an error of 1.5e-5 to 6e-5 of a sum's size).
+ * 8-bit matrix instructions, which drop what lies under 2^-13 of the largest
+ * of 8 consecutive products (1.5e-5 to 6e-5 of a sum's size on normal data).
  * 16-byte aligned w and workspace (tm_fp8_linear_workspace_size); k <= 16384,
  * n_out < 2^24. */
 size_t tm_fp8_linear_workspace_size(int64_t n_rows, int64_t k, int32_t dtype);

@@ -102,6 +102,19 @@ __device__ __forceinline__ void tm_dma16_s(const void *gaddr, uint32_t lds_base)
         : "memory");
 }
 
+// One dword per lane: lane l's to LDS byte lds_base + 4 l.
+__device__ __forceinline__ void tm_dma4_s(const void *gaddr, uint32_t lds_base) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %2\n\t"
+      "global_load_lds_dword %1, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(gaddr), "s"(lds_base)
+      : "memory");
+}
+
 template <int N>
 __device__ __forceinline__ void tm_wait_vm_lgkm0() {
   // s_waitcnt vmcnt(N) lgkmcnt(0), expcnt left at its maximum
