@@ -69,15 +69,15 @@ __device__ __forceinline__ uint2 tm_fp8_scaled_bf16x4(uint32_t q, float s) {
   return r;
 }
 
-// Matrix product of 16 x 128 by 128 x 16 e4m3 values: lane l holds row (column)
-// l % 16 and 32 of the 128, the same ones in both operands; D as in the
-// 16x16x32 form.
+// Matrix product of 32 x 64 by 64 x 32 e4m3 values: lane l holds row (column)
+// l % 32 and 32 of the 64, the same ones in both operands; D as in the 32x32x16
+// form.
 typedef int tm_i32x8 __attribute__((ext_vector_type(8)));
 
-__device__ __forceinline__ tm_f32x4 tm_mfma16x16x128_fp8(const uint4 (&a)[2], const uint4 (&b)[2], tm_f32x4 c) {
+__device__ __forceinline__ tm_f32x16 tm_mfma32x32x64_fp8(const uint4 (&a)[2], const uint4 (&b)[2], tm_f32x16 c) {
   const tm_i32x8 x = {(int)a[0].x, (int)a[0].y, (int)a[0].z, (int)a[0].w,
                       (int)a[1].x, (int)a[1].y, (int)a[1].z, (int)a[1].w};
   const tm_i32x8 y = {(int)b[0].x, (int)b[0].y, (int)b[0].z, (int)b[0].w,
                       (int)b[1].x, (int)b[1].y, (int)b[1].z, (int)b[1].w};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 0, 0, 0, 0, 0);
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 0, 0, 0, 0, 0, 0);
 }

@@ -309,21 +309,27 @@ int stream_launch(const char *name, const Fp8Src &src, const Fp8Rows &rows, cons
 // Many rows: tiles through LDS.
 //
 // Eight waves: wave w owns 64 weight rows of group w % 4 (up: 32 rows of W1 and
-// the same 32 of W3) and NB blocks of 16 activation rows of half w / 4.  A stage
-// is one block of 128 columns, global -> LDS by direct loads, two slots.  Each
-// 16 x 16 product over a stage starts from zero and is added to the fp32
-// accumulators times its scales.
+// the same 32 of W3) and NB blocks of 32 activation rows of half w / 4, in
+// 32 x 32 products.  A stage is 64 columns, global -> LDS by direct loads; LDS
+// holds a ring of as many stages as fit, one barrier per stage: it publishes the
+// stage and frees the slot of the one before.  The products of a block of 128
+// columns (two stages) start from zero and are added to the fp32 accumulators
+// times their scales.
 //
 // Activations come quantised: e4m3 rows (the 8-bit instructions), or the same
 // values as bf16 rows (WIDE: the 16-bit ones, weights converted on the way from
-// LDS), with their scales; up: bf16 rows q * s.  Which rows of its 64 a lane's operand takes is chosen so that its
-// results are 16 (up: 8) consecutive columns; 16-byte chunks of an LDS row are
-// XOR-ed with the row bits that differ among 16 lanes, so operand reads are
-// free of bank conflicts.
+// LDS), with their scales; up: bf16 rows q * s.  Which rows of its 64 a lane's
+// operand takes is chosen so that its results are 32 (up: 16) consecutive
+// columns; 16-byte chunks of an LDS row are XOR-ed with the row bits that differ
+// among 16 lanes, so operand reads are free of bank conflicts.
 // ---------------------------------------------------------------------------
 constexpr int kTileThreads = 512;
+constexpr int kTileLds = 163840;
 constexpr int kTileRows = 256;  // rows per entry of the tile list
-constexpr int kTileCols = 256;  // weight rows per tile (up: 128 of W1 and of W3)
+constexpr int kTileBM = 128;    // rows per workgroup
+constexpr int kTileParts = kTileRows / kTileBM;
+constexpr int kTileCols = 256;  // weight rows per workgroup (up: 128 of W1 and of W3)
+constexpr int kStageK = 64;
 
 struct Fp8Tiles {
   const int32_t *tiles, *offsets, *row_token;  // grouped rows (tm_group_slots); all null: dense
@@ -335,40 +341,54 @@ struct Fp8Tiles {
 // A workgroup barrier that LDS accesses stay on their side of.
 __device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
 
-template <int DT, int MODE, bool WIDE, int NBMAX>
+// Stage layout for NB blocks of 32 rows per half.
+template <int MODE, bool WIDE, int NB>
 struct TileCfg {
-  static constexpr int kBM = 32 * NBMAX;
-  static constexpr int kXRow = WIDE ? 256 : 128;  // bytes of an activation row's stage
-  static constexpr int kW = kTileCols * kFp8Block;
-  static constexpr int kX = kBM * kXRow;
   static constexpr bool kScaled = !WIDE || MODE == kOut;  // rows come with scales
-  static constexpr int kS = !kScaled ? 0 : kBM * 4 < 256 ? 256 : kBM * 4;
+  static constexpr int kXRow = WIDE ? 2 * kStageK : kStageK;
+  static constexpr int kW = kTileCols * kStageK;
+  static constexpr int kX = 64 * NB * kXRow;
+  static constexpr int kS = kScaled ? 64 * NB * 4 : 0;
   static constexpr int kStage = kW + kX + kS;
+  static constexpr int kXLoads = kX / 1024;                        // 1 KiB pieces of a stage's rows
+  static constexpr int kXDma = kXLoads > 8 ? kXLoads / 8 : 1;      // ... per wave
+  static constexpr int kDma = 2 + kXDma + (kScaled ? 1 : 0);
+  static constexpr int kFit = kTileLds / kStage;
+  static constexpr int kSlots = kFit < 8 ? kFit : 8;
 };
 
 template <int MODE>
 __device__ __forceinline__ int w_swz(int row) {
-  return ((row >> 1) & 1) | (((row >> (MODE == kUp ? 3 : 4)) & 3) << 1);
+  return ((row >> (MODE == kUp ? 4 : 5)) & 1) | (((row >> 2) & 1) << 1);
 }
 template <bool WIDE>
-__device__ __forceinline__ int x_swz(int row) { return WIDE ? row & 15 : (row >> 1) & 7; }
+__device__ __forceinline__ int x_swz(int row) { return WIDE ? (row >> 1) & 7 : (row >> 2) & 3; }
 
-template <int DT, int MODE, bool WIDE, int NBMAX>
+// Wait until at most `left` stages of kDma loads are outstanding (and LDS reads
+// are done).
+template <int kDma, int kMost>
+__device__ __forceinline__ void wait_stages(int left) {
+  if constexpr (kMost <= 0) {
+    tm_wait_vm_lgkm0_mem<0>();
+  } else {
+    if (left >= kMost) tm_wait_vm_lgkm0_mem<kMost * kDma>();
+    else wait_stages<kDma, kMost - 1>(left);
+  }
+}
+
+template <int DT, int MODE, bool WIDE>
 __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__restrict__ x, int64_t ld_x,
                                                                const float *__restrict__ xs, int64_t ld_xs, Fp8Mat m0,
                                                                Fp8Mat m1, int n_out, int KT, int n_tiles, Fp8Tiles ts,
                                                                Fp8Dst dst, float *__restrict__ fs, bool vec_out) {
-  using Cfg = TileCfg<DT, MODE, WIDE, NBMAX>;
-  constexpr int kParts = kTileRows / Cfg::kBM;  // work items per entry of the tile list
-  __shared__ uint4 ring[2 * Cfg::kStage / 16];
-  __shared__ uint32_t s_top[MODE == kUp ? 2 * NBMAX * 16 * 4 : 1];
+  __shared__ uint4 ring[kTileLds / 16];
 
   // Work items: (row tile, column tile, part).  Of whole groups of eight row
   // tiles, tile y runs on XCD y % 8 (the dispatcher's round robin), the parts of
   // a column tile next to each other: they share its weights in that L2.
   const int64_t row_tiles = ts.tiles != nullptr ? (ts.tiles[1] < ts.t_max ? ts.tiles[1] : ts.t_max)
                                                 : ((int64_t)ts.rows + kTileRows - 1) / kTileRows;
-  const int per = n_tiles * kParts;
+  const int per = n_tiles * kTileParts;
   const int64_t full = row_tiles / 8 * 8;
   int64_t y;
   int item;
@@ -383,52 +403,55 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
     }
     if (y >= row_tiles) return;  // uniform
   }
-  const int part = item % kParts;
-  const int n0 = (item / kParts) * (MODE == kUp ? kTileCols / 2 : kTileCols);
+  const int part = item % kTileParts;
+  const int n0 = (item / kTileParts) * (MODE == kUp ? kTileCols / 2 : kTileCols);
   int e = 0, r0, r_end;
   if (ts.tiles != nullptr) {
     e = ts.tiles[2 + y];
-    r0 = ts.tiles[2 + ts.t_max + y] + part * Cfg::kBM;
+    const int t0 = ts.tiles[2 + ts.t_max + y];
+    r0 = t0 + part * kTileBM;
     r_end = ts.offsets[e + 1];
-    const int t_end = ts.tiles[2 + ts.t_max + y] + kTileRows;
-    r_end = r_end < t_end ? r_end : t_end;
+    r_end = r_end < t0 + kTileRows ? r_end : t0 + kTileRows;
   } else {
-    r0 = (int)y * kTileRows + part * Cfg::kBM;
+    r0 = (int)y * kTileRows + part * kTileBM;
     r_end = ts.rows;
   }
   if (r0 >= r_end) return;  // uniform
-  const int rows = r_end - r0 < Cfg::kBM ? r_end - r0 : Cfg::kBM;
+  const int rows = r_end - r0 < kTileBM ? r_end - r0 : kTileBM;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int cg = wave & 3, half = wave >> 2, t = lane & 15, g = lane >> 4;
+  const int cg = wave & 3, half = wave >> 2, t = lane & 31, h = lane >> 5;
   const uint32_t lds0 = (uint32_t)(uintptr_t)ring;
   const char *const lds = reinterpret_cast<const char *>(ring);
   const int64_t ld_w = (int64_t)KT * kFp8Block;
   const int n_blk = (n_out + kFp8Block - 1) / kFp8Block;
+  const int steps = 2 * KT;
 
-  // weight loads: 1 KiB pieces wave * 4 + j, eight rows each (up: waves 0-3 W1, waves 4-7 W3)
+  // weight loads: 1 KiB pieces 2 wave + j, 16 rows each (up: waves 0-3 W1, waves 4-7 W3)
   const Fp8Mat &mine = MODE == kUp && wave >= 4 ? m1 : m0;
   constexpr int kWRows = MODE == kUp ? kTileCols / 2 : kTileCols;
   const int w_rows = n_out - n0 < kWRows ? n_out - n0 : kWRows;
   const tm_rsrc_t w_rs = tm_make_rsrc(mine.w + ((int64_t)e * n_out + n0) * ld_w, (uint64_t)w_rows * ld_w);
-  uint32_t w_off[4];
+  uint32_t w_off[2];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    int row = ((MODE == kUp ? wave & 3 : wave) * 4 + j) * 8 + (lane >> 3);
-    const int chunk = (lane & 7) ^ w_swz<MODE>(row);
+  for (int j = 0; j < 2; ++j) {
+    int row = ((MODE == kUp ? wave & 3 : wave) * 2 + j) * 16 + (lane >> 2);
+    const int chunk = (lane & 3) ^ w_swz<MODE>(row);
     row = row < w_rows ? row : w_rows - 1;  // (results of rows past n_out are dropped)
     w_off[j] = (uint32_t)row * (uint32_t)ld_w + (uint32_t)chunk * 16u;
   }
-  // operand offsets: weights (a: blocks of 16 operand rows), activations
-  uint32_t a_off[4][2], b_off[WIDE ? 4 : 2];
+  // operand row t of block a: weight row
+  //   out: 64 cg + 32 (t / 4 % 2) + 16 a + 4 (t / 8) + t % 4
+  //   up:  32 cg + 16 (t / 4 % 2) + 4 (t / 8) + t % 4 of matrix a
+  uint32_t a_off[2];  // chunks h and 2 + h (of block 0)
+  {
+    const int row = MODE == kUp ? 32 * cg + 16 * ((t >> 2) & 1) + 4 * (t >> 3) + (t & 3)
+                                : 64 * cg + 32 * ((t >> 2) & 1) + 4 * (t >> 3) + (t & 3);
 #pragma unroll
-  for (int a = 0; a < 4; ++a) {
-    const int row = MODE == kUp ? (a >> 1) * 128 + cg * 32 + 8 * (t >> 2) + 4 * (a & 1) + (t & 3)
-                                : cg * 64 + 16 * (t >> 2) + 4 * a + (t & 3);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) a_off[a][h] = (uint32_t)(row * 128 + ((4 * h + g) ^ w_swz<MODE>(row)) * 16);
+    for (int c = 0; c < 2; ++c) a_off[c] = (uint32_t)(row * kStageK + ((2 * c + h) ^ w_swz<MODE>(row)) * 16);
   }
-  // the wave's scales of 64 stages, one per lane
+  constexpr uint32_t kABlock = (MODE == kUp ? 128 : 16) * kStageK;  // block 1 (its swizzle is block 0's)
+  // the wave's scales of 64 blocks, one per lane
   const int blk = (MODE == kUp ? n0 : n0 + cg * 64) / kFp8Block;
   const int64_t s_at = ((int64_t)e * n_blk + (blk < n_blk ? blk : n_blk - 1)) * KT;
   float swv[2] = {0.f, 0.f};
@@ -439,29 +462,27 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
   };
   load_sw(0);
 
-  tm_f32x4 acc[4][NBMAX];
+  tm_f32x16 acc[2][2];
 #pragma unroll
-  for (int a = 0; a < 4; ++a)
+  for (int a = 0; a < 2; ++a)
 #pragma unroll
-    for (int q = 0; q < NBMAX; ++q) acc[a][q] = tm_f32x4{};
+    for (int q = 0; q < 2; ++q) acc[a][q] = tm_f32x16{};
 
   auto run = [&](auto nb_c) {
     constexpr int NB = decltype(nb_c)::value;
-    constexpr int kXLoads = 32 * NB * Cfg::kXRow / 1024;               // 1 KiB pieces of a stage's rows
-    constexpr int kXDma = kXLoads / 8 > 1 ? kXLoads / 8 : 1;            // ... per wave
-    constexpr int kRowsPer = 1024 / Cfg::kXRow;
-    constexpr int kChunks = Cfg::kXRow / 16;
-    constexpr int kDma = 4 + kXDma + (Cfg::kScaled ? 1 : 0);
-    const uint8_t *x_src[kXDma];
-    uint32_t x_dst[kXDma];
+    using Cfg = TileCfg<MODE, WIDE, NB>;
+    constexpr int S = Cfg::kSlots;
+    constexpr int kChunks = Cfg::kXRow / 16, kRowsPer = 64 / kChunks;
+    const uint8_t *x_src[Cfg::kXDma];
+    uint32_t x_dst[Cfg::kXDma];
     auto row_of = [&](int tr) {  // a row past the tile: its last one again, results dropped
       int gr = r0 + tr;
       gr = gr < r_end ? gr : r_end - 1;
       return MODE == kUp && ts.row_token != nullptr ? (int64_t)ts.row_token[gr] : (int64_t)gr;
     };
 #pragma unroll
-    for (int j = 0; j < kXDma; ++j) {
-      const int piece = (wave * kXDma + j) % kXLoads;  // (spare waves repeat a piece)
+    for (int j = 0; j < Cfg::kXDma; ++j) {
+      const int piece = (wave * Cfg::kXDma + j) % Cfg::kXLoads;  // (spare waves repeat a piece)
       const int tr = piece * kRowsPer + lane / kChunks;
       x_dst[j] = (uint32_t)(Cfg::kW + piece * 1024);
       x_src[j] = x + row_of(tr) * ld_x + ((lane % kChunks) ^ x_swz<WIDE>(tr)) * 16;
@@ -469,47 +490,44 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
     const float *s_src = nullptr;
     uint32_t s_dst = 0;
     if constexpr (Cfg::kScaled) {
-      constexpr int kPieces = 32 * NB / 64 > 1 ? 32 * NB / 64 : 1;
-      const int piece = wave % kPieces;
-      s_src = xs + row_of((piece * 64 + lane) % (32 * NB)) * ld_xs;
+      const int piece = wave % NB;
+      s_src = xs + row_of(piece * 64 + lane) * ld_xs;
       s_dst = (uint32_t)(Cfg::kW + Cfg::kX + piece * 256);
     }
-    auto issue = [&](int kt) {
-      const uint32_t slot = lds0 + (uint32_t)(kt & 1) * Cfg::kStage;
+    auto issue = [&](int st, uint32_t slot) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        tm_dma16_buf_so(w_rs, w_off[j], (uint32_t)kt * kFp8Block, slot + (uint32_t)(wave * 4 + j) * 1024u);
+      for (int j = 0; j < 2; ++j)
+        tm_dma16_buf_so(w_rs, w_off[j], (uint32_t)st * kStageK, lds0 + slot + (uint32_t)(wave * 2 + j) * 1024u);
 #pragma unroll
-      for (int j = 0; j < kXDma; ++j) tm_dma16_s(x_src[j] + (int64_t)kt * Cfg::kXRow, slot + x_dst[j]);
-      if constexpr (Cfg::kScaled) tm_dma4_s(s_src + kt, slot + s_dst);
+      for (int j = 0; j < Cfg::kXDma; ++j) tm_dma16_s(x_src[j] + (int64_t)st * Cfg::kXRow, lds0 + slot + x_dst[j]);
+      if constexpr (Cfg::kScaled) tm_dma4_s(s_src + (st >> 1), lds0 + slot + s_dst);
     };
-    const int tr0 = half * NB * 16;
+    const int tr0 = half * NB * 32 + t;
+    uint32_t b_off[WIDE ? 4 : 2];
 #pragma unroll
     for (int j = 0; j < (WIDE ? 4 : 2); ++j) {
-      const int c = WIDE ? 8 * (j >> 1) + 2 * g + (j & 1) : 4 * j + g;
-      b_off[j] = (uint32_t)(Cfg::kW + (tr0 + t) * Cfg::kXRow + (c ^ x_swz<WIDE>(tr0 + t)) * 16);
+      const int c = WIDE ? 4 * (j >> 1) + 2 * h + (j & 1) : 2 * j + h;  // k = 32 (j / 2) + 16 h + 8 (j % 2)
+      b_off[j] = (uint32_t)(Cfg::kW + tr0 * Cfg::kXRow + (c ^ x_swz<WIDE>(tr0)) * 16);
     }
-    issue(0);
-    if (KT > 1) issue(1);
-    for (int kt = 0; kt < KT; ++kt) {
-      if (kt + 1 < KT) tm_wait_vm_lgkm0_mem<kDma>();
-      else tm_wait_vm_lgkm0_mem<0>();
-      barrier();  // stage kt landed, in every wave
-      const char *const st = lds + (kt & 1) * Cfg::kStage;
-      if (kt > 0 && (kt & 63) == 0) load_sw(kt);
-      const float sw0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(swv[0]), kt & 63));
-      const float sw1 = MODE == kUp ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(swv[1]), kt & 63)) : sw0;
-      uint4 af[4][WIDE ? 4 : 2];
+    tm_f32x16 p[2][NB];
+    auto step = [&](auto odd_c, int st, uint32_t slot, uint32_t free_slot) {
+      constexpr bool kOdd = decltype(odd_c)::value;
+      const int left = steps - 1 - st;
+      wait_stages<Cfg::kDma, S - 2>(left < S - 2 ? left : S - 2);
+      barrier();  // stage st landed, in every wave; every wave has read stage st - 1
+      if (st - 1 + S < steps && st > 0) issue(st - 1 + S, free_slot);
+      const char *const sp = lds + slot;
+      uint4 af[2][WIDE ? 4 : 2];
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
+      for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4 r = *reinterpret_cast<const uint4 *>(st + a_off[a][h]);
+        for (int c = 0; c < 2; ++c) {
+          const uint4 r = *reinterpret_cast<const uint4 *>(sp + a_off[c] + a * kABlock);
           if constexpr (WIDE) {
-            af[a][2 * h] = tm_fp8_to_bf16x8(r.x, r.y);
-            af[a][2 * h + 1] = tm_fp8_to_bf16x8(r.z, r.w);
+            af[a][2 * c] = tm_fp8_to_bf16x8(r.x, r.y);
+            af[a][2 * c + 1] = tm_fp8_to_bf16x8(r.z, r.w);
           } else {
-            af[a][h] = r;
+            af[a][c] = r;
           }
         }
 #pragma unroll
@@ -517,120 +535,123 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
         uint4 bf[WIDE ? 4 : 2];
 #pragma unroll
         for (int j = 0; j < (WIDE ? 4 : 2); ++j)
-          bf[j] = *reinterpret_cast<const uint4 *>(st + b_off[j] + q * 16 * Cfg::kXRow);
-        float sx = 1.f;
-        if constexpr (Cfg::kScaled)
-          sx = *reinterpret_cast<const float *>(st + Cfg::kW + Cfg::kX + (tr0 + 16 * q + t) * 4);
-        tm_f32x4 p[4];
-#pragma unroll
-        for (int a = 0; a < 4; ++a) p[a] = tm_f32x4{};
+          bf[j] = *reinterpret_cast<const uint4 *>(sp + b_off[j] + q * 32 * Cfg::kXRow);
         if constexpr (WIDE) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int a = 0; a < 4; ++a) p[a] = tm_mfma16x16x32<TM_DT_BF16>(af[a][j], bf[j], p[a]);
+            for (int a = 0; a < 2; ++a)
+              p[a][q] = tm_mfma32x32x16<TM_DT_BF16>(af[a][j], bf[j], !kOdd && j == 0 ? tm_f32x16{} : p[a][q]);
         } else {
 #pragma unroll
-          for (int a = 0; a < 4; ++a) p[a] = tm_mfma16x16x128_fp8(af[a], bf, p[a]);
-        }
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          const float s = (MODE == kUp && a >= 2 ? sw1 : sw0) * sx;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[a][q][i] = fmaf(p[a][i], s, acc[a][q][i]);
+          for (int a = 0; a < 2; ++a) p[a][q] = tm_mfma32x32x64_fp8(af[a], bf, !kOdd ? tm_f32x16{} : p[a][q]);
         }
       }
-      tm_wait_vm_lgkm0_mem<63>();  // this wave has read the stage
-      barrier();                   // ... and every wave
-      if (kt + 2 < KT) issue(kt + 2);
+      if constexpr (kOdd) {
+        const int kb = st >> 1;
+        const float sw0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(swv[0]), kb & 63));
+        const float sw1 = MODE == kUp ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(swv[1]), kb & 63)) : sw0;
+#pragma unroll
+        for (int q = 0; q < NB; ++q) {
+          float sx = 1.f;
+          if constexpr (Cfg::kScaled)
+            sx = *reinterpret_cast<const float *>(sp + Cfg::kW + Cfg::kX + (tr0 + 32 * q) * 4);
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            const float s = (a == 1 ? sw1 : sw0) * sx;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[a][q][i] = fmaf(p[a][q][i], s, acc[a][q][i]);
+          }
+        }
+        if (((kb + 1) & 63) == 0 && kb + 1 < KT) load_sw(kb + 1);
+      }
+    };
+    for (int st = 0; st < S && st < steps; ++st) issue(st, (uint32_t)(st * Cfg::kStage));
+    uint32_t slot = 0, prev = (S - 1) * Cfg::kStage;
+    auto next = [&] {
+      prev = slot;
+      slot = slot == (S - 1) * Cfg::kStage ? 0u : slot + Cfg::kStage;
+    };
+    for (int kt = 0; kt < KT; ++kt) {
+      step(std::false_type{}, 2 * kt, slot, prev);
+      next();
+      step(std::true_type{}, 2 * kt + 1, slot, prev);
+      next();
     }
   };
-  const int nb = (rows + 31) / 32;
-  int used = NBMAX;  // row blocks per half that were multiplied
-  if constexpr (NBMAX >= 8) {
-    if (nb <= 1) { run(std::integral_constant<int, 1>{}); used = 1; }
-    else if (nb <= 2) { run(std::integral_constant<int, 2>{}); used = 2; }
-    else if (nb <= 4) { run(std::integral_constant<int, 4>{}); used = 4; }
-    else run(std::integral_constant<int, NBMAX>{});
-  } else {
-    if (nb <= 1) { run(std::integral_constant<int, 1>{}); used = 1; }
-    else if (nb <= 2) { run(std::integral_constant<int, 2>{}); used = 2; }
-    else run(std::integral_constant<int, NBMAX>{});
-  }
-  const int first = half * used * 16;  // this wave's first row in the tile
+  const int used = rows > 64 ? 2 : 1;  // row blocks per half
+  if (used == 1) run(std::integral_constant<int, 1>{});
+  else run(std::integral_constant<int, 2>{});
+  const int first = half * used * 32 + t;  // this lane's first row in the tile
 
   if constexpr (MODE == kUp) {
-    // lane: row t of each block, columns n0 + 32 cg + 8 g + 4 a + i
-    const int c = n0 + cg * 32 + 8 * g;
+    // lane: row t of each block, columns n0 + 32 cg + 16 h + i
+    tm_wait_vm_lgkm0_mem<0>();
+    barrier();  // the ring is free
+    uint32_t *const top = reinterpret_cast<uint32_t *>(ring);  // [128 rows][4 groups]
+    const int c = n0 + cg * 32 + 16 * h;
 #pragma unroll
-    for (int q = 0; q < NBMAX; ++q) {
+    for (int q = 0; q < 2; ++q) {
       if (q >= used) continue;  // uniform
       uint32_t m = 0;
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float gv = acc[a][q][i];
-          acc[a][q][i] = gv * __builtin_amdgcn_rcpf(1.f + __expf(-gv)) * acc[a + 2][q][i];
-          m = tm_fp8_amax(m, acc[a][q][i]);
-        }
-      m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+      for (int i = 0; i < 16; ++i) {
+        const float gv = acc[0][q][i];
+        acc[0][q][i] = gv * __builtin_amdgcn_rcpf(1.f + __expf(-gv)) * acc[1][q][i];
+        m = tm_fp8_amax(m, acc[0][q][i]);
+      }
       m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-      if (g == 0) s_top[(first + 16 * q + t) * 4 + cg] = m;
+      if (h == 0) top[(first + 32 * q) * 4 + cg] = m;
     }
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < NBMAX; ++q) {
-      if (q >= used) continue;  // uniform
-      const int tr = first + 16 * q + t;
-      const uint4 m4 = *reinterpret_cast<const uint4 *>(&s_top[tr * 4]);
+    for (int q = 0; q < 2; ++q) {
+      const int tr = first + 32 * q;
+      if (q >= used || tr >= rows) continue;
+      const uint4 m4 = *reinterpret_cast<const uint4 *>(&top[tr * 4]);
       float inv;
       const float s = tm_fp8_scale(max(max(m4.x, m4.y), max(m4.z, m4.w)), inv);
-      if (tr < rows) {
-        float v[8];
+      float v[16];
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[4 * a + i] = tm_fp8_quot(acc[a][q][i], inv);
-        *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(dst.y) + (int64_t)(r0 + tr) * dst.ld + c) =
-            make_uint2(tm_fp8_pack4(v[0], v[1], v[2], v[3]), tm_fp8_pack4(v[4], v[5], v[6], v[7]));
-        if (g == 0 && cg == 0) fs[(int64_t)(r0 + tr) * n_blk + n0 / kFp8Block] = s;
-      }
+      for (int i = 0; i < 16; ++i) v[i] = tm_fp8_quot(acc[0][q][i], inv);
+      *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(dst.y) + (int64_t)(r0 + tr) * dst.ld + c) =
+          make_uint4(tm_fp8_pack4(v[0], v[1], v[2], v[3]), tm_fp8_pack4(v[4], v[5], v[6], v[7]),
+                     tm_fp8_pack4(v[8], v[9], v[10], v[11]), tm_fp8_pack4(v[12], v[13], v[14], v[15]));
+      if (h == 0 && cg == 0) fs[(int64_t)(r0 + tr) * n_blk + n0 / kFp8Block] = s;
     }
   } else {
-    const int c = n0 + cg * 64 + 16 * g;
+    const int c = n0 + cg * 64 + 32 * h;
 #pragma unroll
-    for (int q = 0; q < NBMAX; ++q) {
-      const int tr = first + 16 * q + t;
+    for (int q = 0; q < 2; ++q) {
+      const int tr = first + 32 * q;
       if (q >= used || tr >= rows || c >= n_out) continue;
       const int64_t row = r0 + tr;
       const int64_t at = ts.row_out != nullptr ? ts.row_out[row] : row * dst.ld;
 #pragma unroll
-      for (int a = 0; a < 4; ++a) {
+      for (int u = 0; u < 8; ++u) {
         float v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          v[i] = acc[a][q][i];
-          if (dst.add != nullptr && c + 4 * a + i < n_out) v[i] += at_f<DT>(dst.add, row * dst.ld_add + c + 4 * a + i);
+          v[i] = acc[u >> 2][q][4 * (u & 3) + i];
+          if (dst.add != nullptr && c + 4 * u + i < n_out) v[i] += at_f<DT>(dst.add, row * dst.ld_add + c + 4 * u + i);
         }
-        store4<DT>(dst.y, at, v, c + 4 * a, n_out, vec_out);
+        store4<DT>(dst.y, at, v, c + 4 * u, n_out, vec_out);
       }
     }
   }
 }
 
-template <int DT, int MODE, bool WIDE, int NBMAX>
+template <int DT, int MODE, bool WIDE>
 int tile_launch(const char *name, const void *x, int64_t ld_x, const float *xs, int64_t ld_xs, const Fp8Mat &m0,
                 const Fp8Mat &m1, int n_out, int KT, const Fp8Tiles &ts, const Fp8Dst &dst, float *fs, hipStream_t s) {
-  const int cols = MODE == kUp ? kTileCols / 2 : kTileCols;
-  const int n_tiles = (int)tm_cdiv(n_out, cols);
+  const int n_tiles = (int)tm_cdiv(n_out, MODE == kUp ? kTileCols / 2 : kTileCols);
   const int64_t tiles = ts.tiles != nullptr ? (ts.rows < ts.t_max ? ts.rows : ts.t_max) : tm_cdiv(ts.rows, kTileRows);
-  const int64_t grid = tiles * n_tiles * (8 / NBMAX);
+  const int64_t grid = tiles * n_tiles * kTileParts;
   TM_REQUIRE(grid < ((int64_t)1 << 31), TM_EINVAL_SHAPE, "%s: too many rows", name);
   const int64_t esz = Elem<DT>::kBytes;
   const bool vec_out = (reinterpret_cast<uintptr_t>(dst.y) & 15) == 0 && dst.ld * esz % 16 == 0 &&
                        dst.so_b * esz % 16 == 0 && dst.so_s * esz % 16 == 0;
-  hipLaunchKernelGGL((tile_kernel<DT, MODE, WIDE, NBMAX>), dim3((unsigned)grid), dim3(kTileThreads), 0, s,
+  hipLaunchKernelGGL((tile_kernel<DT, MODE, WIDE>), dim3((unsigned)grid), dim3(kTileThreads), 0, s,
                      static_cast<const uint8_t *>(x), ld_x, xs, ld_xs, m0, m1, n_out, KT, n_tiles, ts, dst, fs, vec_out);
   TM_LAUNCH_CHECK(name);
   return TM_OK;
@@ -706,7 +727,7 @@ extern "C" int tm_fp8_linear(int32_t dtype, const void *x, const float *x_scale,
   ts.rows = (int32_t)n_rows;
   return TM_DISPATCH_DTYPE(dtype, DT, [&] {
     constexpr bool kWide = DT == TM_DT_F32;
-    return tile_launch<DT, kOut, kWide, 4>(name, src.x, src.ld * (kWide ? 2 : 1), src.scale, src.ld_s, m, m, (int)n_out,
+    return tile_launch<DT, kOut, kWide>(name, src.x, src.ld * (kWide ? 2 : 1), src.scale, src.ld_s, m, m, (int)n_out,
                                            (int)kb, ts, dst, nullptr, s);
   });
 }
@@ -795,10 +816,10 @@ int mlp_launch(const char *name, const tm_fp8_experts *ex, const void *x, int64_
   int st = tm_internal_fp8_rows(DT, x, n, h, ld_x, base + ws.x, h, nullptr, 0, kFp8RowsScaled, s);
   if (st != TM_OK) return st;
   float *const fs = reinterpret_cast<float *>(base + ws.fs);
-  st = tile_launch<DT, kUp, true, 4>(name, base + ws.x, (int64_t)h * 2, nullptr, 0, w1, w3, inter, h / kFp8Block, *ts,
+  st = tile_launch<DT, kUp, true>(name, base + ws.x, (int64_t)h * 2, nullptr, 0, w1, w3, inter, h / kFp8Block, *ts,
                                      mid, fs, s);
   if (st != TM_OK) return st;
-  return tile_launch<DT, kOut, false, 4>(name, base + ws.f, inter, fs, inter / kFp8Block, w2, w2, h, inter / kFp8Block,
+  return tile_launch<DT, kOut, false>(name, base + ws.f, inter, fs, inter / kFp8Block, w2, w2, h, inter / kFp8Block,
                                          *ts, dst, nullptr, s);
 }
 
