@@ -19,6 +19,15 @@ __device__ __forceinline__ uint32_t tm_fp8_amax(uint32_t m, float v) {
   return a < 0x7f800000u && a > m ? a : m;
 }
 
+// Maximum over each 16-lane row of the wave, in every lane of it.
+__device__ __forceinline__ uint32_t tm_row16_max(uint32_t v) {
+  v = max(v, tm_dpp<0xB1>(v, v));   // quad_perm [1,0,3,2]
+  v = max(v, tm_dpp<0x4E>(v, v));   // quad_perm [2,3,0,1]
+  v = max(v, tm_dpp<0x141>(v, v));  // row_half_mirror
+  v = max(v, tm_dpp<0x140>(v, v));  // row_mirror
+  return v;
+}
+
 // The block scale of max|v| (bits): a / s <= 448 = 1.75 * 2^8 with a = m 2^e,
 // 1 <= m < 2, asks for s = 2^(e - 8), or 2^(e - 7) where m > 1.75.  Subnormal
 // a gives the smallest scale.  `inv` receives 1 / s (exact).

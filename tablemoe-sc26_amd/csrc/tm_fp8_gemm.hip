@@ -33,6 +33,7 @@ struct Fp8Rows {
   const uint8_t *mask;
   int64_t ms_b, ms_s;
   int32_t top_k, n_experts;
+  bool by_expert;  // a workgroup's item is an expert (else a slot)
 };
 
 // Activations: element (row, k) at x[row * ld + k]; kE4M3: with scale[row * ld_s + k / 128].
@@ -86,114 +87,91 @@ __device__ __forceinline__ void store4(void *y, int64_t at, const float (&v)[4],
 // ---------------------------------------------------------------------------
 // Few rows: a stream of the weights.
 //
-// A workgroup of S waves owns 16 weight rows (up: of W1 and of W3); wave w
-// holds their blocks [w KPW, (w + 1) KPW) in registers, loaded at once, and
-// multiplies them with the workgroup's rows, 16 at a time, on the bf16
-// instructions (K of more than S KPW blocks: in passes, loaded again for each
-// 16 rows); the waves' sums are added in wave order through LDS.  Each lane
-// quantises its own piece of a row on the way (32 columns of each block), so
-// neither the activations nor, in the down product, f needs a launch before.
+// A workgroup of S waves owns NA blocks of 16 weight rows (up: of W1 and of W3).
+// Wave w holds blocks [w KPW, (w + 1) KPW) of their 128-column blocks in
+// registers, loaded at once (K of more than S KPW: in passes, loaded again for
+// each chunk of rows).  The workgroup quantises its rows, up to 16 at a time,
+// into LDS (16 lanes own a block of a row), multiplies them on the bf16
+// instructions and adds the waves' sums in wave order through LDS.  No launch
+// before it groups the rows or quantises them: a call is its two products.
+//
+// Quantising in the operand's layout instead, every lane 32 columns of its row,
+// cost the same for one row as for 16 and bound the kernel: 256 slots of 110
+// experts (2048 x 768) up 140 us, down 119.
 // ---------------------------------------------------------------------------
 constexpr int kMaxSlots = 1024;  // (token, slot) pairs of a call that are found in the launch
 constexpr int kMaxWaves = 8;
+constexpr int kStreamLds = 49152;  // bytes of quantised rows
 
-template <int DTX>
-__device__ __forceinline__ void load_x(const Fp8Src &src, int64_t row, int kb, int g, bool live, float (&v)[4][8]) {
-  using T = typename Elem<DTX>::T;
-  const T *const p = static_cast<const T *>(src.x) + row * src.ld;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t c = (int64_t)kb * kFp8Block + 64 * (j >> 1) + 16 * g + 8 * (j & 1);
-    if (live && c + 8 <= src.k) {
-      tm_load8<DTX>(p + c, v[j]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] = live && c + i < src.k ? Elem<DTX>::to_f(p[c + i]) : 0.f;
-    }
-  }
+// Rows of a chunk: what fits, 16 at most.
+__host__ __device__ inline int stream_chunk(int KT, int64_t most) {
+  const int64_t fit = kStreamLds / (KT * (kFp8Block + 4) + 16);
+  const int64_t c = fit < 16 ? fit : 16;
+  return (int)(c < most ? c : most);
 }
 
-// B operands of block kb: this lane's 32 columns of its row, quantised, as
-// bf16 values q * s.
-template <int DTX>
-__device__ __forceinline__ void quantised_frag(const float (&v)[4][8], uint4 (&b)[4]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = tm_fp8_amax(m, v[j][i]);
-  m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-  m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-  float inv;
-  const float s = tm_fp8_scale(m, inv);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float t[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = tm_fp8_quot(v[j][i], inv);
-    const uint2 lo = tm_fp8_scaled_bf16x4(tm_fp8_pack4(t[0], t[1], t[2], t[3]), s);
-    const uint2 hi = tm_fp8_scaled_bf16x4(tm_fp8_pack4(t[4], t[5], t[6], t[7]), s);
-    b[j] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-  }
-}
-
-template <int DT, int DTX, int MODE, int KPW>
+template <int DT, int DTX, int MODE, int NA, int KPW>
 __global__ __launch_bounds__(64 * kMaxWaves) void stream_kernel(Fp8Src src, Fp8Rows rows, Fp8Mat m0, Fp8Mat m1, int n_out,
-                                                                int ld_w, int KT, int n_groups, Fp8Dst dst,
+                                                                int KT, int n_groups, int chunk, Fp8Dst dst,
                                                                 bool vec_out) {
   constexpr int NM = MODE == kUp ? 2 : 1;
-  __shared__ float4 red[kMaxWaves][NM][64];
+  __shared__ float4 red[kMaxWaves][NM * NA][64];
   __shared__ int list[kMaxSlots];
-  __shared__ int s_count;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = (int)blockDim.x >> 6;
+  __shared__ int s_count, s_first;
+  extern __shared__ uint4 xq[];  // [chunk][KT * 128 + 16] bytes, then scales [chunk][KT]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int threads = blockDim.x, S = threads >> 6;
   const int t = lane & 15, g = lane >> 4;
-  const int n0 = (int)(blockIdx.x % n_groups) * 16;
+  const int n0 = (int)(blockIdx.x % n_groups) * (16 * NA);
   const int64_t item = blockIdx.x / n_groups;
   int e = 0;
   int64_t count = rows.n;
   if (rows.ids != nullptr) {
-    // Slot `item` leads if its expert has no earlier slot; the leader's
-    // workgroups take all of the expert's slots, in order.
+    // This workgroup's expert: `item` (by_expert), or that of slot `item`, whose
+    // first slot's workgroups take all of them.
     const int total = (int)rows.n * rows.top_k;
     auto expert_of = [&](int p) {
       const int b = p / rows.top_k, s = p - b * rows.top_k;
       const int64_t id = rows.ids[b * rows.ld_ids + s];
       return rows.mask[b * rows.ms_b + s * rows.ms_s] && id >= 0 && id < rows.n_experts ? (int)id : -1;
     };
-    e = expert_of((int)item);
+    e = rows.by_expert ? (int)item : expert_of((int)item);
     if (e < 0) return;  // uniform
-    if (wave == 0) {
-      int c = 0;
-      for (int p0 = 0; p0 < total; p0 += 64) {
-        const int p = p0 + lane;
-        const bool mine = p < total && expert_of(p) == e;
-        const uint64_t all = __ballot(mine);
-        if (mine) list[c + __popcll(all & ((1ull << lane) - 1))] = p;
-        c += __popcll(all);
-      }
-      if (lane == 0) s_count = c;
+    if (tid == 0) {
+      s_count = 0;
+      s_first = total;
     }
     __syncthreads();
-    if (list[0] != (int)item) return;  // uniform
+    for (int p = tid; p < total; p += threads)
+      if (expert_of(p) == e) {
+        list[atomicAdd(&s_count, 1)] = p;  // (a row's result does not depend on its place)
+        atomicMin(&s_first, p);
+      }
+    __syncthreads();
     count = s_count;
+    if (count == 0 || (!rows.by_expert && s_first != (int)item)) return;  // uniform
   }
 
-  uint4 w[NM][KPW][2];
+  uint4 w[NM][NA][KPW][2];
   float sw[NM][KPW];
   const int nb = (n_out + kFp8Block - 1) / kFp8Block;
+  const int64_t ld_w = (int64_t)KT * kFp8Block;
   auto load_w = [&](int kb0) {
-    const int r = n0 + t < n_out ? n0 + t : n_out - 1;  // (a row past n_out: the last one again, not stored)
 #pragma unroll
     for (int m = 0; m < NM; ++m) {
       const Fp8Mat &mat = m == 0 ? m0 : m1;
-      const uint8_t *const p = mat.w + ((int64_t)e * n_out + r) * ld_w + 16 * g;
       const float *const ps = mat.s + ((int64_t)e * nb + n0 / kFp8Block) * KT;
 #pragma unroll
       for (int j = 0; j < KPW; ++j) {
         const int kb = kb0 + j;
         if (kb < KT) {  // uniform
-          w[m][j][0] = *reinterpret_cast<const uint4 *>(p + (int64_t)kb * kFp8Block);
-          w[m][j][1] = *reinterpret_cast<const uint4 *>(p + (int64_t)kb * kFp8Block + 64);
+#pragma unroll
+          for (int a = 0; a < NA; ++a) {
+            const int r = n0 + 16 * a + t < n_out ? n0 + 16 * a + t : n_out - 1;  // (past n_out: not stored)
+            const uint8_t *const p = mat.w + ((int64_t)e * n_out + r) * ld_w + (int64_t)kb * kFp8Block + 16 * g;
+            w[m][a][j][0] = *reinterpret_cast<const uint4 *>(p);
+            w[m][a][j][1] = *reinterpret_cast<const uint4 *>(p + 64);
+          }
           sw[m][j] = ps[kb];
         }
       }
@@ -201,106 +179,133 @@ __global__ __launch_bounds__(64 * kMaxWaves) void stream_kernel(Fp8Src src, Fp8R
   };
   const bool once = KT <= S * KPW;
   if (once) load_w(wave * KPW);
-  for (int64_t c0 = 0; c0 < count; c0 += 16) {
-    const bool live = c0 + t < count;
-    int64_t xr = c0 + t;
-    if (rows.ids != nullptr) xr = live ? (MODE == kUp ? list[c0 + t] / rows.top_k : list[c0 + t]) : 0;
-    else if (!live) xr = 0;
-    tm_f32x4 acc[NM];
-#pragma unroll
-    for (int m = 0; m < NM; ++m) acc[m] = tm_f32x4{};
-    for (int kb0 = wave * KPW; kb0 < KT; kb0 += S * KPW) {
-    if (!once) load_w(kb0);
-#pragma unroll
-    for (int j = 0; j < KPW; ++j) {
-      const int kb = kb0 + j;
-      if (kb >= KT) continue;  // uniform
-      uint4 b[4];
-      float sx = 1.f;
+  const int x_row = KT * kFp8Block + 16;  // bytes of a row in LDS (16 more: rows start on other banks)
+  char *const xb = reinterpret_cast<char *>(xq);
+  float *const xs = reinterpret_cast<float *>(xb + chunk * x_row);
+  for (int64_t c0 = 0; c0 < count; c0 += chunk) {
+    const int here = (int)(count - c0 < chunk ? count - c0 : chunk);
+    // the chunk's rows to LDS: block b of row r by 16 lanes, 8 columns each
+    for (int i = tid >> 4; i < here * KT; i += threads >> 4) {
+      const int r = i / KT, b = i - r * KT;
+      const int p = rows.ids != nullptr ? list[c0 + r] : 0;
+      const int64_t xr = rows.ids == nullptr ? c0 + r : MODE == kUp ? p / rows.top_k : p;
+      const int c = b * kFp8Block + t * 8;
+      uint2 q;
+      float s;
       if constexpr (DTX == kE4M3) {
-        const uint8_t *const p = static_cast<const uint8_t *>(src.x) + xr * src.ld + (int64_t)kb * kFp8Block + 16 * g;
-        uint4 q0 = make_uint4(0, 0, 0, 0), q1 = q0;
-        if (live) {
-          q0 = *reinterpret_cast<const uint4 *>(p);
-          q1 = *reinterpret_cast<const uint4 *>(p + 64);
-          sx = src.scale[xr * src.ld_s + kb];
-        }
-        b[0] = tm_fp8_to_bf16x8(q0.x, q0.y);
-        b[1] = tm_fp8_to_bf16x8(q0.z, q0.w);
-        b[2] = tm_fp8_to_bf16x8(q1.x, q1.y);
-        b[3] = tm_fp8_to_bf16x8(q1.z, q1.w);
+        q = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(src.x) + xr * src.ld + c);
+        s = src.scale[xr * src.ld_s + b];
       } else {
-        float v[4][8];
-        load_x<DTX>(src, xr, kb, g, live, v);
-        quantised_frag<DTX>(v, b);
-      }
+        float v[8];
+        const auto *const px = static_cast<const typename Elem<DTX>::T *>(src.x) + xr * src.ld;
+        if (c + 8 <= src.k) {
+          tm_load8<DTX>(px + c, v);
+        } else {
 #pragma unroll
-      for (int m = 0; m < NM; ++m) {
-        tm_f32x4 p = {};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          p = tm_mfma16x16x32<TM_DT_BF16>(tm_fp8_to_bf16x8(w[m][j][h].x, w[m][j][h].y), b[2 * h], p);
-          p = tm_mfma16x16x32<TM_DT_BF16>(tm_fp8_to_bf16x8(w[m][j][h].z, w[m][j][h].w), b[2 * h + 1], p);
+          for (int u = 0; u < 8; ++u) v[u] = c + u < src.k ? Elem<DTX>::to_f(px[c + u]) : 0.f;
         }
+        uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(p[i], sw[m][j] * sx, acc[m][i]);
+        for (int u = 0; u < 8; ++u) m = tm_fp8_amax(m, v[u]);
+        m = tm_row16_max(m);
+        float inv;
+        s = tm_fp8_scale(m, inv);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = tm_fp8_quot(v[u], inv);
+        q = make_uint2(tm_fp8_pack4(v[0], v[1], v[2], v[3]), tm_fp8_pack4(v[4], v[5], v[6], v[7]));
+      }
+      *reinterpret_cast<uint2 *>(xb + r * x_row + c) = q;
+      if (t == 0) xs[r * KT + b] = s;
+    }
+    __syncthreads();
+    const int row = t < here ? t : here - 1;  // (lanes past the chunk: its last row again, not stored)
+    tm_f32x4 acc[NM][NA];
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+      for (int a = 0; a < NA; ++a) acc[m][a] = tm_f32x4{};
+    for (int kb0 = wave * KPW; kb0 < KT; kb0 += S * KPW) {
+      if (!once) load_w(kb0);
+#pragma unroll
+      for (int j = 0; j < KPW; ++j) {
+        const int kb = kb0 + j;
+        if (kb >= KT) continue;  // uniform
+        const char *const p = xb + row * x_row + kb * kFp8Block + 16 * g;
+        const uint4 q0 = *reinterpret_cast<const uint4 *>(p), q1 = *reinterpret_cast<const uint4 *>(p + 64);
+        const float sx = xs[row * KT + kb];
+        const uint4 b[4] = {tm_fp8_to_bf16x8(q0.x, q0.y), tm_fp8_to_bf16x8(q0.z, q0.w), tm_fp8_to_bf16x8(q1.x, q1.y),
+                            tm_fp8_to_bf16x8(q1.z, q1.w)};
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+#pragma unroll
+          for (int a = 0; a < NA; ++a) {
+            tm_f32x4 d = {};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint4 &v = w[m][a][j][h];
+              d = tm_mfma16x16x32<TM_DT_BF16>(tm_fp8_to_bf16x8(v.x, v.y), b[2 * h], d);
+              d = tm_mfma16x16x32<TM_DT_BF16>(tm_fp8_to_bf16x8(v.z, v.w), b[2 * h + 1], d);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[m][a][i] = fmaf(d[i], sw[m][j] * sx, acc[m][a][i]);
+          }
       }
     }
-    }
 #pragma unroll
-    for (int m = 0; m < NM; ++m) red[wave][m][lane] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+      for (int a = 0; a < NA; ++a)
+        red[wave][m * NA + a][lane] = make_float4(acc[m][a][0], acc[m][a][1], acc[m][a][2], acc[m][a][3]);
     __syncthreads();
-    if (wave == 0 && live) {
-      // lane: row t, columns n0 + 4 g .. + 3
+    for (int i = tid; i < NA * 64; i += threads) {
+      // row t of the chunk, columns n0 + 16 a + 4 g .. + 3
+      const int a = i >> 6;
       float v[NM][4] = {};
       for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
-          const float4 p = red[s][m][lane];
+          const float4 p = red[s][m * NA + a][i & 63];
           v[m][0] += p.x; v[m][1] += p.y; v[m][2] += p.z; v[m][3] += p.w;
         }
-      const int c = n0 + 4 * g;
+      if (t >= here) continue;
+      const int c = n0 + 16 * a + 4 * g;
+      const int p = rows.ids != nullptr ? list[c0 + t] : 0;
       if constexpr (MODE == kUp) {
         float f[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = v[0][i] * __builtin_amdgcn_rcpf(1.f + __expf(-v[0][i])) * v[NM - 1][i];
-        const int64_t fr = rows.ids != nullptr ? list[c0 + t] : c0 + t;
-        store4<TM_DT_F32>(dst.y, fr * dst.ld, f, c, n_out, true);
+        for (int u = 0; u < 4; ++u) f[u] = v[0][u] * __builtin_amdgcn_rcpf(1.f + __expf(-v[0][u])) * v[NM - 1][u];
+        store4<TM_DT_F32>(dst.y, (rows.ids != nullptr ? p : c0 + t) * dst.ld, f, c, n_out, true);
       } else {
-        int64_t at = xr * dst.ld;
-        if (rows.ids != nullptr) {
-          const int p = list[c0 + t];
-          at = (p / rows.top_k) * dst.so_b + (p % rows.top_k) * dst.so_s;
-        }
+        const int64_t at = rows.ids != nullptr ? (p / rows.top_k) * dst.so_b + (p % rows.top_k) * dst.so_s
+                                               : (c0 + t) * dst.ld;
         if (dst.add != nullptr)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (c + i < n_out) v[0][i] += at_f<DT>(dst.add, xr * dst.ld_add + c + i);
+          for (int u = 0; u < 4; ++u)
+            if (c + u < n_out) v[0][u] += at_f<DT>(dst.add, (c0 + t) * dst.ld_add + c + u);
         store4<DT>(dst.y, at, v[0], c, n_out, vec_out);
       }
     }
-    __syncthreads();
+    // (the next chunk's rows go to LDS that every wave has read: it wrote its sums
+    // after that; its sums go to red after the next barrier)
   }
 }
 
-template <int DT, int DTX, int MODE>
-int stream_launch(const char *name, const Fp8Src &src, const Fp8Rows &rows, const Fp8Mat &m0, const Fp8Mat &m1,
-                  int n_out, int KT, const Fp8Dst &dst, hipStream_t s) {
-  const int n_groups = (int)tm_cdiv(n_out, 16);
-  const int64_t items = rows.ids != nullptr ? rows.n * rows.top_k : 1;
+template <int DT, int DTX, int MODE, int NA, int KPW>
+int stream_launch(const char *name, const Fp8Src &src, Fp8Rows rows, const Fp8Mat &m0, const Fp8Mat &m1, int n_out,
+                  int KT, const Fp8Dst &dst, hipStream_t s) {
+  const int n_groups = (int)tm_cdiv(n_out, 16 * NA);
+  const int64_t total = rows.ids != nullptr ? rows.n * rows.top_k : rows.n;
+  rows.by_expert = rows.ids != nullptr && total >= rows.n_experts;
+  const int64_t items = rows.ids == nullptr ? 1 : rows.by_expert ? rows.n_experts : total;
   TM_REQUIRE(items * n_groups < ((int64_t)1 << 31), TM_EINVAL_SHAPE, "%s: too many rows", name);
   const int64_t esz = Elem<DT>::kBytes;
   const bool vec_out = (reinterpret_cast<uintptr_t>(dst.y) & 15) == 0 && dst.ld * esz % 16 == 0 &&
                        dst.so_b * esz % 16 == 0 && dst.so_s * esz % 16 == 0;
-  const dim3 grid((unsigned)(items * n_groups));
-  const int ld_w = KT * kFp8Block;
-#define TM_STREAM(KPW_)                                                                                            \
-  hipLaunchKernelGGL((stream_kernel<DT, DTX, MODE, KPW_>), grid, dim3(64 * (unsigned)waves(KPW_)), 0, s, src, \
-                     rows, m0, m1, n_out, ld_w, KT, n_groups, dst, vec_out)
-  auto waves = [&](int kpw) { return tm_cdiv(KT, kpw) < kMaxWaves ? tm_cdiv(KT, kpw) : kMaxWaves; };
-  if (KT <= 8) TM_STREAM(2);
-  else TM_STREAM(4);
-#undef TM_STREAM
+  const int waves = (int)(tm_cdiv(KT, KPW) < kMaxWaves ? tm_cdiv(KT, KPW) : kMaxWaves);
+  const int chunk = stream_chunk(KT, total);
+  hipLaunchKernelGGL((stream_kernel<DT, DTX, MODE, NA, KPW>), dim3((unsigned)(items * n_groups)), dim3(64 * waves),
+                     (size_t)chunk * (KT * (kFp8Block + 4) + 16), s, src, rows, m0, m1, n_out, KT, n_groups, chunk, dst,
+                     vec_out);
   TM_LAUNCH_CHECK(name);
   return TM_OK;
 }
@@ -720,8 +725,8 @@ extern "C" int tm_fp8_linear(int32_t dtype, const void *x, const float *x_scale,
   const Fp8Dst dst{out, ld_out, 0, 0, bias, 0};
   if (!tiles)
     return TM_DISPATCH_DTYPE(dtype, DT, [&] {
-      return src.scale ? stream_launch<DT, kE4M3, kOut>(name, src, rows, m, m, (int)n_out, (int)kb, dst, s)
-                       : stream_launch<DT, DT, kOut>(name, src, rows, m, m, (int)n_out, (int)kb, dst, s);
+      return src.scale ? stream_launch<DT, kE4M3, kOut, 1, 4>(name, src, rows, m, m, (int)n_out, (int)kb, dst, s)
+                       : stream_launch<DT, DT, kOut, 1, 4>(name, src, rows, m, m, (int)n_out, (int)kb, dst, s);
     });
   Fp8Tiles ts{};
   ts.rows = (int32_t)n_rows;
@@ -807,10 +812,10 @@ int mlp_launch(const char *name, const tm_fp8_experts *ex, const void *x, int64_
       w2{static_cast<const uint8_t *>(ex->w2), ex->s2};
   const Fp8Dst mid{base + ws.f, inter, 0, 0, nullptr, 0};
   if (ts == nullptr) {
-    const int st = stream_launch<DT, DT, kUp>(name, Fp8Src{x, ld_x, h, nullptr, 0}, *rows, w1, w3, inter, h / kFp8Block,
+    const int st = stream_launch<DT, DT, kUp, 1, 4>(name, Fp8Src{x, ld_x, h, nullptr, 0}, *rows, w1, w3, inter, h / kFp8Block,
                                               mid, s);
     if (st != TM_OK) return st;
-    return stream_launch<DT, TM_DT_F32, kOut>(name, Fp8Src{base + ws.f, inter, inter, nullptr, 0}, *rows, w2, w2, h,
+    return stream_launch<DT, TM_DT_F32, kOut, 4, 2>(name, Fp8Src{base + ws.f, inter, inter, nullptr, 0}, *rows, w2, w2, h,
                                               inter / kFp8Block, dst, s);
   }
   int st = tm_internal_fp8_rows(DT, x, n, h, ld_x, base + ws.x, h, nullptr, 0, kFp8RowsScaled, s);

@@ -10,15 +10,6 @@ namespace {
 
 constexpr int kQThreads = 256;
 
-// Maximum over each 16-lane row of the wave, in every lane of it.
-__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
-  v = max(v, tm_dpp<0xB1>(v, v));   // quad_perm [1,0,3,2]
-  v = max(v, tm_dpp<0x4E>(v, v));   // quad_perm [2,3,0,1]
-  v = max(v, tm_dpp<0x141>(v, v));  // row_half_mirror
-  v = max(v, tm_dpp<0x140>(v, v));  // row_mirror
-  return v;
-}
-
 // Columns [c, c + 8) of a row of k columns, zero past k; VEC: every full piece
 // is one 16-byte (fp32: two) load.
 template <int DT, bool VEC>
@@ -49,7 +40,7 @@ __global__ __launch_bounds__(kQThreads) void quantize_rows_kernel(const typename
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = tm_fp8_amax(m, v[i]);
-  m = row16_max(m);
+  m = tm_row16_max(m);
   float inv;
   const float s = tm_fp8_scale(m, inv);
 #pragma unroll
