@@ -101,12 +101,12 @@ __device__ __forceinline__ void store4(void *y, int64_t at, const float (&v)[4],
 // ---------------------------------------------------------------------------
 constexpr int kMaxSlots = 1024;  // (token, slot) pairs of a call that are found in the launch
 constexpr int kMaxWaves = 8;
-constexpr int kStreamLds = 49152;  // bytes of quantised rows
+constexpr int kStreamLds = 20480;  // bytes of quantised rows
 
 // Rows of a chunk: what fits, 16 at most.
 __host__ __device__ inline int stream_chunk(int KT, int64_t most) {
   const int64_t fit = kStreamLds / (KT * (kFp8Block + 4) + 16);
-  const int64_t c = fit < 16 ? fit : 16;
+  const int64_t c = fit < 1 ? 1 : fit < 16 ? fit : 16;
   return (int)(c < most ? c : most);
 }
 
@@ -115,13 +115,17 @@ __global__ __launch_bounds__(64 * kMaxWaves) void stream_kernel(Fp8Src src, Fp8R
                                                                 int KT, int n_groups, int chunk, Fp8Dst dst,
                                                                 bool vec_out) {
   constexpr int NM = MODE == kUp ? 2 : 1;
-  __shared__ float4 red[kMaxWaves][NM * NA][64];
-  __shared__ int list[kMaxSlots];
+  // the waves' sums [S][NM * NA][64], the chunk's rows [chunk][KT * 128 + 16] bytes,
+  // their scales [chunk][KT], the expert's slots
+  extern __shared__ float4 red[];
   __shared__ int s_count, s_first;
-  extern __shared__ uint4 xq[];  // [chunk][KT * 128 + 16] bytes, then scales [chunk][KT]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int threads = blockDim.x, S = threads >> 6;
   const int t = lane & 15, g = lane >> 4;
+  const int x_row = KT * kFp8Block + 16;  // (16 more: rows start on other banks)
+  char *const xb = reinterpret_cast<char *>(red + S * NM * NA * 64);
+  float *const xs = reinterpret_cast<float *>(xb + chunk * x_row);
+  uint16_t *const list = reinterpret_cast<uint16_t *>(xs + chunk * KT);
   const int n0 = (int)(blockIdx.x % n_groups) * (16 * NA);
   const int64_t item = blockIdx.x / n_groups;
   int e = 0;
@@ -144,7 +148,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void stream_kernel(Fp8Src src, Fp8R
     __syncthreads();
     for (int p = tid; p < total; p += threads)
       if (expert_of(p) == e) {
-        list[atomicAdd(&s_count, 1)] = p;  // (a row's result does not depend on its place)
+        list[atomicAdd(&s_count, 1)] = (uint16_t)p;  // (a row's result does not depend on its place)
         atomicMin(&s_first, p);
       }
     __syncthreads();
@@ -179,9 +183,6 @@ __global__ __launch_bounds__(64 * kMaxWaves) void stream_kernel(Fp8Src src, Fp8R
   };
   const bool once = KT <= S * KPW;
   if (once) load_w(wave * KPW);
-  const int x_row = KT * kFp8Block + 16;  // bytes of a row in LDS (16 more: rows start on other banks)
-  char *const xb = reinterpret_cast<char *>(xq);
-  float *const xs = reinterpret_cast<float *>(xb + chunk * x_row);
   for (int64_t c0 = 0; c0 < count; c0 += chunk) {
     const int here = (int)(count - c0 < chunk ? count - c0 : chunk);
     // the chunk's rows to LDS: block b of row r by 16 lanes, 8 columns each
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void stream_kernel(Fp8Src src, Fp8R
     for (int m = 0; m < NM; ++m)
 #pragma unroll
       for (int a = 0; a < NA; ++a)
-        red[wave][m * NA + a][lane] = make_float4(acc[m][a][0], acc[m][a][1], acc[m][a][2], acc[m][a][3]);
+        red[(wave * (NM * NA) + m * NA + a) * 64 + lane] = make_float4(acc[m][a][0], acc[m][a][1], acc[m][a][2], acc[m][a][3]);
     __syncthreads();
     for (int i = tid; i < NA * 64; i += threads) {
       // row t of the chunk, columns n0 + 16 a + 4 g .. + 3
@@ -264,7 +265,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void stream_kernel(Fp8Src src, Fp8R
       for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
-          const float4 p = red[s][m * NA + a][i & 63];
+          const float4 p = red[(s * (NM * NA) + m * NA + a) * 64 + (i & 63)];
           v[m][0] += p.x; v[m][1] += p.y; v[m][2] += p.z; v[m][3] += p.w;
         }
       if (t >= here) continue;
@@ -304,7 +305,9 @@ int stream_launch(const char *name, const Fp8Src &src, Fp8Rows rows, const Fp8Ma
   const int waves = (int)(tm_cdiv(KT, KPW) < kMaxWaves ? tm_cdiv(KT, KPW) : kMaxWaves);
   const int chunk = stream_chunk(KT, total);
   hipLaunchKernelGGL((stream_kernel<DT, DTX, MODE, NA, KPW>), dim3((unsigned)(items * n_groups)), dim3(64 * waves),
-                     (size_t)chunk * (KT * (kFp8Block + 4) + 16), s, src, rows, m0, m1, n_out, KT, n_groups, chunk, dst,
+                     (size_t)waves * ((MODE == kUp ? 2 : 1) * NA) * 1024 + (size_t)chunk * (KT * (kFp8Block + 4) + 16) +
+                         (rows.ids != nullptr ? (size_t)total * 2 : 0),
+                     s, src, rows, m0, m1, n_out, KT, n_groups, chunk, dst,
                      vec_out);
   TM_LAUNCH_CHECK(name);
   return TM_OK;
