@@ -90,3 +90,13 @@ __device__ __forceinline__ tm_f32x16 tm_mfma32x32x64_fp8(const uint4 (&a)[2], co
                       (int)b[1].x, (int)b[1].y, (int)b[1].z, (int)b[1].w};
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 0, 0, 0, 0, 0, 0);
 }
+
+// The 16 x 128 by 128 x 16 form: row (column) l % 16, 32 of the 128; D as in the
+// 16x16x32 form.
+__device__ __forceinline__ tm_f32x4 tm_mfma16x16x128_fp8(const uint4 (&a)[2], const uint4 (&b)[2], tm_f32x4 c) {
+  const tm_i32x8 x = {(int)a[0].x, (int)a[0].y, (int)a[0].z, (int)a[0].w,
+                      (int)a[1].x, (int)a[1].y, (int)a[1].z, (int)a[1].w};
+  const tm_i32x8 y = {(int)b[0].x, (int)b[0].y, (int)b[0].z, (int)b[0].w,
+                      (int)b[1].x, (int)b[1].y, (int)b[1].z, (int)b[1].w};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 0, 0, 0, 0, 0);
+}

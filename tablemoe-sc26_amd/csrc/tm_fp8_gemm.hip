@@ -95,9 +95,13 @@ __device__ __forceinline__ void store4(void *y, int64_t at, const float (&v)[4],
 // instructions and adds the waves' sums in wave order through LDS.  No launch
 // before it groups the rows or quantises them: a call is its two products.
 //
-// Quantising in the operand's layout instead, every lane 32 columns of its row,
-// cost the same for one row as for 16 and bound the kernel: 256 slots of 110
-// experts (2048 x 768) up 140 us, down 119.
+// Bound by HBM: 256 slots of 110 experts (2048 x 768) stream 352 MB in 65 us (up,
+// 5.4 TB/s) and 176 MB in 37 (down, 4.7); one token's 8 experts take 11 + 6, a
+// chain of latencies (slots, rows, weights, sums).  Up: quantising in the
+// operand's layout, where every lane does 32 columns of its row whether it is
+// live or not, 140; 48 KiB of LDS rows 81; three waves per SIMD instead of four
+// 70; non-temporal weight loads 75; 32 columns per workgroup on eight waves 94.
+// Down: 16 columns 119, 32 columns 38, on the 16-bit instructions 38.
 // ---------------------------------------------------------------------------
 constexpr int kMaxSlots = 1024;  // (token, slot) pairs of a call that are found in the launch
 constexpr int kMaxWaves = 8;
@@ -111,10 +115,11 @@ __host__ __device__ inline int stream_chunk(int KT, int64_t most) {
 }
 
 template <int DT, int DTX, int MODE, int NA, int KPW>
-__global__ __launch_bounds__(64 * kMaxWaves) void stream_kernel(Fp8Src src, Fp8Rows rows, Fp8Mat m0, Fp8Mat m1, int n_out,
+__global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(MODE == kUp ? 4 : 1))) void stream_kernel(Fp8Src src, Fp8Rows rows, Fp8Mat m0, Fp8Mat m1, int n_out,
                                                                 int KT, int n_groups, int chunk, Fp8Dst dst,
                                                                 bool vec_out) {
   constexpr int NM = MODE == kUp ? 2 : 1;
+  constexpr bool WIDE = MODE == kUp || DT == TM_DT_F32;  // on the 16-bit instructions
   // the waves' sums [S][NM * NA][64], the chunk's rows [chunk][KT * 128 + 16] bytes,
   // their scales [chunk][KT], the expert's slots
   extern __shared__ float4 red[];
@@ -186,6 +191,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void stream_kernel(Fp8Src src, Fp8R
   for (int64_t c0 = 0; c0 < count; c0 += chunk) {
     const int here = (int)(count - c0 < chunk ? count - c0 : chunk);
     // the chunk's rows to LDS: block b of row r by 16 lanes, 8 columns each
+    const bool whole = src.k == (int64_t)KT * kFp8Block;  // no row ends inside a block
     for (int i = tid >> 4; i < here * KT; i += threads >> 4) {
       const int r = i / KT, b = i - r * KT;
       const int p = rows.ids != nullptr ? list[c0 + r] : 0;
@@ -199,20 +205,20 @@ __global__ __launch_bounds__(64 * kMaxWaves) void stream_kernel(Fp8Src src, Fp8R
       } else {
         float v[8];
         const auto *const px = static_cast<const typename Elem<DTX>::T *>(src.x) + xr * src.ld;
-        if (c + 8 <= src.k) {
+        if (whole || c + 8 <= src.k) {
           tm_load8<DTX>(px + c, v);
         } else {
 #pragma unroll
-          for (int u = 0; u < 8; ++u) v[u] = c + u < src.k ? Elem<DTX>::to_f(px[c + u]) : 0.f;
+          for (int k = 0; k < 8; ++k) v[k] = c + k < src.k ? Elem<DTX>::to_f(px[c + k]) : 0.f;
         }
         uint32_t m = 0;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) m = tm_fp8_amax(m, v[u]);
+        for (int k = 0; k < 8; ++k) m = tm_fp8_amax(m, v[k]);
         m = tm_row16_max(m);
         float inv;
         s = tm_fp8_scale(m, inv);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = tm_fp8_quot(v[u], inv);
+        for (int k = 0; k < 8; ++k) v[k] = tm_fp8_quot(v[k], inv);
         q = make_uint2(tm_fp8_pack4(v[0], v[1], v[2], v[3]), tm_fp8_pack4(v[4], v[5], v[6], v[7]));
       }
       *reinterpret_cast<uint2 *>(xb + r * x_row + c) = q;
@@ -234,18 +240,30 @@ __global__ __launch_bounds__(64 * kMaxWaves) void stream_kernel(Fp8Src src, Fp8R
         const char *const p = xb + row * x_row + kb * kFp8Block + 16 * g;
         const uint4 q0 = *reinterpret_cast<const uint4 *>(p), q1 = *reinterpret_cast<const uint4 *>(p + 64);
         const float sx = xs[row * KT + kb];
-        const uint4 b[4] = {tm_fp8_to_bf16x8(q0.x, q0.y), tm_fp8_to_bf16x8(q0.z, q0.w), tm_fp8_to_bf16x8(q1.x, q1.y),
-                            tm_fp8_to_bf16x8(q1.z, q1.w)};
+        uint4 b[WIDE ? 4 : 2];
+        if constexpr (WIDE) {
+          b[0] = tm_fp8_to_bf16x8(q0.x, q0.y);
+          b[1] = tm_fp8_to_bf16x8(q0.z, q0.w);
+          b[2] = tm_fp8_to_bf16x8(q1.x, q1.y);
+          b[3] = tm_fp8_to_bf16x8(q1.z, q1.w);
+        } else {
+          b[0] = q0;
+          b[1] = q1;
+        }
 #pragma unroll
         for (int m = 0; m < NM; ++m)
 #pragma unroll
           for (int a = 0; a < NA; ++a) {
             tm_f32x4 d = {};
+            if constexpr (WIDE) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint4 &v = w[m][a][j][h];
-              d = tm_mfma16x16x32<TM_DT_BF16>(tm_fp8_to_bf16x8(v.x, v.y), b[2 * h], d);
-              d = tm_mfma16x16x32<TM_DT_BF16>(tm_fp8_to_bf16x8(v.z, v.w), b[2 * h + 1], d);
+              for (int h = 0; h < 2; ++h) {
+                const uint4 &v = w[m][a][j][h];
+                d = tm_mfma16x16x32<TM_DT_BF16>(tm_fp8_to_bf16x8(v.x, v.y), b[2 * h], d);
+                d = tm_mfma16x16x32<TM_DT_BF16>(tm_fp8_to_bf16x8(v.z, v.w), b[2 * h + 1], d);
+              }
+            } else {
+              d = tm_mfma16x16x128_fp8(w[m][a][j], b, d);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[m][a][i] = fmaf(d[i], sw[m][j] * sx, acc[m][a][i]);
