@@ -52,29 +52,14 @@ __device__ __forceinline__ uint32_t tm_fp8_pack4(float a, float b, float c, floa
 
 typedef __bf16 tm_bf16x2 __attribute__((ext_vector_type(2)));
 
-// Eight e4m3 values as bf16 (exact: 4 significant bits).
-__device__ __forceinline__ uint4 tm_fp8_to_bf16x8(uint32_t lo, uint32_t hi) {
+// Eight e4m3 values, times a power of two, as bf16 (exact: 4 significant bits;
+// apart from products under 2^-126, which blocks of max|v| < 2^-108 alone can have).
+__device__ __forceinline__ uint4 tm_fp8_to_bf16x8(uint32_t lo, uint32_t hi, float s = 1.f) {
   uint4 r;
-  r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
-  r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
-  r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
-  r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
-  return r;
-}
-
-// Two fp32 values whose low 16 bits are zero, as packed bf16.
-__device__ __forceinline__ uint32_t tm_bf16_hi2(float lo, float hi) {
-  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
-}
-
-// Four e4m3 values times a power of two as bf16 (exact, apart from values
-// under 2^-126, which blocks of max|v| < 2^-108 alone can have).
-__device__ __forceinline__ uint2 tm_fp8_scaled_bf16x4(uint32_t q, float s) {
-  typedef float f2 __attribute__((ext_vector_type(2)));
-  const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, true);
-  uint2 r;
-  r.x = tm_bf16_hi2(a.x * s, a.y * s);
-  r.y = tm_bf16_hi2(b.x * s, b.y * s);
+  r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false));
+  r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true));
+  r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false));
+  r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true));
   return r;
 }
 

@@ -336,18 +336,18 @@ int stream_launch(const char *name, const Fp8Src &src, Fp8Rows rows, const Fp8Ma
 //
 // Eight waves: wave w owns 64 weight rows of group w % 4 (up: 32 rows of W1 and
 // the same 32 of W3) and NB blocks of 32 activation rows of half w / 4, in
-// 32 x 32 products.  A stage is 64 columns, global -> LDS by direct loads; LDS
-// holds a ring of as many stages as fit, one barrier per stage: it publishes the
-// stage and frees the slot of the one before.  The products of a block of 128
-// columns (two stages) start from zero and are added to the fp32 accumulators
-// times their scales.
+// 32 x 32 products.  A stage is a block of 128 columns, global -> LDS by direct
+// loads; LDS holds a ring of three, one barrier per stage: it publishes the
+// stage and frees the slot of the one before.  A stage's products start from
+// zero and are added to the fp32 accumulators times their scales.
 //
-// Activations come quantised: e4m3 rows (the 8-bit instructions), or the same
-// values as bf16 rows (WIDE: the 16-bit ones, weights converted on the way from
-// LDS), with their scales; up: bf16 rows q * s.  Which rows of its 64 a lane's
-// operand takes is chosen so that its results are 32 (up: 16) consecutive
-// columns; 16-byte chunks of an LDS row are XOR-ed with the row bits that differ
-// among 16 lanes, so operand reads are free of bank conflicts.
+// Activations come quantised, e4m3 rows and their scales.  The 8-bit
+// instructions take them and the weights as they are; WIDE converts both to bf16
+// on the way from LDS (up: the rows' scales, powers of two, with them).  Which
+// rows of its 64 a lane's operand takes is chosen so that its results are 32
+// (up: 16) consecutive columns; 16-byte chunks of an LDS row are XOR-ed with the
+// row bits that differ among 16 lanes, so operand reads are free of bank
+// conflicts.
 // ---------------------------------------------------------------------------
 constexpr int kTileThreads = 512;
 constexpr int kTileLds = 163840;
@@ -355,7 +355,6 @@ constexpr int kTileRows = 256;  // rows per entry of the tile list
 constexpr int kTileBM = 128;    // rows per workgroup
 constexpr int kTileParts = kTileRows / kTileBM;
 constexpr int kTileCols = 256;  // weight rows per workgroup (up: 128 of W1 and of W3)
-constexpr int kStageK = 64;
 
 struct Fp8Tiles {
   const int32_t *tiles, *offsets, *row_token;  // grouped rows (tm_group_slots); all null: dense
@@ -368,27 +367,21 @@ struct Fp8Tiles {
 __device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 // Stage layout for NB blocks of 32 rows per half.
-template <int MODE, bool WIDE, int NB>
+template <int NB>
 struct TileCfg {
-  static constexpr bool kScaled = !WIDE || MODE == kOut;  // rows come with scales
-  static constexpr int kXRow = WIDE ? 2 * kStageK : kStageK;
-  static constexpr int kW = kTileCols * kStageK;
-  static constexpr int kX = 64 * NB * kXRow;
-  static constexpr int kS = kScaled ? 64 * NB * 4 : 0;
+  static constexpr int kW = kTileCols * kFp8Block;
+  static constexpr int kX = 64 * NB * kFp8Block;
+  static constexpr int kS = 64 * NB * 4;
   static constexpr int kStage = kW + kX + kS;
-  static constexpr int kXLoads = kX / 1024;                        // 1 KiB pieces of a stage's rows
-  static constexpr int kXDma = kXLoads > 8 ? kXLoads / 8 : 1;      // ... per wave
-  static constexpr int kDma = 2 + kXDma + (kScaled ? 1 : 0);
-  static constexpr int kFit = kTileLds / kStage;
-  static constexpr int kSlots = kFit < 8 ? kFit : 8;
+  static constexpr int kDma = 4 + NB + 1;  // loads per wave
+  static constexpr int kSlots = kTileLds / kStage;
 };
 
 template <int MODE>
 __device__ __forceinline__ int w_swz(int row) {
-  return ((row >> (MODE == kUp ? 4 : 5)) & 1) | (((row >> 2) & 1) << 1);
+  return ((row >> 1) & 1) | (((row >> (MODE == kUp ? 4 : 5)) & 1) << 1) | (((row >> 2) & 1) << 2);
 }
-template <bool WIDE>
-__device__ __forceinline__ int x_swz(int row) { return WIDE ? (row >> 1) & 7 : (row >> 2) & 3; }
+__device__ __forceinline__ int x_swz(int row) { return (row >> 1) & 7; }
 
 // Wait until at most `left` stages of kDma loads are outstanding (and LDS reads
 // are done).
@@ -451,32 +444,32 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
   const char *const lds = reinterpret_cast<const char *>(ring);
   const int64_t ld_w = (int64_t)KT * kFp8Block;
   const int n_blk = (n_out + kFp8Block - 1) / kFp8Block;
-  const int steps = 2 * KT;
 
-  // weight loads: 1 KiB pieces 2 wave + j, 16 rows each (up: waves 0-3 W1, waves 4-7 W3)
+  // weight loads: 1 KiB pieces 4 wave + j, 8 rows each (up: waves 0-3 W1, waves 4-7 W3)
   const Fp8Mat &mine = MODE == kUp && wave >= 4 ? m1 : m0;
   constexpr int kWRows = MODE == kUp ? kTileCols / 2 : kTileCols;
   const int w_rows = n_out - n0 < kWRows ? n_out - n0 : kWRows;
   const tm_rsrc_t w_rs = tm_make_rsrc(mine.w + ((int64_t)e * n_out + n0) * ld_w, (uint64_t)w_rows * ld_w);
-  uint32_t w_off[2];
+  uint32_t w_off[4];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    int row = ((MODE == kUp ? wave & 3 : wave) * 2 + j) * 16 + (lane >> 2);
-    const int chunk = (lane & 3) ^ w_swz<MODE>(row);
+  for (int j = 0; j < 4; ++j) {
+    int row = ((MODE == kUp ? wave & 3 : wave) * 4 + j) * 8 + (lane >> 3);
+    const int chunk = (lane & 7) ^ w_swz<MODE>(row);
     row = row < w_rows ? row : w_rows - 1;  // (results of rows past n_out are dropped)
     w_off[j] = (uint32_t)row * (uint32_t)ld_w + (uint32_t)chunk * 16u;
   }
   // operand row t of block a: weight row
   //   out: 64 cg + 32 (t / 4 % 2) + 16 a + 4 (t / 8) + t % 4
   //   up:  32 cg + 16 (t / 4 % 2) + 4 (t / 8) + t % 4 of matrix a
-  uint32_t a_off[2];  // chunks h and 2 + h (of block 0)
+  // its chunk 2 c + h (c = 0 .. 3), of both operands: the same columns
+  uint32_t a_off[4];  // (of block 0)
   {
     const int row = MODE == kUp ? 32 * cg + 16 * ((t >> 2) & 1) + 4 * (t >> 3) + (t & 3)
                                 : 64 * cg + 32 * ((t >> 2) & 1) + 4 * (t >> 3) + (t & 3);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) a_off[c] = (uint32_t)(row * kStageK + ((2 * c + h) ^ w_swz<MODE>(row)) * 16);
+    for (int c = 0; c < 4; ++c) a_off[c] = (uint32_t)(row * kFp8Block + ((2 * c + h) ^ w_swz<MODE>(row)) * 16);
   }
-  constexpr uint32_t kABlock = (MODE == kUp ? 128 : 16) * kStageK;  // block 1 (its swizzle is block 0's)
+  constexpr uint32_t kABlock = (MODE == kUp ? 128 : 16) * kFp8Block;  // block 1 (its swizzle is block 0's)
   // the wave's scales of 64 blocks, one per lane
   const int blk = (MODE == kUp ? n0 : n0 + cg * 64) / kFp8Block;
   const int64_t s_at = ((int64_t)e * n_blk + (blk < n_blk ? blk : n_blk - 1)) * KT;
@@ -496,58 +489,49 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
 
   auto run = [&](auto nb_c) {
     constexpr int NB = decltype(nb_c)::value;
-    using Cfg = TileCfg<MODE, WIDE, NB>;
+    using Cfg = TileCfg<NB>;
     constexpr int S = Cfg::kSlots;
-    constexpr int kChunks = Cfg::kXRow / 16, kRowsPer = 64 / kChunks;
-    const uint8_t *x_src[Cfg::kXDma];
-    uint32_t x_dst[Cfg::kXDma];
     auto row_of = [&](int tr) {  // a row past the tile: its last one again, results dropped
       int gr = r0 + tr;
       gr = gr < r_end ? gr : r_end - 1;
       return MODE == kUp && ts.row_token != nullptr ? (int64_t)ts.row_token[gr] : (int64_t)gr;
     };
+    const uint8_t *x_src[NB];
 #pragma unroll
-    for (int j = 0; j < Cfg::kXDma; ++j) {
-      const int piece = (wave * Cfg::kXDma + j) % Cfg::kXLoads;  // (spare waves repeat a piece)
-      const int tr = piece * kRowsPer + lane / kChunks;
-      x_dst[j] = (uint32_t)(Cfg::kW + piece * 1024);
-      x_src[j] = x + row_of(tr) * ld_x + ((lane % kChunks) ^ x_swz<WIDE>(tr)) * 16;
+    for (int j = 0; j < NB; ++j) {
+      const int tr = (wave * NB + j) * 8 + (lane >> 3);
+      x_src[j] = x + row_of(tr) * ld_x + ((lane & 7) ^ x_swz(tr)) * 16;
     }
-    const float *s_src = nullptr;
-    uint32_t s_dst = 0;
-    if constexpr (Cfg::kScaled) {
-      const int piece = wave % NB;
-      s_src = xs + row_of(piece * 64 + lane) * ld_xs;
-      s_dst = (uint32_t)(Cfg::kW + Cfg::kX + piece * 256);
-    }
-    auto issue = [&](int st, uint32_t slot) {
+    const float *const s_src = xs + row_of((wave % NB) * 64 + lane) * ld_xs;
+    const uint32_t s_dst = (uint32_t)(Cfg::kW + Cfg::kX + (wave % NB) * 256);
+    auto issue = [&](int kt, uint32_t slot) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        tm_dma16_buf_so(w_rs, w_off[j], (uint32_t)st * kStageK, lds0 + slot + (uint32_t)(wave * 2 + j) * 1024u);
+      for (int j = 0; j < 4; ++j)
+        tm_dma16_buf_so(w_rs, w_off[j], (uint32_t)kt * kFp8Block, lds0 + slot + (uint32_t)(wave * 4 + j) * 1024u);
 #pragma unroll
-      for (int j = 0; j < Cfg::kXDma; ++j) tm_dma16_s(x_src[j] + (int64_t)st * Cfg::kXRow, lds0 + slot + x_dst[j]);
-      if constexpr (Cfg::kScaled) tm_dma4_s(s_src + (st >> 1), lds0 + slot + s_dst);
+      for (int j = 0; j < NB; ++j)
+        tm_dma16_s(x_src[j] + (int64_t)kt * kFp8Block, lds0 + slot + (uint32_t)(Cfg::kW + (wave * NB + j) * 1024));
+      tm_dma4_s(s_src + kt, lds0 + slot + s_dst);
     };
     const int tr0 = half * NB * 32 + t;
-    uint32_t b_off[WIDE ? 4 : 2];
+    uint32_t b_off[4];
 #pragma unroll
-    for (int j = 0; j < (WIDE ? 4 : 2); ++j) {
-      const int c = WIDE ? 4 * (j >> 1) + 2 * h + (j & 1) : 2 * j + h;  // k = 32 (j / 2) + 16 h + 8 (j % 2)
-      b_off[j] = (uint32_t)(Cfg::kW + tr0 * Cfg::kXRow + (c ^ x_swz<WIDE>(tr0)) * 16);
-    }
-    tm_f32x16 p[2][NB];
-    auto step = [&](auto odd_c, int st, uint32_t slot, uint32_t free_slot) {
-      constexpr bool kOdd = decltype(odd_c)::value;
-      const int left = steps - 1 - st;
+    for (int c = 0; c < 4; ++c) b_off[c] = (uint32_t)(Cfg::kW + tr0 * kFp8Block + ((2 * c + h) ^ x_swz(tr0)) * 16);
+    for (int kt = 0; kt < S && kt < KT; ++kt) issue(kt, (uint32_t)(kt * Cfg::kStage));
+    uint32_t slot = 0, prev = (S - 1) * Cfg::kStage;
+    for (int kt = 0; kt < KT; ++kt) {
+      const int left = KT - 1 - kt;
       wait_stages<Cfg::kDma, S - 2>(left < S - 2 ? left : S - 2);
-      barrier();  // stage st landed, in every wave; every wave has read stage st - 1
-      if (st - 1 + S < steps && st > 0) issue(st - 1 + S, free_slot);
+      barrier();  // stage kt landed, in every wave; every wave has read stage kt - 1
+      if (kt > 0 && kt - 1 + S < KT) issue(kt - 1 + S, prev);
       const char *const sp = lds + slot;
-      uint4 af[2][WIDE ? 4 : 2];
+      const float sw0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(swv[0]), kt & 63));
+      const float sw1 = MODE == kUp ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(swv[1]), kt & 63)) : sw0;
+      uint4 af[2][WIDE ? 8 : 4];
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int a = 0; a < 2; ++a) {
           const uint4 r = *reinterpret_cast<const uint4 *>(sp + a_off[c] + a * kABlock);
           if constexpr (WIDE) {
             af[a][2 * c] = tm_fp8_to_bf16x8(r.x, r.y);
@@ -558,51 +542,41 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
         }
 #pragma unroll
       for (int q = 0; q < NB; ++q) {
-        uint4 bf[WIDE ? 4 : 2];
-#pragma unroll
-        for (int j = 0; j < (WIDE ? 4 : 2); ++j)
-          bf[j] = *reinterpret_cast<const uint4 *>(sp + b_off[j] + q * 32 * Cfg::kXRow);
+        const float sx = *reinterpret_cast<const float *>(sp + Cfg::kW + Cfg::kX + (tr0 + 32 * q) * 4);
+        tm_f32x16 p[2] = {};
         if constexpr (WIDE) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int c = 0; c < 4; ++c) {
+            const uint4 r = *reinterpret_cast<const uint4 *>(sp + b_off[c] + q * 32 * kFp8Block);
+            const float s = MODE == kUp ? sx : 1.f;
+            const uint4 b[2] = {tm_fp8_to_bf16x8(r.x, r.y, s), tm_fp8_to_bf16x8(r.z, r.w, s)};
 #pragma unroll
-            for (int a = 0; a < 2; ++a)
-              p[a][q] = tm_mfma32x32x16<TM_DT_BF16>(af[a][j], bf[j], !kOdd && j == 0 ? tm_f32x16{} : p[a][q]);
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int a = 0; a < 2; ++a) p[a] = tm_mfma32x32x16<TM_DT_BF16>(af[a][2 * c + u], b[u], p[a]);
+          }
         } else {
 #pragma unroll
-          for (int a = 0; a < 2; ++a) p[a][q] = tm_mfma32x32x64_fp8(af[a], bf, !kOdd ? tm_f32x16{} : p[a][q]);
-        }
-      }
-      if constexpr (kOdd) {
-        const int kb = st >> 1;
-        const float sw0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(swv[0]), kb & 63));
-        const float sw1 = MODE == kUp ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(swv[1]), kb & 63)) : sw0;
+          for (int c = 0; c < 4; c += 2) {
+            const uint4 b[2] = {*reinterpret_cast<const uint4 *>(sp + b_off[c] + q * 32 * kFp8Block),
+                                *reinterpret_cast<const uint4 *>(sp + b_off[c + 1] + q * 32 * kFp8Block)};
 #pragma unroll
-        for (int q = 0; q < NB; ++q) {
-          float sx = 1.f;
-          if constexpr (Cfg::kScaled)
-            sx = *reinterpret_cast<const float *>(sp + Cfg::kW + Cfg::kX + (tr0 + 32 * q) * 4);
-#pragma unroll
-          for (int a = 0; a < 2; ++a) {
-            const float s = (a == 1 ? sw1 : sw0) * sx;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[a][q][i] = fmaf(p[a][q][i], s, acc[a][q][i]);
+            for (int a = 0; a < 2; ++a) {
+              const uint4 w2[2] = {af[a][c], af[a][c + 1]};
+              p[a] = tm_mfma32x32x64_fp8(w2, b, p[a]);
+            }
           }
         }
-        if (((kb + 1) & 63) == 0 && kb + 1 < KT) load_sw(kb + 1);
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const float s = MODE == kUp ? (a == 1 ? sw1 : sw0) : sw0 * sx;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[a][q][i] = fmaf(p[a][i], s, acc[a][q][i]);
+        }
       }
-    };
-    for (int st = 0; st < S && st < steps; ++st) issue(st, (uint32_t)(st * Cfg::kStage));
-    uint32_t slot = 0, prev = (S - 1) * Cfg::kStage;
-    auto next = [&] {
+      if (((kt + 1) & 63) == 0 && kt + 1 < KT) load_sw(kt + 1);
       prev = slot;
       slot = slot == (S - 1) * Cfg::kStage ? 0u : slot + Cfg::kStage;
-    };
-    for (int kt = 0; kt < KT; ++kt) {
-      step(std::false_type{}, 2 * kt, slot, prev);
-      next();
-      step(std::true_type{}, 2 * kt + 1, slot, prev);
-      next();
     }
   };
   const int used = rows > 64 ? 2 : 1;  // row blocks per half
@@ -646,22 +620,51 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
       if (h == 0 && cg == 0) fs[(int64_t)(r0 + tr) * n_blk + n0 / kFp8Block] = s;
     }
   } else {
-    const int c = n0 + cg * 64 + 32 * h;
+    // Through LDS, so that a row's columns are added to and written as whole
+    // lines: every lane storing its own row's columns, 8 bytes at a time, took
+    // 34 us of a 4096 x 2048 product's 87.
+    tm_wait_vm_lgkm0_mem<0>();
+    barrier();  // the ring is free
+    float *const tile = reinterpret_cast<float *>(ring);  // [128 rows][kTileCols + 4]
+    constexpr int kLd = kTileCols + 4;
+    static_assert(kTileBM * kLd * 4 <= kTileLds, "output tile");
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int tr = first + 32 * q;
-      if (q >= used || tr >= rows || c >= n_out) continue;
+      if (q >= used) continue;  // uniform
+      float *const p = tile + (first + 32 * q) * kLd + cg * 64 + 32 * h;
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        *reinterpret_cast<float4 *>(p + 4 * u) =
+            make_float4(acc[u >> 2][q][4 * (u & 3)], acc[u >> 2][q][4 * (u & 3) + 1], acc[u >> 2][q][4 * (u & 3) + 2],
+                        acc[u >> 2][q][4 * (u & 3) + 3]);
+    }
+    __syncthreads();
+    // 32 lanes a row, 8 columns each
+    const int c = (lane & 31) * 8, col = n0 + c;
+    for (int tr = wave * 2 + (lane >> 5); tr < rows; tr += 16) {
+      if (col >= n_out) break;
       const int64_t row = r0 + tr;
-      const int64_t at = ts.row_out != nullptr ? ts.row_out[row] : row * dst.ld;
+      const int64_t at = (ts.row_out != nullptr ? ts.row_out[row] : row * dst.ld) + col;
+      float v[8];
+      const float4 lo = *reinterpret_cast<const float4 *>(tile + tr * kLd + c);
+      const float4 hi = *reinterpret_cast<const float4 *>(tile + tr * kLd + c + 4);
+      v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
+      v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+      using T = typename Elem<DT>::T;
+      T *const y = static_cast<T *>(dst.y) + at;
+      const T *const add = static_cast<const T *>(dst.add) + row * dst.ld_add + col;
+      if (vec_out && col + 8 <= n_out) {
+        if (dst.add != nullptr) {
+          float b[8];
+          tm_load8<DT>(add, b);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        float v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = acc[u >> 2][q][4 * (u & 3) + i];
-          if (dst.add != nullptr && c + 4 * u + i < n_out) v[i] += at_f<DT>(dst.add, row * dst.ld_add + c + 4 * u + i);
+          for (int i = 0; i < 8; ++i) v[i] += b[i];
         }
-        store4<DT>(dst.y, at, v, c + 4 * u, n_out, vec_out);
+        tm_store8<DT>(y, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (col + i < n_out) y[i] = Elem<DT>::from_f(v[i] + (dst.add != nullptr ? Elem<DT>::to_f(add[i]) : 0.f));
       }
     }
   }
@@ -675,8 +678,8 @@ int tile_launch(const char *name, const void *x, int64_t ld_x, const float *xs, 
   const int64_t grid = tiles * n_tiles * kTileParts;
   TM_REQUIRE(grid < ((int64_t)1 << 31), TM_EINVAL_SHAPE, "%s: too many rows", name);
   const int64_t esz = Elem<DT>::kBytes;
-  const bool vec_out = (reinterpret_cast<uintptr_t>(dst.y) & 15) == 0 && dst.ld * esz % 16 == 0 &&
-                       dst.so_b * esz % 16 == 0 && dst.so_s * esz % 16 == 0;
+  const bool vec_out = tm_aligned16(dst.y) && dst.ld * esz % 16 == 0 && dst.so_b * esz % 16 == 0 &&
+                       dst.so_s * esz % 16 == 0 && tm_aligned16(dst.add) && dst.ld_add * esz % 16 == 0;
   hipLaunchKernelGGL((tile_kernel<DT, MODE, WIDE>), dim3((unsigned)grid), dim3(kTileThreads), 0, s,
                      static_cast<const uint8_t *>(x), ld_x, xs, ld_xs, m0, m1, n_out, KT, n_tiles, ts, dst, fs, vec_out);
   TM_LAUNCH_CHECK(name);
@@ -702,8 +705,7 @@ constexpr int64_t kLinearStreamRows = 32;
 extern "C" size_t tm_fp8_linear_workspace_size(int64_t n_rows, int64_t k, int32_t dtype) {
   if (n_rows <= 0 || k <= 0) return 0;
   const int64_t kb = tm_cdiv(k, kFp8Block);
-  return (size_t)(round_up(n_rows * kb * kFp8Block * (dtype == TM_DT_F32 ? 2 : 1), 256) +
-                  round_up(n_rows * kb * 4, 256));
+  return (size_t)(round_up(n_rows * kb * kFp8Block, 256) + round_up(n_rows * kb * 4, 256));
 }
 
 extern "C" int tm_fp8_linear(int32_t dtype, const void *x, const float *x_scale, int64_t n_rows, int64_t k, int64_t ld_x,
@@ -727,17 +729,11 @@ extern "C" int tm_fp8_linear(int32_t dtype, const void *x, const float *x_scale,
   TM_REQUIRE(workspace != nullptr && workspace_bytes >= need && tm_aligned16(workspace), TM_EWORKSPACE,
              "%s: workspace %zu bytes < %zu", name, workspace_bytes, need);
   hipStream_t s = tm_hip_stream(stream);
-  const bool tiles = n_rows > kLinearStreamRows, wide = tiles && dtype == TM_DT_F32;
+  const bool tiles = n_rows > kLinearStreamRows;
   Fp8Src src{x, ld_x, k, x_scale, ld_xs};
   float *const ws_scale = reinterpret_cast<float *>(static_cast<char *>(workspace) + need - round_up(n_rows * kb * 4, 256));
-  if (x_scale && wide) {
-    const int st = tm_internal_fp8_widen(x, n_rows, kp, ld_x, workspace, kp, s);
-    if (st != TM_OK) return st;
-    src.x = workspace;
-    src.ld = kp;
-  } else if (!x_scale && (tiles || !aligned(x, ld_x * (dtype == TM_DT_F32 ? 4 : 2)))) {
-    const int st = tm_internal_fp8_rows(dtype, x, n_rows, k, ld_x, workspace, kp, ws_scale, kb,
-                                        wide ? kFp8Rows16 : kFp8Rows8, s);
+  if (!x_scale && (tiles || !aligned(x, ld_x * (dtype == TM_DT_F32 ? 4 : 2)))) {
+    const int st = tm_internal_fp8_rows(dtype, x, n_rows, k, ld_x, workspace, kp, ws_scale, kb, s);
     if (st != TM_OK) return st;
     src = Fp8Src{workspace, kp, kp, ws_scale, kb};
   }
@@ -752,9 +748,8 @@ extern "C" int tm_fp8_linear(int32_t dtype, const void *x, const float *x_scale,
   Fp8Tiles ts{};
   ts.rows = (int32_t)n_rows;
   return TM_DISPATCH_DTYPE(dtype, DT, [&] {
-    constexpr bool kWide = DT == TM_DT_F32;
-    return tile_launch<DT, kOut, kWide>(name, src.x, src.ld * (kWide ? 2 : 1), src.scale, src.ld_s, m, m, (int)n_out,
-                                           (int)kb, ts, dst, nullptr, s);
+    return tile_launch<DT, kOut, DT == TM_DT_F32>(name, src.x, src.ld, src.scale, src.ld_s, m, m, (int)n_out, (int)kb,
+                                                  ts, dst, nullptr, s);
   });
 }
 
@@ -786,7 +781,7 @@ bool stream_plan(int64_t rows, int32_t n_experts) {
 // Workspace: f (stream: fp32 rows; tiles: 8-bit rows and their scales), the
 // quantised activations and the row lists of the tiles.
 struct ExpertsWs {
-  size_t f, fs, x, offsets, row_token, row_out, tiles, group, total;
+  size_t f, fs, x, xs, offsets, row_token, row_out, tiles, group, total;
 };
 
 ExpertsWs experts_ws(int64_t n, int32_t top_k, const tm_fp8_experts *ex, bool grouped) {
@@ -804,7 +799,8 @@ ExpertsWs experts_ws(int64_t n, int32_t top_k, const tm_fp8_experts *ex, bool gr
   at = 0;
   w.f = take(rows * ex->inter);
   w.fs = take(rows * (ex->inter / kFp8Block) * 4);
-  w.x = take(n * ex->hidden * 2);
+  w.x = take(n * ex->hidden);
+  w.xs = take(n * (ex->hidden / kFp8Block) * 4);
   if (grouped) {
     w.offsets = take(4 * ((int64_t)ex->n_experts + 1));
     w.row_token = take(4 * rows);
@@ -839,10 +835,11 @@ int mlp_launch(const char *name, const tm_fp8_experts *ex, const void *x, int64_
     return stream_launch<DT, TM_DT_F32, kOut, 4, 2>(name, Fp8Src{base + ws.f, inter, inter, nullptr, 0}, *rows, w2, w2, h,
                                               inter / kFp8Block, dst, s);
   }
-  int st = tm_internal_fp8_rows(DT, x, n, h, ld_x, base + ws.x, h, nullptr, 0, kFp8RowsScaled, s);
+  float *const xs = reinterpret_cast<float *>(base + ws.xs);
+  int st = tm_internal_fp8_rows(DT, x, n, h, ld_x, base + ws.x, h, xs, h / kFp8Block, s);
   if (st != TM_OK) return st;
   float *const fs = reinterpret_cast<float *>(base + ws.fs);
-  st = tile_launch<DT, kUp, true>(name, base + ws.x, (int64_t)h * 2, nullptr, 0, w1, w3, inter, h / kFp8Block, *ts,
+  st = tile_launch<DT, kUp, true>(name, base + ws.x, h, xs, h / kFp8Block, w1, w3, inter, h / kFp8Block, *ts,
                                      mid, fs, s);
   if (st != TM_OK) return st;
   return tile_launch<DT, kOut, false>(name, base + ws.f, inter, fs, inter / kFp8Block, w2, w2, h, inter / kFp8Block,

@@ -22,12 +22,10 @@ __device__ __forceinline__ void load8(const typename Elem<DT>::T *row, int64_t c
   }
 }
 
-// OUT: e4m3 values; or, for products on the 16-bit matrix cores, the same
-// values as bf16, or times their scale (no scales are written then).
-template <int DT, bool VEC, int OUT>
+template <int DT, bool VEC>
 __global__ __launch_bounds__(kQThreads) void quantize_rows_kernel(const typename Elem<DT>::T *__restrict__ x, int64_t n,
                                                                  int64_t k, int64_t ld_x, int blocks,
-                                                                 void *__restrict__ q, int64_t ld_q,
+                                                                 uint8_t *__restrict__ q, int64_t ld_q,
                                                                  float *__restrict__ scale, int64_t ld_s) {
   const int64_t item = ((int64_t)blockIdx.x * kQThreads + threadIdx.x) >> 4;  // (row, block)
   const int64_t row = item / blocks;
@@ -46,26 +44,8 @@ __global__ __launch_bounds__(kQThreads) void quantize_rows_kernel(const typename
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = tm_fp8_quot(v[i], inv);
   const uint32_t lo = tm_fp8_pack4(v[0], v[1], v[2], v[3]), hi = tm_fp8_pack4(v[4], v[5], v[6], v[7]);
-  if constexpr (OUT == kFp8Rows8) {
-    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(q) + row * ld_q + c) = make_uint2(lo, hi);
-  } else if constexpr (OUT == kFp8Rows16) {
-    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(q) + row * ld_q + c) = tm_fp8_to_bf16x8(lo, hi);
-  } else {
-    const uint2 a = tm_fp8_scaled_bf16x4(lo, s), d = tm_fp8_scaled_bf16x4(hi, s);
-    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(q) + row * ld_q + c) = make_uint4(a.x, a.y, d.x, d.y);
-  }
-  if (OUT != kFp8RowsScaled && sub == 0) scale[row * ld_s + b] = s;
-}
-
-// e4m3 rows of 8 * pieces columns as bf16.
-__global__ __launch_bounds__(kQThreads) void widen_kernel(const uint8_t *__restrict__ q, int64_t n, int pieces,
-                                                         int64_t ld_q, uint16_t *__restrict__ out, int64_t ld_o) {
-  const int64_t item = (int64_t)blockIdx.x * kQThreads + threadIdx.x;
-  const int64_t row = item / pieces;
-  if (row >= n) return;
-  const int c = (int)(item - row * pieces) * 8;
-  const uint2 v = *reinterpret_cast<const uint2 *>(q + row * ld_q + c);
-  *reinterpret_cast<uint4 *>(out + row * ld_o + c) = tm_fp8_to_bf16x8(v.x, v.y);
+  *reinterpret_cast<uint2 *>(q + row * ld_q + c) = make_uint2(lo, hi);
+  if (sub == 0) scale[row * ld_s + b] = s;
 }
 
 // One workgroup per 128 x 128 block: thread t holds rows t / 16 + 16 j, 8
@@ -116,43 +96,25 @@ bool rows_vec(const void *x, int64_t ld_x) {
   return tm_aligned16(x) && ld_x * Elem<DT>::kBytes % 16 == 0;
 }
 
-template <int OUT>
-int rows_launch(int32_t dtype, const void *x, int64_t n, int64_t k, int64_t ld_x, void *q, int64_t ld_q, float *scale,
-                int64_t ld_s, hipStream_t s) {
+}  // namespace
+
+int tm_internal_fp8_rows(int32_t dtype, const void *x, int64_t n, int64_t k, int64_t ld_x, void *q, int64_t ld_q,
+                         float *scale, int64_t ld_s, hipStream_t s) {
   const int64_t blocks = tm_cdiv(k, kFp8Block);
   const int64_t grid = tm_cdiv(n * blocks, kQThreads / 16);
   TM_REQUIRE(grid < ((int64_t)1 << 31), TM_EINVAL_SHAPE, "tm_fp8_quantize_rows: too many rows");
   return TM_DISPATCH_DTYPE(dtype, DT, [&] {
-    using T = typename Elem<DT>::T;
+    const auto *const p = static_cast<const typename Elem<DT>::T *>(x);
+    auto *const out = static_cast<uint8_t *>(q);
     if (rows_vec<DT>(x, ld_x))
-      hipLaunchKernelGGL((quantize_rows_kernel<DT, true, OUT>), dim3((unsigned)grid), dim3(kQThreads), 0, s,
-                         static_cast<const T *>(x), n, k, ld_x, (int)blocks, q, ld_q, scale, ld_s);
+      hipLaunchKernelGGL((quantize_rows_kernel<DT, true>), dim3((unsigned)grid), dim3(kQThreads), 0, s, p, n, k, ld_x,
+                         (int)blocks, out, ld_q, scale, ld_s);
     else
-      hipLaunchKernelGGL((quantize_rows_kernel<DT, false, OUT>), dim3((unsigned)grid), dim3(kQThreads), 0, s,
-                         static_cast<const T *>(x), n, k, ld_x, (int)blocks, q, ld_q, scale, ld_s);
+      hipLaunchKernelGGL((quantize_rows_kernel<DT, false>), dim3((unsigned)grid), dim3(kQThreads), 0, s, p, n, k, ld_x,
+                         (int)blocks, out, ld_q, scale, ld_s);
     TM_LAUNCH_CHECK("tm_fp8_quantize_rows");
     return TM_OK;
   });
-}
-
-}  // namespace
-
-int tm_internal_fp8_rows(int32_t dtype, const void *x, int64_t n, int64_t k, int64_t ld_x, void *q, int64_t ld_q,
-                         float *scale, int64_t ld_s, int out, hipStream_t s) {
-  switch (out) {
-    case kFp8Rows8: return rows_launch<kFp8Rows8>(dtype, x, n, k, ld_x, q, ld_q, scale, ld_s, s);
-    case kFp8Rows16: return rows_launch<kFp8Rows16>(dtype, x, n, k, ld_x, q, ld_q, scale, ld_s, s);
-    default: return rows_launch<kFp8RowsScaled>(dtype, x, n, k, ld_x, q, ld_q, scale, ld_s, s);
-  }
-}
-
-int tm_internal_fp8_widen(const void *q, int64_t n, int64_t k, int64_t ld_q, void *out, int64_t ld_o, hipStream_t s) {
-  const int64_t grid = tm_cdiv(n * (k / 8), kQThreads);
-  TM_REQUIRE(grid < ((int64_t)1 << 31), TM_EINVAL_SHAPE, "tm_fp8_linear: too many rows");
-  hipLaunchKernelGGL(widen_kernel, dim3((unsigned)grid), dim3(kQThreads), 0, s, static_cast<const uint8_t *>(q), n,
-                     (int)(k / 8), ld_q, static_cast<uint16_t *>(out), ld_o);
-  TM_LAUNCH_CHECK("tm_fp8_linear");
-  return TM_OK;
 }
 
 extern "C" int tm_fp8_quantize_rows(int32_t dtype, const void *x, int64_t n_rows, int64_t k, int64_t ld_x, void *q,
@@ -169,8 +131,7 @@ extern "C" int tm_fp8_quantize_rows(int32_t dtype, const void *x, int64_t n_rows
   if (n_rows == 0) return TM_OK;
   TM_REQUIRE(x && q && scale, TM_EINVAL_ARG, "tm_fp8_quantize_rows: null pointer");
   TM_REQUIRE(tm_aligned16(q), TM_EINVAL_SHAPE, "tm_fp8_quantize_rows: q must be 16-byte aligned");
-  return tm_internal_fp8_rows(dtype, x, n_rows, k, ld_x, q, ld_q, scale, ld_scale, kFp8Rows8,
-                              tm_hip_stream(stream));
+  return tm_internal_fp8_rows(dtype, x, n_rows, k, ld_x, q, ld_q, scale, ld_scale, tm_hip_stream(stream));
 }
 
 extern "C" int tm_fp8_quantize_weight(int32_t dtype, const void *w, int64_t n_mats, int64_t n_rows, int64_t k, void *q,
