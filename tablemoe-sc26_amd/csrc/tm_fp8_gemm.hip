@@ -350,17 +350,17 @@ int stream_launch(const char *name, const Fp8Src &src, Fp8Rows rows, const Fp8Ma
 // conflicts.
 // ---------------------------------------------------------------------------
 constexpr int kTileThreads = 512;
-constexpr int kTileLds = 163840;
-constexpr int kTileRows = 256;  // rows per entry of the tile list
-constexpr int kTileBM = 128;    // rows per workgroup
-constexpr int kTileParts = kTileRows / kTileBM;
-constexpr int kTileCols = 256;  // weight rows per workgroup (up: 128 of W1 and of W3)
+constexpr int kTileBM = 128;    // rows of a tile
+constexpr int kTileCols = 256;  // weight rows of a tile (up: 128 of W1 and of W3)
+constexpr int kTileRing = 3 * (kTileCols * kFp8Block + kTileBM * (kFp8Block + 4));  // LDS bytes of the stages
+constexpr int kMaxExperts = 1024;
 
+// Rows of a tiled call: grouped by expert (what tm_group_slots writes), or
+// (offsets null) all of one matrix.
 struct Fp8Tiles {
-  const int32_t *tiles, *offsets, *row_token;  // grouped rows (tm_group_slots); all null: dense
+  const int32_t *offsets, *row_token;
   const int64_t *row_out;
-  int64_t t_max;
-  int32_t rows;
+  int32_t n_experts, rows;  // rows: dense, their number; grouped, the most
 };
 
 // A workgroup barrier that LDS accesses stay on their side of.
@@ -374,7 +374,7 @@ struct TileCfg {
   static constexpr int kS = 64 * NB * 4;
   static constexpr int kStage = kW + kX + kS;
   static constexpr int kDma = 4 + NB + 1;  // loads per wave
-  static constexpr int kSlots = kTileLds / kStage;
+  static constexpr int kSlots = kTileRing / kStage;
 };
 
 template <int MODE>
@@ -400,43 +400,10 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
                                                                const float *__restrict__ xs, int64_t ld_xs, Fp8Mat m0,
                                                                Fp8Mat m1, int n_out, int KT, int n_tiles, Fp8Tiles ts,
                                                                Fp8Dst dst, float *__restrict__ fs, bool vec_out) {
-  __shared__ uint4 ring[kTileLds / 16];
-
-  // Work items: (row tile, column tile, part).  Of whole groups of eight row
-  // tiles, tile y runs on XCD y % 8 (the dispatcher's round robin), the parts of
-  // a column tile next to each other: they share its weights in that L2.
-  const int64_t row_tiles = ts.tiles != nullptr ? (ts.tiles[1] < ts.t_max ? ts.tiles[1] : ts.t_max)
-                                                : ((int64_t)ts.rows + kTileRows - 1) / kTileRows;
-  const int per = n_tiles * kTileParts;
-  const int64_t full = row_tiles / 8 * 8;
-  int64_t y;
-  int item;
-  {
-    const int64_t b = blockIdx.x;
-    if (b < full * per) {
-      y = (b >> 3) / per * 8 + (b & 7);
-      item = (int)((b >> 3) % per);
-    } else {
-      y = full + (b - full * per) / per;
-      item = (int)((b - full * per) % per);
-    }
-    if (y >= row_tiles) return;  // uniform
-  }
-  const int part = item % kTileParts;
-  const int n0 = (item / kTileParts) * (MODE == kUp ? kTileCols / 2 : kTileCols);
-  int e = 0, r0, r_end;
-  if (ts.tiles != nullptr) {
-    e = ts.tiles[2 + y];
-    const int t0 = ts.tiles[2 + ts.t_max + y];
-    r0 = t0 + part * kTileBM;
-    r_end = ts.offsets[e + 1];
-    r_end = r_end < t0 + kTileRows ? r_end : t0 + kTileRows;
-  } else {
-    r0 = (int)y * kTileRows + part * kTileBM;
-    r_end = ts.rows;
-  }
-  if (r0 >= r_end) return;  // uniform
-  const int rows = r_end - r0 < kTileBM ? r_end - r0 : kTileBM;
+  __shared__ uint4 ring[kTileRing / 16];
+  __shared__ int s_off[kMaxExperts + 1], s_part[kMaxExperts + 1];  // each expert's first row and first row tile
+  __shared__ uint32_t s_top[MODE == kUp ? kTileBM * 4 : 1];
+  __shared__ int s_wave[kTileThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cg = wave & 3, half = wave >> 2, t = lane & 31, h = lane >> 5;
@@ -444,6 +411,60 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
   const char *const lds = reinterpret_cast<const char *>(ring);
   const int64_t ld_w = (int64_t)KT * kFp8Block;
   const int n_blk = (n_out + kFp8Block - 1) / kFp8Block;
+
+  // Row tiles of 128 rows, counted here: no tile is empty.
+  const bool grouped = ts.offsets != nullptr;
+  int n_parts = (ts.rows + kTileBM - 1) / kTileBM;
+  if (grouped) {
+    int o[3], c[2];
+#pragma unroll
+    for (int u = 0; u < 3; ++u) o[u] = ts.offsets[2 * tid + u < ts.n_experts ? 2 * tid + u : ts.n_experts];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) c[u] = (o[u + 1] - o[u] + kTileBM - 1) / kTileBM;
+    const int upto = (int)tm_wave_incl_scan((uint32_t)(c[0] + c[1]));
+    if (lane == 63) s_wave[wave] = upto;
+    __syncthreads();
+    int before = upto - c[0] - c[1];
+    n_parts = 0;
+#pragma unroll
+    for (int w = 0; w < kTileThreads / 64; ++w) {
+      before += w < wave ? s_wave[w] : 0;
+      n_parts += s_wave[w];
+    }
+    s_off[2 * tid] = o[0];
+    s_off[2 * tid + 1] = o[1];
+    s_part[2 * tid] = before;
+    s_part[2 * tid + 1] = before + c[0];
+    if (tid == kTileThreads - 1) {
+      s_off[kMaxExperts] = o[2];
+      s_part[kMaxExperts] = n_parts;
+    }
+    __syncthreads();
+  }
+  n_parts = __builtin_amdgcn_readfirstlane(n_parts);
+
+  // Work items: (row tile, column tile), row tile by row tile; XCD x (the
+  // dispatcher's round robin) takes the x-th eighth of them, so the column tiles
+  // of a row tile and the row tiles of an expert run at the same time on one L2.
+  // A workgroup takes every (its XCD's workgroups)-th of its eighth: a launch
+  // holds one workgroup per CU, whatever the rows.
+  const int64_t total = (int64_t)n_parts * n_tiles;
+  const int xcd = (int)(blockIdx.x & 7), on_xcd = ((int)gridDim.x - xcd + 7) / 8;
+  const int64_t last = total * (xcd + 1) / 8;
+  for (int64_t item = total * xcd / 8 + (blockIdx.x >> 3); item < last; item += on_xcd) {
+  const int part = (int)(item / n_tiles);
+  const int n0 = (int)(item % n_tiles) * (MODE == kUp ? kTileCols / 2 : kTileCols);
+  int e = 0, r0 = part * kTileBM, r_end = ts.rows;
+  if (grouped) {
+    int n = 0;  // experts whose tiles all come before this one
+    for (int i = 0; i < ts.n_experts; i += 64)
+      n += __popcll(__ballot(i + lane < ts.n_experts && s_part[i + lane + 1] <= part));
+    e = n;
+    r0 = __builtin_amdgcn_readfirstlane(s_off[e] + (part - s_part[e]) * kTileBM);
+    r_end = __builtin_amdgcn_readfirstlane(s_off[e + 1]);
+  }
+  const int rows = r_end - r0 < kTileBM ? r_end - r0 : kTileBM;
+  r_end = r0 + rows;
 
   // weight loads: 1 KiB pieces 4 wave + j, 8 rows each (up: waves 0-3 W1, waves 4-7 W3)
   const Fp8Mat &mine = MODE == kUp && wave >= 4 ? m1 : m0;
@@ -585,10 +606,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
   const int first = half * used * 32 + t;  // this lane's first row in the tile
 
   if constexpr (MODE == kUp) {
-    // lane: row t of each block, columns n0 + 32 cg + 16 h + i
-    tm_wait_vm_lgkm0_mem<0>();
-    barrier();  // the ring is free
-    uint32_t *const top = reinterpret_cast<uint32_t *>(ring);  // [128 rows][4 groups]
+    // lane: row t of each block, columns n0 + 32 cg + 16 h + i; s_top: [128 rows][4 groups]
     const int c = n0 + cg * 32 + 16 * h;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -601,14 +619,14 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
         m = tm_fp8_amax(m, acc[0][q][i]);
       }
       m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-      if (h == 0) top[(first + 32 * q) * 4 + cg] = m;
+      if (h == 0) s_top[(first + 32 * q) * 4 + cg] = m;
     }
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int tr = first + 32 * q;
       if (q >= used || tr >= rows) continue;
-      const uint4 m4 = *reinterpret_cast<const uint4 *>(&top[tr * 4]);
+      const uint4 m4 = *reinterpret_cast<const uint4 *>(&s_top[tr * 4]);
       float inv;
       const float s = tm_fp8_scale(max(max(m4.x, m4.y), max(m4.z, m4.w)), inv);
       float v[16];
@@ -627,7 +645,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
     barrier();  // the ring is free
     float *const tile = reinterpret_cast<float *>(ring);  // [128 rows][kTileCols + 4]
     constexpr int kLd = kTileCols + 4;
-    static_assert(kTileBM * kLd * 4 <= kTileLds, "output tile");
+    static_assert(kTileBM * kLd * 4 <= kTileRing, "output tile");
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       if (q >= used) continue;  // uniform
@@ -668,15 +686,17 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
       }
     }
   }
+  __syncthreads();  // the next item's loads come after this one's reads of LDS
+  }
 }
 
 template <int DT, int MODE, bool WIDE>
 int tile_launch(const char *name, const void *x, int64_t ld_x, const float *xs, int64_t ld_xs, const Fp8Mat &m0,
                 const Fp8Mat &m1, int n_out, int KT, const Fp8Tiles &ts, const Fp8Dst &dst, float *fs, hipStream_t s) {
   const int n_tiles = (int)tm_cdiv(n_out, MODE == kUp ? kTileCols / 2 : kTileCols);
-  const int64_t tiles = ts.tiles != nullptr ? (ts.rows < ts.t_max ? ts.rows : ts.t_max) : tm_cdiv(ts.rows, kTileRows);
-  const int64_t grid = tiles * n_tiles * kTileParts;
-  TM_REQUIRE(grid < ((int64_t)1 << 31), TM_EINVAL_SHAPE, "%s: too many rows", name);
+  // one workgroup per CU, or fewer where there cannot be as many tiles
+  const int64_t parts = tm_cdiv(ts.rows, kTileBM) + (ts.offsets != nullptr ? ts.n_experts : 0);
+  const int64_t grid = parts * n_tiles < 256 ? tm_cdiv(parts * n_tiles, 8) * 8 : 256;
   const int64_t esz = Elem<DT>::kBytes;
   const bool vec_out = tm_aligned16(dst.y) && dst.ld * esz % 16 == 0 && dst.so_b * esz % 16 == 0 &&
                        dst.so_s * esz % 16 == 0 && tm_aligned16(dst.add) && dst.ld_add * esz % 16 == 0;
@@ -889,13 +909,12 @@ extern "C" int tm_fp8_grouped_swiglu(const tm_fp8_experts *experts, int32_t dtyp
     int32_t *const offsets = reinterpret_cast<int32_t *>(base + ws.offsets);
     int32_t *const row_token = reinterpret_cast<int32_t *>(base + ws.row_token);
     int64_t *const row_out = reinterpret_cast<int64_t *>(base + ws.row_out);
-    int32_t *const tiles = reinterpret_cast<int32_t *>(base + ws.tiles);
+    int32_t *const tiles = reinterpret_cast<int32_t *>(base + ws.tiles);  // (not used here)
     const int st = tm_group_slots_ws(ids, n_tokens, top_k, ld_ids, mask, ms_b, ms_s, experts->n_experts, so_b, so_s,
                                      offsets, row_token, row_out, tiles, base + ws.group,
                                      tm_group_slots_workspace_size(n_tokens, top_k, experts->n_experts), stream);
     if (st != TM_OK) return st;
-    ts = Fp8Tiles{tiles, offsets, row_token, row_out, tm_group_slots_tiles(max_rows, experts->n_experts),
-                  (int32_t)max_rows};
+    ts = Fp8Tiles{offsets, row_token, row_out, experts->n_experts, (int32_t)max_rows};
   }
   const Fp8Dst dst{out, 0, so_b, so_s, nullptr, 0};
   return dtype == TM_DT_F16
