@@ -382,6 +382,21 @@ def test_experts_uneven_and_masks(hip_device, n):
     _check_experts(xw[:, 8:8 + h], ids, flags, w)           # strided rows
 
 
+@pytest.mark.parametrize("n", [30, 700])
+def test_experts_scales_far_apart(hip_device, n):
+    """Blocks scaled by 0, by 2^-60 of their neighbours, by a negative number."""
+    e, k, h, inter = 5, 3, 512, 256
+    x = _rand(n, n, h, dtype=torch.bfloat16)
+    w = list(_weights(6, e, h, inter))
+    w[1][0, 0, 1] = 0.0
+    w[3][1, 1, 2] = 2.0 ** -60
+    w[1][2, :, 0] = 2.0 ** -70
+    w[3][3, 0, :] *= -1.0
+    w[5][0, 1, 1], w[5][1, 0, 0] = 0.0, -1e-3
+    ids = torch.stack([torch.randperm(e, generator=torch.Generator().manual_seed(i))[:k] for i in range(n)]).to(hip_device)
+    _check_experts(x, ids, torch.ones(n, dtype=torch.bool, device=hip_device), tuple(w))
+
+
 def test_experts_rows_do_not_depend_on_others(hip_device):
     """Two calls give the same bits, and so does another order of the tokens."""
     n, k, e, h, inter = 90, 4, 6, 256, 256
