@@ -361,6 +361,7 @@ struct Fp8Tiles {
   const int32_t *offsets, *row_token;
   const int64_t *row_out;
   int32_t n_experts, rows;  // rows: dense, their number; grouped, the most
+  int32_t bm;               // rows of a tile: kTileBM or (dense) 64
 };
 
 // A workgroup barrier that LDS accesses stay on their side of.
@@ -395,6 +396,54 @@ __device__ __forceinline__ void wait_stages(int left) {
   }
 }
 
+// A tile of results, [rows][COLS + 4] in LDS, added to and written as whole lines.
+template <int DT, int COLS, int THREADS>
+__device__ __forceinline__ void write_tile(const float *tile, int rows, int r0, int n0, int n_out, const Fp8Dst &dst,
+                                           const int64_t *row_out, bool vec_out) {
+  using T = typename Elem<DT>::T;
+  constexpr int kLd = COLS + 4, kLanes = COLS / 8;
+  T *const y = static_cast<T *>(dst.y);
+  const T *const add = static_cast<const T *>(dst.add);
+  const int tid = threadIdx.x;
+  if (vec_out) {  // 8 columns a lane
+    const int c = (tid % kLanes) * 8, col = n0 + c;
+    if (col >= n_out) return;
+    for (int tr = tid / kLanes; tr < rows; tr += THREADS / kLanes) {
+      const int64_t row = r0 + tr;
+      const float4 lo = *reinterpret_cast<const float4 *>(tile + tr * kLd + c);
+      const float4 hi = *reinterpret_cast<const float4 *>(tile + tr * kLd + c + 4);
+      float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      if (add != nullptr) {
+        float b[8];
+        tm_load8<DT>(add + row * dst.ld_add + col, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += b[i];
+      }
+      tm_store8<DT>(y + (row_out != nullptr ? row_out[row] : row * dst.ld) + col, v);
+    }
+  } else {  // a wave a row, a column a lane: 64 neighbours per store
+    for (int tr = tid >> 6; tr < rows; tr += THREADS / 64) {
+      const int64_t row = r0 + tr;
+      const int64_t at = (row_out != nullptr ? row_out[row] : row * dst.ld) + n0;
+#pragma unroll
+      for (int j = 0; j < COLS / 64; ++j) {
+        const int c = (tid & 63) + 64 * j;
+        if (n0 + c >= n_out) break;
+        const float b = add != nullptr ? Elem<DT>::to_f(add[row * dst.ld_add + n0 + c]) : 0.f;
+        y[at + c] = Elem<DT>::from_f(tile[tr * kLd + c] + b);
+      }
+    }
+  }
+}
+
+// Whether write_tile may move 8 columns at a time.
+template <int DT>
+bool can_write8(const Fp8Dst &dst, int n_out) {
+  const int64_t esz = Elem<DT>::kBytes;
+  return n_out % 8 == 0 && tm_aligned16(dst.y) && dst.ld * esz % 16 == 0 && dst.so_b * esz % 16 == 0 &&
+         dst.so_s * esz % 16 == 0 && tm_aligned16(dst.add) && dst.ld_add * esz % 16 == 0;
+}
+
 template <int DT, int MODE, bool WIDE>
 __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__restrict__ x, int64_t ld_x,
                                                                const float *__restrict__ xs, int64_t ld_xs, Fp8Mat m0,
@@ -412,9 +461,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
   const int64_t ld_w = (int64_t)KT * kFp8Block;
   const int n_blk = (n_out + kFp8Block - 1) / kFp8Block;
 
-  // Row tiles of 128 rows, counted here: no tile is empty.
+  // Row tiles, counted here: no tile is empty.
   const bool grouped = ts.offsets != nullptr;
-  int n_parts = (ts.rows + kTileBM - 1) / kTileBM;
+  int n_parts = (ts.rows + ts.bm - 1) / ts.bm;
   if (grouped) {
     int o[3], c[2];
 #pragma unroll
@@ -454,7 +503,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
   for (int64_t item = total * xcd / 8 + (blockIdx.x >> 3); item < last; item += on_xcd) {
   const int part = (int)(item / n_tiles);
   const int n0 = (int)(item % n_tiles) * (MODE == kUp ? kTileCols / 2 : kTileCols);
-  int e = 0, r0 = part * kTileBM, r_end = ts.rows;
+  int e = 0, r0 = part * ts.bm, r_end = ts.rows;
   if (grouped) {
     int n = 0;  // experts whose tiles all come before this one
     for (int i = 0; i < ts.n_experts; i += 64)
@@ -463,7 +512,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
     r0 = __builtin_amdgcn_readfirstlane(s_off[e] + (part - s_part[e]) * kTileBM);
     r_end = __builtin_amdgcn_readfirstlane(s_off[e + 1]);
   }
-  const int rows = r_end - r0 < kTileBM ? r_end - r0 : kTileBM;
+  const int rows = r_end - r0 < ts.bm ? r_end - r0 : ts.bm;
   r_end = r0 + rows;
 
   // weight loads: 1 KiB pieces 4 wave + j, 8 rows each (up: waves 0-3 W1, waves 4-7 W3)
@@ -665,34 +714,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
                         acc[u >> 2][q][4 * (u & 3) + 3]);
     }
     __syncthreads();
-    // 32 lanes a row, 8 columns each
-    const int c = (lane & 31) * 8, col = n0 + c;
-    for (int tr = wave * 2 + (lane >> 5); tr < rows; tr += 16) {
-      if (col >= n_out) break;
-      const int64_t row = r0 + tr;
-      const int64_t at = (ts.row_out != nullptr ? ts.row_out[row] : row * dst.ld) + col;
-      float v[8];
-      const float4 lo = *reinterpret_cast<const float4 *>(tile + tr * kLd + c);
-      const float4 hi = *reinterpret_cast<const float4 *>(tile + tr * kLd + c + 4);
-      v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
-      v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
-      using T = typename Elem<DT>::T;
-      T *const y = static_cast<T *>(dst.y) + at;
-      const T *const add = static_cast<const T *>(dst.add) + row * dst.ld_add + col;
-      if (vec_out && col + 8 <= n_out) {
-        if (dst.add != nullptr) {
-          float b[8];
-          tm_load8<DT>(add, b);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] += b[i];
-        }
-        tm_store8<DT>(y, v);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (col + i < n_out) y[i] = Elem<DT>::from_f(v[i] + (dst.add != nullptr ? Elem<DT>::to_f(add[i]) : 0.f));
-      }
-    }
+    write_tile<DT, kTileCols, kTileThreads>(tile, rows, r0, n0, n_out, dst, ts.row_out, vec_out);
   }
   __syncthreads();  // the next item's loads come after this one's reads of LDS
   }
@@ -700,16 +722,156 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
 
 template <int DT, int MODE, bool WIDE>
 int tile_launch(const char *name, const void *x, int64_t ld_x, const float *xs, int64_t ld_xs, const Fp8Mat &m0,
-                const Fp8Mat &m1, int n_out, int KT, const Fp8Tiles &ts, const Fp8Dst &dst, float *fs, hipStream_t s) {
+                const Fp8Mat &m1, int n_out, int KT, Fp8Tiles ts, const Fp8Dst &dst, float *fs, hipStream_t s) {
   const int n_tiles = (int)tm_cdiv(n_out, MODE == kUp ? kTileCols / 2 : kTileCols);
+  // Tiles of 64 rows where tiles of 128 would leave half of the CUs without one
+  // (linear, 700 rows, 2048 -> 2816 in bf16: 20 us, 26 in tiles of 128; 1000 rows,
+  // 2560 -> 4096: 26 and 33).
+  ts.bm = ts.offsets == nullptr && tm_cdiv(ts.rows, kTileBM) * n_tiles <= 128 ? 64 : kTileBM;
   // one workgroup per CU, or fewer where there cannot be as many tiles
-  const int64_t parts = tm_cdiv(ts.rows, kTileBM) + (ts.offsets != nullptr ? ts.n_experts : 0);
+  const int64_t parts = tm_cdiv(ts.rows, ts.bm) + (ts.offsets != nullptr ? ts.n_experts : 0);
   const int64_t grid = parts * n_tiles < 256 ? tm_cdiv(parts * n_tiles, 8) * 8 : 256;
-  const int64_t esz = Elem<DT>::kBytes;
-  const bool vec_out = tm_aligned16(dst.y) && dst.ld * esz % 16 == 0 && dst.so_b * esz % 16 == 0 &&
-                       dst.so_s * esz % 16 == 0 && tm_aligned16(dst.add) && dst.ld_add * esz % 16 == 0;
   hipLaunchKernelGGL((tile_kernel<DT, MODE, WIDE>), dim3((unsigned)grid), dim3(kTileThreads), 0, s,
-                     static_cast<const uint8_t *>(x), ld_x, xs, ld_xs, m0, m1, n_out, KT, n_tiles, ts, dst, fs, vec_out);
+                     static_cast<const uint8_t *>(x), ld_x, xs, ld_xs, m0, m1, n_out, KT, n_tiles, ts, dst, fs,
+                     can_write8<DT>(dst, n_out));
+  TM_LAUNCH_CHECK(name);
+  return TM_OK;
+}
+
+// ---------------------------------------------------------------------------
+// A linear layer of some rows: 64 x 64 tiles, so that few rows still give many CUs a
+// workgroup.  Four waves, one 32 x 32 product each; a stage is two blocks of 128
+// columns.  Bound by what a CU's direct loads bring, about 45 bytes/ns at any depth
+// of the ring (nine stages of one block: 0.38 us a block as well): 64 rows,
+// 4096 -> 2048 take 18 us with the rows' quantisation, in the large tiles 27;
+// 333 rows, 1000 -> 1111 in fp32 12 and 20.
+// ---------------------------------------------------------------------------
+constexpr int kMidThreads = 256, kMidTile = 64;
+constexpr int kMidW = kMidTile * kFp8Block, kMidBlock = 2 * kMidW + kMidTile * 4;  // LDS bytes of 128 columns
+constexpr int kMidStage = 2 * kMidBlock, kMidSlots = 4, kMidDma = 2 * 5;  // stages in LDS, loads per wave and stage
+
+template <int DT, bool WIDE>
+__global__ __launch_bounds__(kMidThreads, 1) void mid_kernel(const uint8_t *__restrict__ x, int64_t ld_x,
+                                                             const float *__restrict__ xs, int64_t ld_xs, Fp8Mat mat,
+                                                             int n_rows, int n_out, int KT, int n_parts, int total,
+                                                             Fp8Dst dst, bool vec_out) {
+  __shared__ uint4 ring[kMidSlots * kMidStage / 16];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int cg = wave & 1, half = wave >> 1, t = lane & 31, h = lane >> 5;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)ring;
+  const char *const lds = reinterpret_cast<const char *>(ring);
+  // XCD x takes the x-th eighth of the tiles, row tiles first: they share weights
+  const int xcd = (int)(blockIdx.x & 7);
+  const int item = (int)((int64_t)total * xcd / 8) + (int)(blockIdx.x >> 3);
+  if (item >= (int)((int64_t)total * (xcd + 1) / 8)) return;
+  const int n0 = item / n_parts * kMidTile, r0 = item % n_parts * kMidTile;
+  const int rows = n_rows - r0 < kMidTile ? n_rows - r0 : kMidTile;
+  const int w_rows = n_out - n0 < kMidTile ? n_out - n0 : kMidTile;
+
+  const int64_t ld_w = (int64_t)KT * kFp8Block;
+  const float *const sw_src = mat.s + (int64_t)(n0 / kFp8Block) * KT;
+  float swv = 0.f;  // 64 blocks' scales, one per lane
+  auto load_sw = [&](int kt) { swv = sw_src[kt + lane < KT ? kt + lane : KT - 1]; };
+  auto pin_sw = [&] { asm volatile("" : "+v"(swv)); };  // (waited for here: see tile_kernel)
+  load_sw(0);
+  pin_sw();
+  const tm_rsrc_t w_rs = tm_make_rsrc(mat.w + (int64_t)n0 * ld_w, (uint64_t)w_rows * ld_w);
+  uint32_t w_off[2];
+  const uint8_t *x_src[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {  // rows past the end: the last one again, results dropped
+    const int row = (wave * 2 + j) * 8 + (lane >> 3);
+    w_off[j] = (uint32_t)(row < w_rows ? row : w_rows - 1) * (uint32_t)ld_w + (uint32_t)((lane & 7) ^ w_swz<kUp>(row)) * 16u;
+    x_src[j] = x + (int64_t)(r0 + (row < rows ? row : rows - 1)) * ld_x + ((lane & 7) ^ x_swz(row)) * 16;
+  }
+  const float *const s_src = xs + (int64_t)(r0 + (lane < rows ? lane : rows - 1)) * ld_xs;
+  auto issue = [&](int st, uint32_t slot) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int kt = 2 * st + u < KT ? 2 * st + u : KT - 1;  // (a block past the end is not used)
+      const uint32_t at = lds0 + slot + (uint32_t)(u * kMidBlock);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        tm_dma16_buf_so(w_rs, w_off[j], (uint32_t)kt * kFp8Block, at + (uint32_t)(wave * 2 + j) * 1024u);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        tm_dma16_s(x_src[j] + (int64_t)kt * kFp8Block, at + (uint32_t)(kMidW + (wave * 2 + j) * 1024));
+      tm_dma4_s(s_src + kt, at + (uint32_t)(2 * kMidW));
+    }
+  };
+  // operand rows and columns as in the up product of tile_kernel
+  const int a_row = 32 * cg + 16 * ((t >> 2) & 1) + 4 * (t >> 3) + (t & 3), tr = half * 32 + t;
+  const uint32_t a_off = (uint32_t)(a_row * kFp8Block + (h ^ w_swz<kUp>(a_row)) * 16);
+  const uint32_t b_off = (uint32_t)(kMidW + tr * kFp8Block + (h ^ x_swz(tr)) * 16);
+  tm_f32x16 acc = {};
+  const int n_st = (KT + 1) / 2;
+  for (int st = 0; st < kMidSlots && st < n_st; ++st) issue(st, (uint32_t)(st * kMidStage));
+  uint32_t slot = 0, prev = (kMidSlots - 1) * kMidStage;
+  for (int st = 0; st < n_st; ++st) {
+    const int left = n_st - 1 - st;
+    wait_stages<kMidDma, kMidSlots - 2>(left < kMidSlots - 2 ? left : kMidSlots - 2);
+    barrier();  // the stage landed, in every wave; every wave has read the one before
+    uint4 a[2][4], b[2][4];
+    float sc[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const char *const sp = lds + slot + u * kMidBlock;
+      const float sw = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(swv), (2 * st + u) & 63));
+      sc[u] = sw * *reinterpret_cast<const float *>(sp + 2 * kMidW + tr * 4);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        a[u][c] = *reinterpret_cast<const uint4 *>(sp + (a_off ^ (c << 5)));
+        b[u][c] = *reinterpret_cast<const uint4 *>(sp + (b_off ^ (c << 5)));
+      }
+    }
+    if (st > 0 && st - 1 + kMidSlots < n_st) issue(st - 1 + kMidSlots, prev);
+    tm_static_for<2>([&](auto u_c) {
+      constexpr int u = decltype(u_c)::value;
+      if (u == 1 && 2 * st + 1 >= KT) return;
+      tm_f32x16 p = {};
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          p = tm_mfma32x32x16<TM_DT_BF16>(tm_fp8_to_bf16x8(a[u][c].x, a[u][c].y), tm_fp8_to_bf16x8(b[u][c].x, b[u][c].y), p);
+          p = tm_mfma32x32x16<TM_DT_BF16>(tm_fp8_to_bf16x8(a[u][c].z, a[u][c].w), tm_fp8_to_bf16x8(b[u][c].z, b[u][c].w), p);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {
+          const uint4 a2[2] = {a[u][c], a[u][c + 1]}, b2[2] = {b[u][c], b[u][c + 1]};
+          p = tm_mfma32x32x64_fp8(a2, b2, p);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[i] = fmaf(p[i], sc[u], acc[i]);
+    });
+    if (((st + 1) & 31) == 0 && st + 1 < n_st) {
+      load_sw(2 * st + 2);
+      pin_sw();
+    }
+    prev = slot;
+    slot = slot == (kMidSlots - 1) * kMidStage ? 0u : slot + kMidStage;
+  }
+  tm_wait_vm_lgkm0_mem<0>();
+  barrier();  // the ring is free
+  constexpr int kLd = kMidTile + 4;
+  float *const tile = reinterpret_cast<float *>(ring);
+#pragma unroll
+  for (int i = 0; i < 16; i += 4)
+    *reinterpret_cast<float4 *>(tile + tr * kLd + cg * 32 + 16 * h + i) =
+        make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+  __syncthreads();
+  write_tile<DT, kMidTile, kMidThreads>(tile, rows, r0, n0, n_out, dst, nullptr, vec_out);
+}
+
+template <int DT, bool WIDE>
+int mid_launch(const char *name, const void *x, int64_t ld_x, const float *xs, int64_t ld_xs, const Fp8Mat &mat,
+               int64_t n_rows, int n_out, int KT, const Fp8Dst &dst, hipStream_t s) {
+  const int64_t parts = tm_cdiv(n_rows, kMidTile), total = parts * tm_cdiv(n_out, kMidTile);
+  hipLaunchKernelGGL((mid_kernel<DT, WIDE>), dim3((unsigned)(tm_cdiv(total, 8) * 8)), dim3(kMidThreads), 0, s,
+                     static_cast<const uint8_t *>(x), ld_x, xs, ld_xs, mat, (int)n_rows, n_out, KT, (int)parts,
+                     (int)total, dst, can_write8<DT>(dst, n_out));
   TM_LAUNCH_CHECK(name);
   return TM_OK;
 }
@@ -725,8 +887,13 @@ int64_t round_up(int64_t v, int64_t m) { return tm_cdiv(v, m) * m; }
 // ---------------------------------------------------------------------------
 namespace {
 
-// Rows up to which a linear layer streams its weights (stream_kernel).
-constexpr int64_t kLinearStreamRows = 32;
+// Rows up to which a linear layer streams its weights (stream_kernel): 2048 -> 4096
+// in bf16 takes it 8.3 us for 8 rows and 13 for 16, mid_kernel with the rows'
+// quantisation 10.7 and 10.9; 4096 -> 2048 10.5 and 17 against 16.6 and 16.6.
+constexpr int64_t kLinearStreamRows = 12;
+// 64 x 64 tiles up to which it takes mid_kernel, one per CU: 512 rows, 4096 -> 2048
+// (256 tiles) take 22 us, in the large tiles 31; 2048 -> 4096 (512) 24 and 20.
+constexpr int64_t kMidTiles = 256;
 
 }  // namespace
 
@@ -776,6 +943,9 @@ extern "C" int tm_fp8_linear(int32_t dtype, const void *x, const float *x_scale,
   Fp8Tiles ts{};
   ts.rows = (int32_t)n_rows;
   return TM_DISPATCH_DTYPE(dtype, DT, [&] {
+    if (tm_cdiv(n_rows, kMidTile) * tm_cdiv(n_out, kMidTile) <= kMidTiles)
+      return mid_launch<DT, DT == TM_DT_F32>(name, src.x, src.ld, src.scale, src.ld_s, m, n_rows, (int)n_out, (int)kb,
+                                             dst, s);
     return tile_launch<DT, kOut, DT == TM_DT_F32>(name, src.x, src.ld, src.scale, src.ld_s, m, m, (int)n_out, (int)kb,
                                                   ts, dst, nullptr, s);
   });
@@ -922,7 +1092,7 @@ extern "C" int tm_fp8_grouped_swiglu(const tm_fp8_experts *experts, int32_t dtyp
                                      offsets, row_token, row_out, tiles, base + ws.group,
                                      tm_group_slots_workspace_size(n_tokens, top_k, experts->n_experts), stream);
     if (st != TM_OK) return st;
-    ts = Fp8Tiles{offsets, row_token, row_out, experts->n_experts, (int32_t)max_rows};
+    ts = Fp8Tiles{offsets, row_token, row_out, experts->n_experts, (int32_t)max_rows, 0};
   }
   const Fp8Dst dst{out, 0, so_b, so_s, nullptr, 0};
   return dtype == TM_DT_F16

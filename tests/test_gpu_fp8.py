@@ -198,6 +198,19 @@ def test_linear_strides_dims_and_out(hip_device):
     assert torch.equal(layer.forward(x[:1].expand(40, 512)), layer.forward(x[:1].repeat(40, 1)))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,k,n", [
+    (12, 512, 136), (13, 8320, 70), (13, 8192, 64), (70, 128, 1), (64, 8448, 1023),      # few rows; 64 x 64 tiles
+    (512, 300, 2048), (513, 300, 2050), (700, 384, 2816), (2100, 8320, 1025), (1090, 256, 4097),  # the large tiles
+])
+def test_linear_tilings(hip_device, dtype, m, k, n):
+    """Every split of the work, at its first and last rows, with more than 64 blocks
+    of columns and an odd number of them."""
+    x = _rand(m + k, m, k, dtype=dtype)
+    wq, ws = _w8(n, n, k)
+    _check_linear(x, wq, ws, _rand(n + 1, n, dtype=dtype))
+
+
 @pytest.mark.parametrize("m", [2, 70])
 def test_linear_quantised_input(hip_device, m):
     x = _rand(7, m, 1000, dtype=torch.bfloat16)
