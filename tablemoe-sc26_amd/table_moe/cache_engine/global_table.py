@@ -345,9 +345,10 @@ class GlobalTable:
         """A DeepSeek-style MoE layer on the table (models/deepseek_vl2/
         deepseek_layers.py:569-745 shape): the layer call up to the keep set,
         the kept tokens' routed slots recomputed by ``experts``
-        (GroupedExperts, on the device, no host sync), the shared experts
-        ``shared`` = (w1, w3, w2) or a ``SharedExperts`` (packed weights, same
-        bits) run over every token with the residual folded into their down
+        (GroupedExperts or Fp8GroupedExperts, on the device, no host sync),
+        the shared experts ``shared`` = (w1, w3, w2), a ``SharedExperts``
+        (packed weights, same bits) or a ``Fp8SharedExperts`` (8-bit weights)
+        run over every token with the residual folded into their down
         projection (dtype(residual + shared)), then the
         gather + combine on top: out = dtype(dtype(residual + shared) + y),
         y = the renormalised routed slots (kept tokens) or the cached output
@@ -375,6 +376,8 @@ class GlobalTable:
                 nbytes = N.lib().tm_grouped_swiglu_packed_workspace_size(n, shared.inter, 1, N.dtype_tag(self.dtype))
                 if shared._ws is None or shared._ws.numel() < nbytes:
                     shared._ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=self.device)
+                run = lambda: shared.forward(hidden, out=base, addend=residual)  # noqa: E731
+            elif hasattr(shared, "forward"):  # Fp8SharedExperts: its scratch comes from the side stream's pool
                 run = lambda: shared.forward(hidden, out=base, addend=residual)  # noqa: E731
             else:
                 w1, w3, w2 = shared
