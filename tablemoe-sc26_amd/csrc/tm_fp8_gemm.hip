@@ -96,7 +96,7 @@ __device__ __forceinline__ void store4(void *y, int64_t at, const float (&v)[4],
 // before it groups the rows or quantises them: a call is its two products.
 //
 // Bound by HBM: 256 slots of 110 experts (2048 x 768) stream 352 MB in 65 us (up,
-// 5.4 TB/s) and 176 MB in 37 (down, 4.7); one token's 8 experts take 11 + 6, a
+// 5.4 TB/s) and 176 MB in 37 (down, 4.7); one token's 8 experts take 10 + 6, a
 // chain of latencies (slots, rows, weights, sums).  Up: quantising in the
 // operand's layout, where every lane does 32 columns of its row whether it is
 // live or not, 140; 48 KiB of LDS rows 81; three waves per SIMD instead of four
@@ -135,31 +135,39 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(
   const int64_t item = blockIdx.x / n_groups;
   int e = 0;
   int64_t count = rows.n;
+  const bool single = rows.n == 1;
   if (rows.ids != nullptr) {
     // This workgroup's expert: `item` (by_expert), or that of slot `item`, whose
-    // first slot's workgroups take all of them.
+    // first slot's workgroups take all of them; a single token's slots are each by
+    // themselves (8 slots: 10 + 6 us; 11 + 6 when they searched for each other).
     const int total = (int)rows.n * rows.top_k;
     auto expert_of = [&](int p) {
       const int b = p / rows.top_k, s = p - b * rows.top_k;
       const int64_t id = rows.ids[b * rows.ld_ids + s];
-      return rows.mask[b * rows.ms_b + s * rows.ms_s] && id >= 0 && id < rows.n_experts ? (int)id : -1;
+      const bool live = rows.mask[b * rows.ms_b + s * rows.ms_s] != 0;  // (both loads at once)
+      return (live & (id >= 0) & (id < rows.n_experts)) ? (int)id : -1;
     };
     e = rows.by_expert ? (int)item : expert_of((int)item);
     if (e < 0) return;  // uniform
-    if (tid == 0) {
-      s_count = 0;
-      s_first = total;
-    }
-    __syncthreads();
-    for (int p = tid; p < total; p += threads)
-      if (expert_of(p) == e) {
-        list[atomicAdd(&s_count, 1)] = (uint16_t)p;  // (a row's result does not depend on its place)
-        atomicMin(&s_first, p);
+    if (single) {
+      count = 1;
+    } else {
+      if (tid == 0) {
+        s_count = 0;
+        s_first = total;
       }
-    __syncthreads();
-    count = s_count;
-    if (count == 0 || (!rows.by_expert && s_first != (int)item)) return;  // uniform
+      __syncthreads();
+      for (int p = tid; p < total; p += threads)
+        if (expert_of(p) == e) {
+          list[atomicAdd(&s_count, 1)] = (uint16_t)p;  // (a row's result does not depend on its place)
+          atomicMin(&s_first, p);
+        }
+      __syncthreads();
+      count = s_count;
+      if (count == 0 || (!rows.by_expert && s_first != (int)item)) return;  // uniform
+    }
   }
+  auto slot_of = [&](int64_t i) { return rows.ids == nullptr ? 0 : single ? (int)item : (int)list[i]; };
 
   uint4 w[NM][NA][KPW][2];
   float sw[NM][KPW];
@@ -194,7 +202,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(
     const bool whole = src.k == (int64_t)KT * kFp8Block;  // no row ends inside a block
     for (int i = tid >> 4; i < here * KT; i += threads >> 4) {
       const int r = i / KT, b = i - r * KT;
-      const int p = rows.ids != nullptr ? list[c0 + r] : 0;
+      const int p = slot_of(c0 + r);
       const int64_t xr = rows.ids == nullptr ? c0 + r : MODE == kUp ? p / rows.top_k : p;
       const int c = b * kFp8Block + t * 8;
       uint2 q;
@@ -288,7 +296,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(
         }
       if (t >= here) continue;
       const int c = n0 + 16 * a + 4 * g;
-      const int p = rows.ids != nullptr ? list[c0 + t] : 0;
+      const int p = slot_of(c0 + t);
       if constexpr (MODE == kUp) {
         float f[4];
 #pragma unroll
@@ -314,7 +322,7 @@ int stream_launch(const char *name, const Fp8Src &src, Fp8Rows rows, const Fp8Ma
                   int KT, const Fp8Dst &dst, hipStream_t s) {
   const int n_groups = (int)tm_cdiv(n_out, 16 * NA);
   const int64_t total = rows.ids != nullptr ? rows.n * rows.top_k : rows.n;
-  rows.by_expert = rows.ids != nullptr && total >= rows.n_experts;
+  rows.by_expert = rows.ids != nullptr && rows.n > 1 && total >= rows.n_experts;
   const int64_t items = rows.ids == nullptr ? 1 : rows.by_expert ? rows.n_experts : total;
   TM_REQUIRE(items * n_groups < ((int64_t)1 << 31), TM_EINVAL_SHAPE, "%s: too many rows", name);
   const int64_t esz = Elem<DT>::kBytes;

@@ -410,6 +410,19 @@ def test_experts_scales_far_apart(hip_device, n):
     _check_experts(x, ids, torch.ones(n, dtype=torch.bool, device=hip_device), tuple(w))
 
 
+@pytest.mark.parametrize("k", [1, 5, 8])
+def test_experts_of_one_token(hip_device, k):
+    """One token: an expert in several slots, ids out of range, masked slots, as many
+    slots as experts."""
+    e, h, inter = 5, 384, 256
+    x = _rand(k, 1, h, dtype=torch.bfloat16)
+    ids = torch.tensor([[3, 3, -1, 5, 0, 3, 1, 2][:k]], device=hip_device)
+    _check_experts(x, ids, torch.ones(1, dtype=torch.bool, device=hip_device), _weights(8, e, h, inter))
+    flags = torch.tensor([[1, 0, 1, 1, 1, 1, 0, 1][:k]], dtype=torch.bool, device=hip_device)
+    _check_experts(x, ids, flags, _weights(8, e, h, inter))
+    _check_experts(x, ids, torch.zeros(1, dtype=torch.bool, device=hip_device), _weights(8, e, h, inter))
+
+
 def test_experts_rows_do_not_depend_on_others(hip_device):
     """Two calls give the same bits, and so does another order of the tokens."""
     n, k, e, h, inter = 90, 4, 6, 256, 256
