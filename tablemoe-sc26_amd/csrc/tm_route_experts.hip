@@ -29,13 +29,11 @@ struct RouteArgs {
   int n_experts, scoring, n_groups, size, topk_groups, group_rule, top_k, renorm;
   float scale;
   const float *bias;
-  uint32_t inv;  // ceil(2^32 / size)
+  uint32_t inv;  // ceil(2^20 / size)
 };
 
-// e / size: exact for e < 2^16 (e * inv is over e / size * 2^32 by less than e).
-__device__ __forceinline__ int group_of(int e, const RouteArgs &a) {
-  return a.size == 1 ? e : (int)__umulhi((uint32_t)e, a.inv);
-}
+// e / size: exact for e < 2^10 >= size (e * inv is over e / size * 2^20 by less than e).
+__device__ __forceinline__ int group_of(int e, const RouteArgs &a) { return (int)(__umul24((uint32_t)e, a.inv) >> 20); }
 
 template <int CTRL>
 __device__ __forceinline__ float dpp16(float v) {
@@ -274,8 +272,11 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
 #pragma unroll
   for (int j = 0; j < VPL; ++j) {
     const int e = j * 16 + sub;
-    key[j] = l[j] == l[j] ? tm_orderable(scored ? v[j] : l[j]) : kMasked;
-    key[j] = e < a.n_experts ? key[j] : kClosed;
+    const uint32_t u = __float_as_uint(scored ? v[j] : l[j]);  // (both sides of the selects: no branch for each)
+    uint32_t o = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+    asm("" : "+v"(o));
+    o = l[j] == l[j] ? o : kMasked;
+    key[j] = e < a.n_experts ? o : kClosed;
   }
   if (a.n_groups > 1) {  // uniform
 #pragma unroll
@@ -446,7 +447,7 @@ extern "C" int tm_route_experts(int32_t dtype, const void *logits, int64_t n_tok
   TM_REQUIRE(logits && out_weights && out_ids, TM_EINVAL_ARG, "tm_route_experts: null pointer");
   const RouteArgs a{n_tokens, ld_logits, n_experts, scoring, n_groups, n_experts / n_groups, topk_groups, group_rule,
                     top_k, renormalize, scale, bias,
-                    (uint32_t)((((uint64_t)1 << 32) + n_experts / n_groups - 1) / (n_experts / n_groups))};
+                    ((1u << 20) + n_experts / n_groups - 1) / (n_experts / n_groups)};
   hipStream_t s = tm_hip_stream(stream);
   return TM_DISPATCH_DTYPE(dtype, DT, [&] {
     if (n_experts <= 64) launch<DT, 4>(logits, a, out_weights, out_ids, s);
