@@ -15,9 +15,11 @@
 //
 // Bound by latency: each round is a maximum over the lane's keys, four DPP
 // exchanges, the lowest lane that holds it and its key closed, one after the
-// other.  All in 64 bits took 24 us for 8 tokens of 256 experts, 20 us for 4099
-// of 160, 43 us for 12301 of 256 (a first pass in 32 bits that chose again in 64
-// where keys were near: 10, 10 and 36).
+// other; where at most half of the experts are in the groups that stay, over
+// those alone.  8 tokens of 256 experts take 8.2 us, 4099 of 160 8.4 us, 12301 of
+// 256 17 us (rounds over every key: 9.0, 9.3 and 17.7).  All in 64 bits took 24,
+// 20 and 43 (a first pass in 32 bits that chose again in 64 where keys were near:
+// 10, 10 and 36).
 #include "tm_common.h"
 
 #include <type_traits>
@@ -268,16 +270,10 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
       v[j] = l[j] == l[j] ? v[j] : ninf;
     }
   }
-  uint32_t key[VPL];
-#pragma unroll
-  for (int j = 0; j < VPL; ++j) {
-    const int e = j * 16 + sub;
-    const uint32_t u = __float_as_uint(scored ? v[j] : l[j]);  // (both sides of the selects: no branch for each)
-    uint32_t o = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
-    asm("" : "+v"(o));
-    o = l[j] == l[j] ? o : kMasked;
-    key[j] = e < a.n_experts ? o : kClosed;
-  }
+  uint64_t kept = ~0ull;
+  bool compact = false;
+  float *const gmin = vals + 4 * per_tok;
+  int *const glist = reinterpret_cast<int *>(gmin + a.n_groups);  // the groups that stay, ascending
   if (a.n_groups > 1) {  // uniform
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
@@ -285,8 +281,8 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
       const float k = scored || top2 ? v[j] : l[j] == l[j] ? l[j] : ninf;
       vals[e < a.n_experts ? e + group_of(e, a) : per_tok - 1] = k;  // (the last: a group value, written later)
     }
-    float *const gval = vals + a.n_experts + a.n_groups, *const gmin = vals + 4 * per_tok;
-    uint64_t kept;
+    float *const gval = vals + a.n_experts + a.n_groups;
+    compact = 2 * a.topk_groups * a.size <= 16 * VPL && (scored || !top2);  // (vals holds the keys)
     if (scored || top2) {  // uniform
       kept = kept_groups<float, true>(a, sub, vals, gval, gmin, unsure);
       if (__ballot(unsure) != 0) {
@@ -311,13 +307,14 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
         }
         kept = kept_groups<double, false>(a, sub, vals64, vals64 + a.n_experts + a.n_groups, nullptr, unsure);
         unsure = false;
+        compact = false;  // (vals is gone)
       }
     } else {
       kept = kept_groups<float, false>(a, sub, vals, gval, gmin, unsure);
     }
-#pragma unroll
-    for (int j = 0; j < VPL; ++j)
-      if (!((kept >> group_of(j * 16 + sub, a)) & 1)) key[j] = kClosed;
+    for (int g = sub; g < a.n_groups; g += 16)
+      if ((kept >> g) & 1) glist[__popcll(kept & ((1ull << g) - 1))] = g;
+    __syncthreads();
   }
   // Winner r goes to lane r % 16.  With 32-bit keys the rounds go on past the last
   // chosen until the next key is far below: the candidates then hold every
@@ -327,41 +324,80 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
   uint32_t last = 0;
   bool close = false;  // two neighbours of the candidates are near
   int r = 0;
-  for (bool more = true; more; ++r) {
-    uint32_t m = key[0];
+  auto rounds = [&](auto nk_c, auto &key) {
+    constexpr int NK = decltype(nk_c)::value;
+    for (bool more = true; more; ++r) {
+      uint32_t m = key[0];
 #pragma unroll
-    for (int j = 1; j < VPL; ++j) m = max(m, key[j]);
-    m = max(m, tm_dpp<0xB1>(m, m));
-    m = max(m, tm_dpp<0x4E>(m, m));
-    m = max(m, tm_dpp<0x141>(m, m));
-    m = max(m, tm_dpp<0x140>(m, m));
-    uint32_t at = 0xffffu;  // lowest expert with that key
+      for (int j = 1; j < NK; ++j) m = max(m, key[j]);
+      m = max(m, tm_dpp<0xB1>(m, m));
+      m = max(m, tm_dpp<0x4E>(m, m));
+      m = max(m, tm_dpp<0x141>(m, m));
+      m = max(m, tm_dpp<0x140>(m, m));
+      uint32_t at = 0xffffu;  // lowest expert with that key
 #pragma unroll
-    for (int j = VPL - 1; j >= 0; --j) at = key[j] == m ? (uint32_t)j : at;
-    uint32_t w = at * 16 + sub;
-    w = min(w, tm_dpp<0xB1>(w, w));
-    w = min(w, tm_dpp<0x4E>(w, w));
-    w = min(w, tm_dpp<0x141>(w, w));
-    w = min(w, tm_dpp<0x140>(w, w));
-    const uint32_t mine = at * 16 + sub == w ? at : 0xffffu;
+      for (int j = NK - 1; j >= 0; --j) at = key[j] == m ? (uint32_t)j : at;
+      uint32_t w = at * 16 + sub;
+      w = min(w, tm_dpp<0xB1>(w, w));
+      w = min(w, tm_dpp<0x4E>(w, w));
+      w = min(w, tm_dpp<0x141>(w, w));
+      w = min(w, tm_dpp<0x140>(w, w));
+      const uint32_t mine = at * 16 + sub == w ? at : 0xffffu;
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) key[j] = mine == (uint32_t)j ? kClosed : key[j];
-    if ((r & 15) == sub) {
-      if (r < 16) cand[0] = (int)w;
-      else cand[1] = (int)w;
-    }
-    if (scored) {  // uniform
-      const bool touches = (r > 0) & (m > kMasked) & near(tm_from_orderable(last), tm_from_orderable(m), kTol);
-      close |= touches;
-      last = m;
-      more = r + 1 < a.top_k || (r + 1 < n_open && (r + 1 == a.top_k || __ballot(touches) != 0));
-      if (more && r + 1 == 32) {  // a long run of equals: past what the candidates hold
-        unsure = true;
-        more = false;
+      for (int j = 0; j < NK; ++j) key[j] = mine == (uint32_t)j ? kClosed : key[j];
+      if ((r & 15) == sub) {
+        if (r < 16) cand[0] = (int)w;
+        else cand[1] = (int)w;
       }
-    } else {
-      more = r + 1 < a.top_k;
+      if (scored) {  // uniform
+        const bool touches = (r > 0) & (m > kMasked) & near(tm_from_orderable(last), tm_from_orderable(m), kTol);
+        close |= touches;
+        last = m;
+        more = r + 1 < a.top_k || (r + 1 < n_open && (r + 1 == a.top_k || __ballot(touches) != 0));
+        if (more && r + 1 == 32) {  // a long run of equals: past what the candidates hold
+          unsure = true;
+          more = false;
+        }
+      } else {
+        more = r + 1 < a.top_k;
+      }
     }
+  };
+  auto key_of = [&](float f, bool masked) {
+    const uint32_t u = __float_as_uint(f + 0.f);  // (-0 equals 0)
+    uint32_t o = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+    asm("" : "+v"(o));  // (both sides of the select: no branch for each)
+    return masked ? kMasked : o;
+  };
+  if (compact) {
+    // Half of the experts are open at most: a lane takes every 16th of those, in
+    // their order, from LDS.
+    constexpr int NK = VPL / 2;
+    uint32_t key[NK];
+    auto expert_at = [&](int p, int pad) {
+      const int i = group_of(p, a);
+      return glist[i] * (a.size + pad) + p - i * a.size;
+    };
+#pragma unroll
+    for (int j = 0; j < NK; ++j) {
+      const int p = j * 16 + sub;
+      const float f = vals[expert_at(p < n_open ? p : 0, 1)];
+      const uint32_t o = key_of(f, f == ninf);
+      key[j] = p < n_open ? o : kClosed;
+    }
+    rounds(std::integral_constant<int, NK>{}, key);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) cand[u] = expert_at(cand[u], 0);
+  } else {
+    uint32_t key[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      const int e = j * 16 + sub;
+      const uint32_t o = key_of(scored ? v[j] : l[j], l[j] != l[j]);
+      const bool open = (kept >> (a.n_groups > 1 ? group_of(e, a) & 63 : 0)) & 1;
+      key[j] = (open & (e < a.n_experts)) ? o : kClosed;
+    }
+    rounds(std::integral_constant<int, VPL>{}, key);
   }
   int n_cand = r;
   if (__ballot(unsure) != 0) {  // uniform

@@ -55,6 +55,22 @@ def test_matches_definition(hip_device, dtype, n, e, top_k, groups, keep, rule, 
                scale=scale)
 
 
+@pytest.mark.parametrize("scoring,bias,rule", [("sigmoid", True, "top2"), ("softmax", True, "max"),
+                                               ("softmax", False, "max"), ("sigmoid", False, "top2")])
+@pytest.mark.parametrize("e,groups,keep,top_k", [(256, 8, 4, 8), (1024, 2, 1, 32), (60, 20, 10, 12), (64, 64, 32, 31),
+                                                 (99, 3, 1, 9), (500, 4, 2, 16), (112, 7, 3, 6)])
+def test_few_groups_stay(hip_device, e, groups, keep, top_k, scoring, bias, rule):
+    """At most half of the experts open: logits with many equals, experts that are
+    not available (whole groups of them in some rows)."""
+    x = _logits(e, 41, e, hip_device)
+    x[:20] = (x[:20] * 2).round() / 2
+    x[5:15][torch.rand(10, e, generator=torch.Generator().manual_seed(3)).to(hip_device) < 0.4] = float("-inf")
+    x[3, : e // groups] = float("-inf")
+    x[4, e // groups:] = float("nan")
+    b = _logits(5, 1, e, hip_device, spread=0.1)[0] if bias else None
+    _check(x, top_k, b, scoring=scoring, n_groups=groups, topk_groups=keep, group_rule=rule, normalize_topk=True)
+
+
 def test_softmax_matches_topk_softmax(hip_device):
     x = _logits(3, 65, 128, hip_device)
     w, i = route_experts(x, 8, normalize_topk=True)
