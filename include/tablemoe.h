@@ -565,7 +565,7 @@ int tm_fp8_quantize_weight(int32_t dtype, const void *w, int64_t n_mats, int64_t
  * tm_fp8_quantize_rows; w [n_out] rows of ceil(k/128) * 128 bytes (contiguous;
  * what lies past k must not be NaN), w_scale [ceil(n_out/128),
  * ceil(k/128)]; bias [n_out] of `dtype`, nullable; out [n_rows, n_out] of
- * `dtype` (row stride ld_out).  fp32 sums; F32 outputs and the up product of
+ * `dtype` (row stride ld_out, not overlapping x).  fp32 sums; F32 outputs and the up product of
  * the MLPs below take every product exactly, 16-bit outputs may take the
  * 8-bit matrix instructions, which drop what lies under 2^-13 of the largest
  * of 8 consecutive products (1.5e-5 to 6e-5 of a sum's size on normal data).

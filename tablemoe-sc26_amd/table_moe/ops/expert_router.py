@@ -35,8 +35,10 @@ def route_experts(router_logits: torch.Tensor, top_k: int, *, scoring: str = "so
                          f"{sorted(_SCORING)} / {sorted(_GROUP_RULE)}")
     dev = N.require_hip(router_logits, bias)
     tag = N.dtype_tag(router_logits.dtype)
-    logits = router_logits if router_logits.stride(-1) == 1 or router_logits.shape[1] == 1 else router_logits.contiguous()
-    n, n_exp = logits.shape
+    n, n_exp = router_logits.shape
+    logits = router_logits
+    if (logits.stride(1) != 1 and n_exp > 1) or (logits.stride(0) < n_exp and n > 1):  # (stride 0: one row for all)
+        logits = logits.contiguous()
     if bias is not None:
         if bias.shape != (n_exp,):
             raise ValueError(f"route_experts: bias must be [{n_exp}], got {tuple(bias.shape)}")

@@ -90,7 +90,7 @@ class Fp8Linear:
     error of up to 6e-5 of a sum's size before the rounding).  A weight whose
     K is no multiple of 128 is copied once to padded rows.  Calls allocate
     their scratch from torch's allocator: they can be captured in graphs and
-    made on any stream."""
+    made on any stream.  ``out`` must not overlap x."""
 
     def __init__(self, weight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None):
         if weight.dim() != 2:
@@ -107,7 +107,6 @@ class Fp8Linear:
             self.weight = torch.zeros((self.out_features, kp), dtype=torch.uint8, device=self.device)
             self.weight[:, :self.in_features] = weight.view(torch.uint8)
         self.scale, self.bias = scale.contiguous(), bias
-        self._bias: dict = {}
 
     @classmethod
     def from_weight(cls, weight: torch.Tensor, bias: torch.Tensor | None = None) -> "Fp8Linear":
@@ -115,12 +114,7 @@ class Fp8Linear:
         return cls(*quantize_weight_fp8(weight), bias)
 
     def _bias_of(self, dtype):
-        if self.bias is None or (self.bias.dtype == dtype and self.bias.is_contiguous()):
-            return self.bias
-        b = self._bias.get(dtype)
-        if b is None:
-            b = self._bias[dtype] = self.bias.to(dtype).contiguous()
-        return b
+        return None if self.bias is None else self.bias.to(dtype).contiguous()
 
     def forward(self, x, out: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
         k, n = self.in_features, self.out_features
@@ -166,8 +160,9 @@ class Fp8Linear:
         with N.on_device(self.device):
             nbytes = N.lib().tm_fp8_linear_workspace_size(m, k, tag)
             ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=self.device)
+            bias = self._bias_of(dtype)
             N.call("tm_fp8_linear", tag, N.ptr(x2), N.ptr(xs), m, k, ld_x, 0 if xs is None else xs.stride(0),
-                   N.ptr(self.weight), N.ptr(self.scale), n, N.ptr(self._bias_of(dtype)), N.ptr(o2),
+                   N.ptr(self.weight), N.ptr(self.scale), n, N.ptr(bias), N.ptr(o2),
                    max(o2.stride(0), n), N.ptr(ws), ws.numel(), N.stream(self.device))
         return out
 

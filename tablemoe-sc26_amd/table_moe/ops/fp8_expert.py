@@ -75,7 +75,7 @@ class Fp8GroupedExperts:
             raise ValueError(f"slot_out must be [N, {k}, {self.hidden}] with unit stride along hidden")
         if slot_out.stride(0) % 8 or slot_out.stride(1) % 8 or slot_out.data_ptr() % 16:
             raise ValueError("slot_out rows must start on 16-byte boundaries (strides multiples of 8 elements)")
-        if ids.dtype != torch.long or ids.stride(1) != 1:
+        if ids.dtype != torch.long or ids.stride(1) != 1 or ids.stride(0) < k:  # (stride 0: one row for all tokens)
             ids = ids.long().contiguous()
         x = hidden
         if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < self.hidden or x.data_ptr() % 16:

@@ -244,6 +244,23 @@ def test_linear_rows_are_apart(hip_device):
     assert torch.equal(y[same], y0[same])
 
 
+def test_linear_bias_of_another_type(hip_device):
+    """A bias is read at the call, whatever its type and strides."""
+    bias = _rand(21, 300, 2, dtype=torch.float32)[:, 0]
+    was = bias.clone()
+    layer = Fp8Linear(*_w8(22, 300, 256), bias)
+    for m in (3, 40, 3000):
+        x = _rand(m, m, 256, dtype=torch.bfloat16)
+        y = layer.forward(x)
+        bias.copy_(was + 64.0)
+        moved = layer.forward(x)
+        bias.copy_(was)
+        # two roundings of the bias to bf16 and two of the result: 2^-8 of each
+        tol = 2.0 ** -8 * (y.float().abs() + moved.float().abs() + was.abs() + (was + 64.0).abs()) + 1e-3
+        assert bool(((moved.float() - y.float() - 64.0).abs() <= tol).all())
+        assert torch.equal(layer.forward(x), y)
+
+
 def test_linear_stream_and_graph(hip_device):
     x = _rand(13, 24, 512, dtype=torch.float16)
     wq, ws = _w8(14, 300, 512)
@@ -421,6 +438,20 @@ def test_experts_of_one_token(hip_device, k):
     flags = torch.tensor([[1, 0, 1, 1, 1, 1, 0, 1][:k]], dtype=torch.bool, device=hip_device)
     _check_experts(x, ids, flags, _weights(8, e, h, inter))
     _check_experts(x, ids, torch.zeros(1, dtype=torch.bool, device=hip_device), _weights(8, e, h, inter))
+
+
+@pytest.mark.parametrize("n", [7, 600])
+def test_experts_one_row_of_ids_for_all(hip_device, n):
+    """ids and masks of row stride 0."""
+    e, k, h, inter = 6, 3, 256, 128
+    w = _weights(9, e, h, inter)
+    x = _rand(n, n, h, dtype=torch.bfloat16)
+    ids = torch.tensor([[4, 0, 2]], device=hip_device).expand(n, k)
+    flags = torch.tensor([[1, 1, 0]], dtype=torch.uint8, device=hip_device).expand(n, k)
+    _, one = _check_experts(x, ids, flags, w)
+    _, two = _check_experts(x, ids.contiguous(), flags.contiguous().bool(), w)
+    assert torch.equal(one, two)
+    _check_experts(x[:1].expand(n, h), ids, torch.ones(1, dtype=torch.bool, device=hip_device).expand(n), w)
 
 
 def test_experts_rows_do_not_depend_on_others(hip_device):

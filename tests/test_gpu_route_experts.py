@@ -150,6 +150,18 @@ def test_strides_and_empty(hip_device):
     assert w.shape == (0, 5) and i.shape == (0, 5)
 
 
+def test_one_row_for_all_tokens(hip_device):
+    """Row stride 0, and one expert."""
+    x = _logits(4, 1, 100, hip_device)
+    w0, i0 = route_experts(x, 5)
+    w, i = route_experts(x.expand(37, 100), 5)
+    assert torch.equal(w, w0.expand(37, 5)) and torch.equal(i, i0.expand(37, 5))
+    w, i = route_experts(x[:, :1].expand(9, 1), 1)
+    assert bool((w == 1).all()) and bool((i == 0).all())
+    w, i = route_experts(_logits(5, 9, 4, hip_device)[:, 1:2], 1)   # a column
+    assert bool((w == 1).all()) and bool((i == 0).all())
+
+
 def test_other_stream_and_graph(hip_device):
     x = _logits(6, 50, 256, hip_device)
     b = _logits(7, 1, 256, hip_device, spread=0.1)[0]
