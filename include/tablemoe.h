@@ -86,9 +86,8 @@ int tm_topk_softmax(const float *logits, int64_t n_tokens, int32_t n_experts, in
                     tm_stream_t stream);
 
 /* ======================================================================
- * Router of grouped experts with a balancing bias: the routers of the second
- * model family's larger layers (models/deepseek_vl2 gate: softmax or sigmoid
- * scores, groups, correction bias), beside tm_topk_softmax.
+ * Router of grouped experts with a balancing bias, beside tm_topk_softmax
+ * (softmax scores of all experts).
  * For each row of logits [n_tokens, n_experts] (dtype F32, F16 or BF16, row
  * stride ld_logits): scores s = softmax(l) or sigmoid(l); v = s + bias (fp32
  * [n_experts], nullable: 0); order key = v, or l without a bias (the scores

@@ -115,9 +115,9 @@ __host__ __device__ inline int stream_chunk(int KT, int64_t most) {
 }
 
 template <int DT, int DTX, int MODE, int NA, int KPW>
-__global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(MODE == kUp ? 4 : 1))) void stream_kernel(Fp8Src src, Fp8Rows rows, Fp8Mat m0, Fp8Mat m1, int n_out,
-                                                                int KT, int n_groups, int chunk, Fp8Dst dst,
-                                                                bool vec_out) {
+__global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(MODE == kUp ? 4 : 1)))
+void stream_kernel(Fp8Src src, Fp8Rows rows, Fp8Mat m0, Fp8Mat m1, int n_out, int KT, int n_groups, int chunk,
+                   Fp8Dst dst, bool vec_out) {
   constexpr int NM = MODE == kUp ? 2 : 1;
   constexpr bool WIDE = MODE == kUp || DT == TM_DT_F32;  // on the 16-bit instructions
   // the waves' sums [S][NM * NA][64], the chunk's rows [chunk][KT * 128 + 16] bytes,
@@ -282,7 +282,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(
     for (int m = 0; m < NM; ++m)
 #pragma unroll
       for (int a = 0; a < NA; ++a)
-        red[(wave * (NM * NA) + m * NA + a) * 64 + lane] = make_float4(acc[m][a][0], acc[m][a][1], acc[m][a][2], acc[m][a][3]);
+        red[(wave * (NM * NA) + m * NA + a) * 64 + lane] =
+            make_float4(acc[m][a][0], acc[m][a][1], acc[m][a][2], acc[m][a][3]);
     __syncthreads();
     for (int i = tid; i < NA * 64; i += threads) {
       // row t of the chunk, columns n0 + 16 a + 4 g .. + 3
@@ -509,222 +510,222 @@ __global__ __launch_bounds__(kTileThreads, 2) void tile_kernel(const uint8_t *__
   const int xcd = (int)(blockIdx.x & 7), on_xcd = ((int)gridDim.x - xcd + 7) / 8;
   const int64_t last = total * (xcd + 1) / 8;
   for (int64_t item = total * xcd / 8 + (blockIdx.x >> 3); item < last; item += on_xcd) {
-  const int part = (int)(item / n_tiles);
-  const int n0 = (int)(item % n_tiles) * (MODE == kUp ? kTileCols / 2 : kTileCols);
-  int e = 0, r0 = part * ts.bm, r_end = ts.rows;
-  if (grouped) {
-    int n = 0;  // experts whose tiles all come before this one
-    for (int i = 0; i < ts.n_experts; i += 64)
-      n += __popcll(__ballot(i + lane < ts.n_experts && s_part[i + lane + 1] <= part));
-    e = n;
-    r0 = __builtin_amdgcn_readfirstlane(s_off[e] + (part - s_part[e]) * kTileBM);
-    r_end = __builtin_amdgcn_readfirstlane(s_off[e + 1]);
-  }
-  const int rows = r_end - r0 < ts.bm ? r_end - r0 : ts.bm;
-  r_end = r0 + rows;
-
-  // weight loads: 1 KiB pieces 4 wave + j, 8 rows each (up: waves 0-3 W1, waves 4-7 W3)
-  const Fp8Mat &mine = MODE == kUp && wave >= 4 ? m1 : m0;
-  constexpr int kWRows = MODE == kUp ? kTileCols / 2 : kTileCols;
-  const int w_rows = n_out - n0 < kWRows ? n_out - n0 : kWRows;
-  const tm_rsrc_t w_rs = tm_make_rsrc(mine.w + ((int64_t)e * n_out + n0) * ld_w, (uint64_t)w_rows * ld_w);
-  uint32_t w_off[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    int row = ((MODE == kUp ? wave & 3 : wave) * 4 + j) * 8 + (lane >> 3);
-    const int chunk = (lane & 7) ^ w_swz<MODE>(row);
-    row = row < w_rows ? row : w_rows - 1;  // (results of rows past n_out are dropped)
-    w_off[j] = (uint32_t)row * (uint32_t)ld_w + (uint32_t)chunk * 16u;
-  }
-  // operand row t of block a: weight row
-  //   out: 64 cg + 32 (t / 4 % 2) + 16 a + 4 (t / 8) + t % 4
-  //   up:  32 cg + 16 (t / 4 % 2) + 4 (t / 8) + t % 4 of matrix a
-  // its chunk 2 c + h (c = 0 .. 3), of both operands: the same columns
-  uint32_t a_off[4];  // (of block 0)
-  {
-    const int row = MODE == kUp ? 32 * cg + 16 * ((t >> 2) & 1) + 4 * (t >> 3) + (t & 3)
-                                : 64 * cg + 32 * ((t >> 2) & 1) + 4 * (t >> 3) + (t & 3);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) a_off[c] = (uint32_t)(row * kFp8Block + ((2 * c + h) ^ w_swz<MODE>(row)) * 16);
-  }
-  constexpr uint32_t kABlock = (MODE == kUp ? 128 : 16) * kFp8Block;  // block 1 (its swizzle is block 0's)
-  // the wave's scales of 64 blocks, one per lane
-  const int blk = (MODE == kUp ? n0 : n0 + cg * 64) / kFp8Block;
-  const int64_t s_at = ((int64_t)e * n_blk + (blk < n_blk ? blk : n_blk - 1)) * KT;
-  float swv[2] = {0.f, 0.f};
-  auto load_sw = [&](int kt) {
-    const int k = kt + lane < KT ? kt + lane : KT - 1;
-    swv[0] = m0.s[s_at + k];
-    if constexpr (MODE == kUp) swv[1] = m1.s[s_at + k];
-  };
-  // The compiler waits for the scales here; at their use, in the loop, its wait
-  // would be one for every direct load in flight, which it does not count (that took
-  // 149 + 74 us where this takes 132 + 66: 5280 rows of 128 experts).
-  auto pin_sw = [&] { asm volatile("" : "+v"(swv[0]), "+v"(swv[1])); };
-  load_sw(0);
-
-  tm_f32x16 acc[2][2];
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int q = 0; q < 2; ++q) acc[a][q] = tm_f32x16{};
-
-  auto run = [&](auto nb_c) {
-    constexpr int NB = decltype(nb_c)::value;
-    using Cfg = TileCfg<NB>;
-    constexpr int S = Cfg::kSlots;
-    auto row_of = [&](int tr) {  // a row past the tile: its last one again, results dropped
-      int gr = r0 + tr;
-      gr = gr < r_end ? gr : r_end - 1;
-      return MODE == kUp && ts.row_token != nullptr ? (int64_t)ts.row_token[gr] : (int64_t)gr;
-    };
-    const uint8_t *x_src[NB];
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const int tr = (wave * NB + j) * 8 + (lane >> 3);
-      x_src[j] = x + row_of(tr) * ld_x + ((lane & 7) ^ x_swz(tr)) * 16;
+    const int part = (int)(item / n_tiles);
+    const int n0 = (int)(item % n_tiles) * (MODE == kUp ? kTileCols / 2 : kTileCols);
+    int e = 0, r0 = part * ts.bm, r_end = ts.rows;
+    if (grouped) {
+      int n = 0;  // experts whose tiles all come before this one
+      for (int i = 0; i < ts.n_experts; i += 64)
+        n += __popcll(__ballot(i + lane < ts.n_experts && s_part[i + lane + 1] <= part));
+      e = n;
+      r0 = __builtin_amdgcn_readfirstlane(s_off[e] + (part - s_part[e]) * kTileBM);
+      r_end = __builtin_amdgcn_readfirstlane(s_off[e + 1]);
     }
-    const float *const s_src = xs + row_of((wave % NB) * 64 + lane) * ld_xs;
-    const uint32_t s_dst = (uint32_t)(Cfg::kW + Cfg::kX + (wave % NB) * 256);
-    auto issue = [&](int kt, uint32_t slot) {
+    const int rows = r_end - r0 < ts.bm ? r_end - r0 : ts.bm;
+    r_end = r0 + rows;
+
+    // weight loads: 1 KiB pieces 4 wave + j, 8 rows each (up: waves 0-3 W1, waves 4-7 W3)
+    const Fp8Mat &mine = MODE == kUp && wave >= 4 ? m1 : m0;
+    constexpr int kWRows = MODE == kUp ? kTileCols / 2 : kTileCols;
+    const int w_rows = n_out - n0 < kWRows ? n_out - n0 : kWRows;
+    const tm_rsrc_t w_rs = tm_make_rsrc(mine.w + ((int64_t)e * n_out + n0) * ld_w, (uint64_t)w_rows * ld_w);
+    uint32_t w_off[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        tm_dma16_buf_so(w_rs, w_off[j], (uint32_t)kt * kFp8Block, lds0 + slot + (uint32_t)(wave * 4 + j) * 1024u);
+    for (int j = 0; j < 4; ++j) {
+      int row = ((MODE == kUp ? wave & 3 : wave) * 4 + j) * 8 + (lane >> 3);
+      const int chunk = (lane & 7) ^ w_swz<MODE>(row);
+      row = row < w_rows ? row : w_rows - 1;  // (results of rows past n_out are dropped)
+      w_off[j] = (uint32_t)row * (uint32_t)ld_w + (uint32_t)chunk * 16u;
+    }
+    // operand row t of block a: weight row
+    //   out: 64 cg + 32 (t / 4 % 2) + 16 a + 4 (t / 8) + t % 4
+    //   up:  32 cg + 16 (t / 4 % 2) + 4 (t / 8) + t % 4 of matrix a
+    // its chunk 2 c + h (c = 0 .. 3), of both operands: the same columns
+    uint32_t a_off[4];  // (of block 0)
+    {
+      const int row = MODE == kUp ? 32 * cg + 16 * ((t >> 2) & 1) + 4 * (t >> 3) + (t & 3)
+                                  : 64 * cg + 32 * ((t >> 2) & 1) + 4 * (t >> 3) + (t & 3);
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
-        tm_dma16_s(x_src[j] + (int64_t)kt * kFp8Block, lds0 + slot + (uint32_t)(Cfg::kW + (wave * NB + j) * 1024));
-      tm_dma4_s(s_src + kt, lds0 + slot + s_dst);
+      for (int c = 0; c < 4; ++c) a_off[c] = (uint32_t)(row * kFp8Block + ((2 * c + h) ^ w_swz<MODE>(row)) * 16);
+    }
+    constexpr uint32_t kABlock = (MODE == kUp ? 128 : 16) * kFp8Block;  // block 1 (its swizzle is block 0's)
+    // the wave's scales of 64 blocks, one per lane
+    const int blk = (MODE == kUp ? n0 : n0 + cg * 64) / kFp8Block;
+    const int64_t s_at = ((int64_t)e * n_blk + (blk < n_blk ? blk : n_blk - 1)) * KT;
+    float swv[2] = {0.f, 0.f};
+    auto load_sw = [&](int kt) {
+      const int k = kt + lane < KT ? kt + lane : KT - 1;
+      swv[0] = m0.s[s_at + k];
+      if constexpr (MODE == kUp) swv[1] = m1.s[s_at + k];
     };
-    const int tr0 = half * NB * 32 + t;
-    uint32_t b_off[4];
+    // The compiler waits for the scales here; at their use, in the loop, its wait
+    // would be one for every direct load in flight, which it does not count (that took
+    // 149 + 74 us where this takes 132 + 66: 5280 rows of 128 experts).
+    auto pin_sw = [&] { asm volatile("" : "+v"(swv[0]), "+v"(swv[1])); };
+    load_sw(0);
+
+    tm_f32x16 acc[2][2];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) b_off[c] = (uint32_t)(Cfg::kW + tr0 * kFp8Block + ((2 * c + h) ^ x_swz(tr0)) * 16);
-    pin_sw();
-    for (int kt = 0; kt < S && kt < KT; ++kt) issue(kt, (uint32_t)(kt * Cfg::kStage));
-    uint32_t slot = 0, prev = (S - 1) * Cfg::kStage;
-    for (int kt = 0; kt < KT; ++kt) {
-      const int left = KT - 1 - kt;
-      wait_stages<Cfg::kDma, S - 2>(left < S - 2 ? left : S - 2);
-      barrier();  // stage kt landed, in every wave; every wave has read stage kt - 1
-      if (kt > 0 && kt - 1 + S < KT) issue(kt - 1 + S, prev);
-      const char *const sp = lds + slot;
-      const float sw0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(swv[0]), kt & 63));
-      const float sw1 = MODE == kUp ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(swv[1]), kt & 63)) : sw0;
-      uint4 af[2][WIDE ? 8 : 4];
+    for (int a = 0; a < 2; ++a)
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int q = 0; q < 2; ++q) acc[a][q] = tm_f32x16{};
+
+    auto run = [&](auto nb_c) {
+      constexpr int NB = decltype(nb_c)::value;
+      using Cfg = TileCfg<NB>;
+      constexpr int S = Cfg::kSlots;
+      auto row_of = [&](int tr) {  // a row past the tile: its last one again, results dropped
+        int gr = r0 + tr;
+        gr = gr < r_end ? gr : r_end - 1;
+        return MODE == kUp && ts.row_token != nullptr ? (int64_t)ts.row_token[gr] : (int64_t)gr;
+      };
+      const uint8_t *x_src[NB];
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const uint4 r = *reinterpret_cast<const uint4 *>(sp + a_off[c] + a * kABlock);
-          if constexpr (WIDE) {
-            af[a][2 * c] = tm_fp8_to_bf16x8(r.x, r.y);
-            af[a][2 * c + 1] = tm_fp8_to_bf16x8(r.z, r.w);
-          } else {
-            af[a][c] = r;
-          }
-        }
+      for (int j = 0; j < NB; ++j) {
+        const int tr = (wave * NB + j) * 8 + (lane >> 3);
+        x_src[j] = x + row_of(tr) * ld_x + ((lane & 7) ^ x_swz(tr)) * 16;
+      }
+      const float *const s_src = xs + row_of((wave % NB) * 64 + lane) * ld_xs;
+      const uint32_t s_dst = (uint32_t)(Cfg::kW + Cfg::kX + (wave % NB) * 256);
+      auto issue = [&](int kt, uint32_t slot) {
 #pragma unroll
-      for (int q = 0; q < NB; ++q) {
-        const float sx = *reinterpret_cast<const float *>(sp + Cfg::kW + Cfg::kX + (tr0 + 32 * q) * 4);
-        tm_f32x16 p[2] = {};
-        if constexpr (WIDE) {
+        for (int j = 0; j < 4; ++j)
+          tm_dma16_buf_so(w_rs, w_off[j], (uint32_t)kt * kFp8Block, lds0 + slot + (uint32_t)(wave * 4 + j) * 1024u);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint4 r = *reinterpret_cast<const uint4 *>(sp + b_off[c] + q * 32 * kFp8Block);
-            const float s = MODE == kUp ? sx : 1.f;
-            const uint4 b[2] = {tm_fp8_to_bf16x8(r.x, r.y, s), tm_fp8_to_bf16x8(r.z, r.w, s)};
+        for (int j = 0; j < NB; ++j)
+          tm_dma16_s(x_src[j] + (int64_t)kt * kFp8Block, lds0 + slot + (uint32_t)(Cfg::kW + (wave * NB + j) * 1024));
+        tm_dma4_s(s_src + kt, lds0 + slot + s_dst);
+      };
+      const int tr0 = half * NB * 32 + t;
+      uint32_t b_off[4];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+      for (int c = 0; c < 4; ++c) b_off[c] = (uint32_t)(Cfg::kW + tr0 * kFp8Block + ((2 * c + h) ^ x_swz(tr0)) * 16);
+      pin_sw();
+      for (int kt = 0; kt < S && kt < KT; ++kt) issue(kt, (uint32_t)(kt * Cfg::kStage));
+      uint32_t slot = 0, prev = (S - 1) * Cfg::kStage;
+      for (int kt = 0; kt < KT; ++kt) {
+        const int left = KT - 1 - kt;
+        wait_stages<Cfg::kDma, S - 2>(left < S - 2 ? left : S - 2);
+        barrier();  // stage kt landed, in every wave; every wave has read stage kt - 1
+        if (kt > 0 && kt - 1 + S < KT) issue(kt - 1 + S, prev);
+        const char *const sp = lds + slot;
+        const float sw0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(swv[0]), kt & 63));
+        const float sw1 = MODE == kUp ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(swv[1]), kt & 63)) : sw0;
+        uint4 af[2][WIDE ? 8 : 4];
 #pragma unroll
-              for (int a = 0; a < 2; ++a) p[a] = tm_mfma32x32x16<TM_DT_BF16>(af[a][2 * c + u], b[u], p[a]);
-          }
-        } else {
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int c = 0; c < 4; c += 2) {
-            const uint4 b[2] = {*reinterpret_cast<const uint4 *>(sp + b_off[c] + q * 32 * kFp8Block),
-                                *reinterpret_cast<const uint4 *>(sp + b_off[c + 1] + q * 32 * kFp8Block)};
-#pragma unroll
-            for (int a = 0; a < 2; ++a) {
-              const uint4 w2[2] = {af[a][c], af[a][c + 1]};
-              p[a] = tm_mfma32x32x64_fp8(w2, b, p[a]);
+          for (int a = 0; a < 2; ++a) {
+            const uint4 r = *reinterpret_cast<const uint4 *>(sp + a_off[c] + a * kABlock);
+            if constexpr (WIDE) {
+              af[a][2 * c] = tm_fp8_to_bf16x8(r.x, r.y);
+              af[a][2 * c + 1] = tm_fp8_to_bf16x8(r.z, r.w);
+            } else {
+              af[a][c] = r;
             }
           }
-        }
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const float s = MODE == kUp ? (a == 1 ? sw1 : sw0) : sw0 * sx;
+        for (int q = 0; q < NB; ++q) {
+          const float sx = *reinterpret_cast<const float *>(sp + Cfg::kW + Cfg::kX + (tr0 + 32 * q) * 4);
+          tm_f32x16 p[2] = {};
+          if constexpr (WIDE) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[a][q][i] = fmaf(p[a][i], s, acc[a][q][i]);
+            for (int c = 0; c < 4; ++c) {
+              const uint4 r = *reinterpret_cast<const uint4 *>(sp + b_off[c] + q * 32 * kFp8Block);
+              const float s = MODE == kUp ? sx : 1.f;
+              const uint4 b[2] = {tm_fp8_to_bf16x8(r.x, r.y, s), tm_fp8_to_bf16x8(r.z, r.w, s)};
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int a = 0; a < 2; ++a) p[a] = tm_mfma32x32x16<TM_DT_BF16>(af[a][2 * c + u], b[u], p[a]);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+              const uint4 b[2] = {*reinterpret_cast<const uint4 *>(sp + b_off[c] + q * 32 * kFp8Block),
+                                  *reinterpret_cast<const uint4 *>(sp + b_off[c + 1] + q * 32 * kFp8Block)};
+#pragma unroll
+              for (int a = 0; a < 2; ++a) {
+                const uint4 w2[2] = {af[a][c], af[a][c + 1]};
+                p[a] = tm_mfma32x32x64_fp8(w2, b, p[a]);
+              }
+            }
+          }
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            const float s = MODE == kUp ? (a == 1 ? sw1 : sw0) : sw0 * sx;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[a][q][i] = fmaf(p[a][i], s, acc[a][q][i]);
+          }
         }
+        if (((kt + 1) & 63) == 0 && kt + 1 < KT) {
+          load_sw(kt + 1);
+          pin_sw();
+        }
+        prev = slot;
+        slot = slot == (S - 1) * Cfg::kStage ? 0u : slot + Cfg::kStage;
       }
-      if (((kt + 1) & 63) == 0 && kt + 1 < KT) {
-        load_sw(kt + 1);
-        pin_sw();
-      }
-      prev = slot;
-      slot = slot == (S - 1) * Cfg::kStage ? 0u : slot + Cfg::kStage;
-    }
-  };
-  const int used = rows > 64 ? 2 : 1;  // row blocks per half
-  if (used == 1) run(std::integral_constant<int, 1>{});
-  else run(std::integral_constant<int, 2>{});
-  const int first = half * used * 32 + t;  // this lane's first row in the tile
+    };
+    const int used = rows > 64 ? 2 : 1;  // row blocks per half
+    if (used == 1) run(std::integral_constant<int, 1>{});
+    else run(std::integral_constant<int, 2>{});
+    const int first = half * used * 32 + t;  // this lane's first row in the tile
 
-  if constexpr (MODE == kUp) {
-    // lane: row t of each block, columns n0 + 32 cg + 16 h + i; s_top: [128 rows][4 groups]
-    const int c = n0 + cg * 32 + 16 * h;
+    if constexpr (MODE == kUp) {
+      // lane: row t of each block, columns n0 + 32 cg + 16 h + i; s_top: [128 rows][4 groups]
+      const int c = n0 + cg * 32 + 16 * h;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      if (q >= used) continue;  // uniform
-      uint32_t m = 0;
+      for (int q = 0; q < 2; ++q) {
+        if (q >= used) continue;  // uniform
+        uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float gv = acc[0][q][i];
-        acc[0][q][i] = gv * __builtin_amdgcn_rcpf(1.f + __expf(-gv)) * acc[1][q][i];
-        m = tm_fp8_amax(m, acc[0][q][i]);
+        for (int i = 0; i < 16; ++i) {
+          const float gv = acc[0][q][i];
+          acc[0][q][i] = gv * __builtin_amdgcn_rcpf(1.f + __expf(-gv)) * acc[1][q][i];
+          m = tm_fp8_amax(m, acc[0][q][i]);
+        }
+        m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+        if (h == 0) s_top[(first + 32 * q) * 4 + cg] = m;
       }
-      m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-      if (h == 0) s_top[(first + 32 * q) * 4 + cg] = m;
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int tr = first + 32 * q;
+        if (q >= used || tr >= rows) continue;
+        const uint4 m4 = *reinterpret_cast<const uint4 *>(&s_top[tr * 4]);
+        float inv;
+        const float s = tm_fp8_scale(max(max(m4.x, m4.y), max(m4.z, m4.w)), inv);
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = tm_fp8_quot(acc[0][q][i], inv);
+        *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(dst.y) + (int64_t)(r0 + tr) * dst.ld + c) =
+            make_uint4(tm_fp8_pack4(v[0], v[1], v[2], v[3]), tm_fp8_pack4(v[4], v[5], v[6], v[7]),
+                       tm_fp8_pack4(v[8], v[9], v[10], v[11]), tm_fp8_pack4(v[12], v[13], v[14], v[15]));
+        if (h == 0 && cg == 0) fs[(int64_t)(r0 + tr) * n_blk + n0 / kFp8Block] = s;
+      }
+    } else {
+      // Through LDS, so that a row's columns are added to and written as whole
+      // lines: every lane storing its own row's columns, 8 bytes at a time, took
+      // 34 us of a 4096 x 2048 product's 87.
+      tm_wait_vm_lgkm0_mem<0>();
+      barrier();  // the ring is free
+      float *const tile = reinterpret_cast<float *>(ring);  // [128 rows][kTileCols + 4]
+      constexpr int kLd = kTileCols + 4;
+      static_assert(kTileBM * kLd * 4 <= kTileRing, "output tile");
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (q >= used) continue;  // uniform
+        float *const p = tile + (first + 32 * q) * kLd + cg * 64 + 32 * h;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          *reinterpret_cast<float4 *>(p + 4 * u) =
+              make_float4(acc[u >> 2][q][4 * (u & 3)], acc[u >> 2][q][4 * (u & 3) + 1], acc[u >> 2][q][4 * (u & 3) + 2],
+                          acc[u >> 2][q][4 * (u & 3) + 3]);
+      }
+      __syncthreads();
+      write_tile<DT, kTileCols, kTileThreads>(tile, rows, r0, n0, n_out, dst, ts.row_out, vec_out);
     }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int tr = first + 32 * q;
-      if (q >= used || tr >= rows) continue;
-      const uint4 m4 = *reinterpret_cast<const uint4 *>(&s_top[tr * 4]);
-      float inv;
-      const float s = tm_fp8_scale(max(max(m4.x, m4.y), max(m4.z, m4.w)), inv);
-      float v[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = tm_fp8_quot(acc[0][q][i], inv);
-      *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(dst.y) + (int64_t)(r0 + tr) * dst.ld + c) =
-          make_uint4(tm_fp8_pack4(v[0], v[1], v[2], v[3]), tm_fp8_pack4(v[4], v[5], v[6], v[7]),
-                     tm_fp8_pack4(v[8], v[9], v[10], v[11]), tm_fp8_pack4(v[12], v[13], v[14], v[15]));
-      if (h == 0 && cg == 0) fs[(int64_t)(r0 + tr) * n_blk + n0 / kFp8Block] = s;
-    }
-  } else {
-    // Through LDS, so that a row's columns are added to and written as whole
-    // lines: every lane storing its own row's columns, 8 bytes at a time, took
-    // 34 us of a 4096 x 2048 product's 87.
-    tm_wait_vm_lgkm0_mem<0>();
-    barrier();  // the ring is free
-    float *const tile = reinterpret_cast<float *>(ring);  // [128 rows][kTileCols + 4]
-    constexpr int kLd = kTileCols + 4;
-    static_assert(kTileBM * kLd * 4 <= kTileRing, "output tile");
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      if (q >= used) continue;  // uniform
-      float *const p = tile + (first + 32 * q) * kLd + cg * 64 + 32 * h;
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        *reinterpret_cast<float4 *>(p + 4 * u) =
-            make_float4(acc[u >> 2][q][4 * (u & 3)], acc[u >> 2][q][4 * (u & 3) + 1], acc[u >> 2][q][4 * (u & 3) + 2],
-                        acc[u >> 2][q][4 * (u & 3) + 3]);
-    }
-    __syncthreads();
-    write_tile<DT, kTileCols, kTileThreads>(tile, rows, r0, n0, n_out, dst, ts.row_out, vec_out);
-  }
-  __syncthreads();  // the next item's loads come after this one's reads of LDS
+    __syncthreads();  // the next item's loads come after this one's reads of LDS
   }
 }
 
@@ -1035,21 +1036,21 @@ int mlp_launch(const char *name, const tm_fp8_experts *ex, const void *x, int64_
       w2{static_cast<const uint8_t *>(ex->w2), ex->s2};
   const Fp8Dst mid{base + ws.f, inter, 0, 0, nullptr, 0};
   if (ts == nullptr) {
-    const int st = stream_launch<DT, DT, kUp, 1, 4>(name, Fp8Src{x, ld_x, h, nullptr, 0}, *rows, w1, w3, inter, h / kFp8Block,
-                                              mid, s);
+    const int st = stream_launch<DT, DT, kUp, 1, 4>(name, Fp8Src{x, ld_x, h, nullptr, 0}, *rows, w1, w3, inter,
+                                                    h / kFp8Block, mid, s);
     if (st != TM_OK) return st;
-    return stream_launch<DT, TM_DT_F32, kOut, 4, 2>(name, Fp8Src{base + ws.f, inter, inter, nullptr, 0}, *rows, w2, w2, h,
-                                              inter / kFp8Block, dst, s);
+    return stream_launch<DT, TM_DT_F32, kOut, 4, 2>(name, Fp8Src{base + ws.f, inter, inter, nullptr, 0}, *rows, w2,
+                                                    w2, h, inter / kFp8Block, dst, s);
   }
   float *const xs = reinterpret_cast<float *>(base + ws.xs);
   int st = tm_internal_fp8_rows(DT, x, n, h, ld_x, base + ws.x, h, xs, h / kFp8Block, s);
   if (st != TM_OK) return st;
   float *const fs = reinterpret_cast<float *>(base + ws.fs);
-  st = tile_launch<DT, kUp, true>(name, base + ws.x, h, xs, h / kFp8Block, w1, w3, inter, h / kFp8Block, *ts,
-                                     mid, fs, s);
+  st = tile_launch<DT, kUp, true>(name, base + ws.x, h, xs, h / kFp8Block, w1, w3, inter, h / kFp8Block, *ts, mid, fs,
+                                  s);
   if (st != TM_OK) return st;
-  return tile_launch<DT, kOut, false>(name, base + ws.f, inter, fs, inter / kFp8Block, w2, w2, h, inter / kFp8Block,
-                                         *ts, dst, nullptr, s);
+  return tile_launch<DT, kOut, false>(name, base + ws.f, inter, fs, inter / kFp8Block, w2, w2, h, inter / kFp8Block, *ts,
+                                      dst, nullptr, s);
 }
 
 }  // namespace

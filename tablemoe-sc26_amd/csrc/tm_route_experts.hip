@@ -3,8 +3,8 @@
 //
 // 16 lanes own a token, expert e in lane e % 16; a wave holds four tokens.  The
 // keys that decide are those of the definition, in 64 bits: two experts whose
-// scores differ in the eighth digit come out in its order, not in that of
-// somebody's roundings.  They are computed in 32 bits first, whose error is
+// scores differ in the eighth digit come out in its order, not in that of their
+// roundings.  They are computed in 32 bits first, whose error is
 // bounded (kTol); the top_k rounds go on until the next key is far from the
 // last, and where two neighbours are near the candidates (a lane each) are put
 // in the order of their 64-bit keys, whose scores the weights need anyway.  Where
