@@ -3,6 +3,12 @@
 // Rows: 16 lanes own one block of one row, 8 columns each, loaded as 16-byte
 // pieces; the block's maximum is three DPP exchanges and a row_mirror away and
 // the values stay in registers until they are scaled, so a row is read once.
+// Weights: a workgroup holds a block of 128 x 128 in registers between its
+// maximum and its scaling.
+//
+// Bound by HBM: 64 matrices of 1536 x 2560 in bf16 (755 MB) take 138 us, 5.5 TB/s (150
+// when each load waited for the one before); 4099 rows of 2048 (25 MB) 7.4 us, of which
+// a launch is a third.
 #include "tm_fp8_dev.h"
 #include "tm_fp8.h"
 
