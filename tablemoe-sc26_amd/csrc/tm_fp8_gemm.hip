@@ -906,10 +906,18 @@ int64_t round_up(int64_t v, int64_t m) { return tm_cdiv(v, m) * m; }
 // ---------------------------------------------------------------------------
 namespace {
 
-// Rows up to which a linear layer streams its weights (stream_kernel): 2048 -> 4096
-// in bf16 takes it 8.3 us for 8 rows and 13 for 16, mid_kernel with the rows'
-// quantisation 10.7 and 10.9; 4096 -> 2048 10.5 and 17 against 16.6 and 16.6.
-constexpr int64_t kLinearStreamRows = 12;
+// Rows up to which a linear layer streams its weights (stream_kernel), by what the
+// row quantisation in every workgroup costs it against tiles, whose own is a launch.
+// 2048 -> 4096 in bf16: 8 rows 8.3 us (as 64 x 64 tiles 10.7), 16 rows 13 (10.9);
+// 4096 -> 2048: 10.5 (16.6) and 17 (16.6).  K of more than 4096 is read again for
+// each chunk of rows: 8192 -> 2048, 4 rows, two chunks: 18 (28), 8 rows 31 (28).
+// Where 64 x 64 tiles fill half of the CUs they win earlier: 2048 -> 16384, 4 rows
+// 10.3 (11.8), 8 rows 13.8 (11.9); 8192 -> 16384, 2 rows 32 (29).
+int64_t linear_stream_rows(int64_t kb, int64_t n_out) {
+  const int64_t chunk = stream_chunk((int)kb, 16);
+  if (n_out > 128 * kMidTile) return chunk > 2 ? chunk / 2 : 1;
+  return kb <= 32 ? 12 : 2 * chunk;
+}
 // 64 x 64 tiles up to which it takes mid_kernel, one per CU: 512 rows, 4096 -> 2048
 // (256 tiles) take 22 us, in the large tiles 31; 2048 -> 4096 (512) 24 and 20.
 constexpr int64_t kMidTiles = 256;
@@ -943,7 +951,7 @@ extern "C" int tm_fp8_linear(int32_t dtype, const void *x, const float *x_scale,
   TM_REQUIRE(workspace != nullptr && workspace_bytes >= need && tm_aligned16(workspace), TM_EWORKSPACE,
              "%s: workspace %zu bytes < %zu", name, workspace_bytes, need);
   hipStream_t s = tm_hip_stream(stream);
-  const bool tiles = n_rows > kLinearStreamRows;
+  const bool tiles = n_rows > linear_stream_rows(kb, n_out);
   Fp8Src src{x, ld_x, k, x_scale, ld_xs};
   float *const ws_scale = reinterpret_cast<float *>(static_cast<char *>(workspace) + need - round_up(n_rows * kb * 4, 256));
   if (!x_scale && (tiles || !aligned(x, ld_x * (dtype == TM_DT_F32 ? 4 : 2)))) {

@@ -200,7 +200,7 @@ def test_linear_strides_dims_and_out(hip_device):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("m,k,n", [
-    (12, 512, 136), (13, 8320, 70), (13, 8192, 64), (70, 128, 1), (64, 8448, 1023),      # few rows; 64 x 64 tiles
+    (12, 512, 136), (2, 16384, 40), (4, 8320, 33), (5, 8320, 33), (7, 6144, 8300), (13, 8320, 70), (13, 8192, 64), (70, 128, 1), (64, 8448, 1023),      # few rows; 64 x 64 tiles
     (512, 300, 2048), (513, 300, 2050), (700, 384, 2816), (2100, 8320, 1025), (1090, 256, 4097),  # the large tiles
 ])
 def test_linear_tilings(hip_device, dtype, m, k, n):
