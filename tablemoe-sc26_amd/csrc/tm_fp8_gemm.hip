@@ -996,11 +996,17 @@ int check_experts(const char *name, const tm_fp8_experts *ex, int32_t dtype) {
   return TM_OK;
 }
 
-// The plan of a call of up to `rows` rows on n_experts experts: few rows per
-// expert stream the weights (stream_kernel; no launch groups the rows or
-// quantises them), more go through tiles.
-bool stream_plan(int64_t rows, int32_t n_experts) {
-  return rows <= kMaxSlots && rows <= 32 * (int64_t)n_experts;
+// Rows of a call up to which the weights are streamed (stream_kernel; no launch
+// groups the rows or quantises them), more go through tiles: about two rows per
+// expert, and more where there are few experts to fill the CUs; fewer where K is
+// read again for each chunk of rows.  Both, in us: 128 experts (2048 x 768) of 2 rows
+// 109 | 127, of 4 rows 145 | 134; 64 (2560 x 1536) of 1.5 rows 153 | 141, of 3 207 |
+// 158; 16 (4096 x 1024) of 2 rows 46 | 58, of 4 61 | 59; one (2560 x 1536) of 16 rows
+// 31 | 38, of 24 40 | 39; 8 (7168 x 2048) of 2 rows 91 | 100, of 4 143 | 101; one of 8
+// rows 57 | 77, of 12 82 | 77.
+int64_t stream_rows(const tm_fp8_experts *ex) {
+  const int64_t most = 2 * (int64_t)ex->n_experts + (ex->hidden <= 4096 && ex->inter <= 4096 ? 14 : 6);
+  return most < kMaxSlots ? most : kMaxSlots;
 }
 
 // Workspace: f (stream: fp32 rows; tiles: 8-bit rows and their scales), the
@@ -1018,7 +1024,7 @@ ExpertsWs experts_ws(int64_t n, int32_t top_k, const tm_fp8_experts *ex, bool gr
     return here;
   };
   const int64_t rows = n * top_k;
-  const bool stream = stream_plan(rows, ex->n_experts);
+  const bool stream = rows <= stream_rows(ex);
   if (stream) take(rows * ex->inter * 4);  // f, at the start
   const size_t stream_bytes = at;
   at = 0;
@@ -1035,9 +1041,7 @@ ExpertsWs experts_ws(int64_t n, int32_t top_k, const tm_fp8_experts *ex, bool gr
   }
   // never less for more rows: the largest call that streams needs this much
   if (!stream) {
-    int64_t most = 32 * (int64_t)ex->n_experts;
-    most = most < kMaxSlots ? most : kMaxSlots;
-    const size_t largest = (size_t)round_up(most * ex->inter * 4, 256);
+    const size_t largest = (size_t)round_up(stream_rows(ex) * ex->inter * 4, 256);
     at = at > largest ? at : largest;
   } else {
     at = at > stream_bytes ? at : stream_bytes;
@@ -1099,7 +1103,7 @@ extern "C" int tm_fp8_grouped_swiglu(const tm_fp8_experts *experts, int32_t dtyp
   char *const base = static_cast<char *>(workspace);
   hipStream_t s = tm_hip_stream(stream);
   const int64_t max_rows = n_tokens * top_k;
-  const bool stream_w = stream_plan(max_rows, experts->n_experts);
+  const bool stream_w = max_rows <= stream_rows(experts);
   Fp8Rows rows{n_tokens};
   Fp8Tiles ts{};
   if (stream_w) {
@@ -1153,7 +1157,7 @@ extern "C" int tm_fp8_expert_swiglu(const tm_fp8_experts *experts, int32_t dtype
   const Fp8Rows rows{n_rows};
   Fp8Tiles ts{};
   ts.rows = (int32_t)n_rows;
-  const bool stream_w = stream_plan(n_rows, 1);
+  const bool stream_w = n_rows <= stream_rows(experts);
   const Fp8Dst dst{out, ld_out, 0, 0, addend, ld_add};
   const ExpertsWs ws = experts_ws(n_rows, 1, experts, false);
   char *const base = static_cast<char *>(workspace);
