@@ -95,8 +95,8 @@ __device__ __forceinline__ void store4(void *y, int64_t at, const float (&v)[4],
 // instructions and adds the waves' sums in wave order through LDS.  No launch
 // before it groups the rows or quantises them: a call is its two products.
 //
-// Bound by HBM: 256 slots of 110 experts (2048 x 768) stream 352 MB in 65 us (up,
-// 5.4 TB/s) and 176 MB in 37 (down, 4.7); one token's 8 experts take 10 + 6, a
+// Bound by HBM: 256 slots of 110 experts (2048 x 768) stream 352 MB in 64 us (up,
+// 5.5 TB/s) and 176 MB in 35 (down, 5.0); one token's 8 experts take 10 + 6, a
 // chain of latencies (slots, rows, weights, sums).  Up: quantising in the
 // operand's layout, where every lane does 32 columns of its row whether it is
 // live or not, 140; 48 KiB of LDS rows 81; three waves per SIMD instead of four
@@ -115,7 +115,7 @@ __host__ __device__ inline int stream_chunk(int KT, int64_t most) {
 }
 
 template <int DT, int DTX, int MODE, int NA, int KPW>
-__global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(MODE == kUp ? 4 : 1)))
+__global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(MODE != kUp ? 1 : KPW > 4 ? 3 : 4)))
 void stream_kernel(Fp8Src src, Fp8Rows rows, Fp8Mat m0, Fp8Mat m1, int n_out, int KT, int n_groups, int chunk,
                    Fp8Dst dst, bool vec_out) {
   constexpr int NM = MODE == kUp ? 2 : 1;
@@ -1058,11 +1058,21 @@ int mlp_launch(const char *name, const tm_fp8_experts *ex, const void *x, int64_
       w2{static_cast<const uint8_t *>(ex->w2), ex->s2};
   const Fp8Dst mid{base + ws.f, inter, 0, 0, nullptr, 0};
   if (ts == nullptr) {
-    const int st = stream_launch<DT, DT, kUp, 1, 4>(name, Fp8Src{x, ld_x, h, nullptr, 0}, *rows, w1, w3, inter,
-                                                    h / kFp8Block, mid, s);
+    // Blocks per wave: what makes whole sets of four waves, one per SIMD.  Up: five
+    // where four do not (64 experts of 2560 x 1536, 38 of them with rows: 75 us against 89;
+    // not where K takes more than eight waves: 7168, 67 against 59).  Down: two where
+    // that does, or three (the same 38: 38 us against 51, 109 of 2048 x 768: 43 against 45;
+    // but K of 1024: 14.4 against 13.0).
+    const int KT = h / kFp8Block, KT2 = inter / kFp8Block;
+    const Fp8Src src{x, ld_x, h, nullptr, 0}, mid_src{base + ws.f, inter, inter, nullptr, 0};
+    const int w5 = (KT + 4) / 5;
+    const int st = (KT + 3) / 4 % 4 != 0 && w5 % 4 == 0 && w5 <= kMaxWaves
+                       ? stream_launch<DT, DT, kUp, 1, 5>(name, src, *rows, w1, w3, inter, KT, mid, s)
+                       : stream_launch<DT, DT, kUp, 1, 4>(name, src, *rows, w1, w3, inter, KT, mid, s);
     if (st != TM_OK) return st;
-    return stream_launch<DT, TM_DT_F32, kOut, 4, 2>(name, Fp8Src{base + ws.f, inter, inter, nullptr, 0}, *rows, w2,
-                                                    w2, h, inter / kFp8Block, dst, s);
+    return (KT2 + 1) / 2 % 4 == 0
+               ? stream_launch<DT, TM_DT_F32, kOut, 4, 2>(name, mid_src, *rows, w2, w2, h, KT2, dst, s)
+               : stream_launch<DT, TM_DT_F32, kOut, 4, 3>(name, mid_src, *rows, w2, w2, h, KT2, dst, s);
   }
   float *const xs = reinterpret_cast<float *>(base + ws.xs);
   int st = tm_internal_fp8_rows(DT, x, n, h, ld_x, base + ws.x, h, xs, h / kFp8Block, s);
