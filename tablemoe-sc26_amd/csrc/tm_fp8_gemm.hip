@@ -91,9 +91,10 @@ __device__ __forceinline__ void store4(void *y, int64_t at, const float (&v)[4],
 // Wave w holds blocks [w KPW, (w + 1) KPW) of their 128-column blocks in
 // registers, loaded at once (K of more than S KPW: in passes, loaded again for
 // each chunk of rows).  The workgroup quantises its rows, up to 16 at a time,
-// into LDS (16 lanes own a block of a row), multiplies them on the bf16
-// instructions and adds the waves' sums in wave order through LDS.  No launch
-// before it groups the rows or quantises them: a call is its two products.
+// into LDS (16 lanes own a block of a row), multiplies them (16-bit outputs on the
+// 8-bit instructions, else on the bf16 ones) and adds the waves' sums in wave order
+// through LDS.  No launch before it groups the rows or quantises them: a call is
+// its two products.
 //
 // Bound by HBM: 256 slots of 110 experts (2048 x 768) stream 352 MB in 64 us (up,
 // 5.5 TB/s) and 176 MB in 35 (down, 5.0); one token's 8 experts take 10 + 6, a
