@@ -13,6 +13,11 @@
 // makes a wave choose in 64 bits from the start (select64).  Without a bias the
 // logits order the experts, exactly.
 //
+// A softmax's sum has fp32 terms (within two roundings: enough for the weights) until
+// a bias meets a choice in 64 bits: there it scales the scores against the bias, so
+// the sum is taken again of 64-bit terms (sum64; with the fp32 ones two keys 1e-9
+// apart changed places).
+//
 // Bound by latency: each round is a maximum over the lane's keys, four DPP
 // exchanges, the lowest lane that holds it and its key closed, one after the
 // other; where at most half of the experts are in the groups that stay, over
@@ -153,6 +158,19 @@ __device__ __forceinline__ bool available(float l, float b) {  // (false for NaN
   return (l >= -3.402823466e38f) & (b >= -3.402823466e38f);
 }
 
+// A softmax's sum of 64-bit terms, for the choices that are made in 64 bits.
+template <int DT>
+__device__ __forceinline__ double sum64(const typename Elem<DT>::T *lr, const RouteArgs &a, int sub, float mx) {
+  double sum = 0;
+#pragma unroll 1
+  for (int e = sub; e < a.n_experts; e += 16) {
+    const float l = Elem<DT>::to_f(lr[e]);
+    if (available(l, a.bias != nullptr ? a.bias[e] : 0.f))
+      sum += exp((double)fminf(l, 3.402823466e38f) - (double)mx);
+  }
+  return row16_sum(sum);
+}
+
 // The choice in 64 bits: compact, for the few waves that need it.
 template <int DT>
 __device__ __forceinline__ void select64(const typename Elem<DT>::T *lr, const RouteArgs &a, int sub, float mx,
@@ -270,6 +288,14 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
       v[j] = l[j] == l[j] ? v[j] : ninf;
     }
   }
+  // The sum for choices in 64 bits: `sum` where it is a common factor of all keys.
+  // Weights keep `sum`, so they do not hang on the other tokens of the wave.
+  double sum_c = sum;
+  bool exact = SIGMOID || !scored;
+  auto need_sum64 = [&] {
+    if (!exact) sum_c = sum64<DT>(lr, a, sub, mx);
+    exact = true;
+  };
   uint64_t kept = ~0ull;
   bool compact = false;
   float *const gmin = vals + 4 * per_tok;
@@ -287,6 +313,7 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
       kept = kept_groups<float, true>(a, sub, vals, gval, gmin, unsure);
       if (__ballot(unsure) != 0) {
         // again in 64 bits, of the experts that can be among what a group is worth
+        need_sum64();
         Mask<VPL> maybe = 0;
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
@@ -302,7 +329,7 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
           const int e = (int)__builtin_ctzll((uint64_t)maybe) * 16 + sub;
           maybe &= maybe - 1;
           const double s64 = score64(fminf(Elem<DT>::to_f(lr[e]), big), SIGMOID ? TM_ROUTE_SIGMOID : TM_ROUTE_SOFTMAX,
-                                     mx, sum);
+                                     mx, sum_c);
           vals64[e + group_of(e, a)] = s64 + (scored ? (double)a.bias[e] : 0.0);
         }
         kept = kept_groups<double, false>(a, sub, vals64, vals64 + a.n_experts + a.n_groups, nullptr, unsure);
@@ -402,7 +429,8 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
   int n_cand = r;
   if (__ballot(unsure) != 0) {  // uniform
     __syncthreads();
-    select64<DT>(lr, a, sub, mx, sum, lds + tok * per_tok, cand);
+    need_sum64();
+    select64<DT>(lr, a, sub, mx, sum_c, lds + tok * per_tok, cand);
     n_cand = a.top_k;
     close = false;
   }
@@ -418,11 +446,13 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
       w[u] = score64(fminf(x, big), SIGMOID ? TM_ROUTE_SIGMOID : TM_ROUTE_SOFTMAX, mx, sum);
   }
   if (__ballot(close) != 0) {  // uniform: the candidates in the order of their 64-bit keys
+    need_sum64();
     double k64[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const float x = Elem<DT>::to_f(lr[cand[u]]), b = a.bias[cand[u]];
-      k64[u] = available(x, b) ? w[u] + (double)b : -__builtin_huge_val();
+      const double s64 = SIGMOID ? w[u] : score64(fminf(x, big), TM_ROUTE_SOFTMAX, mx, sum_c);
+      k64[u] = available(x, b) ? s64 + (double)b : -__builtin_huge_val();
       place[u] = 16 * u + sub < n_cand ? 0 : 32;
     }
     for (int o = 0; o < n_cand; ++o) {

@@ -1,7 +1,8 @@
 """tm_route_experts / table_moe.ops.route_experts against the definition in 64
-bits: ids equal, weights within a few fp32 roundings (the choice itself is made
-on 64-bit keys; a weight is exp, a sum of at most 1024 terms and two divisions,
-each within 2^-52, rounded once: 2^-24 relative, tested at 2^-22)."""
+bits: ids equal (the choice is that of 64-bit keys), weights within a few fp32
+roundings (a softmax weight is a 64-bit exp over a 64-bit sum of fp32 terms, each
+an expf of one ulp, 2^-23 at most, and a product rounded to 2^-24, then rounded
+once itself: 2^-22 relative)."""
 
 import numpy as np
 import pytest
@@ -202,3 +203,38 @@ def test_refusals(hip_device):
         route_experts(torch.zeros(2, 1025, device=hip_device), 4)
     with pytest.raises(RuntimeError):
         route_experts(x.cpu(), 4)
+
+
+def _near_ties(seed, e, scoring, rows=5):
+    """Logits and a bias that makes every key of row 0 equal up to the bias's own
+    rounding to fp32 (gaps of 1e-11 to 1e-8); row r: row 0's logits moved by r / 2,
+    whose softmax scores are row 0's up to a rounding."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(1, e, generator=g)
+    s = torch.softmax(x[0].double(), 0) if scoring == "softmax" else torch.sigmoid(x[0].double())
+    bias = (0.75 - s).float()
+    return x + 0.5 * torch.arange(rows)[:, None], bias
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e,top_k,groups,keep,rule", [
+    (64, 16, 1, 1, "max"), (256, 8, 1, 1, "max"), (64, 32, 1, 1, "max"), (64, 6, 8, 4, "top2"), (256, 8, 8, 4, "top2"),
+    (256, 8, 8, 3, "max"), (72, 9, 3, 2, "top2"), (512, 16, 4, 2, "max"),
+])
+def test_near_ties_of_many_draws(hip_device, scoring, e, top_k, groups, keep, rule):
+    """The order of keys that only 64 bits tell apart, another bias in every call.  A
+    softmax score's sum of e terms is within e 2^-53 of its size on either side, and a
+    key of under 1 takes a few roundings of 2^-53 more: draws with two keys nearer
+    than that are left out."""
+    taken = 0
+    for seed in range(40):
+        x, bias = _near_ties(1000 * e + seed, e, scoring)
+        z = x.double()
+        score = torch.softmax(z, 1) if scoring == "softmax" else torch.sigmoid(z)
+        error = (8 + (e * float(score.max()) if scoring == "softmax" else 0)) * 2.0 ** -52
+        if float((score + bias.double()).sort(1).values.diff(dim=1).min()) < error:
+            continue
+        taken += 1
+        _check(x.to(hip_device), top_k, bias.to(hip_device), scoring=scoring, n_groups=groups, topk_groups=keep,
+               group_rule=rule)
+    assert taken >= 20
