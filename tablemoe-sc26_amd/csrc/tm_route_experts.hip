@@ -81,7 +81,8 @@ __device__ __forceinline__ K row16_max(K v) {
 // exp2, the sum's reciprocal and a product: of a score s = e^-d / sum, 2.5 d + 8
 // roundings of 2^-24, at most 5.5e-7 (d e^-d < 0.37); adding the bias, one of
 // the key.  Two keys are in the right order if they are further apart than
-// twice that, two sums of two keys if twice as far.
+// twice that.  A sum of two keys has both errors and its own rounding, by the size of
+// its terms, which may cancel: kTol / 2 for each term covers them.
 constexpr float kTol = 1.5e-6f;
 
 __device__ __forceinline__ double score64(float l, int scoring, float mx, double sum) {
@@ -97,10 +98,11 @@ __device__ __forceinline__ bool near(float hi, float lo, float tol) { return hi 
 
 // The groups that stay, from the values in LDS (padded by one per group), as a
 // mask in every lane of the token.  UNSURE: also whether a group that stays and
-// one that does not are too near to be told from each other in 32 bits, and in
-// gmin the least value that a group's own is made of.
+// one that does not are too near to be told from each other in 32 bits, in
+// gmin the least value that a group's own is made of and in gerr the bound on its
+// error (infinite where the value is out of fp32's range).
 template <typename K, bool UNSURE>
-__device__ __forceinline__ uint64_t kept_groups(const RouteArgs &a, int sub, const K *vals, K *gval, K *gmin,
+__device__ __forceinline__ uint64_t kept_groups(const RouteArgs &a, int sub, const K *vals, K *gval, K *gmin, K *gerr,
                                                 bool &unsure) {
   const K ninf = -(K)__builtin_huge_valf();
   const bool top2 = a.group_rule == TM_GROUP_TOP2;
@@ -122,13 +124,25 @@ __device__ __forceinline__ uint64_t kept_groups(const RouteArgs &a, int sub, con
       first = fmax(first, f2);
     }
     if (sub % share == 0) {
-      gval[g] = top2 && second > ninf ? first + second : first;
-      if constexpr (UNSURE) gmin[g] = top2 && second > ninf ? second : first;
+      const bool two = top2 && second > ninf;
+      K v = two ? first + second : first;
+      if constexpr (UNSURE) {
+        constexpr float kBig = 3.402823466e38f;
+        gmin[g] = two ? second : first;
+        K err = kTol / 2 * (fmaxf(1.f, fabsf(first)) + (two ? fmaxf(1.f, fabsf(second)) : 0.f));
+        if (first > ninf && !(fabsf(v) <= kBig)) {  // (an available group stays above the others)
+          v = v > 0 ? kBig : -kBig;
+          err = -ninf;
+        }
+        gerr[g] = err;
+      }
+      gval[g] = v;
     }
   }
   __syncthreads();
   uint64_t kept = 0;
-  float low = __builtin_huge_valf(), high = -low;  // of those that stay, of the others
+  // the least that one that stays can be worth, the most that another (available) one can
+  float low = __builtin_huge_valf(), high = -low;
   for (int g0 = 0; g0 < a.n_groups; g0 += 16) {
     const int g = g0 + sub;
     const bool in = g < a.n_groups;
@@ -140,8 +154,9 @@ __device__ __forceinline__ uint64_t kept_groups(const RouteArgs &a, int sub, con
     }
     const bool stays = ahead < a.topk_groups;
     if constexpr (UNSURE) {
-      low = (in & stays) ? fminf(low, mine) : low;
-      high = (in & !stays) ? fmaxf(high, mine) : high;
+      const K err = gerr[in ? g : 0];
+      low = (in & stays) ? fminf(low, mine - err) : low;
+      high = (in & !stays & (mine > ninf)) ? fmaxf(high, mine + err) : high;
     }
     const uint64_t all = __ballot(in & stays);
     kept |= ((all >> ((threadIdx.x & 63) & ~15)) & 0xffffull) << g0;
@@ -149,7 +164,7 @@ __device__ __forceinline__ uint64_t kept_groups(const RouteArgs &a, int sub, con
   if constexpr (UNSURE) {
     low = -row16_max(-low);
     high = row16_max(high);
-    unsure = high > (float)ninf && near(low, high, 2 * kTol);
+    unsure = high > (float)ninf && high >= low;
   }
   return kept;
 }
@@ -192,7 +207,7 @@ __device__ __forceinline__ void select64(const typename Elem<DT>::T *lr, const R
   }
   if (a.n_groups > 1) {
     bool none = false;
-    const uint64_t kept = kept_groups<double, false>(a, sub, keys, gval, nullptr, none);
+    const uint64_t kept = kept_groups<double, false>(a, sub, keys, gval, nullptr, nullptr, none);
     open = 0;
 #pragma unroll 1
     for (int e = sub, j = 0; e < a.n_experts; e += 16, ++j) {
@@ -298,8 +313,8 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
   };
   uint64_t kept = ~0ull;
   bool compact = false;
-  float *const gmin = vals + 4 * per_tok;
-  int *const glist = reinterpret_cast<int *>(gmin + a.n_groups);  // the groups that stay, ascending
+  float *const gmin = vals + 4 * per_tok, *const gerr = gmin + a.n_groups;  // (3 n_groups <= per_tok)
+  int *const glist = reinterpret_cast<int *>(gerr + a.n_groups);  // the groups that stay, ascending
   if (a.n_groups > 1) {  // uniform
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
@@ -310,7 +325,7 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
     float *const gval = vals + a.n_experts + a.n_groups;
     compact = 2 * a.topk_groups * a.size <= 16 * VPL && (scored || !top2);  // (vals holds the keys)
     if (scored || top2) {  // uniform
-      kept = kept_groups<float, true>(a, sub, vals, gval, gmin, unsure);
+      kept = kept_groups<float, true>(a, sub, vals, gval, gmin, gerr, unsure);
       if (__ballot(unsure) != 0) {
         // again in 64 bits, of the experts that can be among what a group is worth
         need_sum64();
@@ -319,7 +334,8 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
         for (int j = 0; j < VPL; ++j) {
           const int e = j * 16 + sub;
           const float t = gmin[e < a.n_experts ? group_of(e, a) : 0];
-          const bool in = (e < a.n_experts) & (v[j] > ninf) & (v[j] >= t - kTol * fmaxf(1.f, fabsf(t)));
+          // (not `>=`: the bound of an infinite t is NaN)
+          const bool in = (e < a.n_experts) & (v[j] > ninf) & !(v[j] < t - kTol * fmaxf(1.f, fabsf(t)));
           maybe |= (Mask<VPL>)in << j;
         }
         __syncthreads();
@@ -332,12 +348,12 @@ __global__ __launch_bounds__(64) void route_experts_kernel(const typename Elem<D
                                      mx, sum_c);
           vals64[e + group_of(e, a)] = s64 + (scored ? (double)a.bias[e] : 0.0);
         }
-        kept = kept_groups<double, false>(a, sub, vals64, vals64 + a.n_experts + a.n_groups, nullptr, unsure);
+        kept = kept_groups<double, false>(a, sub, vals64, vals64 + a.n_experts + a.n_groups, nullptr, nullptr, unsure);
         unsure = false;
         compact = false;  // (vals is gone)
       }
     } else {
-      kept = kept_groups<float, false>(a, sub, vals, gval, gmin, unsure);
+      kept = kept_groups<float, false>(a, sub, vals, gval, nullptr, nullptr, unsure);
     }
     for (int g = sub; g < a.n_groups; g += 16)
       if ((kept >> g) & 1) glist[__popcll(kept & ((1ull << g) - 1))] = g;

@@ -238,3 +238,35 @@ def test_near_ties_of_many_draws(hip_device, scoring, e, top_k, groups, keep, ru
         _check(x.to(hip_device), top_k, bias.to(hip_device), scoring=scoring, n_groups=groups, topk_groups=keep,
                group_rule=rule)
     assert taken >= 20
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("size", [16.0, 1e3, 1e4, 1e6, 1e30])
+def test_group_values_of_large_biases_that_cancel(hip_device, scoring, size):
+    """A group's two best keys of opposite sign: their sum in fp32 keeps little of
+    the scores, in 64 bits it does."""
+    for seed in range(4):
+        e, groups = 48, 12
+        x = _logits(seed, 401, e, hip_device)
+        b = torch.full((groups, 4), -4 * size)
+        b[:, seed % 3], b[:, 3] = size, -size
+        _check(x, 8, b.reshape(-1).to(hip_device), scoring=scoring, n_groups=groups, topk_groups=5, group_rule="top2")
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("rule", ["max", "top2"])
+def test_group_values_past_fp32(hip_device, scoring, rule):
+    """Sums of two keys over fp32's largest number, under its lowest, and infinite
+    biases, beside groups that are not available."""
+    big, inf = 3.4e38, float("inf")
+    x = _logits(3, 9, 32, hip_device)
+    for rows in ([[big, 1e38], [big, 2e38], [big, big], [3e38, 3e38], [0, 0], [1, 1], [2, 2], [3, 3]],
+                 [[-big, -big], [-inf, -inf], [-big, -2e38], [-3e38, -3e38], [-inf, -big], [-2e38, -big],
+                  [-inf, -inf], [-1e38, -big]],
+                 [[inf, inf], [inf, 1], [inf, -big], [big, big], [2e38, 2e38], [inf, inf], [5, 5], [5.0000005, 5]],
+                 [[-inf, -inf], [-big, -big], [-inf, -inf], [-inf, -inf], [-2e38, -2e38], [-inf, -inf], [-inf, -inf],
+                  [-inf, -inf]]):
+        b = torch.full((8, 4), -inf)
+        b[:, 1:3] = torch.tensor(rows)
+        for keep in (1, 2, 3, 5):
+            _check(x, 4, b.reshape(-1).to(hip_device), scoring=scoring, n_groups=8, topk_groups=keep, group_rule=rule)
