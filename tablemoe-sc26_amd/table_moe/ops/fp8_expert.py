@@ -33,6 +33,20 @@ def _descriptor(name, w1, s1, w3, s3, w2, s2):
     return kept, N.Fp8Experts(e, h, inter, 0, *(t.data_ptr() for t in kept))
 
 
+def _row_stride(t: torch.Tensor, width: int) -> int:
+    """t's row stride; a single row's own means nothing (it may be odd, or 0)."""
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
+def _rows(x: torch.Tensor, width: int):
+    """(x or an aligned copy, its row stride) for rows of ``width`` elements."""
+    ld = _row_stride(x, width)
+    if x.stride(1) != 1 or ld % 8 or ld < width or x.data_ptr() % 16:
+        x = aligned(x)
+        ld = _row_stride(x, width)
+    return x, ld
+
+
 class Fp8GroupedExperts:
     """Stacked 8-bit expert weights; one tm_fp8_grouped_swiglu call per forward
     (grouping included).  Scratch comes from torch's allocator in each call, so
@@ -73,20 +87,19 @@ class Fp8GroupedExperts:
             raise ValueError(f"mask must be [{n}] or [{n}, {k}], got {tuple(mask.shape)}")
         if slot_out.shape != (n, k, self.hidden) or slot_out.stride(-1) != 1:
             raise ValueError(f"slot_out must be [N, {k}, {self.hidden}] with unit stride along hidden")
-        if slot_out.stride(0) % 8 or slot_out.stride(1) % 8 or slot_out.data_ptr() % 16:
+        so_b, so_s = slot_out.stride(0) if n > 1 else 0, slot_out.stride(1) if k > 1 else 0
+        if so_b % 8 or so_s % 8 or slot_out.data_ptr() % 16:
             raise ValueError("slot_out rows must start on 16-byte boundaries (strides multiples of 8 elements)")
         if ids.dtype != torch.long or ids.stride(1) != 1 or ids.stride(0) < k:  # (stride 0: one row for all tokens)
             ids = ids.long().contiguous()
-        x = hidden
-        if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < self.hidden or x.data_ptr() % 16:
-            x = aligned(x)
+        x, ld = _rows(hidden, self.hidden)
         m = N.as_u8(mask)
         ms_b, ms_s = (m.stride(0), 0) if m.dim() == 1 else (m.stride(0), m.stride(1))
         with N.on_device(self.device):
             ws = self._workspace(n, k)
-            N.call("tm_fp8_grouped_swiglu", self._ref, N.dtype_tag(dt), x.data_ptr(), n, x.stride(0), ids.data_ptr(), k,
-                   max(ids.stride(0), k), m.data_ptr(), ms_b, ms_s, slot_out.data_ptr(), slot_out.stride(0),
-                   slot_out.stride(1), ws.data_ptr(), ws.numel(), N.stream(self.device))
+            N.call("tm_fp8_grouped_swiglu", self._ref, N.dtype_tag(dt), x.data_ptr(), n, ld, ids.data_ptr(), k,
+                   max(ids.stride(0), k), m.data_ptr(), ms_b, ms_s, slot_out.data_ptr(), so_b, so_s, ws.data_ptr(),
+                   ws.numel(), N.stream(self.device))
         return slot_out
 
 
@@ -118,16 +131,14 @@ class Fp8SharedExperts:
         if out is None:
             out = torch.empty((m, h), dtype=dt, device=self.device)
         for name, t in (("out", out), ("addend", addend)):
-            if t is not None and (t.shape != (m, h) or t.dtype != dt or t.stride(1) != 1 or t.stride(0) % 8
-                                  or (m > 1 and t.stride(0) < h) or t.data_ptr() % 16):
+            if t is not None and (t.shape != (m, h) or t.dtype != dt or t.stride(1) != 1 or _row_stride(t, h) % 8
+                                  or _row_stride(t, h) < h or t.data_ptr() % 16):
                 raise ValueError(f"{name} must be [{m}, {h}] {dt} with 16-byte aligned rows")
-        x = hidden
-        if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < h or x.data_ptr() % 16:
-            x = aligned(x)
+        x, ld = _rows(hidden, h)
         with N.on_device(self.device):
             nbytes = N.lib().tm_fp8_expert_swiglu_workspace_size(self._ref, m)
             ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=self.device)
-            N.call("tm_fp8_expert_swiglu", self._ref, N.dtype_tag(dt), x.data_ptr(), m, x.stride(0), N.ptr(addend),
-                   0 if addend is None else max(addend.stride(0), h), out.data_ptr(), max(out.stride(0), h),
+            N.call("tm_fp8_expert_swiglu", self._ref, N.dtype_tag(dt), x.data_ptr(), m, ld, N.ptr(addend),
+                   0 if addend is None else _row_stride(addend, h), out.data_ptr(), _row_stride(out, h),
                    ws.data_ptr(), ws.numel(), N.stream(self.device))
         return out

@@ -556,3 +556,28 @@ def test_quantised_from_float_weights(hip_device):
     assert torch.equal(a.forward(x, ids, mask, out[0]), b.forward(x, ids, mask, out[1]))
     l1, l2 = Fp8Linear.from_weight(w1[0]), Fp8Linear(*quantize_weight_fp8(w1[0]))
     assert torch.equal(l1.forward(x), l2.forward(x))
+
+
+@pytest.mark.parametrize("h,inter", [(384, 256), (256, 128)])
+def test_experts_one_row_of_any_stride(hip_device, h, inter):
+    """The row stride of a single row means nothing: it may be odd, or 0."""
+    e, k = 4, 3
+    w = _weights(5, e, h, inter)
+    sh = Fp8SharedExperts(*(t[0] for t in w))
+    row = _rand(1, 1, h, dtype=torch.bfloat16)
+    ids = torch.tensor([[2, 0, 3]], device=hip_device)
+    flag = torch.ones(1, dtype=torch.bool, device=hip_device)
+    _, want = _check_experts(row, ids, flag, w)
+    dense = sh.forward(row, addend=row)
+    odd = torch.zeros(1, h + 3, dtype=torch.bfloat16, device=hip_device)
+    odd[:, :h] = row
+    for x in (odd[:, :h], row[0].expand(1, h), row.as_strided((1, h), (1, 1))):
+        _, got = _check_experts(x, ids, flag, w)
+        assert torch.equal(got, want)
+        assert torch.equal(sh.forward(x, addend=x), dense)
+    out = torch.zeros(1, h + 3, dtype=torch.bfloat16, device=hip_device)
+    sh.forward(row, out=out[:, :h], addend=odd[:, :h])
+    assert torch.equal(out[:, :h], dense) and bool((out[:, h:] == 0).all())
+    slots = torch.zeros(1, k * h + 5, dtype=torch.bfloat16, device=hip_device)
+    _check_experts(row, ids, flag, w, slots=slots[:, :k * h].view(1, k, h))
+    assert bool((slots[:, k * h:] == 0).all())
