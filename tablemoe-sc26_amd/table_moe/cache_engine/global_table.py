@@ -362,7 +362,7 @@ class GlobalTable:
         single-workgroup launches (keep select, slot grouping) and the last
         partial rounds of the routed GEMMs leave idle.  The fork and join are
         stream waits, so the call stays capturable in a HIP graph."""
-        from ..ops import SharedExperts, expert_swiglu
+        from ..ops import Fp8SharedExperts, SharedExperts, expert_swiglu
 
         n = hidden.shape[0]
         main = torch.cuda.current_stream(self.device)
@@ -377,7 +377,7 @@ class GlobalTable:
                 if shared._ws is None or shared._ws.numel() < nbytes:
                     shared._ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=self.device)
                 run = lambda: shared.forward(hidden, out=base, addend=residual)  # noqa: E731
-            elif hasattr(shared, "forward"):  # Fp8SharedExperts: its scratch comes from the side stream's pool
+            elif isinstance(shared, Fp8SharedExperts):  # (its scratch comes from the side stream's pool)
                 run = lambda: shared.forward(hidden, out=base, addend=residual)  # noqa: E731
             else:
                 w1, w3, w2 = shared

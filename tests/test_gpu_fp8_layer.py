@@ -110,3 +110,21 @@ def test_router_to_combine(hip_device, n):
         got = [t.clone() for t in captured]
         for a, b in zip(got, run()):
             assert torch.equal(a, b), rep
+
+
+def test_layer_recompute_refuses_other_modules(hip_device):
+    """`shared` is weights or one of the two classes; any other object with a forward
+    is refused, not called."""
+    wl, routed, _, _, table = _setup(hip_device, 5, torch.bfloat16)
+
+    class Other:
+        called = False
+
+        def forward(self, hidden, out=None, addend=None):
+            Other.called = True
+            return out
+
+    for other in (Other(), torch.nn.Linear(H, H)):
+        with pytest.raises(TypeError):
+            table.layer_forward_recompute(wl.x, wl.is_vision, wl.logits, routed, wl.residual, K, 0.6, shared=other)
+    assert not Other.called
