@@ -153,7 +153,9 @@ class GlobalTable:
         return keep
 
     def gather_combine(self, keep, slot_out, weights, idx, dist, residual=None, out=None):
-        """out = residual + (keep ? sum_s w~ slot_out : blend of values[idx])."""
+        """out = residual + (keep ? sum_s w~ slot_out : blend of values[idx]),
+        w~ = weights / their sum: a factor common to a row's weights is lost
+        (HybridStorageManager.combine_slots(target="orig_sum") keeps it)."""
         N.require_hip(keep, slot_out, weights, idx)
         n, top_k = weights.shape
         if out is None:

@@ -27,7 +27,12 @@ def route_experts(router_logits: torch.Tensor, top_k: int, *, scoring: str = "so
     (default: all) best groups are chosen, a group being worth its best key
     ("max") or the sum of its two best ("top2").  normalize_topk divides the
     weights by their sum; scale multiplies them.  An expert whose logit (or
-    bias) is -inf or NaN is chosen after every other one, with weight 0."""
+    bias) is -inf or NaN is chosen after every other one, with weight 0.
+
+    HybridStorageManager.combine_slots(target="orig_sum") takes the weights as they
+    are; GlobalTable.gather_combine (and the layer calls, which run a softmax router
+    of their own) divides them by their sum, so neither scale nor unnormalised
+    weights reach its output."""
     if router_logits.dim() != 2:
         raise ValueError(f"route_experts expects 2D logits, got {tuple(router_logits.shape)}")
     if scoring not in _SCORING or group_rule not in _GROUP_RULE:

@@ -128,3 +128,41 @@ def test_layer_recompute_refuses_other_modules(hip_device):
         with pytest.raises(TypeError):
             table.layer_forward_recompute(wl.x, wl.is_vision, wl.logits, routed, wl.residual, K, 0.6, shared=other)
     assert not Other.called
+
+
+@pytest.mark.parametrize("normalize", [False, True])
+@pytest.mark.parametrize("n", [1, 70])
+def test_which_combine_keeps_the_scale(hip_device, n, normalize):
+    """combine_slots(target="orig_sum") sums the slots with the router's weights as they
+    are, scale and all; gather_combine divides them by their sum."""
+    from test_gpu_layer import _mode_r_manager
+
+    wl, routed, shared, gate, table = _setup(hip_device, n, torch.bfloat16)
+    mgr, _ = _mode_r_manager(hip_device, E=E, H=H)
+    logits = gate.forward(wl.x).float()
+    kw = dict(scoring="sigmoid", n_groups=4, topk_groups=2, group_rule="top2", normalize_topk=normalize)
+    weights, ids = route_experts(logits, K, scale=2.5, **kw)
+    plain, ids1 = route_experts(logits, K, **kw)
+    assert torch.equal(ids, ids1)
+    keep = torch.ones(n, dtype=torch.bool, device=hip_device)
+    slots = torch.empty(n, K, H, dtype=wl.x.dtype, device=hip_device)
+    routed.forward(wl.x, ids, keep, slots)
+    base = shared.forward(wl.x, addend=wl.residual)
+    every, none = (torch.full((n, K), v, dtype=torch.bool, device=hip_device) for v in (True, False))
+    none_at = torch.zeros(n, K, dtype=torch.long, device=hip_device)
+    got = mgr.combine_slots(weights, ids, keep, every, slots, none, none_at, residual=base, target="orig_sum")
+
+    def check(y, w):
+        want = base.double() + (w[:, :, None] * slots.double()).sum(1)
+        # the coefficient: two sums of K weights, a quotient, a product; K products and
+        # sums in fp32; then half a step of bf16
+        size = base.double().abs() + (w[:, :, None] * slots.double().abs()).sum(1)
+        tol = (3 * K + 6) * 2.0 ** -24 * size
+        tol = tol + 2.0 ** -8 * (want.abs() + tol)
+        assert bool(((y.double() - want).abs() <= tol).all())
+
+    check(got, weights.double())
+    dist = torch.zeros(n, 1, device=hip_device)
+    for w in (weights, plain):
+        y = table.gather_combine(keep, slots, w, none_at[:, :1].contiguous(), dist, base)
+        check(y, w.double() / w.double().sum(1, keepdim=True))
