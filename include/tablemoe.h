@@ -105,7 +105,7 @@ int tm_topk_softmax(const float *logits, int64_t n_tokens, int32_t n_experts, in
  * as the largest finite fp32 number.
  * out_weights fp32, out_ids int64, [n_tokens, top_k] contiguous.
  * Limits: n_experts <= 1024, n_groups divides it and is <= 64, 1 <= top_k <=
- * min(32, topk_groups * n_experts / n_groups).
+ * min(32, topk_groups * n_experts / n_groups), scale finite.
  * ====================================================================== */
 #define TM_ROUTE_SOFTMAX 0
 #define TM_ROUTE_SIGMOID 1

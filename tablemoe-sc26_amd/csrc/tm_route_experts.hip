@@ -524,7 +524,7 @@ extern "C" int tm_route_experts(int32_t dtype, const void *logits, int64_t n_tok
              TM_EINVAL_SHAPE, "tm_route_experts: %d of %d groups of %d experts", topk_groups, n_groups, n_experts);
   TM_REQUIRE(top_k >= 1 && top_k <= 32 && top_k <= topk_groups * (n_experts / n_groups), TM_EINVAL_SHAPE,
              "tm_route_experts: top_k %d out of range", top_k);
-  TM_REQUIRE(scale == scale, TM_EINVAL_ARG, "tm_route_experts: scale is NaN");
+  TM_REQUIRE(scale - scale == 0.f, TM_EINVAL_ARG, "tm_route_experts: scale is not finite");  // (0 * inf is NaN)
   if (n_tokens == 0) return TM_OK;
   TM_REQUIRE(logits && out_weights && out_ids, TM_EINVAL_ARG, "tm_route_experts: null pointer");
   const RouteArgs a{n_tokens, ld_logits, n_experts, scoring, n_groups, n_experts / n_groups, topk_groups, group_rule,

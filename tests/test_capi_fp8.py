@@ -149,3 +149,10 @@ def test_host_tensors_are_refused():
         Fp8Linear(q, s)
     with pytest.raises(RuntimeError):
         Fp8GroupedExperts(*(3 * [q[None], s[None]]))
+
+
+def test_route_experts_refuses_an_infinite_scale(lib):
+    """0 * inf is NaN: an expert that is not available has weight 0."""
+    for scale in (float("inf"), float("-inf"), float("nan")):
+        assert _route(lib, scale=scale, n=0) == N.TM_EINVAL_ARG
+    assert _route(lib, scale=-3.0e38, n=0) == N.TM_OK
