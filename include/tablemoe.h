@@ -593,11 +593,11 @@ typedef struct tm_fp8_experts {
  * selection and the outputs as in tm_group_slots + tm_grouped_swiglu: pair
  * (b, s) is taken when mask[b*ms_b + s*ms_s] != 0 and 0 <= ids[b*ld_ids + s] <
  * n_experts; its row of `hidden` elements goes to out + b*so_b + s*so_s
- * (others are left as they were).  g = x^ W1^T, u = x^ W3^T in fp32, f =
- * silu(g) * u in fp32, f^ = f quantised in blocks of 128 columns, y =
- * dtype(f^ W2^T).  dtype F16 or BF16; x rows, out and the workspace 16-byte
- * aligned, so_b and so_s multiples of 8 elements.  The grouping is part of
- * the call (no host sync). */
+ * (others are left as they were; rows must not overlap).  g = x^ W1^T, u =
+ * x^ W3^T in fp32, f = silu(g) * u in fp32, f^ = f quantised in blocks of 128
+ * columns, y = dtype(f^ W2^T).  dtype F16 or BF16; x rows, out and the
+ * workspace 16-byte aligned, so_b and so_s multiples of 8 elements.  The
+ * grouping is part of the call (no host sync). */
 size_t tm_fp8_grouped_swiglu_workspace_size(const tm_fp8_experts *experts, int64_t n_tokens, int32_t top_k);
 int tm_fp8_grouped_swiglu(const tm_fp8_experts *experts, int32_t dtype, const void *x, int64_t n_tokens, int64_t ld_x,
                           const int64_t *ids, int32_t top_k, int64_t ld_ids, const uint8_t *mask, int64_t ms_b,

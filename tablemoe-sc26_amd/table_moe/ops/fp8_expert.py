@@ -90,6 +90,8 @@ class Fp8GroupedExperts:
         so_b, so_s = slot_out.stride(0) if n > 1 else 0, slot_out.stride(1) if k > 1 else 0
         if so_b % 8 or so_s % 8 or slot_out.data_ptr() % 16:
             raise ValueError("slot_out rows must start on 16-byte boundaries (strides multiples of 8 elements)")
+        if (n > 1 and so_b < self.hidden) or (k > 1 and so_s < self.hidden) or (n > 1 and k > 1 and so_b == so_s):
+            raise ValueError("slot_out rows must not overlap")
         if ids.dtype != torch.long or ids.stride(1) != 1 or ids.stride(0) < k:  # (stride 0: one row for all tokens)
             ids = ids.long().contiguous()
         x, ld = _rows(hidden, self.hidden)

@@ -581,3 +581,18 @@ def test_experts_one_row_of_any_stride(hip_device, h, inter):
     slots = torch.zeros(1, k * h + 5, dtype=torch.bfloat16, device=hip_device)
     _check_experts(row, ids, flag, w, slots=slots[:, :k * h].view(1, k, h))
     assert bool((slots[:, k * h:] == 0).all())
+
+
+def test_experts_overlapping_slots_are_refused(hip_device):
+    """Slots that lie on each other have no defined result."""
+    n, k, e, h = 4, 2, 3, 256
+    ex = Fp8GroupedExperts(*_weights(1, e, h, 128))
+    x = _rand(1, n, h, dtype=torch.bfloat16)
+    ids = torch.zeros(n, k, dtype=torch.long, device=hip_device)
+    mask = torch.ones(n, dtype=torch.bool, device=hip_device)
+    mem = torch.zeros(n * k * h, dtype=torch.bfloat16, device=hip_device)
+    for strides in ((0, h), (k * h, 0), (h, h), (8, n * h), (k * h, 8)):
+        with pytest.raises(ValueError):
+            ex.forward(x, ids, mask, mem.as_strided((n, k, h), (*strides, 1)))
+    assert not bool(mem.any())
+    _check_experts(x, ids, mask, _weights(1, e, h, 128), slots=mem.view(k, n, h).transpose(0, 1))
