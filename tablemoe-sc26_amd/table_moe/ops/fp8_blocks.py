@@ -132,6 +132,9 @@ class Fp8Linear:
             if x.stride(1) != 1 or x.stride(0) < kp or x.stride(0) % 16 or x.data_ptr() % 16 or xs.stride(1) != 1:
                 raise ValueError("Fp8Linear: rows of quantised x must be padded to whole blocks, 16-byte aligned, as "
                                  "quantize_rows_fp8 returns them")
+            end = x.storage_offset() + (x.shape[0] - 1) * x.stride(0) + kp  # (one byte an element)
+            if x.shape[0] > 0 and end > x.untyped_storage().nbytes():
+                raise ValueError("Fp8Linear: the last row of quantised x ends before its last block does")
         else:
             N.require_hip(x, self.weight)
             if dtype is not None and dtype != x.dtype:

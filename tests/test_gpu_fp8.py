@@ -596,3 +596,19 @@ def test_experts_overlapping_slots_are_refused(hip_device):
             ex.forward(x, ids, mask, mem.as_strided((n, k, h), (*strides, 1)))
     assert not bool(mem.any())
     _check_experts(x, ids, mask, _weights(1, e, h, 128), slots=mem.view(k, n, h).transpose(0, 1))
+
+
+def test_linear_quantised_rows_end_inside_their_storage(hip_device):
+    """A row of 8-bit x is read up to its whole last block: where that is not there,
+    the call is refused."""
+    x = _rand(3, 5, 200, dtype=torch.bfloat16)
+    wq, ws = _w8(4, 64, 200)
+    layer = Fp8Linear(wq, ws)
+    q, s = quantize_rows_fp8(x)
+    want = layer.forward((q, s), dtype=torch.bfloat16)
+    short = torch.zeros(4 * 256 + 200, dtype=torch.uint8, device=hip_device)
+    short[:] = torch.as_strided(q.view(torch.uint8), (4 * 256 + 200,), (1,))
+    with pytest.raises(ValueError):
+        layer.forward((short.view(torch.float8_e4m3fn).as_strided((5, 200), (256, 1)), s), dtype=torch.bfloat16)
+    assert torch.equal(layer.forward((q[2:], s[2:]), dtype=torch.bfloat16), want[2:])
+    assert torch.equal(layer.forward((q[:4], s[:4]), dtype=torch.bfloat16), want[:4])
