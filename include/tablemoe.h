@@ -101,8 +101,8 @@ int tm_topk_softmax(const float *logits, int64_t n_tokens, int32_t n_experts, in
  * Keys and group values are compared in 64 bits, weights are rounded once.
  * An expert whose logit is NaN or -inf, or whose key is NaN or -inf, is not
  * available: it comes after every available one (lower id first), in a group
- * without any last of all, with weight 0, and leaves the softmax.  +inf counts
- * as the largest finite fp32 number.
+ * without any last of all, with weight 0, and leaves the softmax.  A +inf logit
+ * counts as the largest finite fp32 number.
  * out_weights fp32, out_ids int64, [n_tokens, top_k] contiguous.
  * Limits: n_experts <= 1024, n_groups divides it and is <= 64, 1 <= top_k <=
  * min(32, topk_groups * n_experts / n_groups), scale finite.
@@ -544,7 +544,9 @@ int tm_grouped_swiglu_packed(int32_t dtype, const void *x, int64_t ld_x, int32_t
  * The quantisers give each block the smallest power of two s with
  * max|v| / s <= 448 over its finite elements (1 if they are all 0, never
  * below 2^-126): v / s is exact and q its nearest e4m3 value (ties to even);
- * a non-finite v becomes NaN.  The products take any fp32 scales.
+ * a non-finite v becomes NaN.  The products take any fp32 scales; the product
+ * of a row's and a weight's has to be a normal fp32 number or 0 (it is formed
+ * in fp32: under 2^-126 it loses digits, past 2^128 it is infinite).
  *
  * tm_fp8_quantize_rows: x [n_rows, k] (F32, F16, BF16, row stride ld_x) -> q
  * (bytes, row stride ld_q, a multiple of 16) and scale [n_rows, ceil(k/128)]
@@ -597,7 +599,8 @@ typedef struct tm_fp8_experts {
  * x^ W3^T in fp32, f = silu(g) * u in fp32, f^ = f quantised in blocks of 128
  * columns, y = dtype(f^ W2^T).  dtype F16 or BF16; x rows, out and the
  * workspace 16-byte aligned, so_b and so_s multiples of 8 elements.  The
- * grouping is part of the call (no host sync). */
+ * grouping is part of the call (no host sync); one workgroup does it for more
+ * than 8192 tokens, 8 slots or 256 experts (tm_group_slots_ws). */
 size_t tm_fp8_grouped_swiglu_workspace_size(const tm_fp8_experts *experts, int64_t n_tokens, int32_t top_k);
 int tm_fp8_grouped_swiglu(const tm_fp8_experts *experts, int32_t dtype, const void *x, int64_t n_tokens, int64_t ld_x,
                           const int64_t *ids, int32_t top_k, int64_t ld_ids, const uint8_t *mask, int64_t ms_b,

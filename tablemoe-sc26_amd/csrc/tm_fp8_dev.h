@@ -53,7 +53,8 @@ __device__ __forceinline__ uint32_t tm_fp8_pack4(float a, float b, float c, floa
 typedef __bf16 tm_bf16x2 __attribute__((ext_vector_type(2)));
 
 // Eight e4m3 values, times a power of two, as bf16 (exact: 4 significant bits;
-// apart from products under 2^-126, which blocks of max|v| < 2^-108 alone can have).
+// apart from products under 2^-126, which blocks of max|v| < 2^-108 alone can have,
+// and of values within 3 % of 2^128, whose e4m3 neighbour is 2^128).
 __device__ __forceinline__ uint4 tm_fp8_to_bf16x8(uint32_t lo, uint32_t hi, float s = 1.f) {
   uint4 r;
   r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false));

@@ -21,8 +21,8 @@
 // Bound by latency: each round is a maximum over the lane's keys, four DPP
 // exchanges, the lowest lane that holds it and its key closed, one after the
 // other; where at most half of the experts are in the groups that stay, over
-// those alone.  8 tokens of 256 experts take 8.2 us, 4099 of 160 8.4 us, 12301 of
-// 256 17 us (rounds over every key: 9.0, 9.3 and 17.7).  All in 64 bits took 24,
+// those alone.  8 tokens of 256 experts take 8.1 us, 4099 of 160 8.7 us, 12301 of
+// 256 15-17 us (rounds over every key: 9.0, 9.3 and 17.7).  All in 64 bits took 24,
 // 20 and 43 (a first pass in 32 bits that chose again in 64 where keys were near:
 // 10, 10 and 36).
 #include "tm_common.h"
