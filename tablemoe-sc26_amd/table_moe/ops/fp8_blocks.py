@@ -85,7 +85,8 @@ class Fp8Linear:
 
     ``forward`` quantises x [..., K] (float32, float16, bfloat16) in the call, or
     takes the pair that ``quantize_rows_fp8`` returns, with ``dtype`` naming the
-    output's; sums are fp32, y is rounded once.  float32 outputs take every
+    output's; sums are fp32, y is rounded once (a bias of another type than the
+    output's is rounded to it first).  float32 outputs take every
     product exactly; 16-bit ones may run on the 8-bit matrix instructions (an
     error of up to 6e-5 of a sum's size before the rounding).  A weight whose
     K is no multiple of 128 is copied once to padded rows.  Calls allocate
