@@ -115,8 +115,9 @@ __global__ __launch_bounds__(kQThreads) void quantize_weight_kernel(const typena
 int tm_internal_fp8_rows(int32_t dtype, const void *x, int64_t n, int64_t k, int64_t ld_x, void *q, int64_t ld_q,
                          float *scale, int64_t ld_s, hipStream_t s) {
   const int64_t blocks = tm_cdiv(k, kFp8Block);
-  const int64_t grid = tm_cdiv(n * blocks, kQThreads / 16);
-  TM_REQUIRE(grid < ((int64_t)1 << 31), TM_EINVAL_SHAPE, "tm_fp8_quantize_rows: too many rows");
+  constexpr int kPer = kQThreads / 16;  // (row, block) pairs of a workgroup
+  TM_REQUIRE(n <= (((int64_t)1 << 31) - 1) * kPer / blocks, TM_EINVAL_SHAPE, "tm_fp8_quantize_rows: too many rows");
+  const int64_t grid = tm_cdiv(n * blocks, kPer);
   return TM_DISPATCH_DTYPE(dtype, DT, [&] {
     const auto *const p = static_cast<const typename Elem<DT>::T *>(x);
     auto *const out = static_cast<uint8_t *>(q);

@@ -156,3 +156,10 @@ def test_route_experts_refuses_an_infinite_scale(lib):
     for scale in (float("inf"), float("-inf"), float("nan")):
         assert _route(lib, scale=scale, n=0) == N.TM_EINVAL_ARG
     assert _route(lib, scale=-3.0e38, n=0) == N.TM_OK
+
+
+def test_quantise_rows_refuses_counts_past_64_bits(lib):
+    """n_rows times a row's blocks out of int64's range."""
+    for n, k in ((1 << 61, 1024), ((1 << 61) + 16, 1024), ((1 << 63) - 1, 129), (1 << 60, 1 << 20)):
+        assert lib.tm_fp8_quantize_rows(N.TM_DT_BF16, P, n, k, k, P, -(-k // 128) * 128, P, -(-k // 128),
+                                        None) == N.TM_EINVAL_SHAPE, (n, k)
