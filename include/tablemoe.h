@@ -615,6 +615,106 @@ int tm_fp8_expert_swiglu(const tm_fp8_experts *experts, int32_t dtype, const voi
                          size_t workspace_bytes, tm_stream_t stream);
 
 /* ======================================================================
+ * Attention side of a layer: positions, an 8-bit cache, attention and
+ * importance over it (beside tm_last_query_importance, whose queries and keys
+ * are rotated and 16-bit; the reference's layers leave attention to their
+ * model code, models/qwen3_vl_moe/hybrid_attention.py:13-110).
+ *
+ * tm_rotate_positions: rotary positions with several axes.  q [n_tokens,
+ * n_heads, head_dim] (strides qs_t, qs_h, unit along head_dim) and, unless k is
+ * NULL, k [n_tokens, n_kv_heads, head_dim].  Frequency i < rotary_dim / 2 turns
+ * with axis a(i) of positions [n_axes, n_tokens] (int64, row stride
+ * ld_positions): sections (host, [n_axes], summing to rotary_dim / 2) are runs
+ * of frequencies in the axes' order, or with interleaved != 0 a(i) = i % n_axes
+ * where i < n_axes * sections[i % n_axes], else 0.  angle = positions * inv_freq[i]
+ * in 64 bits; the pair (x1, x2) = columns (i, i + rotary_dim / 2), or with
+ * adjacent != 0 (2i, 2i + 1), becomes (x1 cos - x2 sin, x2 cos + x1 sin) in
+ * fp32, rounded once.  inverse != 0 turns back (the gradient with respect to
+ * the inputs).  Columns from rotary_dim on are copied.  Outputs have strides of
+ * their own and may be the inputs themselves, but not overlap them otherwise.
+ * Limits: head_dim <= 1024, rotary_dim even and <= head_dim, n_axes <= 4.
+ * ====================================================================== */
+int tm_rotate_positions(int32_t dtype, const void *q, int64_t n_tokens, int32_t n_heads, int64_t qs_t, int64_t qs_h,
+                        const void *k, int32_t n_kv_heads, int64_t ks_t, int64_t ks_h, int32_t head_dim,
+                        int32_t rotary_dim, const int64_t *positions, int64_t ld_positions, int32_t n_axes,
+                        const int32_t *sections, int32_t interleaved, int32_t adjacent, int32_t inverse,
+                        const float *inv_freq, void *q_out, int64_t qo_t, int64_t qo_h, void *k_out, int64_t ko_t,
+                        int64_t ko_h, tm_stream_t stream);
+
+/* A cache of n_pages pages of page_size (32, 64 or 128) tokens for n_kv_heads
+ * heads: k [n_pages, n_kv_heads, page_size / 32, head_dim / 32, 64, 16] bytes
+ * (e4m3), v the same over v_dim columns, k_scale and v_scale [n_pages,
+ * n_kv_heads] fp32, all 16-byte aligned.  A value stands for byte * scale, a
+ * scale being a power of two as tm_kv8_append writes it.  In a tile of 32
+ * tokens byte e of lane l of column block j is, for k, token l % 32 and column
+ * 32 j + 16 (l / 32) + e; for v, column 32 j + l % 32 and token 16 (e / 8) +
+ * 8 (e / 4 % 2) + 4 (l / 32) + e % 4.  (head_dim, v_dim) is one of (64, 64),
+ * (128, 128), (192, 128), (192, 192), (256, 256). */
+typedef struct tm_kv8_cache {
+  int64_t n_pages;
+  int32_t n_kv_heads, head_dim, v_dim, page_size;
+  void *k;
+  void *v;
+  float *k_scale;
+  float *v_scale;
+} tm_kv8_cache;
+
+/* The sequences of one call.  table [n_seqs, max_pages] (row stride ld_table):
+ * each sequence's pages in order.  lengths [n_seqs]: its tokens, the new ones
+ * counted.  starts [n_seqs + 1]: the new tokens of sequence b are rows
+ * [starts[b], starts[b + 1]) of the call's n_tokens rows (non-decreasing, first
+ * 0), its last positions; NULL: one new token each (n_tokens = n_seqs).  All
+ * three are on the device and read there.  Nothing outside the cache is
+ * touched whatever they hold: a page number out of range is a page that is not
+ * there (its tokens are not written, and nobody attends to them), and so is
+ * what lies past the table's width or before position 0. */
+typedef struct tm_kv8_batch {
+  const int32_t *table;
+  int64_t ld_table;
+  const int32_t *lengths;
+  const int32_t *starts;
+  int64_t n_seqs, n_tokens;
+  int32_t max_pages, reserved;
+} tm_kv8_batch;
+
+/* Writes the new tokens' k [n_tokens, n_kv_heads, head_dim] and v (v_dim) of
+ * `dtype` (F32, F16, BF16; strides per token and head, unit along columns,
+ * 16-byte aligned rows) into their pages.  A page's scale is the smallest power
+ * of two s >= 2^-100 with max|x| / s <= 448 over the finite values written (1
+ * where they are all 0), and no less than what it was where the page held
+ * tokens before; where that rises, those tokens' values are rounded again under
+ * the new scale.  Values are rounded to nearest even, a non-finite one becomes NaN.
+ * Cells past a sequence's end keep their bytes.  A page that is written belongs to one sequence. */
+int tm_kv8_append(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *k, int64_t ks_t,
+                  int64_t ks_h, const void *v, int64_t vs_t, int64_t vs_h, tm_stream_t stream);
+
+/* out [n_tokens, n_heads, v_dim] = softmax(scale q K^T) V of each new token over
+ * its sequence's cached positions: those up to its own with causal != 0, all
+ * otherwise.  q [n_tokens, n_heads, head_dim]; head i reads key head
+ * i / (n_heads / n_kv_heads).  fp32 scores, maxima and sums; a probability is
+ * rounded to `dtype` (F16 or BF16) before it meets the values.  lse (nullable,
+ * fp32 [n_tokens, n_heads] contiguous) = log sum exp of the scores, natural.  A
+ * token that sees nothing gets zeros and -inf; rows of no sequence are left as
+ * they were.  16-byte aligned rows of q and out; scale > 0; workspace
+ * tm_kv8_attention_workspace_size (16-byte aligned, one call at a time). */
+size_t tm_kv8_attention_workspace_size(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t n_heads);
+int tm_kv8_attention(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *q, int64_t qs_t,
+                     int64_t qs_h, int32_t n_heads, float scale, int32_t causal, void *out, int64_t os_t, int64_t os_h,
+                     float *lse, void *workspace, size_t workspace_bytes, tm_stream_t stream);
+
+/* tm_last_query_importance over the cache: out[b, t] = mean over heads of the
+ * probability that q[b] ([n_seqs, n_heads, head_dim], one query per sequence)
+ * gives to position t < out_len among lengths[b] cached ones; 0 from there on.
+ * Scores are fp32 (TM_SCORE_F32).  lse (nullable, fp32 [n_seqs, n_heads], row
+ * stride ld_lse): the queries' log sum exp, as tm_kv8_attention gives it;
+ * without it the call computes it first.  batch->starts is not used, n_tokens
+ * = n_seqs.  n_heads <= 256. */
+size_t tm_kv8_importance_workspace_size(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t n_heads);
+int tm_kv8_importance(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *q, int64_t qs_b,
+                      int64_t qs_h, int32_t n_heads, float scale, const float *lse, int64_t ld_lse, int64_t out_len,
+                      float *out, int64_t ld_out, void *workspace, size_t workspace_bytes, tm_stream_t stream);
+
+/* ======================================================================
  * Mode G -- one MoE layer of the table path in ONE call.
  * Enqueues, back to back on `stream`: tm_topk_softmax (router) ->
  * tm_project -> tm_search_global -> tm_keep_select (n_keep =
@@ -680,8 +780,9 @@ typedef struct tm_layer_io {
 #define TM_LAYER_NO_COMBINE 1
 
 /* sizeof(tm_table_layer) for which == 0, sizeof(tm_layer_io) for which == 1,
- * sizeof(tm_fp8_experts) for which == 2 (lets a binding check its mirror of
- * the structs). */
+ * sizeof(tm_fp8_experts) for which == 2, sizeof(tm_kv8_cache) for which == 3,
+ * sizeof(tm_kv8_batch) for which == 4 (lets a binding check its mirror of the
+ * structs). */
 size_t tm_struct_size(int32_t which);
 /* Workspace of tm_table_forward.  Its first TM_LAYER_SYNC_BYTES bytes hold
  * arrival counters and flags (batches of at most 64 tokens hand the

@@ -1,0 +1,433 @@
+// Attention over the 8-bit cache (layout: tm_kv8.h): tm_kv8_attention.
+//
+// Rows of a sequence are its (new token, query head of one key head) pairs, 32 a
+// tile, so a key head's tile of keys serves all its query heads.  Per 32 keys:
+//   S^T = K Q^T on the 16-bit instructions (a byte of K is exact in 16 bits), a
+//   lane holding 16 keys of one row;  x = S^T sk scale log2(e) + log2(sv);
+//   P = 2^(x - m) under a running reference m of the row, so that the values'
+//   scale rides in P and V enters as the bytes stand;  O^T += V^T P.
+// With l = sum P / sv the result is O / l and log sum exp = (m + log2 l) ln 2.
+// m follows the running maximum of x only when that has grown by more than 2^6
+// (P <= 64 then), so O is seldom scaled again.  P is rounded to the queries'
+// type for the second product (half a step of 2^-8 or 2^-11 of each probability,
+// which average out); all sums are fp32.
+//
+// The four waves of a workgroup take every fourth tile of keys and join through
+// LDS.  Where rows alone do not fill the device, the keys are split over
+// workgroups as well, and a second launch joins their parts.
+#include "tm_internal.h"
+#include "tm_kv8_dev.h"
+
+#include <type_traits>
+
+namespace {
+
+constexpr int kAttThreads = 256;
+constexpr int kWaves = kAttThreads / 64;
+constexpr int kMaxSplits = 128;
+constexpr float kGrow = 6.f;
+
+struct AttArgs {
+  tm_kv8_cache c;
+  tm_kv8_batch b;
+  const void *q;
+  int64_t qs_t, qs_h;
+  void *out;
+  int64_t os_t, os_h;
+  float *lse;
+  float2 *stats;  // [row of the call][split]: reference, sum
+  float *part;    // [row of the call][split][v_dim]
+  float scale;
+  int32_t heads, groups, splits, page_log2, causal, tiles1;  // tiles1: row tiles of one token
+};
+
+// A row tile: rows [r0, r0 + rows) of sequence b.
+struct RowTile {
+  Kv8Seq s;
+  int64_t b, r0;
+  int rows;
+  int64_t end;    // keys that its last row sees
+  int64_t tiles;  // of 32 keys
+  int64_t per;    // tiles of a split
+};
+__device__ __forceinline__ int64_t visible(const AttArgs &a, const Kv8Seq &s, int64_t token) {
+  const int64_t cap = (int64_t)a.b.max_pages << a.page_log2;
+  int64_t e = a.causal ? s.len - s.n + token + 1 : s.len;
+  e = e < cap ? e : cap;
+  return e < 0 ? 0 : e;
+}
+__device__ __forceinline__ bool row_tile(const AttArgs &a, int64_t u, RowTile &t) {
+  int64_t j = 0;
+  if (a.b.starts == nullptr) {
+    t.b = u / a.tiles1;
+    j = u - t.b * a.tiles1;
+  } else {
+    t.b = tm_kv8_unit(a.b, u, a.groups, 32, 1, j);
+  }
+  t.s = tm_kv8_seq(a.b, t.b);
+  t.r0 = j * 32;
+  const int64_t all = t.s.n * a.groups;
+  if (j < 0 || t.r0 >= all) return false;
+  t.rows = (int)(all - t.r0 < 32 ? all - t.r0 : 32);
+  t.end = visible(a, t.s, (t.r0 + t.rows - 1) / a.groups);
+  t.tiles = (t.end + 31) >> 5;
+  t.per = tm_kv8_per(t.tiles, a.splits);
+  return true;
+}
+
+// DV = 0: the statistics alone.
+template <int DT, int D, int DV>
+__global__ __launch_bounds__(kAttThreads, D + DV > 320 ? 1 : 2) void attend_kernel(AttArgs a) {
+  using T = typename Elem<DT>::T;
+  constexpr int NK = D / 32, NV = DV / 32;
+  constexpr int kChunk = 64;  // columns joined at a time
+  __shared__ float2 join[kWaves][32];
+  __shared__ __align__(16) float obuf[DV ? kWaves : 1][32][kChunk + 4];
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+  const int c = lane & 31, g = lane >> 5;
+  const int h = blockIdx.y, split = blockIdx.z;
+  RowTile t;
+  if (!row_tile(a, blockIdx.x, t)) return;
+  const int64_t t0 = split * t.per, t1 = t0 + t.per < t.tiles ? t0 + t.per : t.tiles;
+  if (t0 >= t1 && split > 0) return;
+  const int64_t row = t.r0 + (c < t.rows ? c : t.rows - 1);
+  const int64_t token = row / a.groups;
+  const int64_t call_row = (t.s.first + token) * a.heads + h * a.groups + (row - token * a.groups);
+  const int64_t limit = visible(a, t.s, token), first_limit = visible(a, t.s, t.r0 / a.groups);
+
+  uint4 qf[NK][2];
+  {
+    const T *const q = static_cast<const T *>(a.q) + (t.s.first + token) * a.qs_t +
+                       (h * a.groups + (row - token * a.groups)) * a.qs_h + 16 * g;
+#pragma unroll
+    for (int j = 0; j < NK; ++j) {
+      qf[j][0] = *reinterpret_cast<const uint4 *>(q + 32 * j);
+      qf[j][1] = *reinterpret_cast<const uint4 *>(q + 32 * j + 8);
+    }
+  }
+  tm_f32x16 o[NV ? NV : 1];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
+  float m = -__builtin_huge_valf(), l = 0.f;
+  const float unit = a.scale * kLog2e;
+
+  auto step = [&](int64_t tile, const Kv8Place &w, const uint4 (&kf)[NK], uint4 (&vf)[NV ? NV : 1], float sk, float sv) {
+    tm_f32x16 s;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NK; ++j) {
+      s = tm_mfma32x32x16<DT>(tm_kv8_operand<DT>(kf[j].x, kf[j].y), qf[j][0], s);
+      s = tm_mfma32x32x16<DT>(tm_kv8_operand<DT>(kf[j].z, kf[j].w), qf[j][1], s);
+    }
+    const int64_t k0 = tile * 32;
+    const bool edge = !w.there || k0 + 32 > first_limit;
+    uint32_t nan_bytes = 0;
+    if (edge) {
+      const int64_t lim = w.there ? limit : 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int64_t key = k0 + 8 * (i / 4) + 4 * g + i % 4;
+        s[i] = key < lim ? s[i] : -__builtin_huge_valf();
+      }
+      // a NaN among values that some row does not see stays out of the product
+      if constexpr (NV > 0) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          uint32_t *const p = reinterpret_cast<uint32_t *>(&vf[j]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t x = p[e] & 0x7f7f7f7fu;
+            const uint32_t n = (x + 0x01010101u) & 0x80808080u;  // 0x80 where a byte is 0x7f
+            nan_bytes |= n;
+            p[e] &= ~((n >> 7) * 0xffu);
+          }
+        }
+      }
+    }
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+    const float mul = sk * unit, add = tm_exponent(sv);
+    top = fmaf(top, mul, add);
+    top = fmaxf(top, tm_other_half(top));
+    if (__any(top > m + kGrow || (m == -__builtin_huge_valf() && top > m))) {
+      const float to = fmaxf(m, top);
+      const float f = m == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(m - to);
+      m = to;
+      l *= f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[j][i] *= f;
+    }
+    const float off = add - (m == -__builtin_huge_valf() ? 0.f : m);
+    float sum = 0.f;
+    uint32_t pf[8];
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float x = __builtin_amdgcn_exp2f(fmaf(s[i], mul, off)), y = __builtin_amdgcn_exp2f(fmaf(s[i + 1], mul, off));
+      sum += x + y;
+      if constexpr (NV > 0) {
+        typename Elem<DT>::T two[2] = {Elem<DT>::from_f(x), Elem<DT>::from_f(y)};
+        pf[i / 2] = __builtin_bit_cast(uint32_t, two);
+      }
+    }
+    l = fmaf(sum, __builtin_amdgcn_exp2f(-add), l);
+    if constexpr (NV > 0) {
+      const uint4 p0 = make_uint4(pf[0], pf[1], pf[2], pf[3]), p1 = make_uint4(pf[4], pf[5], pf[6], pf[7]);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        o[j] = tm_mfma32x32x16<DT>(tm_kv8_operand<DT>(vf[j].x, vf[j].y), p0, o[j]);
+        o[j] = tm_mfma32x32x16<DT>(tm_kv8_operand<DT>(vf[j].z, vf[j].w), p1, o[j]);
+      }
+      if (edge && __any(nan_bytes != 0)) {  // those that a row does see make its column NaN
+        const uint8_t *const vb = static_cast<const uint8_t *>(a.c.v) +
+                                  ((w.slot << (a.page_log2 - 5)) + w.tile) * (int64_t)(NV * 1024);
+        const int64_t lim = w.there ? limit : 0;
+        for (int key = 0; key < 32 && k0 + key < lim; ++key)
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int col = 8 * (i / 4) + 4 * g + i % 4;
+              const uint8_t x = vb[j * 1024 + ((key / 4 % 2) * 32 + col) * 16 + key / 16 * 8 + key / 8 % 2 * 4 + key % 4];
+              if ((x & 0x7f) == 0x7f) o[j][i] = __builtin_nanf("");
+            }
+      }
+    }
+  };
+
+  const int64_t begin = t0 + wave;
+  if (begin < t1) {
+    uint4 ka[NK], va[NV ? NV : 1], kb[NK], vb[NV ? NV : 1];
+    auto fetch = [&](int64_t tile, Kv8Place &w, uint4 (&kf)[NK], uint4 (&vf)[NV ? NV : 1], float &sk, float &sv) {
+      tile = tile < t1 ? tile : t1 - 1;
+      w = tm_kv8_place(a.c, a.b, t.b, h, tile, a.page_log2);
+      tm_kv8_load<NK>(a.c.k, w, a.page_log2, lane, kf);
+      if constexpr (NV > 0) tm_kv8_load<NV>(a.c.v, w, a.page_log2, lane, vf);
+      sk = w.there ? a.c.k_scale[w.slot] : 1.f;
+      sv = NV && w.there ? a.c.v_scale[w.slot] : 1.f;
+    };
+    Kv8Place wa, wb;
+    float ska, sva, skb, svb;
+    fetch(begin, wa, ka, va, ska, sva);
+    for (int64_t tile = begin; tile < t1; tile += 2 * kWaves) {
+      fetch(tile + kWaves, wb, kb, vb, skb, svb);
+      step(tile, wa, ka, va, ska, sva);
+      if (tile + kWaves >= t1) break;
+      fetch(tile + 2 * kWaves, wa, ka, va, ska, sva);
+      step(tile + kWaves, wb, kb, vb, skb, svb);
+    }
+  }
+  l += tm_other_half(l);
+  if (g == 0) join[wave][c] = make_float2(m, l);
+  __syncthreads();
+  float top = -__builtin_huge_valf(), total = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, join[w][c].x);
+  const float base = top == -__builtin_huge_valf() ? 0.f : top;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) total += join[w][c].y * __builtin_amdgcn_exp2f(join[w][c].x - base);
+  const float f = __builtin_amdgcn_exp2f(m - base);
+  const bool whole = t.per >= t.tiles;  // nothing to join with other workgroups
+  if (wave == 0 && g == 0 && c < t.rows) {
+    if (DV == 0 || !whole) a.stats[call_row * a.splits + split] = make_float2(top, total);
+    if (whole && a.lse) a.lse[call_row] = total == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(total)) * kLn2;
+  }
+  if constexpr (NV > 0) {
+    __shared__ float inv[32];
+    if (wave == 0 && g == 0) inv[c] = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int half = 0; half < DV / kChunk; ++half) {
+#pragma unroll
+      for (int jj = 0; jj < kChunk / 32; ++jj)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const tm_f32x16 &v = o[half * (kChunk / 32) + jj];
+          *reinterpret_cast<float4 *>(&obuf[wave][c][32 * jj + 2 * i + 4 * g]) =
+              make_float4(v[i] * f, v[i + 1] * f, v[i + 2] * f, v[i + 3] * f);
+        }
+      __syncthreads();
+      for (int e = threadIdx.x; e < t.rows * (kChunk / 4); e += kAttThreads) {
+        const int r = e / (kChunk / 4), col = e % (kChunk / 4) * 4;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const float4 x = *reinterpret_cast<const float4 *>(&obuf[w][r][col]);
+          v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+        }
+        const int64_t rr = t.r0 + r, tok = rr / a.groups, head = h * a.groups + (rr - tok * a.groups);
+        const int to = half * kChunk + col;
+        if (whole) {
+          T y[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[k] = Elem<DT>::from_f(v[k] * inv[r]);
+          __builtin_memcpy(static_cast<T *>(a.out) + (t.s.first + tok) * a.os_t + head * a.os_h + to, y, 8);
+        } else {
+          *reinterpret_cast<float4 *>(a.part + (((t.s.first + tok) * a.heads + head) * a.splits + split) * DV + to) =
+              make_float4(v[0], v[1], v[2], v[3]);
+        }
+      }
+      if (half + 1 < DV / kChunk) __syncthreads();
+    }
+  }
+}
+
+// Joins the splits of a row tile: a wave per row.
+template <int DT, int DV>
+__global__ __launch_bounds__(kAttThreads) void join_kernel(AttArgs a) {
+  using T = typename Elem<DT>::T;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = blockIdx.y;
+  RowTile t;
+  if (!row_tile(a, blockIdx.x, t) || t.per >= t.tiles) return;
+  const int n = (int)((t.tiles + t.per - 1) / t.per);
+  for (int r = blockIdx.z * kWaves + wave; r < t.rows; r += kWaves * gridDim.z) {
+    const int64_t rr = t.r0 + r, tok = rr / a.groups, head = h * a.groups + (rr - tok * a.groups);
+    const int64_t row = (t.s.first + tok) * a.heads + head;
+    const float2 *const st = a.stats + row * a.splits;
+    const float2 x0 = lane < n ? st[lane] : make_float2(-__builtin_huge_valf(), 0.f);
+    const float2 x1 = lane + 64 < n ? st[lane + 64] : make_float2(-__builtin_huge_valf(), 0.f);
+    const float top = tm_wave_max(fmaxf(x0.x, x1.x));
+    const float base = top == -__builtin_huge_valf() ? 0.f : top;
+    const float f0 = __builtin_amdgcn_exp2f(x0.x - base), f1 = __builtin_amdgcn_exp2f(x1.x - base);
+    const float total = tm_wave_sum(x0.y * f0 + x1.y * f1);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    if (a.lse && lane == 0) a.lse[row] = total == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(total)) * kLn2;
+    constexpr int kPer = DV / 64;
+    float v[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) v[k] = 0.f;
+    const float *const p = a.part + row * a.splits * DV + lane * kPer;
+    for (int s = 0; s < n; ++s) {
+      const float f = __shfl(s < 64 ? f0 : f1, s & 63, 64);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) v[k] = fmaf(p[(int64_t)s * DV + k], f, v[k]);
+    }
+    T *const y = static_cast<T *>(a.out) + (t.s.first + tok) * a.os_t + head * a.os_h + lane * kPer;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) y[k] = Elem<DT>::from_f(v[k] * inv);
+  }
+}
+
+int page_log2(int page) { return page == 32 ? 5 : page == 64 ? 6 : 7; }
+
+// Row tiles of a call (an upper bound), and the splits of the keys.
+int64_t row_tiles(const tm_kv8_batch *b, int groups) {
+  return b->starts ? b->n_tokens * groups / 32 + b->n_seqs : b->n_seqs * tm_cdiv(groups, 32);
+}
+int key_splits(const tm_kv8_cache *c, const tm_kv8_batch *b, int64_t tiles) {
+  const int64_t units = tiles * c->n_kv_heads, keys = (int64_t)b->max_pages * c->page_size / 32;
+  if (units <= 0) return 1;
+  int64_t s = 512 / units;  // two workgroups per CU
+  s = s < keys / 8 ? s : keys / 8;
+  return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+}
+
+}  // namespace
+
+int tm_internal_kv8_splits(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups) {
+  return key_splits(c, b, row_tiles(b, groups));
+}
+int tm_internal_kv8_stats(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *q, int64_t qs_b,
+                          int64_t qs_h, int32_t n_heads, float scale, float2 *stats, hipStream_t s) {
+  AttArgs a = {};
+  a.c = *cache;
+  a.b = *batch;
+  a.groups = n_heads / cache->n_kv_heads;
+  const int64_t tiles = row_tiles(batch, a.groups);
+  a.splits = key_splits(cache, batch, tiles);
+  a.q = q, a.qs_t = qs_b, a.qs_h = qs_h;
+  a.stats = stats;
+  a.scale = scale;
+  a.heads = n_heads;
+  a.page_log2 = page_log2(cache->page_size);
+  a.tiles1 = (int)tm_cdiv(a.groups, 32);
+  const dim3 grid((unsigned)tiles, (unsigned)cache->n_kv_heads, (unsigned)a.splits);
+  auto run = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    switch (cache->head_dim) {
+      case 64: hipLaunchKernelGGL((attend_kernel<DT, 64, 0>), grid, dim3(kAttThreads), 0, s, a); break;
+      case 128: hipLaunchKernelGGL((attend_kernel<DT, 128, 0>), grid, dim3(kAttThreads), 0, s, a); break;
+      case 192: hipLaunchKernelGGL((attend_kernel<DT, 192, 0>), grid, dim3(kAttThreads), 0, s, a); break;
+      default: hipLaunchKernelGGL((attend_kernel<DT, 256, 0>), grid, dim3(kAttThreads), 0, s, a); break;
+    }
+  };
+  if (dtype == TM_DT_F16) run(std::integral_constant<int, TM_DT_F16>{});
+  else run(std::integral_constant<int, TM_DT_BF16>{});
+  TM_LAUNCH_CHECK("tm_kv8_importance(statistics)");
+  return TM_OK;
+}
+
+extern "C" size_t tm_kv8_attention_workspace_size(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t n_heads) {
+  if (!cache || !batch || n_heads < 1 || cache->n_kv_heads < 1 || n_heads % cache->n_kv_heads || batch->n_tokens <= 0)
+    return 0;
+  const int s = key_splits(cache, batch, row_tiles(batch, n_heads / cache->n_kv_heads));
+  if (s == 1) return 0;
+  return (size_t)batch->n_tokens * n_heads * s * (cache->v_dim + 2) * sizeof(float) + 16;
+}
+
+extern "C" int tm_kv8_attention(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *q,
+                                int64_t qs_t, int64_t qs_h, int32_t n_heads, float scale, int32_t causal, void *out,
+                                int64_t os_t, int64_t os_h, float *lse, void *workspace, size_t workspace_bytes,
+                                tm_stream_t stream) {
+  TM_REQUIRE(dtype == TM_DT_F16 || dtype == TM_DT_BF16, TM_EINVAL_DTYPE, "tm_kv8_attention: unsupported dtype tag %d",
+             (int)dtype);
+  const int bad = tm_kv8_check("tm_kv8_attention", cache, batch);
+  if (bad != TM_OK) return bad;
+  TM_REQUIRE(n_heads >= 1 && n_heads <= 4096 && n_heads % cache->n_kv_heads == 0, TM_EINVAL_SHAPE,
+             "tm_kv8_attention: %d query heads on %d key heads", n_heads, cache->n_kv_heads);
+  TM_REQUIRE(scale > 0.f && scale < __builtin_huge_valf(), TM_EINVAL_ARG, "tm_kv8_attention: scale must be positive and finite");
+  if (batch->n_tokens == 0 || batch->n_seqs == 0) return TM_OK;
+  TM_REQUIRE(q && out, TM_EINVAL_ARG, "tm_kv8_attention: null pointer");
+  TM_REQUIRE(tm_aligned16(q) && tm_aligned16(out) && qs_t % 8 == 0 && qs_h % 8 == 0 && os_t % 8 == 0 && os_h % 8 == 0,
+             TM_EINVAL_SHAPE, "tm_kv8_attention: rows of q and out must be 16-byte aligned, strides multiples of 8 elements");
+  AttArgs a = {};
+  a.c = *cache;
+  a.b = *batch;
+  if (cache->n_pages == 0) a.b.max_pages = 0;  // no page is there
+  a.groups = n_heads / cache->n_kv_heads;
+  const int64_t tiles = row_tiles(batch, a.groups);
+  TM_REQUIRE(tiles < ((int64_t)1 << 31), TM_EINVAL_SHAPE, "tm_kv8_attention: too many rows");
+  a.splits = key_splits(cache, batch, tiles);
+  const size_t need = tm_kv8_attention_workspace_size(cache, batch, n_heads);
+  TM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && tm_aligned16(workspace)), TM_EWORKSPACE,
+             "tm_kv8_attention: workspace %zu bytes < %zu", workspace_bytes, need);
+  a.q = q, a.qs_t = qs_t, a.qs_h = qs_h;
+  a.out = out, a.os_t = os_t, a.os_h = os_h;
+  a.lse = lse;
+  const int64_t rows = batch->n_tokens * n_heads * a.splits;
+  a.part = static_cast<float *>(workspace);
+  a.stats = reinterpret_cast<float2 *>(a.part + rows * cache->v_dim);
+  a.scale = scale;
+  a.heads = n_heads;
+  a.page_log2 = page_log2(cache->page_size);
+  a.causal = causal != 0;
+  a.tiles1 = (int)tm_cdiv(a.groups, 32);
+  hipStream_t s = tm_hip_stream(stream);
+  auto run = [&](auto dt, auto d, auto dv) {
+    constexpr int DT = decltype(dt)::value, D = decltype(d)::value, DV = decltype(dv)::value;
+    hipLaunchKernelGGL((attend_kernel<DT, D, DV>), dim3((unsigned)tiles, (unsigned)cache->n_kv_heads, (unsigned)a.splits),
+                       dim3(kAttThreads), 0, s, a);
+    TM_LAUNCH_CHECK("tm_kv8_attention");
+    if (a.splits > 1) {
+      const unsigned z = (unsigned)tm_cdiv(a.groups < 32 ? a.groups : 32, kWaves);
+      hipLaunchKernelGGL((join_kernel<DT, DV>), dim3((unsigned)tiles, (unsigned)cache->n_kv_heads, z), dim3(kAttThreads),
+                         0, s, a);
+      TM_LAUNCH_CHECK("tm_kv8_attention(join)");
+    }
+    return TM_OK;
+  };
+  auto columns = [&](auto dt) {
+    using std::integral_constant;
+    if (cache->head_dim == 64) return run(dt, integral_constant<int, 64>{}, integral_constant<int, 64>{});
+    if (cache->head_dim == 128) return run(dt, integral_constant<int, 128>{}, integral_constant<int, 128>{});
+    if (cache->head_dim == 256) return run(dt, integral_constant<int, 256>{}, integral_constant<int, 256>{});
+    if (cache->v_dim == 128) return run(dt, integral_constant<int, 192>{}, integral_constant<int, 128>{});
+    return run(dt, integral_constant<int, 192>{}, integral_constant<int, 192>{});
+  };
+  if (dtype == TM_DT_F16) return columns(std::integral_constant<int, TM_DT_F16>{});
+  return columns(std::integral_constant<int, TM_DT_BF16>{});
+}

@@ -1,0 +1,224 @@
+// Importance over the 8-bit cache: tm_kv8_importance.
+//
+// out[t] = 1/H sum over heads of exp(scale q_h . k_t - lse_h): with the rows'
+// log sum exp at hand (from the attention of the same query, or from a first
+// launch that reads K for the statistics alone) K is read once and nothing is
+// kept between.  Per 32 keys and key head one 32x32 product S = Q K^T, rows =
+// that head's queries: a lane has 16 rows of one key and adds them itself.  The
+// waves of a workgroup take the key heads and tiles of its keys between them and
+// join through LDS in a fixed order.
+#include "tm_internal.h"
+#include "tm_kv8_dev.h"
+
+#include <type_traits>
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kMaxHeads = 256;
+constexpr int kMaxPer = 16;  // tiles of a workgroup
+
+struct ImpArgs {
+  tm_kv8_cache c;
+  tm_kv8_batch b;
+  const void *q;
+  int64_t qs_b, qs_h;
+  const float *lse;
+  int64_t ld_lse;
+  const float2 *stats;
+  float *out;
+  int64_t ld_out, out_len;
+  float scale;
+  int32_t heads, groups, splits, page_log2, per, head_waves, lanes_log2;
+};
+
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void importance_kernel(ImpArgs a) {
+  using T = typename Elem<DT>::T;
+  constexpr int NK = D / 32;
+  __shared__ float norm[kMaxHeads];                // the rows' log2 sum exp
+  __shared__ float acc[kWaves][kMaxPer][32];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int c = lane & 31, g = lane >> 5;
+  const int64_t b = blockIdx.y, tile0 = (int64_t)blockIdx.x * a.per;
+  const int64_t cap = (int64_t)a.b.max_pages << a.page_log2;
+  int64_t len = a.b.lengths[b];
+  len = len < 0 ? 0 : len < cap ? len : cap;
+  const int64_t tiles = (len + 31) >> 5;
+  const int64_t end = tile0 + a.per < tiles ? tile0 + a.per : tiles;  // tiles to compute
+  if (tile0 < tiles) {
+    if (a.lse != nullptr) {
+      if (tid < a.heads) norm[tid] = a.lse[b * a.ld_lse + tid] * kLog2e;
+    } else {
+      const int lanes = 1 << a.lanes_log2, at = tid & (lanes - 1);
+      const int used = (int)((tiles + tm_kv8_per(tiles, a.splits) - 1) / tm_kv8_per(tiles, a.splits));
+      for (int h0 = 0; h0 < a.heads; h0 += kThreads >> a.lanes_log2) {
+        const int h = h0 + (tid >> a.lanes_log2);
+        const float2 *const st = a.stats + (b * a.heads + (h < a.heads ? h : a.heads - 1)) * a.splits;
+        float m = -__builtin_huge_valf(), l = 0.f;
+        for (int s = at; s < used; s += lanes) {
+          const float2 x = st[s];
+          const float to = fmaxf(m, x.x), base = to == -__builtin_huge_valf() ? 0.f : to;
+          l = l * __builtin_amdgcn_exp2f(m - base) + x.y * __builtin_amdgcn_exp2f(x.x - base);
+          m = to;
+        }
+        for (int o = 1; o < lanes; o <<= 1) {
+          const float om = __shfl_xor(m, o, 64), ol = __shfl_xor(l, o, 64);
+          const float to = fmaxf(m, om), base = to == -__builtin_huge_valf() ? 0.f : to;
+          l = l * __builtin_amdgcn_exp2f(m - base) + ol * __builtin_amdgcn_exp2f(om - base);
+          m = to;
+        }
+        if (at == 0 && h < a.heads) norm[h] = m + __builtin_amdgcn_logf(l);
+      }
+    }
+  }
+  for (int i = tid; i < kWaves * kMaxPer * 32; i += kThreads) (&acc[0][0][0])[i] = 0.f;
+  __syncthreads();
+
+  const int hw = a.head_waves;  // waves that share a tile's heads
+  const int my_head = wave % hw, my_tile = wave / hw, tile_waves = kWaves / hw;
+  const float unit = a.scale * kLog2e;
+  if (tile0 + my_tile < end)
+    for (int h = my_head; h < a.c.n_kv_heads; h += hw)
+      for (int r0 = 0; r0 < a.groups; r0 += 32) {
+        uint4 qf[NK][2];
+        const int row = r0 + c < a.groups ? r0 + c : a.groups - 1;
+        const T *const q = static_cast<const T *>(a.q) + b * a.qs_b + (h * a.groups + row) * a.qs_h + 16 * g;
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+          qf[j][0] = *reinterpret_cast<const uint4 *>(q + 32 * j);
+          qf[j][1] = *reinterpret_cast<const uint4 *>(q + 32 * j + 8);
+        }
+        float nr[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int r = r0 + 8 * (i / 4) + 4 * g + i % 4;
+          nr[i] = norm[h * a.groups + (r < a.groups ? r : a.groups - 1)];
+        }
+        auto step = [&](int64_t tile, const Kv8Place &w, const uint4 (&kf)[NK], float sk) {
+          tm_f32x16 s;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+          for (int j = 0; j < NK; ++j) {
+            s = tm_mfma32x32x16<DT>(qf[j][0], tm_kv8_operand<DT>(kf[j].x, kf[j].y), s);
+            s = tm_mfma32x32x16<DT>(qf[j][1], tm_kv8_operand<DT>(kf[j].z, kf[j].w), s);
+          }
+          const float mul = sk * unit;
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[i], mul, -nr[i]));
+            sum += r0 + 8 * (i / 4) + 4 * g + i % 4 < a.groups ? p : 0.f;
+          }
+          sum += tm_other_half(sum);
+          const int at = (int)(tile - tile0);
+          if (g == 0 && w.there) acc[wave][at][c] += sum;
+        };
+        uint4 ka[NK], kb[NK];
+        Kv8Place wa, wb;
+        float sa, sb;
+        auto fetch = [&](int64_t tile, Kv8Place &w, uint4 (&kf)[NK], float &sk) {
+          tile = tile < end ? tile : end - 1;
+          w = tm_kv8_place(a.c, a.b, b, h, tile, a.page_log2);
+          tm_kv8_load<NK>(a.c.k, w, a.page_log2, lane, kf);
+          sk = w.there ? a.c.k_scale[w.slot] : 1.f;
+        };
+        fetch(tile0 + my_tile, wa, ka, sa);
+        for (int64_t tile = tile0 + my_tile; tile < end; tile += 2 * tile_waves) {
+          fetch(tile + tile_waves, wb, kb, sb);
+          step(tile, wa, ka, sa);
+          if (tile + tile_waves >= end) break;
+          fetch(tile + 2 * tile_waves, wa, ka, sa);
+          step(tile + tile_waves, wb, kb, sb);
+        }
+      }
+  __syncthreads();
+  for (int i = tid; i < a.per * 32; i += kThreads) {
+    const int64_t t = tile0 * 32 + i;
+    if (t >= a.out_len) break;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v += acc[w][i >> 5][i & 31];
+    a.out[b * a.ld_out + t] = t < len ? v / (float)a.heads : 0.f;
+  }
+}
+
+}  // namespace
+
+extern "C" size_t tm_kv8_importance_workspace_size(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t n_heads) {
+  if (!cache || !batch || n_heads < 1 || cache->n_kv_heads < 1 || n_heads % cache->n_kv_heads || batch->n_seqs <= 0)
+    return 0;
+  tm_kv8_batch one = *batch;
+  one.starts = nullptr;
+  one.n_tokens = one.n_seqs;
+  return (size_t)batch->n_seqs * n_heads * tm_internal_kv8_splits(cache, &one, n_heads / cache->n_kv_heads) * sizeof(float2);
+}
+
+extern "C" int tm_kv8_importance(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *q,
+                                 int64_t qs_b, int64_t qs_h, int32_t n_heads, float scale, const float *lse,
+                                 int64_t ld_lse, int64_t out_len, float *out, int64_t ld_out, void *workspace,
+                                 size_t workspace_bytes, tm_stream_t stream) {
+  TM_REQUIRE(dtype == TM_DT_F16 || dtype == TM_DT_BF16, TM_EINVAL_DTYPE, "tm_kv8_importance: unsupported dtype tag %d",
+             (int)dtype);
+  TM_REQUIRE(cache && batch, TM_EINVAL_ARG, "tm_kv8_importance: null pointer");
+  tm_kv8_batch one = *batch;
+  one.starts = nullptr;
+  const int bad = tm_kv8_check("tm_kv8_importance", cache, &one);
+  if (bad != TM_OK) return bad;
+  TM_REQUIRE(n_heads >= 1 && n_heads <= kMaxHeads && n_heads % cache->n_kv_heads == 0, TM_EINVAL_SHAPE,
+             "tm_kv8_importance: %d query heads (at most %d) on %d key heads", n_heads, kMaxHeads, cache->n_kv_heads);
+  TM_REQUIRE(scale > 0.f && scale < __builtin_huge_valf(), TM_EINVAL_ARG, "tm_kv8_importance: scale must be positive and finite");
+  TM_REQUIRE(out_len >= 0 && out_len < ((int64_t)1 << 31) && ld_out >= out_len && batch->n_seqs < 65536 &&
+                 (lse == nullptr || ld_lse >= n_heads),
+             TM_EINVAL_SHAPE, "tm_kv8_importance: bad sizes (out_len %lld, %lld sequences)", (long long)out_len,
+             (long long)batch->n_seqs);
+  if (batch->n_seqs == 0 || out_len == 0) return TM_OK;
+  TM_REQUIRE(q && out, TM_EINVAL_ARG, "tm_kv8_importance: null pointer");
+  TM_REQUIRE(tm_aligned16(q) && qs_b % 8 == 0 && qs_h % 8 == 0, TM_EINVAL_SHAPE,
+             "tm_kv8_importance: rows of q must be 16-byte aligned, strides multiples of 8 elements");
+  ImpArgs a = {};
+  a.c = *cache;
+  if (cache->n_pages == 0) one.max_pages = 0;
+  a.b = one;
+  a.groups = n_heads / cache->n_kv_heads;
+  hipStream_t s = tm_hip_stream(stream);
+  a.splits = tm_internal_kv8_splits(cache, &one, a.groups);
+  if (lse == nullptr) {
+    const size_t need = tm_kv8_importance_workspace_size(cache, batch, n_heads);
+    TM_REQUIRE(workspace && workspace_bytes >= need && tm_aligned16(workspace), TM_EWORKSPACE,
+               "tm_kv8_importance: workspace %zu bytes < %zu", workspace_bytes, need);
+    a.stats = static_cast<const float2 *>(workspace);
+    const int st = tm_internal_kv8_stats(cache, &one, dtype, q, qs_b, qs_h, n_heads, scale,
+                                         static_cast<float2 *>(workspace), s);
+    if (st != TM_OK) return st;
+  }
+  a.q = q, a.qs_b = qs_b, a.qs_h = qs_h;
+  a.lse = lse, a.ld_lse = ld_lse;
+  a.out = out, a.ld_out = ld_out, a.out_len = out_len;
+  a.scale = scale;
+  a.heads = n_heads;
+  a.page_log2 = cache->page_size == 32 ? 5 : cache->page_size == 64 ? 6 : 7;
+  a.head_waves = cache->n_kv_heads >= 4 ? 4 : cache->n_kv_heads >= 2 ? 2 : 1;
+  while (a.lanes_log2 < 6 && (kThreads >> (a.lanes_log2 + 1)) >= n_heads) ++a.lanes_log2;
+  const int64_t tiles = tm_cdiv(out_len, 32);
+  int64_t per = tm_cdiv(tiles * one.n_seqs, 1024);
+  const int tile_waves = kWaves / a.head_waves;
+  per = tm_cdiv(per, tile_waves) * tile_waves;
+  a.per = (int)(per > kMaxPer ? kMaxPer : per);
+  const dim3 grid((unsigned)tm_cdiv(tiles, a.per), (unsigned)one.n_seqs);
+  auto run = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    switch (cache->head_dim) {
+      case 64: hipLaunchKernelGGL((importance_kernel<DT, 64>), grid, dim3(kThreads), 0, s, a); break;
+      case 128: hipLaunchKernelGGL((importance_kernel<DT, 128>), grid, dim3(kThreads), 0, s, a); break;
+      case 192: hipLaunchKernelGGL((importance_kernel<DT, 192>), grid, dim3(kThreads), 0, s, a); break;
+      default: hipLaunchKernelGGL((importance_kernel<DT, 256>), grid, dim3(kThreads), 0, s, a); break;
+    }
+  };
+  if (dtype == TM_DT_F16) run(std::integral_constant<int, TM_DT_F16>{});
+  else run(std::integral_constant<int, TM_DT_BF16>{});
+  TM_LAUNCH_CHECK("tm_kv8_importance");
+  return TM_OK;
+}

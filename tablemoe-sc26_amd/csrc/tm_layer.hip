@@ -274,6 +274,8 @@ extern "C" size_t tm_struct_size(int32_t which) {
     case 0: return sizeof(tm_table_layer);
     case 1: return sizeof(tm_layer_io);
     case 2: return sizeof(tm_fp8_experts);
+    case 3: return sizeof(tm_kv8_cache);
+    case 4: return sizeof(tm_kv8_batch);
     default: return 0;
   }
 }

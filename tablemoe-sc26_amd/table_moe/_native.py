@@ -63,6 +63,20 @@ class Fp8Experts(C.Structure):
                 ("w3", vp), ("s3", vp), ("w2", vp), ("s2", vp)]
 
 
+class Kv8Cache(C.Structure):
+    """Mirror of tm_kv8_cache (include/tablemoe.h)."""
+
+    _fields_ = [("n_pages", i64), ("n_kv_heads", i32), ("head_dim", i32), ("v_dim", i32), ("page_size", i32), ("k", vp),
+                ("v", vp), ("k_scale", vp), ("v_scale", vp)]
+
+
+class Kv8Batch(C.Structure):
+    """Mirror of tm_kv8_batch (include/tablemoe.h)."""
+
+    _fields_ = [("table", vp), ("ld_table", i64), ("lengths", vp), ("starts", vp), ("n_seqs", i64), ("n_tokens", i64),
+                ("max_pages", i32), ("reserved", i32)]
+
+
 # name -> (restype, argtypes); mirrors include/tablemoe.h
 PROTOTYPES = {
     "tm_version": (C.c_int, []),
@@ -78,6 +92,13 @@ PROTOTYPES = {
     "tm_fp8_grouped_swiglu": (C.c_int, [vp, i32, vp, i64, i64, vp, i32, i64, vp, i64, i64, vp, i64, i64, vp, sz, vp]),
     "tm_fp8_expert_swiglu_workspace_size": (sz, [vp, i64]),
     "tm_fp8_expert_swiglu": (C.c_int, [vp, i32, vp, i64, i64, vp, i64, vp, i64, vp, sz, vp]),
+    "tm_rotate_positions": (C.c_int, [i32, vp, i64, i32, i64, i64, vp, i32, i64, i64, i32, i32, vp, i64, i32, vp, i32, i32,
+                                      i32, vp, vp, i64, i64, vp, i64, i64, vp]),
+    "tm_kv8_append": (C.c_int, [vp, vp, i32, vp, i64, i64, vp, i64, i64, vp]),
+    "tm_kv8_attention_workspace_size": (sz, [vp, vp, i32]),
+    "tm_kv8_attention": (C.c_int, [vp, vp, i32, vp, i64, i64, i32, f32, i32, vp, i64, i64, vp, vp, sz, vp]),
+    "tm_kv8_importance_workspace_size": (sz, [vp, vp, i32]),
+    "tm_kv8_importance": (C.c_int, [vp, vp, i32, vp, i64, i64, i32, f32, vp, i64, i64, vp, i64, vp, sz, vp]),
     "tm_project_workspace_size": (sz, [i64, i32, i32]),
     "tm_project_packed_size": (sz, [i32, i32, i32]),
     "tm_project_pack": (C.c_int, [i32, vp, i32, i32, i64, i64, vp, sz, vp]),
@@ -159,7 +180,7 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
-        for which, struct in ((0, TableLayer), (1, LayerIO), (2, Fp8Experts)):
+        for which, struct in ((0, TableLayer), (1, LayerIO), (2, Fp8Experts), (3, Kv8Cache), (4, Kv8Batch)):
             if lib.tm_struct_size(which) != C.sizeof(struct):
                 raise RuntimeError(f"{struct.__name__} mirror ({C.sizeof(struct)} bytes) does not match the library "
                                    f"({lib.tm_struct_size(which)} bytes)")

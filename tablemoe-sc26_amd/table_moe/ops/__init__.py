@@ -12,6 +12,8 @@ _LAZY = {
     "Fp8Linear": "fp8_blocks",
     "Fp8GroupedExperts": "fp8_expert",
     "Fp8SharedExperts": "fp8_expert",
+    "rotate_positions": "rotary",
+    "Fp8KVCache": "fp8_cache",
 }
 
 __all__ = ["maybe_run_fp16_fused_expert", "qwen_topk_softmax", "expert_swiglu", "GroupedExperts", "SharedExperts",

@@ -1,0 +1,154 @@
+"""Rotary positions with several axes: text, images (row, column) and video
+(time, row, column), for the queries and keys whose scores the importance and
+the attention of this package take.
+
+One tm_rotate_positions call turns q and k: angles in 64 bits, the rotation in
+fp32, one rounding.  It is differentiable (the gradient is the rotation back).
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import functools
+
+import torch
+
+from .. import _native as N
+
+
+@functools.lru_cache(maxsize=64)
+def _sections(sections: tuple):
+    return (C.c_int32 * len(sections))(*sections)
+
+
+def rows_apart(t: torch.Tensor) -> bool:
+    """Whether the [T, H, D] view's rows of D do not overlap each other."""
+    (n, h, d), (st, sh, sd) = t.shape, t.stride()
+    if sd != 1 and d > 1:
+        return False
+    pairs = sorted((s, m) for s, m in ((st, n), (sh, h)) if m > 1)
+    end = d
+    for s, m in pairs:
+        if s < end:
+            return False
+        end = s * (m - 1) + end
+    return True
+
+
+def _span(t: torch.Tensor):
+    last = sum((m - 1) * s for m, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _check_out(name: str, out: torch.Tensor, x: torch.Tensor) -> None:
+    if out.shape != x.shape or out.dtype != x.dtype or not rows_apart(out):
+        raise ValueError(f"rotate_positions: {name} must be {tuple(x.shape)} {x.dtype} with unit stride along its last "
+                         "dimension and rows that do not overlap")
+    if out.numel() and not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
+        (a, b), (c, d) = _span(out), _span(x)
+        if a < d and c < b:
+            raise ValueError(f"rotate_positions: {name} may be the input itself, not overlap it otherwise")
+
+
+def _strides(t: torch.Tensor):
+    st, sh, _ = t.stride()
+    return st if t.shape[0] > 1 else 0, sh if t.shape[1] > 1 else 0
+
+
+def _run(q, k, positions, inv_freq, sections, interleaved, adjacent, inverse, q_out, k_out, dev):
+    n, h, d = q.shape
+    qs_t, qs_h = _strides(q)
+    qo_t, qo_h = _strides(q_out)
+    ks_t, ks_h = (0, 0) if k is None else _strides(k)
+    ko_t, ko_h = (0, 0) if k is None else _strides(k_out)
+    with N.on_device(dev):
+        N.call("tm_rotate_positions", N.dtype_tag(q.dtype), q.data_ptr(), n, h, qs_t, qs_h, N.ptr(k),
+               0 if k is None else k.shape[1], ks_t, ks_h, d, 2 * inv_freq.shape[0], positions.data_ptr(),
+               positions.stride(0) if positions.shape[0] > 1 else n, positions.shape[0], _sections(sections),
+               interleaved, adjacent, inverse, inv_freq.data_ptr(), q_out.data_ptr(), qo_t, qo_h, N.ptr(k_out), ko_t,
+               ko_h, N.stream(dev))
+
+
+def _unit_rows(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+class _Rotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, how):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.how = how
+        qq = _unit_rows(q)
+        kk = None if k is None else _unit_rows(k)
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        _run(qq, kk, positions, inv_freq, *how, q_out, k_out, q.device)
+        return q_out, k_out
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        positions, inv_freq = ctx.saved_tensors
+        sections, interleaved, adjacent, inverse = ctx.how
+        how = (sections, interleaved, adjacent, 1 - inverse)
+        # (the gradient of the part that is not asked for is not computed)
+        if not ctx.needs_input_grad[0]:
+            return None, _Rotate.apply(dk, None, positions, inv_freq, how)[0], None, None, None
+        dq, dk = _Rotate.apply(dq, dk if ctx.needs_input_grad[1] else None, positions, inv_freq, how)
+        return dq, dk, None, None, None
+
+
+def rotate_positions(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
+                     sections=None, *, interleaved: bool = False, adjacent: bool = False, inverse: bool = False,
+                     out=None):
+    """(q', k') of q [T, H, D] and k [T, Hkv, D] (or None), float32, float16 or
+    bfloat16, any strides with unit stride along D (others are copied).
+
+    positions: [A, T] integers, or [T] for one axis.  inv_freq [R / 2] float32:
+    frequency i turns with axis a(i); columns R .. D are copied.  sections (A
+    numbers summing to R / 2; default: all of one axis): runs of frequencies in
+    the axes' order; with ``interleaved`` a(i) = i % A where i < A * sections[i %
+    A], else 0.  Pairs are columns (i, i + R / 2), or (2i, 2i + 1) with
+    ``adjacent``.  ``inverse`` turns back.  angle = positions * inv_freq in 64
+    bits, the rest in fp32, rounded once.
+
+    out: a pair (q_out, k_out) to write to, which may be (q, k) themselves; then
+    there are no gradients.  Otherwise gradients of any order flow to q and k."""
+    dev = N.require_hip(q, k, positions, inv_freq)
+    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]
+                                           or k.dtype != q.dtype)):
+        raise ValueError("rotate_positions expects q [T, H, D] and k [T, Hkv, D] of one dtype")
+    N.dtype_tag(q.dtype)
+    n = q.shape[0]
+    if positions.dim() == 1:
+        positions = positions[None]
+    if positions.dim() != 2 or positions.shape[1] != n or positions.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"rotate_positions: positions must be [A, {n}] or [{n}] integers, got {tuple(positions.shape)} "
+                         f"{positions.dtype}")
+    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
+        raise ValueError("rotate_positions: inv_freq must be [R / 2] float32")
+    sections = (inv_freq.shape[0],) if sections is None else tuple(int(s) for s in sections)
+    if len(sections) != positions.shape[0]:
+        raise ValueError(f"rotate_positions: {len(sections)} sections for {positions.shape[0]} axes")
+    if positions.dtype != torch.int64:
+        positions = positions.long()
+    if (positions.stride(1) != 1 and n > 1) or (positions.stride(0) < n and positions.shape[0] > 1):
+        positions = positions.contiguous()
+    inv_freq = inv_freq if inv_freq.is_contiguous() else inv_freq.contiguous()
+    how = (sections, int(bool(interleaved)), int(bool(adjacent)), int(bool(inverse)))
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        if out is not None:
+            raise ValueError("rotate_positions: no gradients through out")
+        return _Rotate.apply(q, k, positions, inv_freq, how)
+    if out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
+    else:
+        q_out, k_out = out
+        if (k is None) != (k_out is None):
+            raise ValueError("rotate_positions: out holds a tensor for each of q and k")
+        N.require_hip(q, q_out, k_out)
+        _check_out("out[0]", q_out, q)
+        if k is not None:
+            _check_out("out[1]", k_out, k)
+    _run(_unit_rows(q), None if k is None else _unit_rows(k), positions, inv_freq, *how, q_out, k_out, dev)
+    return q_out, k_out

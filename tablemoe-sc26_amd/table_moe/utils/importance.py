@@ -87,3 +87,22 @@ def cache_last_token_attention(query_states: torch.Tensor, key_states: torch.Ten
     except (ValueError, RuntimeError):
         ModalityContext.set_attn_weights(None)
         return None
+
+
+def cached_importance(cache, query_states: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+                      scaling: float | None = None, lse: torch.Tensor | None = None,
+                      query_length: int | None = None):
+    """cache_last_token_attention over keys that live in an 8-bit cache
+    (table_moe.ops.Fp8KVCache): query_states [B, H, D], the last query of each
+    sequence after RoPE.  Stores and returns the scores of the first
+    query_length positions [B, query_length] (default: the table's width)."""
+    try:
+        with torch.no_grad():
+            mean_score = cache.importance(query_states, table, lengths, scale=scaling, lse=lse, out_len=query_length)
+            ModalityContext.set_attn_weights(mean_score.reshape(-1))
+            return mean_score
+    except N.NativeLibraryMissing:
+        raise
+    except (ValueError, RuntimeError):
+        ModalityContext.set_attn_weights(None)
+        return None
