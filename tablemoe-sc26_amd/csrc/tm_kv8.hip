@@ -29,82 +29,38 @@ __device__ __forceinline__ uint4 rescale16(uint4 v, float f) {
   return make_uint4(rescale4(v.x, f), rescale4(v.y, f), rescale4(v.z, f), rescale4(v.w, f));
 }
 
-// K: the rows [lo, hi) of the page from src (row 0 = the page's first token), the rows before lo times f.
-template <int DT, int D>
-__device__ void write_k(const typename Elem<DT>::T *src, int64_t s_t, int lo, int hi, float inv, float f,
-                        uint8_t *__restrict__ page) {
-  constexpr int kPieces = D / 16;  // of 16 columns
-  auto at = [&](int row, int p) {
-    return reinterpret_cast<uint4 *>(page + ((int64_t)(row >> 5) * (D / 32) + (p >> 1)) * 1024 + (p & 1) * 512 + (row & 31) * 16);
-  };
-  if (f != 1.f)
-    for (int i = threadIdx.x; i < lo * kPieces; i += kAppThreads) {
-      uint4 *const w = at(i / kPieces, i % kPieces);
-      *w = rescale16(*w, f);
-    }
-  for (int i = threadIdx.x; i < (hi - lo) * kPieces; i += kAppThreads) {
-    const int row = lo + i / kPieces, p = i % kPieces;
-    float a[8], b[8];
-    tm_load8<DT>(src + row * s_t + p * 16, a);
-    tm_load8<DT>(src + row * s_t + p * 16 + 8, b);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      a[e] = tm_fp8_quot(a[e], inv);
-      b[e] = tm_fp8_quot(b[e], inv);
-    }
-    *at(row, p) = make_uint4(tm_fp8_pack4(a[0], a[1], a[2], a[3]), tm_fp8_pack4(a[4], a[5], a[6], a[7]),
-                             tm_fp8_pack4(b[0], b[1], b[2], b[3]), tm_fp8_pack4(b[4], b[5], b[6], b[7]));
-  }
-}
-
-// V: a thread's 16 bytes hold 16 tokens of one column.
-template <int DT, int D>
-__device__ void write_v(const typename Elem<DT>::T *src, int64_t s_t, int lo, int hi, float inv, float f,
-                        uint8_t *__restrict__ page) {
-  const int t0 = f != 1.f ? 0 : lo >> 5, t1 = (hi + 31) >> 5;
-  for (int i = threadIdx.x; i < (t1 - t0) * D * 2; i += kAppThreads) {
-    const int tile = t0 + i / (D * 2), lane = i & 63, col = (i % (D * 2) >> 6) * 32 + (lane & 31), g = lane >> 5;
-    const int first = tile * 32 + 4 * g;  // byte e: token first + 16 (e / 8) + 8 (e / 4 % 2) + e % 4
-    uint4 *const w = reinterpret_cast<uint4 *>(page + ((int64_t)tile * (D / 32) + (col >> 5)) * 1024 + lane * 16);
-    // the tokens of this piece: [first, first + 28)
-    const bool whole = first >= lo && first + 28 <= hi;
-    if (!whole && (first >= hi || (first + 28 <= lo && f == 1.f))) continue;
-    uint4 old = make_uint4(0, 0, 0, 0);
-    if (!whole) old = *w;
-    uint32_t r[4] = {old.x, old.y, old.z, old.w};
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int tq = first + 8 * q;
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = tq + e;
-        v[e] = t >= lo && t < hi ? tm_fp8_quot(Elem<DT>::to_f(src[t * s_t + col]), inv) : 0.f;
-      }
-      const uint32_t now = tm_fp8_pack4(v[0], v[1], v[2], v[3]);
-      const uint32_t was = f != 1.f ? rescale4(r[q], f) : r[q];
-      uint32_t out = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = tq + e;
-        out |= (t < lo ? was : t < hi ? now : r[q]) & (0xffu << (8 * e));
-      }
-      r[q] = out;
-    }
-    *w = make_uint4(r[0], r[1], r[2], r[3]);
-  }
-}
-
-template <int DT, int D, bool V>
-__device__ void write_page(const typename Elem<DT>::T *src, int64_t s_t, int lo, int hi, uint8_t *page, float *scale) {
+// The new rows [lo, hi) of a page from src (row 0: the page's first token).  A thread owns four consecutive tokens by
+// 8 columns, read once and kept in registers over the search for the maximum: as bytes they are whole dwords of
+// V's pieces and halves of K's.  These meet in an image of the page in LDS, and what changes goes out as 16-byte pieces.
+template <int DT, int PAGE, int D, bool V>
+__device__ __forceinline__ void write_page(const typename Elem<DT>::T *src, int64_t s_t, int lo, int hi, uint8_t *image,
+                                           uint8_t *__restrict__ page, float *scale) {
+  using T = typename Elem<DT>::T;
   __shared__ uint32_t top[kAppThreads / 64];
-  constexpr int kVecs = D / 8;
+  constexpr int kCols = D / 8, kItems = PAGE / 4 * kCols, kOwn = (kItems + kAppThreads - 1) / kAppThreads;
+  struct alignas(16) Eight {
+    T v[8];
+  };
+  Eight r[kOwn][4];
   uint32_t m = 0;
-  for (int i = threadIdx.x; i < (hi - lo) * kVecs; i += kAppThreads) {
-    float v[8];
-    tm_load8<DT>(src + (lo + i / kVecs) * s_t + i % kVecs * 8, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = tm_fp8_amax(m, v[e]);
+  for (int o = 0; o < kOwn; ++o) {
+    const int i = o * kAppThreads + threadIdx.x, t = i / kCols * 4, c = i % kCols * 8;
+    if (i >= kItems || t >= hi || t + 4 <= lo) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {  // (a row that is not new: one that is again)
+      const int row = t + e < lo ? lo : t + e < hi ? t + e : hi - 1;
+      r[o][e] = *reinterpret_cast<const Eight *>(src + row * s_t + c);
+    }
+  }
+#pragma unroll
+  for (int o = 0; o < kOwn; ++o) {
+    const int i = o * kAppThreads + threadIdx.x, t = i / kCols * 4;
+    if (i >= kItems || t >= hi || t + 4 <= lo) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int x = 0; x < 8; ++x) m = tm_fp8_amax(m, Elem<DT>::to_f(r[o][e].v[x]));
   }
   const float before = *scale;
   m = tm_wave_max_u32(m);
@@ -113,23 +69,75 @@ __device__ void write_page(const typename Elem<DT>::T *src, int64_t s_t, int lo,
   m = max(max(top[0], top[1]), max(top[2], top[3]));
   float inv;
   float s = fmaxf(tm_fp8_scale(m, inv), kKv8MinScale);
-  float f = 1.f;
+  float f = 1.f;  // what the page held is taken times this
   if (lo > 0) {
     if (before > s) s = before;
     else f = before / s;  // powers of two
   }
   inv = 1.f / s;
   if (threadIdx.x == 0) *scale = s;
-  if constexpr (V) write_v<DT, D>(src, s_t, lo, hi, inv, f, page);
-  else write_k<DT, D>(src, s_t, lo, hi, inv, f, page);
+#pragma unroll
+  for (int o = 0; o < kOwn; ++o) {
+    const int i = o * kAppThreads + threadIdx.x, t = i / kCols * 4, c = i % kCols * 8;
+    if (i >= kItems || t >= hi || t + 4 <= lo) continue;
+    uint8_t *const tile = image + (t >> 5) * (32 * D) + (c >> 5) * 1024;
+    auto q = [&](int e, int x) { return tm_fp8_quot(Elem<DT>::to_f(r[o][e].v[x]), inv); };
+    if constexpr (V) {
+      uint8_t *const at = tile + ((t >> 2 & 1) * 32 + (c & 31)) * 16 + (t >> 3 & 3) * 4;
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        *reinterpret_cast<uint32_t *>(at + x * 16) = tm_fp8_pack4(q(0, x), q(1, x), q(2, x), q(3, x));
+    } else {
+      uint8_t *const at = tile + ((c >> 4 & 1) * 32 + (t & 31)) * 16 + (c & 8);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<uint2 *>(at + e * 16) = make_uint2(tm_fp8_pack4(q(e, 0), q(e, 1), q(e, 2), q(e, 3)),
+                                                            tm_fp8_pack4(q(e, 4), q(e, 5), q(e, 6), q(e, 7)));
+    }
+  }
+  __syncthreads();
+  // the tiles with new tokens, those before them too where they are rounded again
+  const int first = f != 1.f ? 0 : lo >> 5, last = (hi - 1) >> 5;
+  for (int i = first * (2 * D) + threadIdx.x; i < (last + 1) * (2 * D); i += kAppThreads) {
+    const int lane = i & 63, t = i / (2 * D) * 32;
+    uint4 *const w = reinterpret_cast<uint4 *>(page) + i;
+    const uint4 now = reinterpret_cast<const uint4 *>(image)[i];
+    if constexpr (!V) {
+      const int row = t + (lane & 31);
+      if (row >= hi || (row < lo && f == 1.f)) continue;
+      *w = row < lo ? rescale16(*w, f) : now;
+    } else {
+      const int t0 = t + 4 * (lane >> 5);  // dword q: tokens t0 + 8 q ..+3
+      if (t0 >= lo && t0 + 28 <= hi) {
+        *w = now;
+        continue;
+      }
+      if (t0 >= hi || (t0 + 28 <= lo && f == 1.f)) continue;
+      const uint4 old = *w;
+      const uint32_t o[4] = {old.x, old.y, old.z, old.w}, n[4] = {now.x, now.y, now.z, now.w};
+      uint32_t out[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t was = f != 1.f ? rescale4(o[q], f) : o[q];
+        out[q] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int x = t0 + 8 * q + e;
+          out[q] |= (x < lo ? was : x < hi ? n[q] : o[q]) & (0xffu << (8 * e));
+        }
+      }
+      *w = make_uint4(out[0], out[1], out[2], out[3]);
+    }
+  }
 }
 
-template <int DT, int D, int DV>
+template <int DT, int PAGE, int D, int DV>
 __global__ __launch_bounds__(kAppThreads) void append_kernel(AppArgs a) {
   using T = typename Elem<DT>::T;
   const int h = blockIdx.y;
   const bool vals = blockIdx.z != 0;
-  const int page = a.c.page_size;
+  __shared__ __align__(16) uint8_t image[PAGE * (D > DV ? D : DV)];
+  constexpr int page = PAGE;
   int64_t b = blockIdx.x, j = 0;
   if (a.b.starts != nullptr) b = tm_kv8_unit(a.b, blockIdx.x, 1, page, 2, j);
   const Kv8Seq s = tm_kv8_seq(a.b, b);
@@ -145,10 +153,10 @@ __global__ __launch_bounds__(kAppThreads) void append_kernel(AppArgs a) {
   const int64_t at = id * a.c.n_kv_heads + h;
   if (vals) {
     const T *const src = static_cast<const T *>(a.src[1]) + row0 * a.s_t[1] + h * a.s_h[1];
-    write_page<DT, DV, true>(src, a.s_t[1], lo, hi, static_cast<uint8_t *>(a.c.v) + at * page * DV, a.c.v_scale + at);
+    write_page<DT, PAGE, DV, true>(src, a.s_t[1], lo, hi, image, static_cast<uint8_t *>(a.c.v) + at * page * DV, a.c.v_scale + at);
   } else {
     const T *const src = static_cast<const T *>(a.src[0]) + row0 * a.s_t[0] + h * a.s_h[0];
-    write_page<DT, D, false>(src, a.s_t[0], lo, hi, static_cast<uint8_t *>(a.c.k) + at * page * D, a.c.k_scale + at);
+    write_page<DT, PAGE, D, false>(src, a.s_t[0], lo, hi, image, static_cast<uint8_t *>(a.c.k) + at * page * D, a.c.k_scale + at);
   }
 }
 
@@ -193,10 +201,16 @@ extern "C" int tm_kv8_append(const tm_kv8_cache *cache, const tm_kv8_batch *batc
   const dim3 grid((unsigned)units, (unsigned)cache->n_kv_heads, 2);
   hipStream_t s = tm_hip_stream(stream);
   return TM_DISPATCH_DTYPE(dtype, DT, [&] {
-    auto launch = [&](auto d, auto dv) {
-      hipLaunchKernelGGL((append_kernel<DT, decltype(d)::value, decltype(dv)::value>), grid, dim3(kAppThreads), 0, s, a);
-    };
     using std::integral_constant;
+    auto launch = [&](auto d, auto dv) {
+      auto go = [&](auto page) {
+        hipLaunchKernelGGL((append_kernel<DT, decltype(page)::value, decltype(d)::value, decltype(dv)::value>), grid,
+                           dim3(kAppThreads), 0, s, a);
+      };
+      if (cache->page_size == 32) go(integral_constant<int, 32>{});
+      else if (cache->page_size == 64) go(integral_constant<int, 64>{});
+      else go(integral_constant<int, 128>{});
+    };
     if (cache->head_dim == 64) launch(integral_constant<int, 64>{}, integral_constant<int, 64>{});
     else if (cache->head_dim == 128) launch(integral_constant<int, 128>{}, integral_constant<int, 128>{});
     else if (cache->head_dim == 256) launch(integral_constant<int, 256>{}, integral_constant<int, 256>{});
