@@ -692,7 +692,7 @@ int tm_kv8_append(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t 
  * its sequence's cached positions: those up to its own with causal != 0, all
  * otherwise.  q [n_tokens, n_heads, head_dim]; head i reads key head
  * i / (n_heads / n_kv_heads).  fp32 scores, maxima and sums; a probability is
- * rounded to `dtype` (F16 or BF16) before it meets the values.  lse (nullable,
+ * rounded to fp16 before it meets the values.  lse (nullable,
  * fp32 [n_tokens, n_heads] contiguous) = log sum exp of the scores, natural.  A
  * token that sees nothing gets zeros and -inf; rows of no sequence are left as
  * they were.  16-byte aligned rows of q and out; scale > 0; workspace

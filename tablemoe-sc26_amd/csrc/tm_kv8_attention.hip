@@ -6,11 +6,15 @@
 //   lane holding 16 keys of one row;  x = S^T sk scale log2(e) + log2(sv);
 //   P = 2^(x - m) under a running reference m of the row, so that the values'
 //   scale rides in P and V enters as the bytes stand;  O^T += V^T P.
-// With l = sum P / sv the result is O / l and log sum exp = (m + log2 l) ln 2.
-// m follows the running maximum of x only when that has grown by more than 2^6
-// (P <= 64 then), so O is seldom scaled again.  P is rounded to the queries'
-// type for the second product (half a step of 2^-8 or 2^-11 of each probability,
-// which average out); all sums are fp32.
+// With l = sum P / sv the result is O / l and log sum exp = (m + log2 l) ln 2 (sv >=
+// 2^-100: l stays in range).
+// m is 2^8 under a running maximum of x and follows it only when that has grown by
+// more than 2^6, so O is seldom scaled again and P lies in [0, 2^14].  P is rounded
+// to fp16 for the second product whatever the queries' type, and V's bytes become
+// fp16 (exact): half a step is 2^-12 of a probability, where bf16 would leave
+// 2^-9 (an output's error against 64 bits 1.9e-3 of its size instead of 1.6e-3, which
+// is its own rounding); what lies under 2^-33 of a row's largest is lost.  All
+// sums are fp32.
 //
 // The four waves of a workgroup take every fourth tile of keys and join through
 // LDS.  Where rows alone do not fill the device, the keys are split over
@@ -25,7 +29,7 @@ namespace {
 constexpr int kAttThreads = 256;
 constexpr int kWaves = kAttThreads / 64;
 constexpr int kMaxSplits = 128;
-constexpr float kGrow = 6.f;
+constexpr float kRoom = 8.f, kGrow = 6.f;  // log2 of a new maximum's P, of what it may grow by
 
 struct AttArgs {
   tm_kv8_cache c;
@@ -153,8 +157,8 @@ __global__ __launch_bounds__(kAttThreads, D + DV > 320 ? 1 : 2) void attend_kern
     const float mul = sk * unit, add = tm_exponent(sv);
     top = fmaf(top, mul, add);
     top = fmaxf(top, tm_other_half(top));
-    if (__any(top > m + kGrow || (m == -__builtin_huge_valf() && top > m))) {
-      const float to = fmaxf(m, top);
+    if (__any(top > m + (kRoom + kGrow) || (m == -__builtin_huge_valf() && top > m))) {
+      const float to = fmaxf(m, top - kRoom);
       const float f = m == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(m - to);
       m = to;
       l *= f;
@@ -171,17 +175,17 @@ __global__ __launch_bounds__(kAttThreads, D + DV > 320 ? 1 : 2) void attend_kern
       const float x = __builtin_amdgcn_exp2f(fmaf(s[i], mul, off)), y = __builtin_amdgcn_exp2f(fmaf(s[i + 1], mul, off));
       sum += x + y;
       if constexpr (NV > 0) {
-        typename Elem<DT>::T two[2] = {Elem<DT>::from_f(x), Elem<DT>::from_f(y)};
+        const _Float16 two[2] = {(_Float16)x, (_Float16)y};
         pf[i / 2] = __builtin_bit_cast(uint32_t, two);
       }
     }
-    l = fmaf(sum, __builtin_amdgcn_exp2f(-add), l);
+    l = fmaf(sum, __builtin_amdgcn_exp2f(-add - kRoom), l);
     if constexpr (NV > 0) {
       const uint4 p0 = make_uint4(pf[0], pf[1], pf[2], pf[3]), p1 = make_uint4(pf[4], pf[5], pf[6], pf[7]);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        o[j] = tm_mfma32x32x16<DT>(tm_kv8_operand<DT>(vf[j].x, vf[j].y), p0, o[j]);
-        o[j] = tm_mfma32x32x16<DT>(tm_kv8_operand<DT>(vf[j].z, vf[j].w), p1, o[j]);
+        o[j] = tm_mfma32x32x16<TM_DT_F16>(tm_kv8_operand<TM_DT_F16>(vf[j].x, vf[j].y), p0, o[j]);
+        o[j] = tm_mfma32x32x16<TM_DT_F16>(tm_kv8_operand<TM_DT_F16>(vf[j].z, vf[j].w), p1, o[j]);
       }
       if (edge && __any(nan_bytes != 0)) {  // those that a row does see make its column NaN
         const uint8_t *const vb = static_cast<const uint8_t *>(a.c.v) +
@@ -223,6 +227,7 @@ __global__ __launch_bounds__(kAttThreads, D + DV > 320 ? 1 : 2) void attend_kern
     }
   }
   l += tm_other_half(l);
+  m += kRoom;  // (a P of 1 stands for 2^(x - m) now, O for 2^kRoom times its sum)
   if (g == 0) join[wave][c] = make_float2(m, l);
   __syncthreads();
   float top = -__builtin_huge_valf(), total = 0.f;
@@ -239,7 +244,7 @@ __global__ __launch_bounds__(kAttThreads, D + DV > 320 ? 1 : 2) void attend_kern
   }
   if constexpr (NV > 0) {
     __shared__ float inv[32];
-    if (wave == 0 && g == 0) inv[c] = total == 0.f ? 0.f : 1.f / total;
+    if (wave == 0 && g == 0) inv[c] = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(-kRoom) / total;
 #pragma unroll
     for (int half = 0; half < DV / kChunk; ++half) {
 #pragma unroll
@@ -276,40 +281,63 @@ __global__ __launch_bounds__(kAttThreads, D + DV > 320 ? 1 : 2) void attend_kern
   }
 }
 
-// Joins the splits of a row tile: a wave per row.
-template <int DT, int DV>
+// Joins the splits of a row: a workgroup per row, a thread owning 4 columns of some splits, whose
+// parts are requested together with the statistics.
+template <int DT, int DV, int OWN>
 __global__ __launch_bounds__(kAttThreads) void join_kernel(AttArgs a) {
   using T = typename Elem<DT>::T;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = blockIdx.y;
+  constexpr int kCols = DV / 4, kSets = kAttThreads / kCols;  // OWN: splits of a thread
+  __shared__ float fac[kMaxSplits];
+  __shared__ __align__(16) float4 red[kSets][kCols];
+  const int h = blockIdx.y;
   RowTile t;
-  if (!row_tile(a, blockIdx.x, t) || t.per >= t.tiles) return;
+  if (!row_tile(a, blockIdx.x, t) || t.per >= t.tiles || (int)blockIdx.z >= t.rows) return;
   const int n = (int)((t.tiles + t.per - 1) / t.per);
-  for (int r = blockIdx.z * kWaves + wave; r < t.rows; r += kWaves * gridDim.z) {
-    const int64_t rr = t.r0 + r, tok = rr / a.groups, head = h * a.groups + (rr - tok * a.groups);
-    const int64_t row = (t.s.first + tok) * a.heads + head;
-    const float2 *const st = a.stats + row * a.splits;
-    const float2 x0 = lane < n ? st[lane] : make_float2(-__builtin_huge_valf(), 0.f);
-    const float2 x1 = lane + 64 < n ? st[lane + 64] : make_float2(-__builtin_huge_valf(), 0.f);
-    const float top = tm_wave_max(fmaxf(x0.x, x1.x));
-    const float base = top == -__builtin_huge_valf() ? 0.f : top;
-    const float f0 = __builtin_amdgcn_exp2f(x0.x - base), f1 = __builtin_amdgcn_exp2f(x1.x - base);
-    const float total = tm_wave_sum(x0.y * f0 + x1.y * f1);
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    if (a.lse && lane == 0) a.lse[row] = total == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(total)) * kLn2;
-    constexpr int kPer = DV / 64;
-    float v[kPer];
+  const int64_t rr = t.r0 + blockIdx.z, tok = rr / a.groups, head = h * a.groups + (rr - tok * a.groups);
+  const int64_t row = (t.s.first + tok) * a.heads + head;
+  const int col = threadIdx.x % kCols, set = threadIdx.x / kCols, lane = threadIdx.x & 63;
+  const float *const p = a.part + row * a.splits * DV + col * 4;
+  float4 v[OWN];
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) v[k] = 0.f;
-    const float *const p = a.part + row * a.splits * DV + lane * kPer;
-    for (int s = 0; s < n; ++s) {
-      const float f = __shfl(s < 64 ? f0 : f1, s & 63, 64);
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) v[k] = fmaf(p[(int64_t)s * DV + k], f, v[k]);
-    }
-    T *const y = static_cast<T *>(a.out) + (t.s.first + tok) * a.os_t + head * a.os_h + lane * kPer;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) y[k] = Elem<DT>::from_f(v[k] * inv);
+  for (int i = 0; i < OWN; ++i) {
+    const int s = set + i * kSets;
+    v[i] = *reinterpret_cast<const float4 *>(p + (int64_t)(s < n ? s : 0) * DV);
   }
+  const float2 *const st = a.stats + row * a.splits;
+  const float2 none = make_float2(-__builtin_huge_valf(), 0.f);
+  const float2 x0 = lane < n ? st[lane] : none, x1 = lane + 64 < n ? st[lane + 64] : none;
+  const float top = tm_wave_max(fmaxf(x0.x, x1.x));
+  const float base = top == -__builtin_huge_valf() ? 0.f : top;
+  const float f0 = __builtin_amdgcn_exp2f(x0.x - base), f1 = __builtin_amdgcn_exp2f(x1.x - base);
+  const float total = tm_wave_sum(x0.y * f0 + x1.y * f1);
+  if (threadIdx.x < 64) {
+    fac[lane] = f0;
+    fac[lane + 64] = f1;
+  }
+  __syncthreads();
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (set < kSets) {
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      const int s = set + i * kSets;
+      if (s < n) {
+        const float f = fac[s];
+        y.x = fmaf(v[i].x, f, y.x), y.y = fmaf(v[i].y, f, y.y), y.z = fmaf(v[i].z, f, y.z), y.w = fmaf(v[i].w, f, y.w);
+      }
+    }
+    red[set][col] = y;
+  }
+  __syncthreads();
+  if (set != 0) return;
+#pragma unroll
+  for (int s = 1; s < kSets; ++s) {
+    const float4 x = red[s][col];
+    y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
+  }
+  const float inv = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(-kRoom) / total;
+  T o[4] = {Elem<DT>::from_f(y.x * inv), Elem<DT>::from_f(y.y * inv), Elem<DT>::from_f(y.z * inv), Elem<DT>::from_f(y.w * inv)};
+  __builtin_memcpy(static_cast<T *>(a.out) + (t.s.first + tok) * a.os_t + head * a.os_h + col * 4, o, 8);
+  if (a.lse && threadIdx.x == 0) a.lse[row] = total == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
 int page_log2(int page) { return page == 32 ? 5 : page == 64 ? 6 : 7; }
@@ -413,9 +441,11 @@ extern "C" int tm_kv8_attention(const tm_kv8_cache *cache, const tm_kv8_batch *b
                        dim3(kAttThreads), 0, s, a);
     TM_LAUNCH_CHECK("tm_kv8_attention");
     if (a.splits > 1) {
-      const unsigned z = (unsigned)tm_cdiv(a.groups < 32 ? a.groups : 32, kWaves);
-      hipLaunchKernelGGL((join_kernel<DT, DV>), dim3((unsigned)tiles, (unsigned)cache->n_kv_heads, z), dim3(kAttThreads),
-                         0, s, a);
+      // (rows of a tile: one token's heads, or 32 of several tokens)
+      const dim3 grid((unsigned)tiles, (unsigned)cache->n_kv_heads, (unsigned)(!batch->starts && a.groups < 32 ? a.groups : 32));
+      constexpr int kSets = kAttThreads / (DV / 4);
+      if (a.splits <= 4 * kSets) hipLaunchKernelGGL((join_kernel<DT, DV, 4>), grid, dim3(kAttThreads), 0, s, a);
+      else hipLaunchKernelGGL((join_kernel<DT, DV, (kMaxSplits + kSets - 1) / kSets>), grid, dim3(kAttThreads), 0, s, a);
       TM_LAUNCH_CHECK("tm_kv8_attention(join)");
     }
     return TM_OK;
