@@ -192,6 +192,8 @@ extern "C" int tm_kv8_append(const tm_kv8_cache *cache, const tm_kv8_batch *batc
   if (bad != TM_OK) return bad;
   if (batch->n_tokens == 0 || batch->n_seqs == 0 || cache->n_pages == 0 || batch->max_pages == 0) return TM_OK;
   TM_REQUIRE(k && v, TM_EINVAL_ARG, "tm_kv8_append: null pointer");
+  if (batch->n_tokens == 1) ks_t = vs_t = 0;  // (the stride of a single row means nothing)
+  if (cache->n_kv_heads == 1) ks_h = vs_h = 0;
   TM_REQUIRE(tm_aligned16(k) && tm_aligned16(v) && ks_t % 8 == 0 && ks_h % 8 == 0 && vs_t % 8 == 0 && vs_h % 8 == 0,
              TM_EINVAL_SHAPE, "tm_kv8_append: rows of k and v must be 16-byte aligned, strides multiples of 8 elements");
   AppArgs a = {*cache, *batch, {k, v}, {ks_t, vs_t}, {ks_h, vs_h}};

@@ -410,6 +410,8 @@ extern "C" int tm_kv8_attention(const tm_kv8_cache *cache, const tm_kv8_batch *b
   TM_REQUIRE(scale > 0.f && scale < __builtin_huge_valf(), TM_EINVAL_ARG, "tm_kv8_attention: scale must be positive and finite");
   if (batch->n_tokens == 0 || batch->n_seqs == 0) return TM_OK;
   TM_REQUIRE(q && out, TM_EINVAL_ARG, "tm_kv8_attention: null pointer");
+  if (batch->n_tokens == 1) qs_t = os_t = 0;  // (the stride of a single row means nothing)
+  if (n_heads == 1) qs_h = os_h = 0;
   TM_REQUIRE(tm_aligned16(q) && tm_aligned16(out) && qs_t % 8 == 0 && qs_h % 8 == 0 && os_t % 8 == 0 && os_h % 8 == 0,
              TM_EINVAL_SHAPE, "tm_kv8_attention: rows of q and out must be 16-byte aligned, strides multiples of 8 elements");
   AttArgs a = {};

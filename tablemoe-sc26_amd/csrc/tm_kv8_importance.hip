@@ -176,6 +176,8 @@ extern "C" int tm_kv8_importance(const tm_kv8_cache *cache, const tm_kv8_batch *
              (long long)batch->n_seqs);
   if (batch->n_seqs == 0 || out_len == 0) return TM_OK;
   TM_REQUIRE(q && out, TM_EINVAL_ARG, "tm_kv8_importance: null pointer");
+  if (batch->n_seqs == 1) qs_b = 0;  // (the stride of a single row means nothing)
+  if (n_heads == 1) qs_h = 0;
   TM_REQUIRE(tm_aligned16(q) && qs_b % 8 == 0 && qs_h % 8 == 0, TM_EINVAL_SHAPE,
              "tm_kv8_importance: rows of q must be 16-byte aligned, strides multiples of 8 elements");
   ImpArgs a = {};

@@ -166,9 +166,12 @@ extern "C" int tm_rotate_positions(int32_t dtype, const void *q, int64_t n_token
   RotArgs a = {};
   a.in[0] = q, a.in[1] = k;
   a.out[0] = q_out, a.out[1] = k_out;
-  a.in_t[0] = qs_t, a.in_h[0] = qs_h, a.in_t[1] = ks_t, a.in_h[1] = ks_h;
-  a.out_t[0] = qo_t, a.out_h[0] = qo_h, a.out_t[1] = ko_t, a.out_h[1] = ko_h;
   a.heads[0] = n_heads, a.heads[1] = k ? n_kv_heads : 0;
+  const int64_t in_t[2] = {qs_t, ks_t}, in_h[2] = {qs_h, ks_h}, out_t[2] = {qo_t, ko_t}, out_h[2] = {qo_h, ko_h};
+  for (int w = 0; w < 2; ++w) {  // (the stride of a single token or head means nothing)
+    a.in_t[w] = n_tokens > 1 ? in_t[w] : 0, a.in_h[w] = a.heads[w] > 1 ? in_h[w] : 0;
+    a.out_t[w] = n_tokens > 1 ? out_t[w] : 0, a.out_h[w] = a.heads[w] > 1 ? out_h[w] : 0;
+  }
   a.n = n_tokens;
   a.pos = positions, a.ld_pos = ld_positions, a.inv = inv_freq;
   a.half = rotary_dim / 2, a.dim = head_dim, a.axes = n_axes, a.interleaved = interleaved != 0;

@@ -15,6 +15,7 @@ from .. import _native as N
 from .rotary import _strides, rows_apart
 
 TILE = 32
+_TAG16 = {torch.float16: N.TM_DT_F16, torch.bfloat16: N.TM_DT_BF16}
 
 
 def _int32(name: str, t: torch.Tensor, dims: int) -> torch.Tensor:
@@ -23,13 +24,16 @@ def _int32(name: str, t: torch.Tensor, dims: int) -> torch.Tensor:
     return t if t.dtype == torch.int32 else t.to(torch.int32)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t [T, H, D], or a copy of it, with 16-byte aligned rows."""
-    st, sh = _strides(t)
-    if t.stride(2) != 1 or st % 8 or sh % 8 or t.data_ptr() % 16:
+def _rows(t: torch.Tensor):
+    """(t [T, H, D] or a copy of it with 16-byte aligned rows, its strides)."""
+    if not t.is_contiguous() or t.data_ptr() % 16:
+        st, sh = _strides(t)
+        if t.stride(2) == 1 and st % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0:
+            return t, st, sh
         t = t.contiguous()
         t = t if t.data_ptr() % 16 == 0 else t.clone()
-    return t
+    _, h, d = t.shape
+    return t, h * d, d
 
 
 class Fp8KVCache:
@@ -94,6 +98,7 @@ class Fp8KVCache:
         self._desc = N.Kv8Cache(self.n_pages, self.n_kv_heads, self.head_dim, self.v_dim, self.page_size, k.data_ptr(),
                                 v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
         self._ref = C.byref(self._desc)
+        self._scale = self.head_dim ** -0.5
 
     def read_pages(self, pages: torch.Tensor | None = None):
         """(K [n, heads, page_size, head_dim], V [n, heads, page_size, v_dim]) float32 of the given pages (all)."""
@@ -106,21 +111,27 @@ class Fp8KVCache:
         v = v.permute(0, 1, 2, 6, 7, 4, 8, 3, 5).reshape(n, h, self.page_size, self.v_dim)
         return k.float() * pick(self.k_scale)[:, :, None, None], v.float() * pick(self.v_scale)[:, :, None, None]
 
-    def _batch(self, table, lengths, starts, n_tokens, *others):
-        N.require_hip(self.k, table, lengths, starts, *others)
-        table, lengths = _int32("table", table, 2), _int32("lengths", lengths, 1)
+    def _batch(self, table, lengths, starts, n_tokens):
+        """(tm_kv8_batch, the tensors that it points to): int32, as they are or converted."""
+        dev = self.device
+        if table.device != dev or lengths.device != dev or (starts is not None and starts.device != dev):
+            N.require_hip(self.k, table, lengths, starts)
+        if table.dtype is not torch.int32 or table.dim() != 2:
+            table = _int32("table", table, 2)
+        if lengths.dtype is not torch.int32 or lengths.dim() != 1:
+            lengths = _int32("lengths", lengths, 1)
         b, most = table.shape
-        if table.stride(1) != 1 and most > 1 or table.stride(0) < most and b > 1:
+        if not table.is_contiguous() and (table.stride(1) != 1 and most > 1 or table.stride(0) < most and b > 1):
             table = table.contiguous()
-        lengths = lengths if lengths.is_contiguous() else lengths.contiguous()
+        if not lengths.is_contiguous():
+            lengths = lengths.contiguous()
         if starts is not None:
-            starts = _int32("starts", starts, 1)
-            starts = starts if starts.is_contiguous() else starts.contiguous()
+            starts = _int32("starts", starts, 1).contiguous()
         if lengths.shape[0] != b or (n_tokens != b if starts is None else starts.shape[0] != b + 1):
             raise ValueError(f"Fp8KVCache: table {tuple(table.shape)}, lengths {tuple(lengths.shape)}, starts "
                              f"{None if starts is None else tuple(starts.shape)} and {n_tokens} rows do not go together")
-        batch = N.Kv8Batch(table.data_ptr(), table.stride(0) if b > 1 else most, lengths.data_ptr(), N.ptr(starts), b,
-                           n_tokens, most, 0)
+        batch = N.Kv8Batch(table.data_ptr(), table.stride(0) if b > 1 else most, lengths.data_ptr(),
+                           None if starts is None else starts.data_ptr(), b, n_tokens, most, 0)
         return batch, (table, lengths, starts)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
@@ -132,25 +143,30 @@ class Fp8KVCache:
         stored as NaN.  A page that is written belongs to one sequence."""
         n = k.shape[0]
         if k.shape != (n, self.n_kv_heads, self.head_dim) or v.shape != (n, self.n_kv_heads, self.v_dim) \
-                or k.dtype != v.dtype:
+                or k.dtype is not v.dtype:
             raise ValueError(f"Fp8KVCache.append: k must be [T, {self.n_kv_heads}, {self.head_dim}] and v [T, "
                              f"{self.n_kv_heads}, {self.v_dim}] of one dtype, got {tuple(k.shape)} {k.dtype} and "
                              f"{tuple(v.shape)} {v.dtype}")
         tag = N.dtype_tag(k.dtype)
-        batch, kept = self._batch(table, lengths, starts, n, k, v)
-        k, v = _rows(k), _rows(v)
-        ks_t, ks_h = _strides(k)
-        vs_t, vs_h = _strides(v)
-        with N.on_device(self.device):
+        dev = self.device
+        if k.device != dev or v.device != dev:
+            N.require_hip(self.k, k, v)
+        batch, kept = self._batch(table, lengths, starts, n)
+        k, ks_t, ks_h = _rows(k)
+        v, vs_t, vs_h = _rows(v)
+        with N.on_device(dev):
             N.call("tm_kv8_append", self._ref, C.byref(batch), tag, k.data_ptr(), ks_t, ks_h, v.data_ptr(), vs_t, vs_h,
-                   N.stream(self.device))
+                   N.stream(dev))
 
     def _queries(self, q, scale):
-        if q.dim() != 3 or q.shape[2] != self.head_dim or q.shape[1] % self.n_kv_heads or q.shape[1] == 0 \
-                or q.dtype not in (torch.float16, torch.bfloat16):
+        """(dtype tag, scale) of checked queries."""
+        tag = _TAG16.get(q.dtype)
+        if tag is None or q.dim() != 3 or q.shape[2] != self.head_dim or q.shape[1] % self.n_kv_heads or q.shape[1] == 0:
             raise ValueError(f"Fp8KVCache: q must be [T, heads, {self.head_dim}] float16 or bfloat16, its heads a "
                              f"multiple of {self.n_kv_heads}, got {tuple(q.shape)} {q.dtype}")
-        return self.head_dim ** -0.5 if scale is None else float(scale)
+        if q.device != self.device:
+            N.require_hip(self.k, q)
+        return tag, (self._scale if scale is None else float(scale))
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None = None, *,
                scale: float | None = None, causal: bool = True, out: torch.Tensor | None = None,
@@ -162,25 +178,28 @@ class Fp8KVCache:
         log sum exp of the scores [T, heads] float32.  A token that sees nothing
         gets zeros and -inf; rows that ``starts`` leaves out are not written.
         ``out`` must not overlap q."""
-        scale = self._queries(q, scale)
+        tag, scale = self._queries(q, scale)
         n, h, _ = q.shape
-        batch, kept = self._batch(table, lengths, starts, n, q, out)
-        q = _rows(q)
+        batch, kept = self._batch(table, lengths, starts, n)
+        dev = self.device
+        q, qs_t, qs_h = _rows(q)
         if out is None:
-            out = torch.empty((n, h, self.v_dim), dtype=q.dtype, device=self.device)
-        elif out.shape != (n, h, self.v_dim) or out.dtype != q.dtype or not rows_apart(out) or out.data_ptr() % 16 \
-                or any(s % 8 for s in _strides(out)):
-            raise ValueError(f"Fp8KVCache.attend: out must be {(n, h, self.v_dim)} {q.dtype} with 16-byte aligned rows "
-                             "that do not overlap")
-        lse = torch.empty((n, h), dtype=torch.float32, device=self.device) if return_lse else None
-        qs_t, qs_h = _strides(q)
-        os_t, os_h = _strides(out)
-        with N.on_device(self.device):
-            ref = C.byref(batch)
-            nbytes = N.lib().tm_kv8_attention_workspace_size(self._ref, ref, h)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
-            N.call("tm_kv8_attention", self._ref, ref, N.dtype_tag(q.dtype), q.data_ptr(), qs_t, qs_h, h, scale,
-                   1 if causal else 0, out.data_ptr(), os_t, os_h, N.ptr(lse), N.ptr(ws), nbytes, N.stream(self.device))
+            out = q.new_empty((n, h, self.v_dim))
+            os_t, os_h = h * self.v_dim, self.v_dim
+        else:
+            N.require_hip(q, out)
+            os_t, os_h = _strides(out) if out.dim() == 3 else (0, 0)
+            if out.shape != (n, h, self.v_dim) or out.dtype != q.dtype or not rows_apart(out) or out.data_ptr() % 16 \
+                    or os_t % 8 or os_h % 8:
+                raise ValueError(f"Fp8KVCache.attend: out must be {(n, h, self.v_dim)} {q.dtype} with 16-byte aligned "
+                                 "rows that do not overlap")
+        lse = torch.empty((n, h), dtype=torch.float32, device=dev) if return_lse else None
+        ref = C.byref(batch)
+        nbytes = N.lib().tm_kv8_attention_workspace_size(self._ref, ref, h)
+        ws = q.new_empty(nbytes // 2) if nbytes else None
+        with N.on_device(dev):
+            N.call("tm_kv8_attention", self._ref, ref, tag, q.data_ptr(), qs_t, qs_h, h, scale, 1 if causal else 0,
+                   out.data_ptr(), os_t, os_h, N.ptr(lse), N.ptr(ws), nbytes, N.stream(dev))
         return (out, lse) if return_lse else out
 
     def importance(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *, scale: float | None = None,
@@ -192,25 +211,27 @@ class Fp8KVCache:
         given it (keys are read once then).  At most 256 heads.
         ``table_moe.utils.importance.cached_importance`` also stores the scores
         for the keep rule."""
-        scale = self._queries(q, scale)
+        tag, scale = self._queries(q, scale)
         b, h, _ = q.shape
-        batch, kept = self._batch(table, lengths, None, b, q, lse)
-        q = _rows(q)
+        batch, kept = self._batch(table, lengths, None, b)
+        dev = self.device
+        q, qs_t, qs_h = _rows(q)
         out_len = batch.max_pages * self.page_size if out_len is None else int(out_len)
         if out_len < 0:
             raise ValueError("Fp8KVCache.importance: out_len must not be negative")
+        out = torch.empty((b, out_len), dtype=torch.float32, device=dev)
+        ref, ld_lse, ws, nbytes = C.byref(batch), 0, None, 0
         if lse is not None:
+            N.require_hip(q, lse)
             if lse.shape != (b, h) or lse.dtype != torch.float32:
                 raise ValueError(f"Fp8KVCache.importance: lse must be {(b, h)} float32")
             if lse.stride(1) != 1 and h > 1 or lse.stride(0) < h and b > 1:
                 lse = lse.contiguous()
-        out = torch.empty((b, out_len), dtype=torch.float32, device=self.device)
-        qs_t, qs_h = _strides(q)
-        with N.on_device(self.device):
-            ref = C.byref(batch)
-            nbytes = 0 if lse is not None else N.lib().tm_kv8_importance_workspace_size(self._ref, ref, h)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
-            N.call("tm_kv8_importance", self._ref, ref, N.dtype_tag(q.dtype), q.data_ptr(), qs_t, qs_h, h, scale,
-                   N.ptr(lse), 0 if lse is None else (lse.stride(0) if b > 1 else h), out_len, out.data_ptr(), out_len,
-                   N.ptr(ws), nbytes, N.stream(self.device))
+            ld_lse = lse.stride(0) if b > 1 else h
+        else:
+            nbytes = N.lib().tm_kv8_importance_workspace_size(self._ref, ref, h)
+            ws = q.new_empty(nbytes // 2) if nbytes else None
+        with N.on_device(dev):
+            N.call("tm_kv8_importance", self._ref, ref, tag, q.data_ptr(), qs_t, qs_h, h, scale, N.ptr(lse), ld_lse,
+                   out_len, out.data_ptr(), out_len, N.ptr(ws), nbytes, N.stream(dev))
         return out

@@ -15,6 +15,8 @@ import torch
 
 from .. import _native as N
 
+_INTEGERS = (torch.int64, torch.int32)
+
 
 @functools.lru_cache(maxsize=64)
 def _sections(sections: tuple):
@@ -57,20 +59,26 @@ def _strides(t: torch.Tensor):
 
 def _run(q, k, positions, inv_freq, sections, interleaved, adjacent, inverse, q_out, k_out, dev):
     n, h, d = q.shape
-    qs_t, qs_h = _strides(q)
-    qo_t, qo_h = _strides(q_out)
-    ks_t, ks_h = (0, 0) if k is None else _strides(k)
-    ko_t, ko_h = (0, 0) if k is None else _strides(k_out)
+    qs_t, qs_h, _ = q.stride()
+    qo_t, qo_h, _ = q_out.stride()
+    kp = kv = ks_t = ks_h = kop = ko_t = ko_h = 0
+    if k is not None:
+        kp, kv, kop = k.data_ptr(), k.shape[1], k_out.data_ptr()
+        ks_t, ks_h, _ = k.stride()
+        ko_t, ko_h, _ = k_out.stride()
     with N.on_device(dev):
-        N.call("tm_rotate_positions", N.dtype_tag(q.dtype), q.data_ptr(), n, h, qs_t, qs_h, N.ptr(k),
-               0 if k is None else k.shape[1], ks_t, ks_h, d, 2 * inv_freq.shape[0], positions.data_ptr(),
-               positions.stride(0) if positions.shape[0] > 1 else n, positions.shape[0], _sections(sections),
-               interleaved, adjacent, inverse, inv_freq.data_ptr(), q_out.data_ptr(), qo_t, qo_h, N.ptr(k_out), ko_t,
-               ko_h, N.stream(dev))
+        N.call("tm_rotate_positions", N.dtype_tag(q.dtype), q.data_ptr(), n, h, qs_t, qs_h, kp, kv, ks_t, ks_h, d,
+               2 * inv_freq.shape[0], positions.data_ptr(), positions.stride(0) if len(sections) > 1 else n,
+               len(sections), _sections(sections), interleaved, adjacent, inverse, inv_freq.data_ptr(), q_out.data_ptr(),
+               qo_t, qo_h, kop, ko_t, ko_h, N.stream(dev))
 
 
 def _unit_rows(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+    return t if t.is_contiguous() or t.stride(2) == 1 else t.contiguous()
+
+
+def _new(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 class _Rotate(torch.autograd.Function):
@@ -80,8 +88,7 @@ class _Rotate(torch.autograd.Function):
         ctx.how = how
         qq = _unit_rows(q)
         kk = None if k is None else _unit_rows(k)
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        q_out, k_out = _new(qq), None if k is None else _new(kk)
         _run(qq, kk, positions, inv_freq, *how, q_out, k_out, q.device)
         return q_out, k_out
 
@@ -115,33 +122,34 @@ def rotate_positions(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
     there are no gradients.  Otherwise gradients of any order flow to q and k."""
     dev = N.require_hip(q, k, positions, inv_freq)
     if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]
-                                           or k.dtype != q.dtype)):
+                                           or k.dtype is not q.dtype)):
         raise ValueError("rotate_positions expects q [T, H, D] and k [T, Hkv, D] of one dtype")
-    N.dtype_tag(q.dtype)
     n = q.shape[0]
     if positions.dim() == 1:
         positions = positions[None]
-    if positions.dim() != 2 or positions.shape[1] != n or positions.dtype not in (torch.int64, torch.int32):
+    if positions.dim() != 2 or positions.shape[1] != n or positions.dtype not in _INTEGERS:
         raise ValueError(f"rotate_positions: positions must be [A, {n}] or [{n}] integers, got {tuple(positions.shape)} "
                          f"{positions.dtype}")
-    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
+    if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float32:
         raise ValueError("rotate_positions: inv_freq must be [R / 2] float32")
-    sections = (inv_freq.shape[0],) if sections is None else tuple(int(s) for s in sections)
+    sections = (inv_freq.shape[0],) if sections is None else tuple(map(int, sections))
     if len(sections) != positions.shape[0]:
         raise ValueError(f"rotate_positions: {len(sections)} sections for {positions.shape[0]} axes")
-    if positions.dtype != torch.int64:
+    if positions.dtype is not torch.int64:
         positions = positions.long()
-    if (positions.stride(1) != 1 and n > 1) or (positions.stride(0) < n and positions.shape[0] > 1):
+    if not positions.is_contiguous() and ((positions.stride(1) != 1 and n > 1)
+                                          or (positions.stride(0) < n and positions.shape[0] > 1)):
         positions = positions.contiguous()
-    inv_freq = inv_freq if inv_freq.is_contiguous() else inv_freq.contiguous()
-    how = (sections, int(bool(interleaved)), int(bool(adjacent)), int(bool(inverse)))
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if not inv_freq.is_contiguous():
+        inv_freq = inv_freq.contiguous()
+    how = (sections, 1 if interleaved else 0, 1 if adjacent else 0, 1 if inverse else 0)
+    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("rotate_positions: no gradients through out")
         return _Rotate.apply(q, k, positions, inv_freq, how)
+    q, k = _unit_rows(q), None if k is None else _unit_rows(k)
     if out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
+        q_out, k_out = _new(q), None if k is None else _new(k)
     else:
         q_out, k_out = out
         if (k is None) != (k_out is None):
@@ -150,5 +158,5 @@ def rotate_positions(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
         _check_out("out[0]", q_out, q)
         if k is not None:
             _check_out("out[1]", k_out, k)
-    _run(_unit_rows(q), None if k is None else _unit_rows(k), positions, inv_freq, *how, q_out, k_out, dev)
+    _run(q, k, positions, inv_freq, *how, q_out, k_out, dev)
     return q_out, k_out
