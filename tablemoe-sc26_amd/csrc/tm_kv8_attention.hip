@@ -29,6 +29,9 @@ namespace {
 constexpr int kAttThreads = 256;
 constexpr int kWaves = kAttThreads / 64;
 constexpr int kMaxSplits = 128;
+typedef float tm_f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 tm_f16x2 __attribute__((ext_vector_type(2)));
+
 constexpr float kRoom = 8.f, kGrow = 6.f;  // log2 of a new maximum's P, of what it may grow by
 
 struct AttArgs {
@@ -45,16 +48,17 @@ struct AttArgs {
   int32_t heads, groups, splits, page_log2, causal, tiles1;  // tiles1: row tiles of one token
 };
 
-// A row tile: rows [r0, r0 + rows) of sequence b.
+// A row tile: rows [r0, r0 + rows) of sequence b (tokens times heads of a key head: under 2^31).
 struct RowTile {
   Kv8Seq s;
-  int64_t b, r0;
+  int64_t b;
+  uint32_t r0;
   int rows;
   int64_t end;    // keys that its last row sees
   int64_t tiles;  // of 32 keys
   int64_t per;    // tiles of a split
 };
-__device__ __forceinline__ int64_t visible(const AttArgs &a, const Kv8Seq &s, int64_t token) {
+__device__ __forceinline__ int64_t visible(const AttArgs &a, const Kv8Seq &s, uint32_t token) {
   const int64_t cap = (int64_t)a.b.max_pages << a.page_log2;
   int64_t e = a.causal ? s.len - s.n + token + 1 : s.len;
   e = e < cap ? e : cap;
@@ -62,21 +66,27 @@ __device__ __forceinline__ int64_t visible(const AttArgs &a, const Kv8Seq &s, in
 }
 __device__ __forceinline__ bool row_tile(const AttArgs &a, int64_t u, RowTile &t) {
   int64_t j = 0;
+  uint32_t last = 0;  // the tile's last token
   if (a.b.starts == nullptr) {
-    t.b = u / a.tiles1;
+    t.b = a.tiles1 == 1 ? (uint32_t)u : (uint32_t)u / (uint32_t)a.tiles1;
     j = u - t.b * a.tiles1;
   } else {
     t.b = tm_kv8_unit(a.b, u, a.groups, 32, 1, j);
   }
   t.s = tm_kv8_seq(a.b, t.b);
-  t.r0 = j * 32;
   const int64_t all = t.s.n * a.groups;
-  if (j < 0 || t.r0 >= all) return false;
+  if (j < 0 || j * 32 >= all) return false;
+  t.r0 = (uint32_t)(j * 32);
   t.rows = (int)(all - t.r0 < 32 ? all - t.r0 : 32);
-  t.end = visible(a, t.s, (t.r0 + t.rows - 1) / a.groups);
+  if (a.b.starts != nullptr) last = (t.r0 + t.rows - 1) / (uint32_t)a.groups;
+  t.end = visible(a, t.s, last);
   t.tiles = (t.end + 31) >> 5;
-  t.per = tm_kv8_per(t.tiles, a.splits);
+  t.per = a.splits == 1 ? t.tiles + 3 : tm_kv8_per(t.tiles, a.splits);
   return true;
+}
+// A row's token (of its sequence) and its head among the key head's.
+__device__ __forceinline__ uint32_t token_of(const AttArgs &a, uint32_t row) {
+  return a.b.starts == nullptr ? 0 : row / (uint32_t)a.groups;
 }
 
 // DV = 0: the statistics alone.
@@ -91,13 +101,13 @@ __global__ __launch_bounds__(kAttThreads, D + DV > 320 ? 1 : 2) void attend_kern
   const int c = lane & 31, g = lane >> 5;
   const int h = blockIdx.y, split = blockIdx.z;
   RowTile t;
-  if (!row_tile(a, blockIdx.x, t)) return;
+  if (!row_tile(a, gridDim.x - 1 - blockIdx.x, t)) return;  // the last tokens of a prompt see most: they go first
   const int64_t t0 = split * t.per, t1 = t0 + t.per < t.tiles ? t0 + t.per : t.tiles;
   if (t0 >= t1 && split > 0) return;
-  const int64_t row = t.r0 + (c < t.rows ? c : t.rows - 1);
-  const int64_t token = row / a.groups;
+  const uint32_t row = t.r0 + (c < t.rows ? c : t.rows - 1);
+  const uint32_t token = token_of(a, row);
   const int64_t call_row = (t.s.first + token) * a.heads + h * a.groups + (row - token * a.groups);
-  const int64_t limit = visible(a, t.s, token), first_limit = visible(a, t.s, t.r0 / a.groups);
+  const int64_t limit = visible(a, t.s, token), first_limit = visible(a, t.s, token_of(a, t.r0));
 
   uint4 qf[NK][2];
   {
@@ -154,7 +164,7 @@ __global__ __launch_bounds__(kAttThreads, D + DV > 320 ? 1 : 2) void attend_kern
     float top = s[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-    const float mul = sk * unit, add = tm_exponent(sv);
+    const float mul = (w.there ? sk : 1.f) * unit, add = w.there ? tm_exponent(sv) : 0.f;
     top = fmaf(top, mul, add);
     top = fmaxf(top, tm_other_half(top));
     if (__any(top > m + (kRoom + kGrow) || (m == -__builtin_huge_valf() && top > m))) {
@@ -175,8 +185,7 @@ __global__ __launch_bounds__(kAttThreads, D + DV > 320 ? 1 : 2) void attend_kern
       const float x = __builtin_amdgcn_exp2f(fmaf(s[i], mul, off)), y = __builtin_amdgcn_exp2f(fmaf(s[i + 1], mul, off));
       sum += x + y;
       if constexpr (NV > 0) {
-        const _Float16 two[2] = {(_Float16)x, (_Float16)y};
-        pf[i / 2] = __builtin_bit_cast(uint32_t, two);
+        pf[i / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(tm_f32x2{x, y}, tm_f16x2));
       }
     }
     l = fmaf(sum, __builtin_amdgcn_exp2f(-add - kRoom), l);
@@ -207,22 +216,26 @@ __global__ __launch_bounds__(kAttThreads, D + DV > 320 ? 1 : 2) void attend_kern
   const int64_t begin = t0 + wave;
   if (begin < t1) {
     uint4 ka[NK], va[NV ? NV : 1], kb[NK], vb[NV ? NV : 1];
-    auto fetch = [&](int64_t tile, Kv8Place &w, uint4 (&kf)[NK], uint4 (&vf)[NV ? NV : 1], float &sk, float &sv) {
-      tile = tile < t1 ? tile : t1 - 1;
-      w = tm_kv8_place(a.c, a.b, t.b, h, tile, a.page_log2);
+    const int32_t *const pages = a.b.table + t.b * a.b.ld_table;
+    auto page_of = [&](int64_t tile) { return tm_kv8_page(a.b, pages, tile < t1 ? tile : t1 - 1, a.page_log2); };
+    auto fetch = [&](int64_t tile, int id, Kv8Place &w, uint4 (&kf)[NK], uint4 (&vf)[NV ? NV : 1], float &sk, float &sv) {
+      w = tm_kv8_place(a.c, id, h, tile < t1 ? tile : t1 - 1, a.page_log2);
       tm_kv8_load<NK>(a.c.k, w, a.page_log2, lane, kf);
       if constexpr (NV > 0) tm_kv8_load<NV>(a.c.v, w, a.page_log2, lane, vf);
-      sk = w.there ? a.c.k_scale[w.slot] : 1.f;
-      sv = NV && w.there ? a.c.v_scale[w.slot] : 1.f;
+      sk = a.c.k_scale[w.slot];
+      sv = NV ? a.c.v_scale[w.slot] : 1.f;
     };
     Kv8Place wa, wb;
     float ska, sva, skb, svb;
-    fetch(begin, wa, ka, va, ska, sva);
+    int ida = page_of(begin), idb = page_of(begin + kWaves);
+    fetch(begin, ida, wa, ka, va, ska, sva);
     for (int64_t tile = begin; tile < t1; tile += 2 * kWaves) {
-      fetch(tile + kWaves, wb, kb, vb, skb, svb);
+      ida = page_of(tile + 2 * kWaves);
+      fetch(tile + kWaves, idb, wb, kb, vb, skb, svb);
       step(tile, wa, ka, va, ska, sva);
       if (tile + kWaves >= t1) break;
-      fetch(tile + 2 * kWaves, wa, ka, va, ska, sva);
+      idb = page_of(tile + 3 * kWaves);
+      fetch(tile + 2 * kWaves, ida, wa, ka, va, ska, sva);
       step(tile + kWaves, wb, kb, vb, skb, svb);
     }
   }
@@ -264,7 +277,8 @@ __global__ __launch_bounds__(kAttThreads, D + DV > 320 ? 1 : 2) void attend_kern
           const float4 x = *reinterpret_cast<const float4 *>(&obuf[w][r][col]);
           v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
         }
-        const int64_t rr = t.r0 + r, tok = rr / a.groups, head = h * a.groups + (rr - tok * a.groups);
+        const uint32_t rr = t.r0 + r, tok = token_of(a, rr);
+        const int64_t head = h * a.groups + (rr - tok * a.groups);
         const int to = half * kChunk + col;
         if (whole) {
           T y[4];
@@ -293,7 +307,8 @@ __global__ __launch_bounds__(kAttThreads) void join_kernel(AttArgs a) {
   RowTile t;
   if (!row_tile(a, blockIdx.x, t) || t.per >= t.tiles || (int)blockIdx.z >= t.rows) return;
   const int n = (int)((t.tiles + t.per - 1) / t.per);
-  const int64_t rr = t.r0 + blockIdx.z, tok = rr / a.groups, head = h * a.groups + (rr - tok * a.groups);
+  const uint32_t rr = t.r0 + blockIdx.z, tok = token_of(a, rr);
+  const int64_t head = h * a.groups + (rr - tok * a.groups);
   const int64_t row = (t.s.first + tok) * a.heads + head;
   const int col = threadIdx.x % kCols, set = threadIdx.x / kCols, lane = threadIdx.x & 63;
   const float *const p = a.part + row * a.splits * DV + col * 4;
@@ -420,7 +435,8 @@ extern "C" int tm_kv8_attention(const tm_kv8_cache *cache, const tm_kv8_batch *b
   if (cache->n_pages == 0) a.b.max_pages = 0;  // no page is there
   a.groups = n_heads / cache->n_kv_heads;
   const int64_t tiles = row_tiles(batch, a.groups);
-  TM_REQUIRE(tiles < ((int64_t)1 << 31), TM_EINVAL_SHAPE, "tm_kv8_attention: too many rows");
+  TM_REQUIRE(batch->n_tokens * a.groups + 32 * batch->n_seqs < ((int64_t)1 << 31), TM_EINVAL_SHAPE,
+             "tm_kv8_attention: too many rows");
   a.splits = key_splits(cache, batch, tiles);
   const size_t need = tm_kv8_attention_workspace_size(cache, batch, n_heads);
   TM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && tm_aligned16(workspace)), TM_EWORKSPACE,

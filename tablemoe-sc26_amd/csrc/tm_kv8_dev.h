@@ -15,16 +15,18 @@ struct Kv8Place {
   int tile;      // within the page
   bool there;
 };
-__device__ __forceinline__ Kv8Place tm_kv8_place(const tm_kv8_cache &c, const tm_kv8_batch &bt, int64_t b, int h,
-                                                 int64_t tile, int page_log2) {
-  const int tl = page_log2 - 5;  // tiles of a page: 1 << tl
-  const int64_t p = tile >> tl;
+// The page of a tile, as its sequence's row of the table names it (-1: past the table's width).  Loaded a round before
+// the tile itself: the bytes wait for it.
+__device__ __forceinline__ int tm_kv8_page(const tm_kv8_batch &bt, const int32_t *row, int64_t tile, int page_log2) {
+  const int64_t p = tile >> (page_log2 - 5);
+  const int id = row[p < bt.max_pages ? p : bt.max_pages - 1];
+  return p < bt.max_pages ? id : -1;
+}
+__device__ __forceinline__ Kv8Place tm_kv8_place(const tm_kv8_cache &c, int id, int h, int64_t tile, int page_log2) {
   Kv8Place r;
-  int64_t id = p < bt.max_pages ? bt.table[b * bt.ld_table + p] : -1;
   r.there = id >= 0 && id < c.n_pages;
-  id = r.there ? id : 0;
-  r.slot = id * c.n_kv_heads + h;
-  r.tile = (int)(tile & ((1 << tl) - 1));
+  r.slot = (int64_t)(r.there ? id : 0) * c.n_kv_heads + h;
+  r.tile = (int)(tile & ((1 << (page_log2 - 5)) - 1));
   return r;
 }
 

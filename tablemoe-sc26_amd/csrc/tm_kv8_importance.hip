@@ -119,18 +119,23 @@ __global__ __launch_bounds__(kThreads) void importance_kernel(ImpArgs a) {
         uint4 ka[NK], kb[NK];
         Kv8Place wa, wb;
         float sa, sb;
-        auto fetch = [&](int64_t tile, Kv8Place &w, uint4 (&kf)[NK], float &sk) {
-          tile = tile < end ? tile : end - 1;
-          w = tm_kv8_place(a.c, a.b, b, h, tile, a.page_log2);
+        const int32_t *const pages = a.b.table + b * a.b.ld_table;
+        auto page_of = [&](int64_t tile) { return tm_kv8_page(a.b, pages, tile < end ? tile : end - 1, a.page_log2); };
+        auto fetch = [&](int64_t tile, int id, Kv8Place &w, uint4 (&kf)[NK], float &sk) {
+          w = tm_kv8_place(a.c, id, h, tile < end ? tile : end - 1, a.page_log2);
           tm_kv8_load<NK>(a.c.k, w, a.page_log2, lane, kf);
-          sk = w.there ? a.c.k_scale[w.slot] : 1.f;
+          sk = a.c.k_scale[w.slot];
         };
-        fetch(tile0 + my_tile, wa, ka, sa);
-        for (int64_t tile = tile0 + my_tile; tile < end; tile += 2 * tile_waves) {
-          fetch(tile + tile_waves, wb, kb, sb);
+        const int64_t begin = tile0 + my_tile;
+        int ida = page_of(begin), idb = page_of(begin + tile_waves);
+        fetch(begin, ida, wa, ka, sa);
+        for (int64_t tile = begin; tile < end; tile += 2 * tile_waves) {
+          ida = page_of(tile + 2 * tile_waves);
+          fetch(tile + tile_waves, idb, wb, kb, sb);
           step(tile, wa, ka, sa);
           if (tile + tile_waves >= end) break;
-          fetch(tile + 2 * tile_waves, wa, ka, sa);
+          idb = page_of(tile + 3 * tile_waves);
+          fetch(tile + 2 * tile_waves, ida, wa, ka, sa);
           step(tile + tile_waves, wb, kb, sb);
         }
       }
