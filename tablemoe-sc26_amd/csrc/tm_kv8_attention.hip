@@ -1,24 +1,33 @@
 // Attention over the 8-bit cache (layout: tm_kv8.h): tm_kv8_attention.
 //
-// Rows of a sequence are its (new token, query head of one key head) pairs, 32 a
-// tile, so a key head's tile of keys serves all its query heads.  Per 32 keys:
+// Rows of a sequence are its (new token, query head of one key head) pairs, so a
+// key head's keys serve all its query heads.  A workgroup owns R x 32 rows; its
+// four waves take every fourth tile of 32 keys and join through LDS.  Per tile and
+// 32 rows:
 //   S^T = K Q^T on the 16-bit instructions (a byte of K is exact in 16 bits), a
 //   lane holding 16 keys of one row;  x = S^T sk scale log2(e) + log2(sv);
-//   P = 2^(x - m) under a running reference m of the row, so that the values'
-//   scale rides in P and V enters as the bytes stand;  O^T += V^T P.
+//   P = 2^(x - m) under a reference m of the row, so that the values' scale
+//   rides in P and V enters as the bytes stand;  O^T += V^T P.
 // With l = sum P / sv the result is O / l and log sum exp = (m + log2 l) ln 2 (sv >=
 // 2^-100: l stays in range).
-// m is 2^8 under a running maximum of x and follows it only when that has grown by
-// more than 2^6, so O is seldom scaled again and P lies in [0, 2^14].  P is rounded
-// to fp16 for the second product whatever the queries' type, and V's bytes become
-// fp16 (exact): half a step is 2^-12 of a probability, where bf16 would leave
-// 2^-9 (an output's error against 64 bits 1.9e-3 of its size instead of 1.6e-3, which
-// is its own rounding); what lies under 2^-33 of a row's largest is lost.  All
-// sums are fp32.
+// m is set 2^8 under the first tile's largest x and raised only where the
+// probabilities of a lane's 16 keys sum to more than 2^15: no maximum is taken of
+// the other tiles, and O is seldom scaled again.  P is rounded to fp16 for the
+// second product whatever the queries' type, and V's bytes become fp16 (exact):
+// half a step is 2^-12 of a probability, where bf16 would leave 2^-9 (an output's
+// error against 64 bits 1.9e-3 of its size instead of 1.6e-3, which is its own
+// rounding); what lies under 2^-33 of a row's largest is lost.  All sums are fp32.
 //
-// The four waves of a workgroup take every fourth tile of keys and join through
-// LDS.  Where rows alone do not fill the device, the keys are split over
-// workgroups as well, and a second launch joins their parts.
+// A prompt is bound by instructions: per 32 keys and 64 rows the products take 1024
+// cycles of the matrix units, of which about half keep the vector units from
+// issuing, and the conversions of K and V (64, 5 cycles each), exponentials (32, 8.5)
+// and the rest (about 110, 3 to 6) another 1000.  So a long prompt's waves own 64 rows,
+// which share the conversions, with the queries' operands in LDS (in registers they
+// would leave one wave per SIMD, which issues a vector instruction every 5 to 12
+// cycles where two issue one every 3).  Tried and slower: the tile converted once per
+// workgroup into LDS; one wave per SIMD with the next tile's scores among this tile's exponentials.
+// A decode step is bound by HBM; where rows alone do not fill the device, the keys
+// are split over workgroups too, and a second launch joins their parts.
 #include "tm_internal.h"
 #include "tm_kv8_dev.h"
 
@@ -26,13 +35,14 @@
 
 namespace {
 
-constexpr int kAttThreads = 256;
-constexpr int kWaves = kAttThreads / 64;
-constexpr int kMaxSplits = 128;
 typedef float tm_f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 tm_f16x2 __attribute__((ext_vector_type(2)));
 
-constexpr float kRoom = 8.f, kGrow = 6.f;  // log2 of a new maximum's P, of what it may grow by
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kMaxSplits = 128;
+constexpr float kRoom = 8.f;  // log2 of the first maximum's P
+// What the probabilities of 16 keys may sum to before the reference is raised (each is rounded to fp16: at most 65504).
+constexpr float kMost = 32768.f;
 
 struct AttArgs {
   tm_kv8_cache c;
@@ -64,6 +74,7 @@ __device__ __forceinline__ int64_t visible(const AttArgs &a, const Kv8Seq &s, ui
   e = e < cap ? e : cap;
   return e < 0 ? 0 : e;
 }
+template <int ROWS = 32>
 __device__ __forceinline__ bool row_tile(const AttArgs &a, int64_t u, RowTile &t) {
   int64_t j = 0;
   uint32_t last = 0;  // the tile's last token
@@ -71,13 +82,13 @@ __device__ __forceinline__ bool row_tile(const AttArgs &a, int64_t u, RowTile &t
     t.b = a.tiles1 == 1 ? (uint32_t)u : (uint32_t)u / (uint32_t)a.tiles1;
     j = u - t.b * a.tiles1;
   } else {
-    t.b = tm_kv8_unit(a.b, u, a.groups, 32, 1, j);
+    t.b = tm_kv8_unit(a.b, u, a.groups, ROWS, 1, j);
   }
   t.s = tm_kv8_seq(a.b, t.b);
   const int64_t all = t.s.n * a.groups;
-  if (j < 0 || j * 32 >= all) return false;
-  t.r0 = (uint32_t)(j * 32);
-  t.rows = (int)(all - t.r0 < 32 ? all - t.r0 : 32);
+  if (j < 0 || j * ROWS >= all) return false;
+  t.r0 = (uint32_t)(j * ROWS);
+  t.rows = (int)(all - t.r0 < ROWS ? all - t.r0 : ROWS);
   if (a.b.starts != nullptr) last = (t.r0 + t.rows - 1) / (uint32_t)a.groups;
   t.end = visible(a, t.s, last);
   t.tiles = (t.end + 31) >> 5;
@@ -89,208 +100,259 @@ __device__ __forceinline__ uint32_t token_of(const AttArgs &a, uint32_t row) {
   return a.b.starts == nullptr ? 0 : row / (uint32_t)a.groups;
 }
 
+
 // DV = 0: the statistics alone.
-template <int DT, int D, int DV>
-__global__ __launch_bounds__(kAttThreads, D + DV > 320 ? 1 : 2) void attend_kernel(AttArgs a) {
+template <int DT, int D, int DV, int R>
+__global__ __launch_bounds__(kThreads, R == 2 || D + DV > 320 ? 2 : 3) void attend_kernel(AttArgs a) {
   using T = typename Elem<DT>::T;
   constexpr int NK = D / 32, NV = DV / 32;
   constexpr int kChunk = 64;  // columns joined at a time
+  constexpr size_t kQ = R * NK * 2 * 64 * 16, kJoin = DV ? sizeof(float) * kWaves * 32 * (kChunk + 4) : 0;
+  __shared__ __align__(16) uint8_t lds[kQ > kJoin ? kQ : kJoin];  // the queries' operands, then the parts to join
   __shared__ float2 join[kWaves][32];
-  __shared__ __align__(16) float obuf[DV ? kWaves : 1][32][kChunk + 4];
+  __shared__ float inv_s[32];
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
   const int c = lane & 31, g = lane >> 5;
-  const int h = blockIdx.y, split = blockIdx.z;
+  const uint32_t heads = a.c.n_kv_heads, block = gridDim.x - 1 - blockIdx.x;  // the last tokens see most: they go first
+  const int h = (int)(block % heads);
   RowTile t;
-  if (!row_tile(a, gridDim.x - 1 - blockIdx.x, t)) return;  // the last tokens of a prompt see most: they go first
-  const int64_t t0 = split * t.per, t1 = t0 + t.per < t.tiles ? t0 + t.per : t.tiles;
-  if (t0 >= t1 && split > 0) return;
-  const uint32_t row = t.r0 + (c < t.rows ? c : t.rows - 1);
-  const uint32_t token = token_of(a, row);
-  const int64_t call_row = (t.s.first + token) * a.heads + h * a.groups + (row - token * a.groups);
-  const int64_t limit = visible(a, t.s, token), first_limit = visible(a, t.s, token_of(a, t.r0));
+  if (!row_tile<32 * R>(a, block / heads, t)) return;
+  const int split = blockIdx.y;
+  const int t0 = (int)(split * t.per < t.tiles ? split * t.per : t.tiles), n = (int)(t0 + t.per < t.tiles ? t0 + t.per : t.tiles);
+  if (t0 >= n && split > 0) return;
+  const bool whole = t.per >= t.tiles;  // nothing to join with other workgroups
+  auto head_of = [&](uint32_t row, uint32_t token) { return (int64_t)h * a.groups + (row - token * a.groups); };
 
-  uint4 qf[NK][2];
-  {
-    const T *const q = static_cast<const T *>(a.q) + (t.s.first + token) * a.qs_t +
-                       (h * a.groups + (row - token * a.groups)) * a.qs_h + 16 * g;
-#pragma unroll
-    for (int j = 0; j < NK; ++j) {
-      qf[j][0] = *reinterpret_cast<const uint4 *>(q + 32 * j);
-      qf[j][1] = *reinterpret_cast<const uint4 *>(q + 32 * j + 8);
-    }
-  }
-  tm_f32x16 o[NV ? NV : 1];
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[j][i] = 0.f;
-  float m = -__builtin_huge_valf(), l = 0.f;
   const float unit = a.scale * kLog2e;
+  const int seen_whole = (int)(visible(a, t.s, token_of(a, t.r0)) >> 5);  // tiles that every row sees whole
+  const int32_t *const pages = a.b.table + t.b * a.b.ld_table;
+  auto page_of = [&](int tile) { return tm_kv8_page(a.b, pages, tile < n ? tile : n - 1, a.page_log2); };
+  auto place = [&](int tile, int id) { return tm_kv8_place(a.c, id, h, tile < n ? tile : n - 1, a.page_log2); };
 
-  auto step = [&](int64_t tile, const Kv8Place &w, const uint4 (&kf)[NK], uint4 (&vf)[NV ? NV : 1], float sk, float sv) {
-    tm_f32x16 s;
+  // the first tile of the wave is on its way while the queries are laid out
+  uint4 kf[NK], vf[NV ? NV : 1];
+  const int begin = t0 + wave;
+  Kv8Place w = {};
+  int id = -1;
+  float sk = 1.f, sv = 1.f;
+  if (begin < n) {
+    w = place(begin, page_of(begin));
+    id = page_of(begin + kWaves);
+    tm_kv8_load<NK>(a.c.k, w, a.page_log2, lane, kf);
+    if constexpr (NV > 0) tm_kv8_load<NV>(a.c.v, w, a.page_log2, lane, vf);
+    sk = a.c.k_scale[w.slot];
+    if constexpr (NV > 0) sv = a.c.v_scale[w.slot];
+  }
+
+  uint4(*const qs)[64] = reinterpret_cast<uint4(*)[64]>(lds);  // [r][j][e]
+  int64_t limit[R];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+  for (int r = 0; r < R; ++r) {
+    const uint32_t in = 32 * r + c, row = t.r0 + (in < (uint32_t)t.rows ? in : t.rows - 1), token = token_of(a, row);
+    limit[r] = visible(a, t.s, token);
+    const T *const q = static_cast<const T *>(a.q) + (t.s.first + token) * a.qs_t + head_of(row, token) * a.qs_h + 16 * g;
 #pragma unroll
-    for (int j = 0; j < NK; ++j) {
-      s = tm_mfma32x32x16<DT>(tm_kv8_operand<DT>(kf[j].x, kf[j].y), qf[j][0], s);
-      s = tm_mfma32x32x16<DT>(tm_kv8_operand<DT>(kf[j].z, kf[j].w), qf[j][1], s);
-    }
-    const int64_t k0 = tile * 32;
-    const bool edge = !w.there || k0 + 32 > first_limit;
-    uint32_t nan_bytes = 0;
-    if (edge) {
-      const int64_t lim = w.there ? limit : 0;
+    for (int j = 0; j < NK; ++j)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int64_t key = k0 + 8 * (i / 4) + 4 * g + i % 4;
-        s[i] = key < lim ? s[i] : -__builtin_huge_valf();
+      for (int e = 0; e < 2; ++e) {
+        const int at = (r * NK + j) * 2 + e;
+        if (at % kWaves == wave) qs[at][lane] = *reinterpret_cast<const uint4 *>(q + 32 * j + 8 * e);
       }
-      // a NaN among values that some row does not see stays out of the product
-      if constexpr (NV > 0) {
+  }
+  __syncthreads();
+  tm_f32x16 o[R][NV ? NV : 1];
+  float m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -__builtin_huge_valf();
+    l[r] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[r][j][i] = 0.f;
+  }
+  bool first = true;      // some row has no reference yet, or may have none
+  bool seen_nan = false;  // among values that some row does not see
+#pragma unroll 1
+  for (int tile = begin; tile < n; tile += kWaves) {
+      tm_f32x16 s[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[r][i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NK; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint4 k = e ? tm_kv8_operand<DT>(kf[j].z, kf[j].w) : tm_kv8_operand<DT>(kf[j].x, kf[j].y);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            s[r] = tm_mfma32x32x16<DT>(k, qs[(r * NK + j) * 2 + e][lane], s[r]);
+          }
+        }
+      const Kv8Place wn = place(tile + kWaves, id);
+      id = page_of(tile + 2 * kWaves);
+      tm_kv8_load<NK>(a.c.k, wn, a.page_log2, lane, kf);
+      const float mul = (w.there ? sk : 1.f) * unit, add = w.there ? tm_exponent(sv) : 0.f;
+      sk = a.c.k_scale[wn.slot];
+      if constexpr (NV > 0) sv = a.c.v_scale[wn.slot];
+      if (!w.there || tile >= seen_whole) {
+        first = true;
+        uint32_t nan = 0;  // a NaN among values that some row does not see stays out of the product
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           uint32_t *const p = reinterpret_cast<uint32_t *>(&vf[j]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t x = p[e] & 0x7f7f7f7fu;
-            const uint32_t n = (x + 0x01010101u) & 0x80808080u;  // 0x80 where a byte is 0x7f
-            nan_bytes |= n;
-            p[e] &= ~((n >> 7) * 0xffu);
+            const uint32_t x = ((p[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // 0x80 where a byte is NaN
+            nan |= x;
+            p[e] &= ~((x >> 7) * 0xffu);
           }
         }
+        seen_nan = seen_nan || nan != 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int64_t left = (w.there ? limit[r] : 0) - (int64_t)tile * 32;
+          int lim = left > 32 ? 32 : left < 0 ? 0 : (int)left;
+          asm volatile("" : "+v"(lim));  // (what follows stays in this branch)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[r][i] = 8 * (i / 4) + 4 * g + i % 4 < lim ? s[r][i] : -__builtin_huge_valf();
+        }
       }
-    }
-    float top = s[0];
+      w = wn;
+      const float back = __builtin_amdgcn_exp2f(-add - kRoom);
+      bool none = false;
+      uint4 p[R][2];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-    const float mul = (w.there ? sk : 1.f) * unit, add = w.there ? tm_exponent(sv) : 0.f;
-    top = fmaf(top, mul, add);
-    top = fmaxf(top, tm_other_half(top));
-    if (__any(top > m + (kRoom + kGrow) || (m == -__builtin_huge_valf() && top > m))) {
-      const float to = fmaxf(m, top - kRoom);
-      const float f = m == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(m - to);
-      m = to;
-      l *= f;
+      for (int r = 0; r < R; ++r) {
+        auto settle = [&] {  // the row's reference 2^8 under its largest score so far
+          float top = s[r][0];
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[j][i] *= f;
-    }
-    const float off = add - (m == -__builtin_huge_valf() ? 0.f : m);
-    float sum = 0.f;
-    uint32_t pf[8];
-#pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-      const float x = __builtin_amdgcn_exp2f(fmaf(s[i], mul, off)), y = __builtin_amdgcn_exp2f(fmaf(s[i + 1], mul, off));
-      sum += x + y;
-      if constexpr (NV > 0) {
-        pf[i / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(tm_f32x2{x, y}, tm_f16x2));
-      }
-    }
-    l = fmaf(sum, __builtin_amdgcn_exp2f(-add - kRoom), l);
-    if constexpr (NV > 0) {
-      const uint4 p0 = make_uint4(pf[0], pf[1], pf[2], pf[3]), p1 = make_uint4(pf[4], pf[5], pf[6], pf[7]);
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        o[j] = tm_mfma32x32x16<TM_DT_F16>(tm_kv8_operand<TM_DT_F16>(vf[j].x, vf[j].y), p0, o[j]);
-        o[j] = tm_mfma32x32x16<TM_DT_F16>(tm_kv8_operand<TM_DT_F16>(vf[j].z, vf[j].w), p1, o[j]);
-      }
-      if (edge && __any(nan_bytes != 0)) {  // those that a row does see make its column NaN
-        const uint8_t *const vb = static_cast<const uint8_t *>(a.c.v) +
-                                  ((w.slot << (a.page_log2 - 5)) + w.tile) * (int64_t)(NV * 1024);
-        const int64_t lim = w.there ? limit : 0;
-        for (int key = 0; key < 32 && k0 + key < lim; ++key)
+          for (int i = 1; i < 16; ++i) top = fmaxf(top, s[r][i]);
+          top = fmaf(top, mul, add);
+          top = fmaxf(top, tm_other_half(top));
+          const float to = fmaxf(m[r], top - kRoom);
+          const float f = m[r] == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(m[r] - to);
+          m[r] = to;
+          l[r] *= f;
 #pragma unroll
           for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int col = 8 * (i / 4) + 4 * g + i % 4;
-              const uint8_t x = vb[j * 1024 + ((key / 4 % 2) * 32 + col) * 16 + key / 16 * 8 + key / 8 % 2 * 4 + key % 4];
-              if ((x & 0x7f) == 0x7f) o[j][i] = __builtin_nanf("");
-            }
+            for (int i = 0; i < 16; ++i) o[r][j][i] *= f;
+        };
+        if (first) {
+          settle();
+          none = none || m[r] == -__builtin_huge_valf();
+        }
+        float sum;
+        auto probabilities = [&] {
+          const float off = add - (m[r] == -__builtin_huge_valf() ? 0.f : m[r]);
+          uint32_t pf[8];
+          sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const tm_f32x2 x = {__builtin_amdgcn_exp2f(fmaf(s[r][i], mul, off)), __builtin_amdgcn_exp2f(fmaf(s[r][i + 1], mul, off))};
+            sum += x.x + x.y;
+            pf[i / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, tm_f16x2));
+          }
+          p[r][0] = make_uint4(pf[0], pf[1], pf[2], pf[3]);
+          p[r][1] = make_uint4(pf[4], pf[5], pf[6], pf[7]);
+        };
+        probabilities();
+        if (__any(sum > kMost)) {
+          settle();
+          probabilities();
+        }
+        l[r] = fmaf(sum, back, l[r]);
       }
-    }
-  };
-
-  const int64_t begin = t0 + wave;
-  if (begin < t1) {
-    uint4 ka[NK], va[NV ? NV : 1], kb[NK], vb[NV ? NV : 1];
-    const int32_t *const pages = a.b.table + t.b * a.b.ld_table;
-    auto page_of = [&](int64_t tile) { return tm_kv8_page(a.b, pages, tile < t1 ? tile : t1 - 1, a.page_log2); };
-    auto fetch = [&](int64_t tile, int id, Kv8Place &w, uint4 (&kf)[NK], uint4 (&vf)[NV ? NV : 1], float &sk, float &sv) {
-      w = tm_kv8_place(a.c, id, h, tile < t1 ? tile : t1 - 1, a.page_log2);
-      tm_kv8_load<NK>(a.c.k, w, a.page_log2, lane, kf);
+      if (first) first = __any(none);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint4 v = e ? tm_kv8_operand<TM_DT_F16>(vf[j].z, vf[j].w) : tm_kv8_operand<TM_DT_F16>(vf[j].x, vf[j].y);
+#pragma unroll
+          for (int r = 0; r < R; ++r) o[r][j] = tm_mfma32x32x16<TM_DT_F16>(v, p[r][e], o[r][j]);
+        }
       if constexpr (NV > 0) tm_kv8_load<NV>(a.c.v, w, a.page_log2, lane, vf);
-      sk = a.c.k_scale[w.slot];
-      sv = NV ? a.c.v_scale[w.slot] : 1.f;
-    };
-    Kv8Place wa, wb;
-    float ska, sva, skb, svb;
-    int ida = page_of(begin), idb = page_of(begin + kWaves);
-    fetch(begin, ida, wa, ka, va, ska, sva);
-    for (int64_t tile = begin; tile < t1; tile += 2 * kWaves) {
-      ida = page_of(tile + 2 * kWaves);
-      fetch(tile + kWaves, idb, wb, kb, vb, skb, svb);
-      step(tile, wa, ka, va, ska, sva);
-      if (tile + kWaves >= t1) break;
-      idb = page_of(tile + 3 * kWaves);
-      fetch(tile + 2 * kWaves, ida, wa, ka, va, ska, sva);
-      step(tile + kWaves, wb, kb, vb, skb, svb);
+  }
+  const bool patch = __syncthreads_or(seen_nan) != 0;  // (the queries are done with, too)
+  float(*const obuf)[32][kChunk + 4] = reinterpret_cast<float(*)[32][kChunk + 4]>(lds);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (32 * r >= t.rows) break;
+    const float total_w = l[r] + tm_other_half(l[r]), mw = m[r] + kRoom;  // (O stands for 2^kRoom times its sum)
+    if (r > 0) __syncthreads();
+    if (g == 0) join[wave][c] = make_float2(mw, total_w);
+    __syncthreads();
+    float top = -__builtin_huge_valf(), total = 0.f;
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x) top = fmaxf(top, join[x][c].x);
+    const float base = top == -__builtin_huge_valf() ? 0.f : top;
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x) total += join[x][c].y * __builtin_amdgcn_exp2f(join[x][c].x - base);
+    const float f = __builtin_amdgcn_exp2f(mw - base);
+    const int rows = t.rows - 32 * r < 32 ? t.rows - 32 * r : 32;
+    if (wave == 0 && g == 0) {
+      if (NV > 0) inv_s[c] = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(-kRoom) / total;
+      if (c < rows) {
+        const uint32_t row = t.r0 + 32 * r + c, token = token_of(a, row);
+        const int64_t at = (t.s.first + token) * a.heads + head_of(row, token);
+        if (NV == 0 || !whole) a.stats[at * a.splits + split] = make_float2(top, total);
+        else if (a.lse) a.lse[at] = total == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(total)) * kLn2;
+      }
     }
-  }
-  l += tm_other_half(l);
-  m += kRoom;  // (a P of 1 stands for 2^(x - m) now, O for 2^kRoom times its sum)
-  if (g == 0) join[wave][c] = make_float2(m, l);
-  __syncthreads();
-  float top = -__builtin_huge_valf(), total = 0.f;
+    if constexpr (NV > 0) {
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, join[w][c].x);
-  const float base = top == -__builtin_huge_valf() ? 0.f : top;
+      for (int part = 0; part < DV / kChunk; ++part) {
+        if (part) __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) total += join[w][c].y * __builtin_amdgcn_exp2f(join[w][c].x - base);
-  const float f = __builtin_amdgcn_exp2f(m - base);
-  const bool whole = t.per >= t.tiles;  // nothing to join with other workgroups
-  if (wave == 0 && g == 0 && c < t.rows) {
-    if (DV == 0 || !whole) a.stats[call_row * a.splits + split] = make_float2(top, total);
-    if (whole && a.lse) a.lse[call_row] = total == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(total)) * kLn2;
-  }
-  if constexpr (NV > 0) {
-    __shared__ float inv[32];
-    if (wave == 0 && g == 0) inv[c] = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(-kRoom) / total;
+        for (int jj = 0; jj < kChunk / 32; ++jj)
 #pragma unroll
-    for (int half = 0; half < DV / kChunk; ++half) {
+          for (int i = 0; i < 16; i += 4) {
+            const tm_f32x16 &v = o[r][part * (kChunk / 32) + jj];
+            *reinterpret_cast<float4 *>(&obuf[wave][c][32 * jj + 2 * i + 4 * g]) =
+                make_float4(v[i] * f, v[i + 1] * f, v[i + 2] * f, v[i + 3] * f);
+          }
+        __syncthreads();
+        for (int e = threadIdx.x; e < rows * (kChunk / 8); e += kThreads) {
+          const int rr = e / (kChunk / 8), col = e % (kChunk / 8) * 8;
+          float v[8];
 #pragma unroll
-      for (int jj = 0; jj < kChunk / 32; ++jj)
+          for (int k = 0; k < 8; ++k) v[k] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const tm_f32x16 &v = o[half * (kChunk / 32) + jj];
-          *reinterpret_cast<float4 *>(&obuf[wave][c][32 * jj + 2 * i + 4 * g]) =
-              make_float4(v[i] * f, v[i + 1] * f, v[i + 2] * f, v[i + 3] * f);
-        }
-      __syncthreads();
-      for (int e = threadIdx.x; e < t.rows * (kChunk / 4); e += kAttThreads) {
-        const int r = e / (kChunk / 4), col = e % (kChunk / 4) * 4;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int x = 0; x < kWaves; ++x)
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-          const float4 x = *reinterpret_cast<const float4 *>(&obuf[w][r][col]);
-          v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
-        }
-        const uint32_t rr = t.r0 + r, tok = token_of(a, rr);
-        const int64_t head = h * a.groups + (rr - tok * a.groups);
-        const int to = half * kChunk + col;
-        if (whole) {
-          T y[4];
+            for (int k = 0; k < 8; ++k) v[k] += obuf[x][rr][col + k];
+          const uint32_t row = t.r0 + 32 * r + rr, token = token_of(a, row);
+          if (patch) {  // the NaN that this row does see: columns of NaN
+            const int64_t seen = visible(a, t.s, token);
+            const int end = seen < (int64_t)n * 32 ? (int)seen : n * 32;
+            for (int key = (seen_whole > t0 ? seen_whole : t0) * 32; key < end; ++key) {
+              const Kv8Place at = place(key >> 5, page_of(key >> 5));
+              if (!at.there) continue;
+              const int in = key & 31;
+              const uint8_t *const vb = static_cast<const uint8_t *>(a.c.v) +
+                                        ((at.slot << (a.page_log2 - 5)) + at.tile) * (int64_t)(NV * 1024) +
+                                        (in / 4 % 2) * 512 + in / 16 * 8 + in / 8 % 2 * 4 + in % 4;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) y[k] = Elem<DT>::from_f(v[k] * inv[r]);
-          __builtin_memcpy(static_cast<T *>(a.out) + (t.s.first + tok) * a.os_t + head * a.os_h + to, y, 8);
-        } else {
-          *reinterpret_cast<float4 *>(a.part + (((t.s.first + tok) * a.heads + head) * a.splits + split) * DV + to) =
-              make_float4(v[0], v[1], v[2], v[3]);
+              for (int k = 0; k < 8; ++k) {
+                const int to = part * kChunk + col + k;
+                if ((vb[to / 32 * 1024 + to % 32 * 16] & 0x7f) == 0x7f) v[k] = __builtin_nanf("");
+              }
+            }
+          }
+          if (whole) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] *= inv_s[rr];
+            tm_store8<DT>(static_cast<T *>(a.out) + (t.s.first + token) * a.os_t + head_of(row, token) * a.os_h +
+                              part * kChunk + col, v);
+          } else {
+            tm_store8<TM_DT_F32>(a.part + (((t.s.first + token) * a.heads + head_of(row, token)) * a.splits + split) * DV +
+                                     part * kChunk + col, v);
+          }
         }
       }
-      if (half + 1 < DV / kChunk) __syncthreads();
     }
   }
 }
@@ -298,9 +360,9 @@ __global__ __launch_bounds__(kAttThreads, D + DV > 320 ? 1 : 2) void attend_kern
 // Joins the splits of a row: a workgroup per row, a thread owning 4 columns of some splits, whose
 // parts are requested together with the statistics.
 template <int DT, int DV, int OWN>
-__global__ __launch_bounds__(kAttThreads) void join_kernel(AttArgs a) {
+__global__ __launch_bounds__(kThreads) void join_kernel(AttArgs a) {
   using T = typename Elem<DT>::T;
-  constexpr int kCols = DV / 4, kSets = kAttThreads / kCols;  // OWN: splits of a thread
+  constexpr int kCols = DV / 4, kSets = kThreads / kCols;  // OWN: splits of a thread
   __shared__ float fac[kMaxSplits];
   __shared__ __align__(16) float4 red[kSets][kCols];
   const int h = blockIdx.y;
@@ -355,47 +417,70 @@ __global__ __launch_bounds__(kAttThreads) void join_kernel(AttArgs a) {
   if (a.lse && threadIdx.x == 0) a.lse[row] = total == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
-int page_log2(int page) { return page == 32 ? 5 : page == 64 ? 6 : 7; }
-
-// Row tiles of a call (an upper bound), and the splits of the keys.
-int64_t row_tiles(const tm_kv8_batch *b, int groups) {
-  return b->starts ? b->n_tokens * groups / 32 + b->n_seqs : b->n_seqs * tm_cdiv(groups, 32);
+// How a call is cut up: R x 32 rows a workgroup, at most `tiles` of these per key head, keys split `splits` times.
+struct Plan {
+  int r, splits;
+  int64_t tiles;
+};
+Plan plan_of(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups) {
+  const int64_t rows = b->n_tokens * groups, heads = c->n_kv_heads;
+  Plan p = {1, 1, b->starts ? rows / 32 + b->n_seqs : b->n_seqs * tm_cdiv(groups, 32)};
+  // 64 rows a wave where that leaves four workgroups for each that a CU holds (32 heads on 4, us with 32 and 64 rows:
+  // 2048 tokens 53, 58; 4099 173, 167; 8192 599, 554); wider values leave no registers for them
+  if (b->starts && c->v_dim <= 128 && (rows / 64 + b->n_seqs) * heads >= 2048) {
+    p.r = 2;
+    p.tiles = rows / 64 + b->n_seqs;
+    return p;
+  }
+  const int64_t units = p.tiles * heads, keys = (int64_t)b->max_pages * c->page_size / kKv8Tile;
+  // Up to 1024 keys (eight rounds of the four waves) one launch: a round is 0.7 us, joining parts 3 of the host's and 2
+  // of the device's.  Then one workgroup per CU, from 4096 keys on two (32 heads on 4, one sequence, us by splits: 4000
+  // keys 1 28, 4 13.6, 16 9.4; eight sequences of 4000: 1 29, 4 14.7, 8 11.9, 16 12.4).
+  if (units <= 0 || keys <= 32) return p;
+  int64_t s = (keys <= 128 ? 256 : 512) / units;
+  s = s < keys / kWaves ? s : keys / kWaves;
+  p.splits = (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+  return p;
 }
-int key_splits(const tm_kv8_cache *c, const tm_kv8_batch *b, int64_t tiles) {
-  const int64_t units = tiles * c->n_kv_heads, keys = (int64_t)b->max_pages * c->page_size / 32;
-  if (units <= 0) return 1;
-  int64_t s = 512 / units;  // two workgroups per CU
-  s = s < keys / 8 ? s : keys / 8;
-  return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+
+AttArgs args_of(const tm_kv8_cache *c, const tm_kv8_batch *b, const void *q, int64_t qs_t, int64_t qs_h, int n_heads,
+                float scale, const Plan &p) {
+  AttArgs a = {};
+  a.c = *c;
+  a.b = *b;
+  a.q = q, a.qs_t = qs_t, a.qs_h = qs_h;
+  a.scale = scale;
+  a.heads = n_heads;
+  a.groups = n_heads / c->n_kv_heads;
+  a.splits = p.splits;
+  a.page_log2 = c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
+  a.tiles1 = (int)tm_cdiv(a.groups, 32);
+  return a;
+}
+
+template <int DT, int D, int DV, int R>
+void launch(const AttArgs &a, const Plan &p, hipStream_t s) {
+  const dim3 grid((unsigned)(p.tiles * a.c.n_kv_heads), (unsigned)p.splits);
+  hipLaunchKernelGGL((attend_kernel<DT, D, DV, R>), grid, dim3(kThreads), 0, s, a);
 }
 
 }  // namespace
 
 int tm_internal_kv8_splits(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups) {
-  return key_splits(c, b, row_tiles(b, groups));
+  return plan_of(c, b, groups).splits;
 }
 int tm_internal_kv8_stats(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *q, int64_t qs_b,
                           int64_t qs_h, int32_t n_heads, float scale, float2 *stats, hipStream_t s) {
-  AttArgs a = {};
-  a.c = *cache;
-  a.b = *batch;
-  a.groups = n_heads / cache->n_kv_heads;
-  const int64_t tiles = row_tiles(batch, a.groups);
-  a.splits = key_splits(cache, batch, tiles);
-  a.q = q, a.qs_t = qs_b, a.qs_h = qs_h;
+  const Plan p = plan_of(cache, batch, n_heads / cache->n_kv_heads);
+  AttArgs a = args_of(cache, batch, q, qs_b, qs_h, n_heads, scale, p);
   a.stats = stats;
-  a.scale = scale;
-  a.heads = n_heads;
-  a.page_log2 = page_log2(cache->page_size);
-  a.tiles1 = (int)tm_cdiv(a.groups, 32);
-  const dim3 grid((unsigned)tiles, (unsigned)cache->n_kv_heads, (unsigned)a.splits);
   auto run = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     switch (cache->head_dim) {
-      case 64: hipLaunchKernelGGL((attend_kernel<DT, 64, 0>), grid, dim3(kAttThreads), 0, s, a); break;
-      case 128: hipLaunchKernelGGL((attend_kernel<DT, 128, 0>), grid, dim3(kAttThreads), 0, s, a); break;
-      case 192: hipLaunchKernelGGL((attend_kernel<DT, 192, 0>), grid, dim3(kAttThreads), 0, s, a); break;
-      default: hipLaunchKernelGGL((attend_kernel<DT, 256, 0>), grid, dim3(kAttThreads), 0, s, a); break;
+      case 64: launch<DT, 64, 0, 1>(a, p, s); break;
+      case 128: launch<DT, 128, 0, 1>(a, p, s); break;
+      case 192: launch<DT, 192, 0, 1>(a, p, s); break;
+      default: launch<DT, 256, 0, 1>(a, p, s); break;
     }
   };
   if (dtype == TM_DT_F16) run(std::integral_constant<int, TM_DT_F16>{});
@@ -407,7 +492,7 @@ int tm_internal_kv8_stats(const tm_kv8_cache *cache, const tm_kv8_batch *batch, 
 extern "C" size_t tm_kv8_attention_workspace_size(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t n_heads) {
   if (!cache || !batch || n_heads < 1 || cache->n_kv_heads < 1 || n_heads % cache->n_kv_heads || batch->n_tokens <= 0)
     return 0;
-  const int s = key_splits(cache, batch, row_tiles(batch, n_heads / cache->n_kv_heads));
+  const int s = plan_of(cache, batch, n_heads / cache->n_kv_heads).splits;
   if (s == 1) return 0;
   return (size_t)batch->n_tokens * n_heads * s * (cache->v_dim + 2) * sizeof(float) + 16;
 }
@@ -429,41 +514,37 @@ extern "C" int tm_kv8_attention(const tm_kv8_cache *cache, const tm_kv8_batch *b
   if (n_heads == 1) qs_h = os_h = 0;
   TM_REQUIRE(tm_aligned16(q) && tm_aligned16(out) && qs_t % 8 == 0 && qs_h % 8 == 0 && os_t % 8 == 0 && os_h % 8 == 0,
              TM_EINVAL_SHAPE, "tm_kv8_attention: rows of q and out must be 16-byte aligned, strides multiples of 8 elements");
-  AttArgs a = {};
-  a.c = *cache;
-  a.b = *batch;
-  if (cache->n_pages == 0) a.b.max_pages = 0;  // no page is there
-  a.groups = n_heads / cache->n_kv_heads;
-  const int64_t tiles = row_tiles(batch, a.groups);
-  TM_REQUIRE(batch->n_tokens * a.groups + 32 * batch->n_seqs < ((int64_t)1 << 31), TM_EINVAL_SHAPE,
-             "tm_kv8_attention: too many rows");
-  a.splits = key_splits(cache, batch, tiles);
+  const int groups = n_heads / cache->n_kv_heads;
+  TM_REQUIRE((batch->n_tokens * groups + 64 * batch->n_seqs) / 32 * cache->n_kv_heads < ((int64_t)1 << 31) &&
+                 batch->n_tokens * groups < ((int64_t)1 << 31),
+             TM_EINVAL_SHAPE, "tm_kv8_attention: too many rows");
+  const Plan p = plan_of(cache, batch, groups);
   const size_t need = tm_kv8_attention_workspace_size(cache, batch, n_heads);
   TM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && tm_aligned16(workspace)), TM_EWORKSPACE,
              "tm_kv8_attention: workspace %zu bytes < %zu", workspace_bytes, need);
-  a.q = q, a.qs_t = qs_t, a.qs_h = qs_h;
+  AttArgs a = args_of(cache, batch, q, qs_t, qs_h, n_heads, scale, p);
+  if (cache->n_pages == 0) a.b.max_pages = 0;  // no page is there
   a.out = out, a.os_t = os_t, a.os_h = os_h;
   a.lse = lse;
-  const int64_t rows = batch->n_tokens * n_heads * a.splits;
-  a.part = static_cast<float *>(workspace);
-  a.stats = reinterpret_cast<float2 *>(a.part + rows * cache->v_dim);
-  a.scale = scale;
-  a.heads = n_heads;
-  a.page_log2 = page_log2(cache->page_size);
   a.causal = causal != 0;
-  a.tiles1 = (int)tm_cdiv(a.groups, 32);
+  a.part = static_cast<float *>(workspace);
+  a.stats = reinterpret_cast<float2 *>(a.part + batch->n_tokens * n_heads * p.splits * cache->v_dim);
   hipStream_t s = tm_hip_stream(stream);
   auto run = [&](auto dt, auto d, auto dv) {
     constexpr int DT = decltype(dt)::value, D = decltype(d)::value, DV = decltype(dv)::value;
-    hipLaunchKernelGGL((attend_kernel<DT, D, DV>), dim3((unsigned)tiles, (unsigned)cache->n_kv_heads, (unsigned)a.splits),
-                       dim3(kAttThreads), 0, s, a);
+    if constexpr (DV <= 128) {
+      if (p.r == 2) launch<DT, D, DV, 2>(a, p, s);
+      else launch<DT, D, DV, 1>(a, p, s);
+    } else {
+      launch<DT, D, DV, 1>(a, p, s);
+    }
     TM_LAUNCH_CHECK("tm_kv8_attention");
-    if (a.splits > 1) {
+    if (p.splits > 1) {
       // (rows of a tile: one token's heads, or 32 of several tokens)
-      const dim3 grid((unsigned)tiles, (unsigned)cache->n_kv_heads, (unsigned)(!batch->starts && a.groups < 32 ? a.groups : 32));
-      constexpr int kSets = kAttThreads / (DV / 4);
-      if (a.splits <= 4 * kSets) hipLaunchKernelGGL((join_kernel<DT, DV, 4>), grid, dim3(kAttThreads), 0, s, a);
-      else hipLaunchKernelGGL((join_kernel<DT, DV, (kMaxSplits + kSets - 1) / kSets>), grid, dim3(kAttThreads), 0, s, a);
+      const dim3 grid((unsigned)p.tiles, (unsigned)cache->n_kv_heads, (unsigned)(!batch->starts && groups < 32 ? groups : 32));
+      constexpr int kSets = kThreads / (DV / 4);
+      if (p.splits <= 4 * kSets) hipLaunchKernelGGL((join_kernel<DT, DV, 4>), grid, dim3(kThreads), 0, s, a);
+      else hipLaunchKernelGGL((join_kernel<DT, DV, (kMaxSplits + kSets - 1) / kSets>), grid, dim3(kThreads), 0, s, a);
       TM_LAUNCH_CHECK("tm_kv8_attention(join)");
     }
     return TM_OK;

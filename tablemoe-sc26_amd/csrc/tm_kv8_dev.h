@@ -17,16 +17,16 @@ struct Kv8Place {
 };
 // The page of a tile, as its sequence's row of the table names it (-1: past the table's width).  Loaded a round before
 // the tile itself: the bytes wait for it.
-__device__ __forceinline__ int tm_kv8_page(const tm_kv8_batch &bt, const int32_t *row, int64_t tile, int page_log2) {
-  const int64_t p = tile >> (page_log2 - 5);
+__device__ __forceinline__ int tm_kv8_page(const tm_kv8_batch &bt, const int32_t *row, int tile, int page_log2) {
+  const int p = tile >> (page_log2 - 5);  // (max_pages < 2^24: a tile's number fits 32 bits)
   const int id = row[p < bt.max_pages ? p : bt.max_pages - 1];
   return p < bt.max_pages ? id : -1;
 }
-__device__ __forceinline__ Kv8Place tm_kv8_place(const tm_kv8_cache &c, int id, int h, int64_t tile, int page_log2) {
+__device__ __forceinline__ Kv8Place tm_kv8_place(const tm_kv8_cache &c, int id, int h, int tile, int page_log2) {
   Kv8Place r;
   r.there = id >= 0 && id < c.n_pages;
   r.slot = (int64_t)(r.there ? id : 0) * c.n_kv_heads + h;
-  r.tile = (int)(tile & ((1 << (page_log2 - 5)) - 1));
+  r.tile = tile & ((1 << (page_log2 - 5)) - 1);
   return r;
 }
 

@@ -41,12 +41,13 @@ __global__ __launch_bounds__(kThreads) void importance_kernel(ImpArgs a) {
   __shared__ float acc[kWaves][kMaxPer][32];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int c = lane & 31, g = lane >> 5;
-  const int64_t b = blockIdx.y, tile0 = (int64_t)blockIdx.x * a.per;
+  const int64_t b = blockIdx.y;
+  const int tile0 = (int)(blockIdx.x * a.per);
   const int64_t cap = (int64_t)a.b.max_pages << a.page_log2;
   int64_t len = a.b.lengths[b];
   len = len < 0 ? 0 : len < cap ? len : cap;
-  const int64_t tiles = (len + 31) >> 5;
-  const int64_t end = tile0 + a.per < tiles ? tile0 + a.per : tiles;  // tiles to compute
+  const int tiles = (int)((len + 31) >> 5);
+  const int end = tile0 + a.per < tiles ? tile0 + a.per : tiles;  // tiles to compute
   if (tile0 < tiles) {
     if (a.lse != nullptr) {
       if (tid < a.heads) norm[tid] = a.lse[b * a.ld_lse + tid] * kLog2e;
@@ -96,7 +97,16 @@ __global__ __launch_bounds__(kThreads) void importance_kernel(ImpArgs a) {
           const int r = r0 + 8 * (i / 4) + 4 * g + i % 4;
           nr[i] = norm[h * a.groups + (r < a.groups ? r : a.groups - 1)];
         }
-        auto step = [&](int64_t tile, const Kv8Place &w, const uint4 (&kf)[NK], float sk) {
+        const int32_t *const pages = a.b.table + b * a.b.ld_table;
+        auto page_of = [&](int tile) { return tm_kv8_page(a.b, pages, tile < end ? tile : end - 1, a.page_log2); };
+        auto place = [&](int tile, int id) { return tm_kv8_place(a.c, id, h, tile < end ? tile : end - 1, a.page_log2); };
+        uint4 kf[NK];
+        Kv8Place w = place(tile0 + my_tile, page_of(tile0 + my_tile));
+        int id = page_of(tile0 + my_tile + tile_waves);
+        tm_kv8_load<NK>(a.c.k, w, a.page_log2, lane, kf);
+        float sk = a.c.k_scale[w.slot];
+#pragma unroll 1
+        for (int tile = tile0 + my_tile; tile < end; tile += tile_waves) {
           tm_f32x16 s;
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[i] = 0.f;
@@ -105,7 +115,12 @@ __global__ __launch_bounds__(kThreads) void importance_kernel(ImpArgs a) {
             s = tm_mfma32x32x16<DT>(qf[j][0], tm_kv8_operand<DT>(kf[j].x, kf[j].y), s);
             s = tm_mfma32x32x16<DT>(qf[j][1], tm_kv8_operand<DT>(kf[j].z, kf[j].w), s);
           }
-          const float mul = sk * unit;
+          const bool there = w.there;
+          const float mul = there ? sk * unit : unit;
+          w = place(tile + tile_waves, id);
+          id = page_of(tile + 2 * tile_waves);
+          tm_kv8_load<NK>(a.c.k, w, a.page_log2, lane, kf);
+          sk = a.c.k_scale[w.slot];
           float sum = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -113,35 +128,12 @@ __global__ __launch_bounds__(kThreads) void importance_kernel(ImpArgs a) {
             sum += r0 + 8 * (i / 4) + 4 * g + i % 4 < a.groups ? p : 0.f;
           }
           sum += tm_other_half(sum);
-          const int at = (int)(tile - tile0);
-          if (g == 0 && w.there) acc[wave][at][c] += sum;
-        };
-        uint4 ka[NK], kb[NK];
-        Kv8Place wa, wb;
-        float sa, sb;
-        const int32_t *const pages = a.b.table + b * a.b.ld_table;
-        auto page_of = [&](int64_t tile) { return tm_kv8_page(a.b, pages, tile < end ? tile : end - 1, a.page_log2); };
-        auto fetch = [&](int64_t tile, int id, Kv8Place &w, uint4 (&kf)[NK], float &sk) {
-          w = tm_kv8_place(a.c, id, h, tile < end ? tile : end - 1, a.page_log2);
-          tm_kv8_load<NK>(a.c.k, w, a.page_log2, lane, kf);
-          sk = a.c.k_scale[w.slot];
-        };
-        const int64_t begin = tile0 + my_tile;
-        int ida = page_of(begin), idb = page_of(begin + tile_waves);
-        fetch(begin, ida, wa, ka, sa);
-        for (int64_t tile = begin; tile < end; tile += 2 * tile_waves) {
-          ida = page_of(tile + 2 * tile_waves);
-          fetch(tile + tile_waves, idb, wb, kb, sb);
-          step(tile, wa, ka, sa);
-          if (tile + tile_waves >= end) break;
-          idb = page_of(tile + 3 * tile_waves);
-          fetch(tile + 2 * tile_waves, ida, wa, ka, sa);
-          step(tile + tile_waves, wb, kb, sb);
+          if (g == 0 && there) acc[wave][tile - tile0][c] += sum;
         }
       }
   __syncthreads();
   for (int i = tid; i < a.per * 32; i += kThreads) {
-    const int64_t t = tile0 * 32 + i;
+    const int64_t t = (int64_t)tile0 * 32 + i;
     if (t >= a.out_len) break;
     float v = 0.f;
 #pragma unroll

@@ -66,11 +66,12 @@ def _run(q, k, positions, inv_freq, sections, interleaved, adjacent, inverse, q_
         kp, kv, kop = k.data_ptr(), k.shape[1], k_out.data_ptr()
         ks_t, ks_h, _ = k.stride()
         ko_t, ko_h, _ = k_out.stride()
+    axes = len(sections)
     with N.on_device(dev):
         N.call("tm_rotate_positions", N.dtype_tag(q.dtype), q.data_ptr(), n, h, qs_t, qs_h, kp, kv, ks_t, ks_h, d,
-               2 * inv_freq.shape[0], positions.data_ptr(), positions.stride(0) if len(sections) > 1 else n,
-               len(sections), _sections(sections), interleaved, adjacent, inverse, inv_freq.data_ptr(), q_out.data_ptr(),
-               qo_t, qo_h, kop, ko_t, ko_h, N.stream(dev))
+               2 * inv_freq.shape[0], positions.data_ptr(), positions.stride(0) if axes > 1 else n, axes,
+               _sections(sections), interleaved, adjacent, inverse, inv_freq.data_ptr(), q_out.data_ptr(), qo_t, qo_h,
+               kop, ko_t, ko_h, N.stream(dev))
 
 
 def _unit_rows(t: torch.Tensor) -> torch.Tensor:
@@ -78,7 +79,7 @@ def _unit_rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _new(t: torch.Tensor) -> torch.Tensor:
-    return torch.empty_like(t, memory_format=torch.contiguous_format)
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 class _Rotate(torch.autograd.Function):
