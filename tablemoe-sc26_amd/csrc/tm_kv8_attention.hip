@@ -100,7 +100,6 @@ __device__ __forceinline__ uint32_t token_of(const AttArgs &a, uint32_t row) {
   return a.b.starts == nullptr ? 0 : row / (uint32_t)a.groups;
 }
 
-
 // DV = 0: the statistics alone.
 template <int DT, int D, int DV, int R>
 __global__ __launch_bounds__(kThreads, R == 2 || D + DV > 320 ? 2 : 3) void attend_kernel(AttArgs a) {
@@ -175,106 +174,106 @@ __global__ __launch_bounds__(kThreads, R == 2 || D + DV > 320 ? 2 : 3) void atte
   bool seen_nan = false;  // among values that some row does not see
 #pragma unroll 1
   for (int tile = begin; tile < n; tile += kWaves) {
-      tm_f32x16 s[R];
+    tm_f32x16 s[R];
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[r][i] = 0.f;
+      for (int i = 0; i < 16; ++i) s[r][i] = 0.f;
 #pragma unroll
-      for (int j = 0; j < NK; ++j)
+    for (int j = 0; j < NK; ++j)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint4 k = e ? tm_kv8_operand<DT>(kf[j].z, kf[j].w) : tm_kv8_operand<DT>(kf[j].x, kf[j].y);
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            s[r] = tm_mfma32x32x16<DT>(k, qs[(r * NK + j) * 2 + e][lane], s[r]);
-          }
-        }
-      const Kv8Place wn = place(tile + kWaves, id);
-      id = page_of(tile + 2 * kWaves);
-      tm_kv8_load<NK>(a.c.k, wn, a.page_log2, lane, kf);
-      const float mul = (w.there ? sk : 1.f) * unit, add = w.there ? tm_exponent(sv) : 0.f;
-      sk = a.c.k_scale[wn.slot];
-      if constexpr (NV > 0) sv = a.c.v_scale[wn.slot];
-      if (!w.there || tile >= seen_whole) {
-        first = true;
-        uint32_t nan = 0;  // a NaN among values that some row does not see stays out of the product
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          uint32_t *const p = reinterpret_cast<uint32_t *>(&vf[j]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t x = ((p[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // 0x80 where a byte is NaN
-            nan |= x;
-            p[e] &= ~((x >> 7) * 0xffu);
-          }
-        }
-        seen_nan = seen_nan || nan != 0;
+      for (int e = 0; e < 2; ++e) {
+        const uint4 k = e ? tm_kv8_operand<DT>(kf[j].z, kf[j].w) : tm_kv8_operand<DT>(kf[j].x, kf[j].y);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const int64_t left = (w.there ? limit[r] : 0) - (int64_t)tile * 32;
-          int lim = left > 32 ? 32 : left < 0 ? 0 : (int)left;
-          asm volatile("" : "+v"(lim));  // (what follows stays in this branch)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[r][i] = 8 * (i / 4) + 4 * g + i % 4 < lim ? s[r][i] : -__builtin_huge_valf();
+        s[r] = tm_mfma32x32x16<DT>(k, qs[(r * NK + j) * 2 + e][lane], s[r]);
         }
       }
-      w = wn;
-      const float back = __builtin_amdgcn_exp2f(-add - kRoom);
-      bool none = false;
-      uint4 p[R][2];
+    const Kv8Place wn = place(tile + kWaves, id);
+    id = page_of(tile + 2 * kWaves);
+    tm_kv8_load<NK>(a.c.k, wn, a.page_log2, lane, kf);
+    const float mul = (w.there ? sk : 1.f) * unit, add = w.there ? tm_exponent(sv) : 0.f;
+    sk = a.c.k_scale[wn.slot];
+    if constexpr (NV > 0) sv = a.c.v_scale[wn.slot];
+    if (!w.there || tile >= seen_whole) {
+      first = true;
+      uint32_t nan = 0;  // a NaN among values that some row does not see stays out of the product
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        uint32_t *const p = reinterpret_cast<uint32_t *>(&vf[j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t x = ((p[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // 0x80 where a byte is NaN
+          nan |= x;
+          p[e] &= ~((x >> 7) * 0xffu);
+        }
+      }
+      seen_nan = seen_nan || nan != 0;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        auto settle = [&] {  // the row's reference 2^8 under its largest score so far
-          float top = s[r][0];
+        const int64_t left = (w.there ? limit[r] : 0) - (int64_t)tile * 32;
+        int lim = left > 32 ? 32 : left < 0 ? 0 : (int)left;
+        asm volatile("" : "+v"(lim));  // (what follows stays in this branch)
 #pragma unroll
-          for (int i = 1; i < 16; ++i) top = fmaxf(top, s[r][i]);
-          top = fmaf(top, mul, add);
-          top = fmaxf(top, tm_other_half(top));
-          const float to = fmaxf(m[r], top - kRoom);
-          const float f = m[r] == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(m[r] - to);
-          m[r] = to;
-          l[r] *= f;
-#pragma unroll
-          for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[r][j][i] *= f;
-        };
-        if (first) {
-          settle();
-          none = none || m[r] == -__builtin_huge_valf();
-        }
-        float sum;
-        auto probabilities = [&] {
-          const float off = add - (m[r] == -__builtin_huge_valf() ? 0.f : m[r]);
-          uint32_t pf[8];
-          sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const tm_f32x2 x = {__builtin_amdgcn_exp2f(fmaf(s[r][i], mul, off)), __builtin_amdgcn_exp2f(fmaf(s[r][i + 1], mul, off))};
-            sum += x.x + x.y;
-            pf[i / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, tm_f16x2));
-          }
-          p[r][0] = make_uint4(pf[0], pf[1], pf[2], pf[3]);
-          p[r][1] = make_uint4(pf[4], pf[5], pf[6], pf[7]);
-        };
-        probabilities();
-        if (__any(sum > kMost)) {
-          settle();
-          probabilities();
-        }
-        l[r] = fmaf(sum, back, l[r]);
+        for (int i = 0; i < 16; ++i) s[r][i] = 8 * (i / 4) + 4 * g + i % 4 < lim ? s[r][i] : -__builtin_huge_valf();
       }
-      if (first) first = __any(none);
+    }
+    w = wn;
+    const float back = __builtin_amdgcn_exp2f(-add - kRoom);
+    bool none = false;
+    uint4 p[R][2];
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+    for (int r = 0; r < R; ++r) {
+      auto settle = [&] {  // the row's reference 2^8 under its largest score so far
+        float top = s[r][0];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint4 v = e ? tm_kv8_operand<TM_DT_F16>(vf[j].z, vf[j].w) : tm_kv8_operand<TM_DT_F16>(vf[j].x, vf[j].y);
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[r][i]);
+        top = fmaf(top, mul, add);
+        top = fmaxf(top, tm_other_half(top));
+        const float to = fmaxf(m[r], top - kRoom);
+        const float f = m[r] == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(m[r] - to);
+        m[r] = to;
+        l[r] *= f;
 #pragma unroll
-          for (int r = 0; r < R; ++r) o[r][j] = tm_mfma32x32x16<TM_DT_F16>(v, p[r][e], o[r][j]);
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[r][j][i] *= f;
+      };
+      if (first) {
+        settle();
+        none = none || m[r] == -__builtin_huge_valf();
+      }
+      float sum;
+      auto probabilities = [&] {
+        const float off = add - (m[r] == -__builtin_huge_valf() ? 0.f : m[r]);
+        uint32_t pf[8];
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const tm_f32x2 x = {__builtin_amdgcn_exp2f(fmaf(s[r][i], mul, off)), __builtin_amdgcn_exp2f(fmaf(s[r][i + 1], mul, off))};
+          sum += x.x + x.y;
+          pf[i / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, tm_f16x2));
         }
-      if constexpr (NV > 0) tm_kv8_load<NV>(a.c.v, w, a.page_log2, lane, vf);
+        p[r][0] = make_uint4(pf[0], pf[1], pf[2], pf[3]);
+        p[r][1] = make_uint4(pf[4], pf[5], pf[6], pf[7]);
+      };
+      probabilities();
+      if (__any(sum > kMost)) {
+        settle();
+        probabilities();
+      }
+      l[r] = fmaf(sum, back, l[r]);
+    }
+    if (first) first = __any(none);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint4 v = e ? tm_kv8_operand<TM_DT_F16>(vf[j].z, vf[j].w) : tm_kv8_operand<TM_DT_F16>(vf[j].x, vf[j].y);
+#pragma unroll
+        for (int r = 0; r < R; ++r) o[r][j] = tm_mfma32x32x16<TM_DT_F16>(v, p[r][e], o[r][j]);
+      }
+    if constexpr (NV > 0) tm_kv8_load<NV>(a.c.v, w, a.page_log2, lane, vf);
   }
   const bool patch = __syncthreads_or(seen_nan) != 0;  // (the queries are done with, too)
   float(*const obuf)[32][kChunk + 4] = reinterpret_cast<float(*)[32][kChunk + 4]>(lds);
@@ -427,7 +426,7 @@ Plan plan_of(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups) {
   Plan p = {1, 1, b->starts ? rows / 32 + b->n_seqs : b->n_seqs * tm_cdiv(groups, 32)};
   // 64 rows a wave where that leaves four workgroups for each that a CU holds (32 heads on 4, us with 32 and 64 rows:
   // 2048 tokens 53, 58; 4099 173, 167; 8192 599, 554); wider values leave no registers for them
-  if (b->starts && c->v_dim <= 128 && (rows / 64 + b->n_seqs) * heads >= 2048) {
+  if (b->starts && c->v_dim <= 128 && rows / 64 * heads >= 2048) {
     p.r = 2;
     p.tiles = rows / 64 + b->n_seqs;
     return p;

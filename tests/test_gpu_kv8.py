@@ -227,6 +227,25 @@ def test_append(hip_device, page, d, dv, kv, lens, new, dt):
     assert torch.equal(vd.cpu().double()[0], vc[table[-1, 0]] * vs[table[-1, 0]][:, None, None])
 
 
+def test_append_draft_then_rollback(hip_device):
+    """A few tokens written, some taken back by a shorter length, others written in their place: scales stay, cells
+    past the end keep their bytes until they are written again."""
+    g = torch.Generator().manual_seed(12)
+    dev, page, d, kv = hip_device, 32, 64, 1
+    cache, (kc, ks, vc, vs) = filled(g, 4, kv, page, d, d, dev)
+    table = torch.tensor([[2, 0], [1, 3]], dtype=torch.int32)
+    for lens, new, size in (([30, 20], [30, 20], 1.0), ([35, 24], [5, 4], 3.0), ([33, 21], [2, 1], 0.1), ([37, 33], [4, 12], 9.0)):
+        n = sum(new)
+        k, v = (size * torch.randn(n, kv, d, generator=g)).to(BF16), (size * torch.randn(n, kv, d, generator=g)).to(BF16)
+        lengths, starts = torch.tensor(lens, dtype=torch.int32), torch.tensor([0, new[0], n], dtype=torch.int32)
+        cache.append(k.to(dev), v.to(dev), table.to(dev), lengths.to(dev), starts.to(dev))
+        for rows, c, s in ((k, kc, ks), (v, vc, vs)):
+            R.append(c, s, rows, table, lengths, starts)
+        assert torch.equal(cache.k_scale.cpu().double(), ks) and torch.equal(cache.v_scale.cpu().double(), vs)
+        same_cells(cache.k, kc, False)
+        same_cells(cache.v, vc, True)
+
+
 def test_append_odd_batches(hip_device):
     """Non-finite values, zeros, tiny and huge ones; pages that are not there; more new tokens than positions; positions
     past the table; rows of no sequence; 64-bit lists; strided rows."""
@@ -340,6 +359,51 @@ def test_attend_long(hip_device, n, page, dt):
     imp2 = cache.importance(q.to(dev), table.to(dev), lengths.to(dev), scale=0.2, lse=lse, out_len=n)
     check_importance(plain, q, table, lengths, 0.2, imp)
     check_importance(plain, q, table, lengths, 0.2, imp2)
+
+
+@pytest.mark.parametrize("d,dv,dt,causal", [(64, 64, BF16, True), (128, 128, F16, True), (192, 128, BF16, False)])
+def test_attend_many_rows(hip_device, d, dv, dt, causal):
+    """Enough rows that a wave takes 64 of them (tokens times heads from 131072 on): two prompts with 256 heads to a key
+    head, rows that end inside a tile, NaN among what later tokens bring."""
+    g = torch.Generator().manual_seed(d + dv)
+    dev, page, kv, h = hip_device, 32, 2, 512
+    lens, new = [150, 133], [150, 110]
+    counts = [5, 5]
+    cache, plain = filled(g, 12, kv, page, d, dv, dev)
+    table = table_of(g, counts, 6, 12)
+    if causal:  # position 141 of the first prompt, in V: later tokens see it
+        plain[2][table[0, 4], 1, 13, 7] = math.nan
+        cache.v.view(torch.uint8).copy_(R.pack(plain[2], True).view(torch.uint8))
+    lengths, starts = torch.tensor(lens, dtype=torch.int32), torch.tensor([0, 150, 260], dtype=torch.int32)
+    q = (1.5 * torch.randn(260, h, d, generator=g)).to(dt)
+    y, lse = cache.attend(q.to(dev), table.to(dev), lengths.to(dev), starts.to(dev), causal=causal, return_lse=True)
+    if causal:
+        bad = torch.isnan(y).cpu()
+        assert bool(bad[141:150, 256:, 7].all()) and int(bad.sum()) == 9 * 256
+        y = torch.where(torch.isnan(y), torch.zeros_like(y), y)
+        plain[2] = torch.nan_to_num(plain[2])
+    rows = {0, 1, 31, 64, 127, 140, 150, 151, 200, 259} if causal else {0, 149, 150, 222}
+    check_attend(cache, plain, q, table, lengths, starts, y, lse, d ** -0.5, causal, rows)
+
+
+def test_attend_small_scales(hip_device):
+    """Values so small that their scales sit at the floor of 2^-100."""
+    g = torch.Generator().manual_seed(77)
+    dev, d = hip_device, 64
+    from table_moe.ops import Fp8KVCache
+
+    cache = Fp8KVCache(20, 1, d, page_size=32, device=dev)
+    k, v = torch.randn(600, 1, d, generator=g), torch.randn(600, 1, d, generator=g) * 1e-29
+    table, lengths = torch.arange(20, dtype=torch.int32, device=dev)[None], torch.tensor([600], device=dev)
+    cache.append(k.to(dev), v.to(dev), table, lengths, torch.tensor([0, 600], device=dev))
+    assert float(cache.v_scale[:19].max()) == 2.0 ** -100
+    q = torch.randn(1, 4, d, generator=g).to(BF16)
+    y, lse = cache.attend(q.to(dev), table, lengths, return_lse=True)
+    kk, vv = (t.cpu().double().transpose(1, 2).flatten(0, 1)[:600] for t in cache.read_pages())
+    # (bf16 holds these magnitudes: its exponents are fp32's)
+    want = R.attend(q[0].double(), kk, vv, torch.ones(600, dtype=torch.bool), d ** -0.5)
+    attend_close(y[0].float() * 2.0 ** 90, lse[0], want[0] * 2.0 ** 90, want[1], want[2] * 2.0 ** 90, want[3], want[4].amax(0), BF16,
+                 d, 600, 1.0)
 
 
 def test_attend_offsets_past_32_bits(hip_device):
