@@ -38,12 +38,14 @@ THETA = 5000000.0
 
 
 def _ops():
-    root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "tablemoe-sc26_amd")
-    if root not in sys.path:
-        sys.path.insert(0, root)
-    from table_moe import ops
+    if not hasattr(_ops, "module"):  # imported once, as a user's program does
+        root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "tablemoe-sc26_amd")
+        if root not in sys.path:
+            sys.path.insert(0, root)
+        from table_moe import ops
 
-    return ops
+        _ops.module = ops
+    return _ops.module
 
 
 # --------------------------------------------------------------------- cases
@@ -385,8 +387,10 @@ def run(state):
     kind = c["kind"]
     if kind == "rotate":
         if own:
+            if "sections" not in state:
+                state["sections"] = [int(v) for v in c["sections"].split(",")]
             return list(_ops().rotate_positions(
-                state["q"], state["k"], state["positions"], state["inv"], [int(v) for v in c["sections"].split(",")],
+                state["q"], state["k"], state["positions"], state["inv"], state["sections"],
                 interleaved=c["interleaved"], adjacent=c["adjacent"], inverse=c["inverse"]))
         return [_rotate_plain(state["q"], state, c), _rotate_plain(state["k"], state, c)]
     if kind == "append":
