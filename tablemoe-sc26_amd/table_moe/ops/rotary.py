@@ -43,6 +43,8 @@ def _span(t: torch.Tensor):
 
 
 def _check_out(name: str, out: torch.Tensor, x: torch.Tensor) -> None:
+    if out is x and x.is_contiguous():
+        return
     if out.shape != x.shape or out.dtype != x.dtype or not rows_apart(out):
         raise ValueError(f"rotate_positions: {name} must be {tuple(x.shape)} {x.dtype} with unit stride along its last "
                          "dimension and rows that do not overlap")
@@ -128,18 +130,18 @@ def rotate_positions(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
     n = q.shape[0]
     if positions.dim() == 1:
         positions = positions[None]
+    axes = positions.shape[0]
     if positions.dim() != 2 or positions.shape[1] != n or positions.dtype not in _INTEGERS:
         raise ValueError(f"rotate_positions: positions must be [A, {n}] or [{n}] integers, got {tuple(positions.shape)} "
                          f"{positions.dtype}")
     if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float32:
         raise ValueError("rotate_positions: inv_freq must be [R / 2] float32")
     sections = (inv_freq.shape[0],) if sections is None else tuple(map(int, sections))
-    if len(sections) != positions.shape[0]:
-        raise ValueError(f"rotate_positions: {len(sections)} sections for {positions.shape[0]} axes")
+    if len(sections) != axes:
+        raise ValueError(f"rotate_positions: {len(sections)} sections for {axes} axes")
     if positions.dtype is not torch.int64:
         positions = positions.long()
-    if not positions.is_contiguous() and ((positions.stride(1) != 1 and n > 1)
-                                          or (positions.stride(0) < n and positions.shape[0] > 1)):
+    if not positions.is_contiguous() and (positions.stride(1) != 1 and n > 1 or positions.stride(0) < n and axes > 1):
         positions = positions.contiguous()
     if not inv_freq.is_contiguous():
         inv_freq = inv_freq.contiguous()
