@@ -365,23 +365,34 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttArgs a) {
   __shared__ float fac[kMaxSplits];
   __shared__ __align__(16) float4 red[kSets][kCols];
   const int h = blockIdx.y;
-  RowTile t;
-  if (!row_tile(a, blockIdx.x, t) || t.per >= t.tiles || (int)blockIdx.z >= t.rows) return;
-  const int n = (int)((t.tiles + t.per - 1) / t.per);
-  const uint32_t rr = t.r0 + blockIdx.z, tok = token_of(a, rr);
-  const int64_t head = h * a.groups + (rr - tok * a.groups);
-  const int64_t row = (t.s.first + tok) * a.heads + head;
+  RowTile t = {};
+  int64_t tok, head;
+  if (a.b.starts == nullptr) {  // the row is known without the lists: its parts are on their way before the length is read
+    tok = a.tiles1 == 1 ? blockIdx.x : blockIdx.x / (uint32_t)a.tiles1;
+    const int64_t in = (blockIdx.x - tok * a.tiles1) * 32 + blockIdx.z;
+    if (in >= a.groups) return;
+    head = h * a.groups + in;
+  } else {
+    if (!row_tile(a, blockIdx.x, t) || t.per >= t.tiles || (int)blockIdx.z >= t.rows) return;
+    const uint32_t rr = t.r0 + blockIdx.z, in = token_of(a, rr);
+    tok = t.s.first + in;
+    head = h * a.groups + (rr - in * a.groups);
+  }
+  const int64_t row = tok * a.heads + head;
   const int col = threadIdx.x % kCols, set = threadIdx.x / kCols, lane = threadIdx.x & 63;
   const float *const p = a.part + row * a.splits * DV + col * 4;
-  float4 v[OWN];
+  float4 v[OWN];  // (parts that were not written are read, not used)
 #pragma unroll
   for (int i = 0; i < OWN; ++i) {
     const int s = set + i * kSets;
-    v[i] = *reinterpret_cast<const float4 *>(p + (int64_t)(s < n ? s : 0) * DV);
+    v[i] = *reinterpret_cast<const float4 *>(p + (int64_t)(s < a.splits ? s : 0) * DV);
   }
   const float2 *const st = a.stats + row * a.splits;
+  const float2 s0 = st[lane < a.splits ? lane : 0], s1 = st[lane + 64 < a.splits ? lane + 64 : 0];
+  if (a.b.starts == nullptr && (!row_tile(a, blockIdx.x, t) || t.per >= t.tiles)) return;
+  const int n = (int)((t.tiles + t.per - 1) / t.per);
   const float2 none = make_float2(-__builtin_huge_valf(), 0.f);
-  const float2 x0 = lane < n ? st[lane] : none, x1 = lane + 64 < n ? st[lane + 64] : none;
+  const float2 x0 = lane < n ? s0 : none, x1 = lane + 64 < n ? s1 : none;
   const float top = tm_wave_max(fmaxf(x0.x, x1.x));
   const float base = top == -__builtin_huge_valf() ? 0.f : top;
   const float f0 = __builtin_amdgcn_exp2f(x0.x - base), f1 = __builtin_amdgcn_exp2f(x1.x - base);
@@ -412,7 +423,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttArgs a) {
   }
   const float inv = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(-kRoom) / total;
   T o[4] = {Elem<DT>::from_f(y.x * inv), Elem<DT>::from_f(y.y * inv), Elem<DT>::from_f(y.z * inv), Elem<DT>::from_f(y.w * inv)};
-  __builtin_memcpy(static_cast<T *>(a.out) + (t.s.first + tok) * a.os_t + head * a.os_h + col * 4, o, 8);
+  __builtin_memcpy(static_cast<T *>(a.out) + tok * a.os_t + head * a.os_h + col * 4, o, 8);
   if (a.lse && threadIdx.x == 0) a.lse[row] = total == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
