@@ -8,8 +8,10 @@
 //   lane holding 16 keys of one row;  x = S^T sk scale log2(e) + log2(sv);
 //   P = 2^(x - m) under a reference m of the row, so that the values' scale
 //   rides in P and V enters as the bytes stand;  O^T += V^T P.
-// With l = sum P / sv the result is O / l and log sum exp = (m + log2 l) ln 2 (sv >=
-// 2^-100: l stays in range).
+// With l = sum P / sv the result is O / l and log sum exp = (m + log2 l) ln 2.  sv is
+// 2^-100 to 2^120 and l stays in range, but a factor of it may not: where P falls
+// under fp32's smallest number for sv's sake, or a reference moves that far, l is
+// taken apart from P or in two factors.
 // m is set 2^8 under the first tile's largest x and raised only where the
 // probabilities of a lane's 16 keys sum to more than 2^15: no maximum is taken of
 // the other tiles, and O is seldom scaled again.  P is rounded to fp16 for the
@@ -40,9 +42,10 @@ typedef _Float16 tm_f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kMaxSplits = 128;
-constexpr float kRoom = 8.f;  // log2 of the first maximum's P
+constexpr int kRoom = 8;  // log2 of the first maximum's P
 // What the probabilities of 16 keys may sum to before the reference is raised (each is rounded to fp16: at most 65504).
 constexpr float kMost = 32768.f;
+constexpr int kFar = 80;  // of 126: what is left to P is 2^-46 of its row's largest
 
 struct AttArgs {
   tm_kv8_cache c;
@@ -57,6 +60,12 @@ struct AttArgs {
   float scale;
   int32_t heads, groups, splits, page_log2, causal, tiles1;  // tiles1: row tiles of one token
 };
+
+// l 2^x, where 2^x alone may be too small for fp32.
+__device__ __forceinline__ float scaled(float l, float x) {
+  const float root = __builtin_amdgcn_exp2f(0.5f * x);
+  return l * root * root;
+}
 
 // A row tile: rows [r0, r0 + rows) of sequence b (tokens times heads of a key head: under 2^31).
 struct RowTile {
@@ -170,6 +179,7 @@ __global__ __launch_bounds__(kThreads, R == 2 || D + DV > 320 ? 2 : 3) void atte
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[r][j][i] = 0.f;
   }
+  int most = -127;  // log2 of the largest value scale so far
   bool first = true;      // some row has no reference yet, or may have none
   bool seen_nan = false;  // among values that some row does not see
 #pragma unroll 1
@@ -192,7 +202,8 @@ __global__ __launch_bounds__(kThreads, R == 2 || D + DV > 320 ? 2 : 3) void atte
     const Kv8Place wn = place(tile + kWaves, id);
     id = page_of(tile + 2 * kWaves);
     tm_kv8_load<NK>(a.c.k, wn, a.page_log2, lane, kf);
-    const float mul = (w.there ? sk : 1.f) * unit, add = w.there ? tm_exponent(sv) : 0.f;
+    const int power = w.there ? tm_exponent(sv) : 0;
+    const float mul = (w.there ? sk : 1.f) * unit, add = (float)power;
     sk = a.c.k_scale[wn.slot];
     if constexpr (NV > 0) sv = a.c.v_scale[wn.slot];
     if (!w.there || tile >= seen_whole) {
@@ -219,7 +230,8 @@ __global__ __launch_bounds__(kThreads, R == 2 || D + DV > 320 ? 2 : 3) void atte
       }
     }
     w = wn;
-    const float back = __builtin_amdgcn_exp2f(-add - kRoom);
+    const bool low = power < most - kFar;  // P may vanish where P / sv counts
+    most = power > most ? power : most;
     bool none = false;
     uint4 p[R][2];
 #pragma unroll
@@ -231,9 +243,9 @@ __global__ __launch_bounds__(kThreads, R == 2 || D + DV > 320 ? 2 : 3) void atte
         top = fmaf(top, mul, add);
         top = fmaxf(top, tm_other_half(top));
         const float to = fmaxf(m[r], top - kRoom);
-        const float f = m[r] == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(m[r] - to);
+        const float root = m[r] == -__builtin_huge_valf() ? 0.f : __builtin_amdgcn_exp2f(0.5f * (m[r] - to)), f = root * root;
         m[r] = to;
-        l[r] *= f;
+        l[r] = l[r] * root * root;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -262,7 +274,17 @@ __global__ __launch_bounds__(kThreads, R == 2 || D + DV > 320 ? 2 : 3) void atte
         settle();
         probabilities();
       }
-      l[r] = fmaf(sum, back, l[r]);
+      if (low) {
+        float top = s[r][0], apart = 0.f;
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[r][i]);
+        top = top == -__builtin_huge_valf() ? 0.f : top * mul;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) apart += __builtin_amdgcn_exp2f(fmaf(s[r][i], mul, -top));
+        l[r] += scaled(apart, top - (m[r] == -__builtin_huge_valf() ? 0.f : m[r]) - kRoom);
+      } else {
+        l[r] += __builtin_ldexpf(sum, -kRoom - power);
+      }
     }
     if (first) first = __any(none);
 #pragma unroll
@@ -289,11 +311,11 @@ __global__ __launch_bounds__(kThreads, R == 2 || D + DV > 320 ? 2 : 3) void atte
     for (int x = 0; x < kWaves; ++x) top = fmaxf(top, join[x][c].x);
     const float base = top == -__builtin_huge_valf() ? 0.f : top;
 #pragma unroll
-    for (int x = 0; x < kWaves; ++x) total += join[x][c].y * __builtin_amdgcn_exp2f(join[x][c].x - base);
+    for (int x = 0; x < kWaves; ++x) total += scaled(join[x][c].y, join[x][c].x - base);
     const float f = __builtin_amdgcn_exp2f(mw - base);
     const int rows = t.rows - 32 * r < 32 ? t.rows - 32 * r : 32;
     if (wave == 0 && g == 0) {
-      if (NV > 0) inv_s[c] = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(-kRoom) / total;
+      if (NV > 0) inv_s[c] = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(-(float)kRoom) / total;
       if (c < rows) {
         const uint32_t row = t.r0 + 32 * r + c, token = token_of(a, row);
         const int64_t at = (t.s.first + token) * a.heads + head_of(row, token);
@@ -396,7 +418,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttArgs a) {
   const float top = tm_wave_max(fmaxf(x0.x, x1.x));
   const float base = top == -__builtin_huge_valf() ? 0.f : top;
   const float f0 = __builtin_amdgcn_exp2f(x0.x - base), f1 = __builtin_amdgcn_exp2f(x1.x - base);
-  const float total = tm_wave_sum(x0.y * f0 + x1.y * f1);
+  const float total = tm_wave_sum(scaled(x0.y, x0.x - base) + scaled(x1.y, x1.x - base));
   if (threadIdx.x < 64) {
     fac[lane] = f0;
     fac[lane + 64] = f1;
@@ -421,7 +443,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttArgs a) {
     const float4 x = red[s][col];
     y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
   }
-  const float inv = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(-kRoom) / total;
+  const float inv = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(-(float)kRoom) / total;
   T o[4] = {Elem<DT>::from_f(y.x * inv), Elem<DT>::from_f(y.y * inv), Elem<DT>::from_f(y.z * inv), Elem<DT>::from_f(y.w * inv)};
   __builtin_memcpy(static_cast<T *>(a.out) + tok * a.os_t + head * a.os_h + col * 4, o, 8);
   if (a.lse && threadIdx.x == 0) a.lse[row] = total == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(total)) * kLn2;

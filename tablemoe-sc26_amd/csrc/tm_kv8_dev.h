@@ -40,4 +40,4 @@ __device__ __forceinline__ void tm_kv8_load(const void *base, const Kv8Place &w,
 }
 
 // Exponent of a power of two.
-__device__ __forceinline__ float tm_exponent(float s) { return (float)((int)(__float_as_uint(s) >> 23 & 0xff) - 127); }
+__device__ __forceinline__ int tm_exponent(float s) { return (int)(__float_as_uint(s) >> 23 & 0xff) - 127; }

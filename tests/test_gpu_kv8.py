@@ -510,6 +510,33 @@ def test_attend_scales_far_apart_and_large_scores(hip_device):
     check_attend(cache, plain, q, table, lengths, starts, y, lse, d ** -0.5, True, set(range(0, 250, 11)) | {249})
 
 
+@pytest.mark.parametrize("order,one_token", [("big first", False), ("big last", False), ("by turns", False), ("big first", True),
+                                             ("big last", True), ("all big", True)])
+def test_attend_value_scales_of_any_ratio(hip_device, order, one_token):
+    """Value scales from 2^-100 to 2^120 among keys of like probability: each counts in the sum. One token of 2048 keys
+    has its keys split over workgroups; pages of 32 go to the four waves in turn."""
+    g = torch.Generator().manual_seed(31)
+    dev, page, d, kv, pages = hip_device, 32, 64, 1, 64 if one_token else 16
+    cache, plain = filled(g, pages, kv, page, d, d, dev)
+    big = {"big first": lambda p: p < pages // 2, "big last": lambda p: p >= pages // 2, "by turns": lambda p: p % 2 == 0,
+           "all big": lambda p: True}[order]
+    for p in range(pages):
+        plain[3][p] = 2.0 ** (120 if big(p) else -100)
+    plain[2] *= 1 / 4.0  # (means of them stay under bf16's largest)
+    cache.v.view(torch.uint8).copy_(R.pack(R.e4m3(plain[2]), True).view(torch.uint8))
+    plain[2] = R.raw(cache.v, True)
+    cache.v_scale.copy_(plain[3].float())
+    table, n = torch.arange(pages, dtype=torch.int32)[None], pages * page
+    t = 1 if one_token else n
+    q = (0.5 * torch.randn(t, 4, d, generator=g)).to(BF16)
+    lengths, starts = torch.tensor([n], dtype=torch.int32), None if one_token else torch.tensor([0, n], dtype=torch.int32)
+    y, lse = cache.attend(q.to(dev), table.to(dev), lengths.to(dev), None if one_token else starts.to(dev), return_lse=True)
+    # (in units of 2^120, where the tolerance's own arithmetic holds them)
+    plain[3] = plain[3] * 2.0 ** -120
+    check_attend(cache, plain, q, table, lengths, starts, y.double() * 2.0 ** -120, lse, d ** -0.5, True,
+                 None if one_token else set(range(0, n, 37)) | {n - 1})
+
+
 # ----------------------------------------------------------------- importance
 def check_importance(plain, q, table, lengths, scale, got):
     k = plain[0] * plain[1][:, :, None, None]
