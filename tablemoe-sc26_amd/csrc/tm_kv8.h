@@ -19,6 +19,7 @@
 #include "tm_mfma.h"
 
 constexpr int kKv8Tile = 32;
+constexpr int64_t kKv8MaxGrid = (int64_t)1 << 24;  // workgroups of 256: a launch holds under 2^32 threads in a direction
 constexpr float kKv8MinScale = 0x1p-100f;
 
 // A batch's sequence: its new tokens are [first, first + n) of the caller's rows,

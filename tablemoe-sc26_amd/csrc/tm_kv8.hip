@@ -205,7 +205,7 @@ extern "C" int tm_kv8_append(const tm_kv8_cache *cache, const tm_kv8_batch *batc
   AppArgs a = {*cache, *batch, {k, v}, {ks_t, vs_t}, {ks_h, vs_h}};
   // a sequence of n new tokens touches at most (n - 2) / page + 2 pages
   const int64_t units = batch->starts ? batch->n_tokens / cache->page_size + 2 * batch->n_seqs : batch->n_seqs;
-  TM_REQUIRE(units < ((int64_t)1 << 31), TM_EINVAL_SHAPE, "tm_kv8_append: too many pages");
+  TM_REQUIRE(units < kKv8MaxGrid, TM_EINVAL_SHAPE, "tm_kv8_append: too many pages");
   const dim3 grid((unsigned)units, (unsigned)cache->n_kv_heads, 2);
   hipStream_t s = tm_hip_stream(stream);
   return TM_DISPATCH_DTYPE(dtype, DT, [&] {

@@ -547,10 +547,9 @@ extern "C" int tm_kv8_attention(const tm_kv8_cache *cache, const tm_kv8_batch *b
   TM_REQUIRE(tm_aligned16(q) && tm_aligned16(out) && qs_t % 8 == 0 && qs_h % 8 == 0 && os_t % 8 == 0 && os_h % 8 == 0,
              TM_EINVAL_SHAPE, "tm_kv8_attention: rows of q and out must be 16-byte aligned, strides multiples of 8 elements");
   const int groups = n_heads / cache->n_kv_heads;
-  TM_REQUIRE((batch->n_tokens * groups + 64 * batch->n_seqs) / 32 * cache->n_kv_heads < ((int64_t)1 << 31) &&
-                 batch->n_tokens * groups < ((int64_t)1 << 31),
-             TM_EINVAL_SHAPE, "tm_kv8_attention: too many rows");
   const Plan p = plan_of(cache, batch, groups);
+  TM_REQUIRE(p.tiles * cache->n_kv_heads < kKv8MaxGrid && batch->n_tokens * groups < ((int64_t)1 << 31), TM_EINVAL_SHAPE,
+             "tm_kv8_attention: too many rows");
   const size_t need = tm_kv8_attention_workspace_size(cache, batch, n_heads);
   TM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && tm_aligned16(workspace)), TM_EWORKSPACE,
              "tm_kv8_attention: workspace %zu bytes < %zu", workspace_bytes, need);

@@ -22,6 +22,7 @@ namespace {
 constexpr int kRotThreads = 256;
 constexpr int kRotPairs = 1024;  // sines and cosines that a workgroup holds
 constexpr int kRotMaxAxes = 4;
+constexpr int64_t kMaxGrid = (int64_t)1 << 24;  // workgroups: a launch holds under 2^32 threads in a direction
 
 struct RotArgs {
   const void *in[2];
@@ -189,6 +190,7 @@ extern "C" int tm_rotate_positions(int32_t dtype, const void *q, int64_t n_token
            a.out_t[w] % 8 == 0 && a.out_h[w] % 8 == 0;
   a.tokens = 4;
   while (a.tokens > 1 && a.tokens * a.half > kRotPairs) --a.tokens;
+  TM_REQUIRE(tm_cdiv(n_tokens, a.tokens) < kMaxGrid, TM_EINVAL_SHAPE, "tm_rotate_positions: too many tokens");
   const dim3 grid((unsigned)tm_cdiv(n_tokens, a.tokens));
   hipStream_t s = tm_hip_stream(stream);
   return TM_DISPATCH_DTYPE(dtype, DT, [&] {

@@ -12,7 +12,7 @@ import ctypes as C
 import torch
 
 from .. import _native as N
-from .rotary import _strides, rows_apart
+from .rotary import _strides, overlap, rows_apart, written
 
 TILE = 32
 _TAG16 = {torch.float16: N.TM_DT_F16, torch.bfloat16: N.TM_DT_BF16}
@@ -193,6 +193,9 @@ class Fp8KVCache:
                     or os_t % 8 or os_h % 8:
                 raise ValueError(f"Fp8KVCache.attend: out must be {(n, h, self.v_dim)} {q.dtype} with 16-byte aligned "
                                  "rows that do not overlap")
+            if overlap(out, q):
+                raise ValueError("Fp8KVCache.attend: out must not overlap q")
+            written(out)
         lse = torch.empty((n, h), dtype=torch.float32, device=dev) if return_lse else None
         ref = C.byref(batch)
         nbytes = N.lib().tm_kv8_attention_workspace_size(self._ref, ref, h)

@@ -42,16 +42,40 @@ def _span(t: torch.Tensor):
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
-def _check_out(name: str, out: torch.Tensor, x: torch.Tensor) -> None:
-    if out is x and x.is_contiguous():
-        return
-    if out.shape != x.shape or out.dtype != x.dtype or not rows_apart(out):
-        raise ValueError(f"rotate_positions: {name} must be {tuple(x.shape)} {x.dtype} with unit stride along its last "
-                         "dimension and rows that do not overlap")
-    if out.numel() and not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
-        (a, b), (c, d) = _span(out), _span(x)
-        if a < d and c < b:
+def written(*tensors) -> None:
+    """Tells autograd, for a graph that has saved one of them (an error in its backward, as after any write in place)."""
+    for t in tensors:
+        if t is None or t.is_inference():
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("out has no gradient")
+        torch.autograd.graph.increment_version(t)
+
+
+def overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether the [T, H, D] views may share memory; views of one fused projection's rows that take different columns do
+    not."""
+    if x.numel() == 0 or y.numel() == 0:
+        return False
+    (a, b), (c, d) = _span(x), _span(y)
+    if a >= d or c >= b:
+        return False
+    step = x.stride(0) * x.element_size()
+    if x.shape[0] == 1 or y.shape[0] == 1 or step != y.stride(0) * y.element_size() or step == 0:
+        return True
+    (a, b), (c, d) = _span(x[0]), _span(y[0])  # what a token takes of its row, modulo the rows' distance
+    return (c - a) % step < b - a or (a - c) % step < d - c
+
+
+def _check_out(name: str, out: torch.Tensor, x: torch.Tensor, others) -> None:
+    if not (out is x and x.is_contiguous()):
+        if out.shape != x.shape or out.dtype != x.dtype or not rows_apart(out):
+            raise ValueError(f"rotate_positions: {name} must be {tuple(x.shape)} {x.dtype} with unit stride along its last "
+                             "dimension and rows that do not overlap")
+        if not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()) and overlap(out, x):
             raise ValueError(f"rotate_positions: {name} may be the input itself, not overlap it otherwise")
+    if any(overlap(out, t) for t in others):
+        raise ValueError(f"rotate_positions: {name} overlaps the other input or output")
 
 
 def _strides(t: torch.Tensor):
@@ -134,8 +158,8 @@ def rotate_positions(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
     if positions.dim() != 2 or positions.shape[1] != n or positions.dtype not in _INTEGERS:
         raise ValueError(f"rotate_positions: positions must be [A, {n}] or [{n}] integers, got {tuple(positions.shape)} "
                          f"{positions.dtype}")
-    if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float32:
-        raise ValueError("rotate_positions: inv_freq must be [R / 2] float32")
+    if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float32 or inv_freq.requires_grad and torch.is_grad_enabled():
+        raise ValueError("rotate_positions: inv_freq must be [R / 2] float32 and has no gradient")
     sections = (inv_freq.shape[0],) if sections is None else tuple(map(int, sections))
     if len(sections) != axes:
         raise ValueError(f"rotate_positions: {len(sections)} sections for {axes} axes")
@@ -158,8 +182,9 @@ def rotate_positions(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
         if (k is None) != (k_out is None):
             raise ValueError("rotate_positions: out holds a tensor for each of q and k")
         N.require_hip(q, q_out, k_out)
-        _check_out("out[0]", q_out, q)
+        _check_out("out[0]", q_out, q, () if k is None else (k, k_out))
         if k is not None:
-            _check_out("out[1]", k_out, k)
+            _check_out("out[1]", k_out, k, (q,))
+        written(q_out, k_out)
     _run(q, k, positions, inv_freq, *how, q_out, k_out, dev)
     return q_out, k_out

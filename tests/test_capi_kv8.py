@@ -113,3 +113,22 @@ def test_importance_refusals(lib):
                      (dict(out=None), N.TM_EINVAL_ARG), (dict(q=ODD), N.TM_EINVAL_SHAPE), (dict(qt=4), N.TM_EINVAL_SHAPE),
                      (dict(ws=None), N.TM_EWORKSPACE), (dict(nb=need - 1), N.TM_EWORKSPACE), (dict(ws=ODD), N.TM_EWORKSPACE)):
         assert f(**kw) == want, kw
+
+
+def test_more_workgroups_than_a_launch_holds(lib):
+    """2^24 workgroups of 256 threads are 2^32 threads: refused, not left to the runtime."""
+    sections = (C.c_int32 * 1)(64)
+
+    def rotate(n):
+        return lib.tm_rotate_positions(N.TM_DT_BF16, P, n, 1, 128, 128, None, 0, 0, 0, 128, 128, P, n, 1, sections, 0, 0, 0,
+                                       P, P, 128, 128, None, 0, 0, None)
+
+    assert rotate(1 << 26) == N.TM_EINVAL_SHAPE and rotate((1 << 26) - 3) == N.TM_EINVAL_SHAPE
+    assert rotate((1 << 31) - 1) == N.TM_EINVAL_SHAPE and rotate(1 << 31) == N.TM_EINVAL_SHAPE
+    c = _cache(page=32)
+    many = _batch(seqs=1 << 23, tokens=1 << 23, starts=1 << 12)
+    assert lib.tm_kv8_append(C.byref(c), C.byref(many), N.TM_DT_BF16, P, 256, 128, P, 256, 128, None) == N.TM_EINVAL_SHAPE
+    for seqs, tokens, starts in ((1 << 23, 1 << 23, None), (3, (1 << 28) - 8, 1 << 12), (3, 1 << 29, 1 << 12)):
+        b = _batch(seqs=seqs, tokens=tokens, starts=starts)
+        assert lib.tm_kv8_attention(C.byref(c), C.byref(b), N.TM_DT_BF16, P, 512, 128, 4, 0.1, 1, P, 512, 128, None, P,
+                                    1 << 40, None) == N.TM_EINVAL_SHAPE, seqs

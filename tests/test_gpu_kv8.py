@@ -164,6 +164,57 @@ def test_rotate_refusals(hip_device):
         rotate_positions(q.cpu(), None, pos, inv, (10, 11, 11))
 
 
+def test_rotate_outputs_that_overlap(hip_device):
+    """Outputs may be their inputs, or other columns of the same rows; not each other's, nor the other's input."""
+    from table_moe.ops import rotate_positions
+
+    dev = hip_device
+    g = torch.Generator().manual_seed(12)
+    n, d = 9, 64
+    fused = torch.randn(n, 8 * d, generator=g).to(dev)
+    part = lambda a, b: fused[:, a * d:b * d].view(n, b - a, d)  # noqa: E731
+    pos, inv = torch.arange(n, device=dev), torch.rand(d // 2, generator=g).to(dev)
+    q, k = part(0, 2), part(2, 4)
+    want = rotate_positions(q, k, pos, inv)
+    got = rotate_positions(q, k, pos, inv, out=(part(4, 6), part(6, 8)))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(got[0], part(4, 6))
+    one = torch.zeros(n, 2, d, device=dev)
+    for out in ((k, q), (one, one), (part(2, 4), part(6, 8)), (part(4, 6), part(5, 7)), (part(1, 3), part(6, 8)),
+                (one, fused.view(-1)[d:d + n * 2 * d].view(n, 2, d))):
+        with pytest.raises(ValueError, match="overlap"):
+            rotate_positions(q, k, pos, inv, out=out)
+    with pytest.raises(ValueError, match="overlap"):  # one tensor as both inputs, turned twice in place
+        rotate_positions(one, one, pos, inv, out=(one, one))
+    rotate_positions(one, one, pos, inv)
+
+
+def test_outputs_that_a_graph_has_saved(hip_device):
+    """A write to a tensor that a backward needs is an error there, as after torch's own writes in place."""
+    from table_moe.ops import Fp8KVCache, rotate_positions
+
+    dev = hip_device
+    q = torch.randn(3, 2, 64, device=dev)
+    w = torch.ones(3, 2, 64, device=dev, requires_grad=True)
+    pos, inv = torch.arange(3, device=dev), torch.ones(32, device=dev)
+    y = (q * w).sum()
+    rotate_positions(q, None, pos, inv, out=(q, None))
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+    cache = Fp8KVCache(1, 1, 64, device=dev)
+    table, one = torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    out = torch.ones(1, 1, 64, dtype=F16, device=dev)
+    v = torch.ones(1, 1, 64, dtype=F16, device=dev, requires_grad=True)
+    y = (out * v).sum()
+    cache.attend(torch.ones(1, 1, 64, dtype=F16, device=dev), table, one, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+    with torch.inference_mode():
+        r = torch.ones(3, 2, 64, device=dev)
+        rotate_positions(r, None, pos, inv, out=(r, None))
+    with pytest.raises(ValueError, match="gradient"):
+        rotate_positions(w, None, pos, inv.clone().requires_grad_())
+
+
 # --------------------------------------------------------------------- append
 def filled(g, pages, kv, page, d, dv, dev):
     """A cache in use: (Fp8KVCache, plain cells and scales of K and V)."""
@@ -693,6 +744,8 @@ def test_cache_refusals(hip_device):
             if name != "starts":
                 with pytest.raises(ValueError):
                     c.importance(q, **{k: v for k, v in kw.items() if k != "starts"})
+    with pytest.raises(ValueError, match="overlap"):
+        c.attend(q, t, n, out=q)
     for k, v in ((kv[:, :1], kv), (kv, kv.half()), (kv.double(), kv.double()), (kv[..., :64], kv), (kv[:2], kv)):
         with pytest.raises(ValueError):
             c.append(k, v, t, n)
