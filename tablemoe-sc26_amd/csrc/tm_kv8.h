@@ -76,16 +76,21 @@ __device__ __forceinline__ uint4 tm_kv8_operand(uint32_t lo, uint32_t hi) {
 // What the entry points refuse about a cache and a batch (host).
 int tm_kv8_check(const char *what, const tm_kv8_cache *c, const tm_kv8_batch *b) __attribute__((visibility("hidden")));
 
-// Splits of the keys of a call with one query per sequence (`groups` heads to a key head), and the softmax
+// How a call's keys are cut up for workgroups: at most `splits` parts, of at least `least` tiles of 32.
+struct Kv8Cut {
+  int splits, least;
+};
+// Cut of the keys of a call with one query per sequence (`groups` heads to a key head), and the softmax
 // statistics of its rows: stats[row][split] = (reference in units of log2, sum), the
 // first ceil(tiles / per) of them written, with tiles of 32 keys and per as
 // tm_kv8_per gives it.  Arguments as checked by tm_kv8_importance.
-__attribute__((visibility("hidden"))) int tm_internal_kv8_splits(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups);
+__attribute__((visibility("hidden"))) Kv8Cut tm_internal_kv8_cut(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups);
 __attribute__((visibility("hidden"))) int tm_internal_kv8_stats(const tm_kv8_cache *cache, const tm_kv8_batch *batch,
                                                                 int32_t dtype, const void *q, int64_t qs_b, int64_t qs_h,
                                                                 int32_t n_heads, float scale, float2 *stats,
                                                                 hipStream_t s);
-// Tiles of a split: whole rounds of a workgroup's four waves.
-__device__ __forceinline__ int64_t tm_kv8_per(int64_t tiles, int splits) {
-  return ((tiles + splits - 1) / splits + 3) / 4 * 4;
+// Tiles of a part: whole rounds of a workgroup's four waves.
+__device__ __forceinline__ int64_t tm_kv8_per(int64_t tiles, Kv8Cut cut) {
+  const int64_t n = ((tiles + cut.splits - 1) / cut.splits + 3) / 4 * 4;
+  return n > cut.least ? n : cut.least;
 }

@@ -58,7 +58,8 @@ struct AttArgs {
   float2 *stats;  // [row of the call][split]: reference, sum
   float *part;    // [row of the call][split][v_dim]
   float scale;
-  int32_t heads, groups, splits, page_log2, causal, tiles1;  // tiles1: row tiles of one token
+  Kv8Cut cut;
+  int32_t heads, groups, page_log2, causal, tiles1;  // tiles1: row tiles of one token
 };
 
 // l 2^x, where 2^x alone may be too small for fp32.
@@ -101,7 +102,7 @@ __device__ __forceinline__ bool row_tile(const AttArgs &a, int64_t u, RowTile &t
   if (a.b.starts != nullptr) last = (t.r0 + t.rows - 1) / (uint32_t)a.groups;
   t.end = visible(a, t.s, last);
   t.tiles = (t.end + 31) >> 5;
-  t.per = a.splits == 1 ? t.tiles + 3 : tm_kv8_per(t.tiles, a.splits);
+  t.per = a.cut.splits == 1 ? t.tiles + 3 : tm_kv8_per(t.tiles, a.cut);
   return true;
 }
 // A row's token (of its sequence) and its head among the key head's.
@@ -319,7 +320,7 @@ __global__ __launch_bounds__(kThreads, R == 2 || D + DV > 320 ? 2 : 3) void atte
       if (c < rows) {
         const uint32_t row = t.r0 + 32 * r + c, token = token_of(a, row);
         const int64_t at = (t.s.first + token) * a.heads + head_of(row, token);
-        if (NV == 0 || !whole) a.stats[at * a.splits + split] = make_float2(top, total);
+        if (NV == 0 || !whole) a.stats[at * a.cut.splits + split] = make_float2(top, total);
         else if (a.lse) a.lse[at] = total == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(total)) * kLn2;
       }
     }
@@ -369,7 +370,7 @@ __global__ __launch_bounds__(kThreads, R == 2 || D + DV > 320 ? 2 : 3) void atte
             tm_store8<DT>(static_cast<T *>(a.out) + (t.s.first + token) * a.os_t + head_of(row, token) * a.os_h +
                               part * kChunk + col, v);
           } else {
-            tm_store8<TM_DT_F32>(a.part + (((t.s.first + token) * a.heads + head_of(row, token)) * a.splits + split) * DV +
+            tm_store8<TM_DT_F32>(a.part + (((t.s.first + token) * a.heads + head_of(row, token)) * a.cut.splits + split) * DV +
                                      part * kChunk + col, v);
           }
         }
@@ -389,7 +390,10 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttArgs a) {
   const int h = blockIdx.y;
   RowTile t = {};
   int64_t tok, head;
-  if (a.b.starts == nullptr) {  // the row is known without the lists: its parts are on their way before the length is read
+  // with one token each the row is known without the lists; where most rows have parts these are on their way before
+  // the length is read
+  const bool early = a.b.starts == nullptr && a.cut.least == 4;
+  if (early) {
     tok = a.tiles1 == 1 ? blockIdx.x : blockIdx.x / (uint32_t)a.tiles1;
     const int64_t in = (blockIdx.x - tok * a.tiles1) * 32 + blockIdx.z;
     if (in >= a.groups) return;
@@ -402,16 +406,16 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttArgs a) {
   }
   const int64_t row = tok * a.heads + head;
   const int col = threadIdx.x % kCols, set = threadIdx.x / kCols, lane = threadIdx.x & 63;
-  const float *const p = a.part + row * a.splits * DV + col * 4;
+  const float *const p = a.part + row * a.cut.splits * DV + col * 4;
   float4 v[OWN];  // (parts that were not written are read, not used)
 #pragma unroll
   for (int i = 0; i < OWN; ++i) {
     const int s = set + i * kSets;
-    v[i] = *reinterpret_cast<const float4 *>(p + (int64_t)(s < a.splits ? s : 0) * DV);
+    v[i] = *reinterpret_cast<const float4 *>(p + (int64_t)(s < a.cut.splits ? s : 0) * DV);
   }
-  const float2 *const st = a.stats + row * a.splits;
-  const float2 s0 = st[lane < a.splits ? lane : 0], s1 = st[lane + 64 < a.splits ? lane + 64 : 0];
-  if (a.b.starts == nullptr && (!row_tile(a, blockIdx.x, t) || t.per >= t.tiles)) return;
+  const float2 *const st = a.stats + row * a.cut.splits;
+  const float2 s0 = st[lane < a.cut.splits ? lane : 0], s1 = st[lane + 64 < a.cut.splits ? lane + 64 : 0];
+  if (early && (!row_tile(a, blockIdx.x, t) || t.per >= t.tiles)) return;
   const int n = (int)((t.tiles + t.per - 1) / t.per);
   const float2 none = make_float2(-__builtin_huge_valf(), 0.f);
   const float2 x0 = lane < n ? s0 : none, x1 = lane + 64 < n ? s1 : none;
@@ -451,12 +455,13 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttArgs a) {
 
 // How a call is cut up: R x 32 rows a workgroup, at most `tiles` of these per key head, keys split `splits` times.
 struct Plan {
-  int r, splits;
+  int r;
+  Kv8Cut cut;
   int64_t tiles;
 };
 Plan plan_of(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups) {
   const int64_t rows = b->n_tokens * groups, heads = c->n_kv_heads;
-  Plan p = {1, 1, b->starts ? rows / 32 + b->n_seqs : b->n_seqs * tm_cdiv(groups, 32)};
+  Plan p = {1, {1, 4}, b->starts ? rows / 32 + b->n_seqs : b->n_seqs * tm_cdiv(groups, 32)};
   // 64 rows a wave where that leaves four workgroups for each that a CU holds (32 heads on 4, us with 32 and 64 rows:
   // 2048 tokens 53, 58; 4099 173, 167; 8192 599, 554); wider values leave no registers for them
   if (b->starts && c->v_dim <= 128 && rows / 64 * heads >= 2048) {
@@ -471,7 +476,15 @@ Plan plan_of(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups) {
   if (units <= 0 || keys <= 32) return p;
   int64_t s = (keys <= 128 ? 256 : 512) / units;
   s = s < keys / kWaves ? s : keys / kWaves;
-  p.splits = (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+  // Sequences of one table may differ much: a part has about 4096 keys of the longest, from two workgroups per CU on
+  // 8192, and a short sequence no more parts than above (32 heads on 4, us before and now: one of 65536 among 31 of 1000
+  // keys 153, 60, among 127 434, 104; but 128 of 500 in a table of 65536 16.7, 21.7, of 2000 46, 51).
+  const int64_t most = keys / (units >= 512 ? 256 : 128);
+  if (!b->starts && most > s) {
+    p.cut.least = (int)(units >= 512 ? 64 : (units + 31) / 32 * 4);
+    s = most;
+  }
+  p.cut.splits = (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
   return p;
 }
 
@@ -484,7 +497,7 @@ AttArgs args_of(const tm_kv8_cache *c, const tm_kv8_batch *b, const void *q, int
   a.scale = scale;
   a.heads = n_heads;
   a.groups = n_heads / c->n_kv_heads;
-  a.splits = p.splits;
+  a.cut = p.cut;
   a.page_log2 = c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
   a.tiles1 = (int)tm_cdiv(a.groups, 32);
   return a;
@@ -492,14 +505,14 @@ AttArgs args_of(const tm_kv8_cache *c, const tm_kv8_batch *b, const void *q, int
 
 template <int DT, int D, int DV, int R>
 void launch(const AttArgs &a, const Plan &p, hipStream_t s) {
-  const dim3 grid((unsigned)(p.tiles * a.c.n_kv_heads), (unsigned)p.splits);
+  const dim3 grid((unsigned)(p.tiles * a.c.n_kv_heads), (unsigned)p.cut.splits);
   hipLaunchKernelGGL((attend_kernel<DT, D, DV, R>), grid, dim3(kThreads), 0, s, a);
 }
 
 }  // namespace
 
-int tm_internal_kv8_splits(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups) {
-  return plan_of(c, b, groups).splits;
+Kv8Cut tm_internal_kv8_cut(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups) {
+  return plan_of(c, b, groups).cut;
 }
 int tm_internal_kv8_stats(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *q, int64_t qs_b,
                           int64_t qs_h, int32_t n_heads, float scale, float2 *stats, hipStream_t s) {
@@ -524,7 +537,7 @@ int tm_internal_kv8_stats(const tm_kv8_cache *cache, const tm_kv8_batch *batch, 
 extern "C" size_t tm_kv8_attention_workspace_size(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t n_heads) {
   if (!cache || !batch || n_heads < 1 || cache->n_kv_heads < 1 || n_heads % cache->n_kv_heads || batch->n_tokens <= 0)
     return 0;
-  const int s = plan_of(cache, batch, n_heads / cache->n_kv_heads).splits;
+  const int s = plan_of(cache, batch, n_heads / cache->n_kv_heads).cut.splits;
   if (s == 1) return 0;
   return (size_t)batch->n_tokens * n_heads * s * (cache->v_dim + 2) * sizeof(float) + 16;
 }
@@ -559,7 +572,7 @@ extern "C" int tm_kv8_attention(const tm_kv8_cache *cache, const tm_kv8_batch *b
   a.lse = lse;
   a.causal = causal != 0;
   a.part = static_cast<float *>(workspace);
-  a.stats = reinterpret_cast<float2 *>(a.part + batch->n_tokens * n_heads * p.splits * cache->v_dim);
+  a.stats = reinterpret_cast<float2 *>(a.part + batch->n_tokens * n_heads * p.cut.splits * cache->v_dim);
   hipStream_t s = tm_hip_stream(stream);
   auto run = [&](auto dt, auto d, auto dv) {
     constexpr int DT = decltype(dt)::value, D = decltype(d)::value, DV = decltype(dv)::value;
@@ -570,11 +583,11 @@ extern "C" int tm_kv8_attention(const tm_kv8_cache *cache, const tm_kv8_batch *b
       launch<DT, D, DV, 1>(a, p, s);
     }
     TM_LAUNCH_CHECK("tm_kv8_attention");
-    if (p.splits > 1) {
+    if (p.cut.splits > 1) {
       // (rows of a tile: one token's heads, or 32 of several tokens)
       const dim3 grid((unsigned)p.tiles, (unsigned)cache->n_kv_heads, (unsigned)(!batch->starts && groups < 32 ? groups : 32));
       constexpr int kSets = kThreads / (DV / 4);
-      if (p.splits <= 4 * kSets) hipLaunchKernelGGL((join_kernel<DT, DV, 4>), grid, dim3(kThreads), 0, s, a);
+      if (p.cut.splits <= 4 * kSets) hipLaunchKernelGGL((join_kernel<DT, DV, 4>), grid, dim3(kThreads), 0, s, a);
       else hipLaunchKernelGGL((join_kernel<DT, DV, (kMaxSplits + kSets - 1) / kSets>), grid, dim3(kThreads), 0, s, a);
       TM_LAUNCH_CHECK("tm_kv8_attention(join)");
     }

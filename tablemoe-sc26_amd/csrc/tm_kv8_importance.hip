@@ -34,7 +34,8 @@ struct ImpArgs {
   float *out;
   int64_t ld_out, out_len;
   float scale;
-  int32_t heads, groups, splits, page_log2, per, head_waves, lanes_log2;
+  Kv8Cut cut;
+  int32_t heads, groups, page_log2, per, head_waves, lanes_log2;
 };
 
 template <int DT, int D>
@@ -57,10 +58,10 @@ __global__ __launch_bounds__(kThreads) void importance_kernel(ImpArgs a) {
       if (tid < a.heads) norm[tid] = a.lse[b * a.ld_lse + tid] * kLog2e;
     } else {
       const int lanes = 1 << a.lanes_log2, at = tid & (lanes - 1);
-      const int used = (int)((tiles + tm_kv8_per(tiles, a.splits) - 1) / tm_kv8_per(tiles, a.splits));
+      const int used = (int)((tiles + tm_kv8_per(tiles, a.cut) - 1) / tm_kv8_per(tiles, a.cut));
       for (int h0 = 0; h0 < a.heads; h0 += kThreads >> a.lanes_log2) {
         const int h = h0 + (tid >> a.lanes_log2);
-        const float2 *const st = a.stats + (b * a.heads + (h < a.heads ? h : a.heads - 1)) * a.splits;
+        const float2 *const st = a.stats + (b * a.heads + (h < a.heads ? h : a.heads - 1)) * a.cut.splits;
         float m = -__builtin_huge_valf(), l = 0.f;
         for (int s = at; s < used; s += lanes) {
           const float2 x = st[s];
@@ -154,7 +155,7 @@ extern "C" size_t tm_kv8_importance_workspace_size(const tm_kv8_cache *cache, co
   tm_kv8_batch one = *batch;
   one.starts = nullptr;
   one.n_tokens = one.n_seqs;
-  return (size_t)batch->n_seqs * n_heads * tm_internal_kv8_splits(cache, &one, n_heads / cache->n_kv_heads) * sizeof(float2);
+  return (size_t)batch->n_seqs * n_heads * tm_internal_kv8_cut(cache, &one, n_heads / cache->n_kv_heads).splits * sizeof(float2);
 }
 
 extern "C" int tm_kv8_importance(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *q,
@@ -187,7 +188,7 @@ extern "C" int tm_kv8_importance(const tm_kv8_cache *cache, const tm_kv8_batch *
   a.b = one;
   a.groups = n_heads / cache->n_kv_heads;
   hipStream_t s = tm_hip_stream(stream);
-  a.splits = tm_internal_kv8_splits(cache, &one, a.groups);
+  a.cut = tm_internal_kv8_cut(cache, &one, a.groups);
   if (lse == nullptr) {
     const size_t need = tm_kv8_importance_workspace_size(cache, batch, n_heads);
     TM_REQUIRE(workspace && workspace_bytes >= need && tm_aligned16(workspace), TM_EWORKSPACE,

@@ -588,6 +588,29 @@ def test_attend_value_scales_of_any_ratio(hip_device, order, one_token):
                  None if one_token else set(range(0, n, 37)) | {n - 1})
 
 
+@pytest.mark.parametrize("h,kv,seqs,longest", [(4, 2, 64, 21000), (16, 8, 66, 20000), (40, 1, 70, 41000)])
+def test_attend_lengths_that_differ(hip_device, h, kv, seqs, longest):
+    """One long sequence among many short ones, one token each: its keys are split, theirs are not."""
+    g = torch.Generator().manual_seed(seqs)
+    dev, page, d = hip_device, 128, 64
+    lens = [int(x) for x in torch.randint(0, 700, (seqs,), generator=g)]
+    lens[seqs // 2], lens[3], lens[4], lens[5] = longest, 0, 1, 4200
+    counts = [-(-x // page) for x in lens]
+    cache, plain = filled(g, sum(counts) + 1, kv, page, d, d, dev)
+    table, lengths = table_of(g, counts, max(counts), sum(counts) + 1), torch.tensor(lens, dtype=torch.int32)
+    q = (1.5 * torch.randn(seqs, h, d, generator=g)).to(BF16)
+    args = (q.to(dev), table.to(dev), lengths.to(dev))
+    y, lse = cache.attend(*args, return_lse=True)
+    imp = cache.importance(*args)
+    some = [0, 3, 4, 5, seqs // 2, seqs - 1]
+    check_attend(cache, plain, q, table, lengths, None, y, lse, d ** -0.5, True, set(some))
+    check_importance(plain, q[some], table[some], lengths[some], d ** -0.5, imp[some])
+    # the others alone, whose table is narrow: the same up to two roundings of the result and those of its sums
+    rest = [i for i in range(seqs) if i not in (seqs // 2, 5)]
+    z = cache.attend(q[rest].to(dev), table[rest, :6].contiguous().to(dev), lengths[rest].to(dev))
+    assert bool(((z.double() - y[rest].double()).abs() <= 2 * half_step(BF16) * y[rest].double().abs() + 1e-5 * 448 * float(plain[3].max())).all())
+
+
 # ----------------------------------------------------------------- importance
 def check_importance(plain, q, table, lengths, scale, got):
     k = plain[0] * plain[1][:, :, None, None]
