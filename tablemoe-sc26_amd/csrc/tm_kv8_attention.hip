@@ -59,7 +59,7 @@ struct AttArgs {
   float *part;    // [row of the call][split][v_dim]
   float scale;
   Kv8Cut cut;
-  int32_t heads, groups, page_log2, causal, tiles1;  // tiles1: row tiles of one token
+  int32_t heads, groups, page_log2, causal, tiles1, rows, early;  // tiles1: row tiles of one token; rows: of a tile
 };
 
 // l 2^x, where 2^x alone may be too small for fp32.
@@ -102,7 +102,8 @@ __device__ __forceinline__ bool row_tile(const AttArgs &a, int64_t u, RowTile &t
   if (a.b.starts != nullptr) last = (t.r0 + t.rows - 1) / (uint32_t)a.groups;
   t.end = visible(a, t.s, last);
   t.tiles = (t.end + 31) >> 5;
-  t.per = a.cut.splits == 1 ? t.tiles + 3 : tm_kv8_per(t.tiles, a.cut);
+  const bool fills = a.cut.least > 4 && all * a.c.n_kv_heads >= 256 * 32;  // one workgroup per CU of its own
+  t.per = a.cut.splits == 1 || fills ? t.tiles + 3 : tm_kv8_per(t.tiles, a.cut);
   return true;
 }
 // A row's token (of its sequence) and its head among the key head's.
@@ -379,7 +380,7 @@ __global__ __launch_bounds__(kThreads, R == 2 || D + DV > 320 ? 2 : 3) void atte
   }
 }
 
-// Joins the splits of a row: a workgroup per row, a thread owning 4 columns of some splits, whose
+// Joins the splits of rows: a workgroup takes a row at a time, a thread 4 columns of some splits, whose
 // parts are requested together with the statistics.
 template <int DT, int DV, int OWN>
 __global__ __launch_bounds__(kThreads) void join_kernel(AttArgs a) {
@@ -388,69 +389,77 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttArgs a) {
   __shared__ float fac[kMaxSplits];
   __shared__ __align__(16) float4 red[kSets][kCols];
   const int h = blockIdx.y;
-  RowTile t = {};
-  int64_t tok, head;
-  // with one token each the row is known without the lists; where most rows have parts these are on their way before
-  // the length is read
-  const bool early = a.b.starts == nullptr && a.cut.least == 4;
-  if (early) {
-    tok = a.tiles1 == 1 ? blockIdx.x : blockIdx.x / (uint32_t)a.tiles1;
-    const int64_t in = (blockIdx.x - tok * a.tiles1) * 32 + blockIdx.z;
-    if (in >= a.groups) return;
-    head = h * a.groups + in;
-  } else {
-    if (!row_tile(a, blockIdx.x, t) || t.per >= t.tiles || (int)blockIdx.z >= t.rows) return;
-    const uint32_t rr = t.r0 + blockIdx.z, in = token_of(a, rr);
-    tok = t.s.first + in;
-    head = h * a.groups + (rr - in * a.groups);
-  }
-  const int64_t row = tok * a.heads + head;
   const int col = threadIdx.x % kCols, set = threadIdx.x / kCols, lane = threadIdx.x & 63;
-  const float *const p = a.part + row * a.cut.splits * DV + col * 4;
-  float4 v[OWN];  // (parts that were not written are read, not used)
-#pragma unroll
-  for (int i = 0; i < OWN; ++i) {
-    const int s = set + i * kSets;
-    v[i] = *reinterpret_cast<const float4 *>(p + (int64_t)(s < a.cut.splits ? s : 0) * DV);
-  }
-  const float2 *const st = a.stats + row * a.cut.splits;
-  const float2 s0 = st[lane < a.cut.splits ? lane : 0], s1 = st[lane + 64 < a.cut.splits ? lane + 64 : 0];
-  if (early && (!row_tile(a, blockIdx.x, t) || t.per >= t.tiles)) return;
-  const int n = (int)((t.tiles + t.per - 1) / t.per);
-  const float2 none = make_float2(-__builtin_huge_valf(), 0.f);
-  const float2 x0 = lane < n ? s0 : none, x1 = lane + 64 < n ? s1 : none;
-  const float top = tm_wave_max(fmaxf(x0.x, x1.x));
-  const float base = top == -__builtin_huge_valf() ? 0.f : top;
-  const float f0 = __builtin_amdgcn_exp2f(x0.x - base), f1 = __builtin_amdgcn_exp2f(x1.x - base);
-  const float total = tm_wave_sum(scaled(x0.y, x0.x - base) + scaled(x1.y, x1.x - base));
-  if (threadIdx.x < 64) {
-    fac[lane] = f0;
-    fac[lane + 64] = f1;
-  }
-  __syncthreads();
-  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (set < kSets) {
+  float4 v[OWN];
+  float2 s0, s1;
+  auto request = [&](int64_t row) {  // (parts that were not written are read, not used)
+    const float *const p = a.part + row * a.cut.splits * DV + col * 4;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
       const int s = set + i * kSets;
-      if (s < n) {
-        const float f = fac[s];
-        y.x = fmaf(v[i].x, f, y.x), y.y = fmaf(v[i].y, f, y.y), y.z = fmaf(v[i].z, f, y.z), y.w = fmaf(v[i].w, f, y.w);
-      }
+      v[i] = *reinterpret_cast<const float4 *>(p + (int64_t)(s < a.cut.splits ? s : 0) * DV);
     }
-    red[set][col] = y;
-  }
-  __syncthreads();
-  if (set != 0) return;
+    const float2 *const st = a.stats + row * a.cut.splits;
+    s0 = st[lane < a.cut.splits ? lane : 0], s1 = st[lane + 64 < a.cut.splits ? lane + 64 : 0];
+  };
+  auto join = [&](int64_t tok, int64_t head, int n) {
+    const float2 none = make_float2(-__builtin_huge_valf(), 0.f);
+    const float2 x0 = lane < n ? s0 : none, x1 = lane + 64 < n ? s1 : none;
+    const float top = tm_wave_max(fmaxf(x0.x, x1.x));
+    const float base = top == -__builtin_huge_valf() ? 0.f : top;
+    const float f0 = __builtin_amdgcn_exp2f(x0.x - base), f1 = __builtin_amdgcn_exp2f(x1.x - base);
+    const float total = tm_wave_sum(scaled(x0.y, x0.x - base) + scaled(x1.y, x1.x - base));
+    if (threadIdx.x < 64) {
+      fac[lane] = f0;
+      fac[lane + 64] = f1;
+    }
+    __syncthreads();
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (set < kSets) {
 #pragma unroll
-  for (int s = 1; s < kSets; ++s) {
-    const float4 x = red[s][col];
-    y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
+      for (int i = 0; i < OWN; ++i) {
+        const int s = set + i * kSets;
+        if (s < n) {
+          const float f = fac[s];
+          y.x = fmaf(v[i].x, f, y.x), y.y = fmaf(v[i].y, f, y.y), y.z = fmaf(v[i].z, f, y.z), y.w = fmaf(v[i].w, f, y.w);
+        }
+      }
+      red[set][col] = y;
+    }
+    __syncthreads();
+    if (set != 0) return;
+#pragma unroll
+    for (int s = 1; s < kSets; ++s) {
+      const float4 x = red[s][col];
+      y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
+    }
+    const float inv = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(-(float)kRoom) / total;
+    T o[4] = {Elem<DT>::from_f(y.x * inv), Elem<DT>::from_f(y.y * inv), Elem<DT>::from_f(y.z * inv), Elem<DT>::from_f(y.w * inv)};
+    __builtin_memcpy(static_cast<T *>(a.out) + tok * a.os_t + head * a.os_h + col * 4, o, 8);
+    if (a.lse && threadIdx.x == 0)
+      a.lse[tok * a.heads + head] = total == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(total)) * kLn2;
+  };
+  auto parts = [](const RowTile &t) { return (int)((t.tiles + t.per - 1) / t.per); };
+  RowTile t = {};
+  if (a.early) {
+    // one token each: a row is known without the lists, its parts are on their way before the length is read
+    const int64_t tok = a.tiles1 == 1 ? blockIdx.x : blockIdx.x / (uint32_t)a.tiles1;
+    const int64_t in = (blockIdx.x - tok * a.tiles1) * 32 + blockIdx.z;
+    if (in >= a.groups) return;
+    request(tok * a.heads + h * a.groups + in);
+    if (!row_tile(a, blockIdx.x, t) || t.per >= t.tiles) return;
+    join(tok, h * a.groups + in, parts(t));
+    return;
   }
-  const float inv = total == 0.f ? 0.f : __builtin_amdgcn_exp2f(-(float)kRoom) / total;
-  T o[4] = {Elem<DT>::from_f(y.x * inv), Elem<DT>::from_f(y.y * inv), Elem<DT>::from_f(y.z * inv), Elem<DT>::from_f(y.w * inv)};
-  __builtin_memcpy(static_cast<T *>(a.out) + tok * a.os_t + head * a.os_h + col * 4, o, 8);
-  if (a.lse && threadIdx.x == 0) a.lse[row] = total == 0.f ? -__builtin_huge_valf() : (top + __builtin_amdgcn_logf(total)) * kLn2;
+  const bool any = a.rows == 64 ? row_tile<64>(a, blockIdx.x, t) : row_tile(a, blockIdx.x, t);
+  if (!any || t.per >= t.tiles) return;
+  for (int r = blockIdx.z; r < t.rows; r += gridDim.z) {
+    const uint32_t rr = t.r0 + r, in = token_of(a, rr);
+    const int64_t tok = t.s.first + in, head = h * a.groups + (rr - in * a.groups);
+    request(tok * a.heads + head);
+    if (r >= (int)gridDim.z) __syncthreads();  // (the row before is summed)
+    join(tok, head, parts(t));
+  }
 }
 
 // How a call is cut up: R x 32 rows a workgroup, at most `tiles` of these per key head, keys split `splits` times.
@@ -462,27 +471,35 @@ struct Plan {
 Plan plan_of(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups) {
   const int64_t rows = b->n_tokens * groups, heads = c->n_kv_heads;
   Plan p = {1, {1, 4}, b->starts ? rows / 32 + b->n_seqs : b->n_seqs * tm_cdiv(groups, 32)};
+  const int64_t keys = (int64_t)b->max_pages * c->page_size / kKv8Tile;
+  // workgroups that have rows, if the sequences have as many each
+  const int64_t units = b->n_seqs > 0 ? b->n_seqs * tm_cdiv(tm_cdiv(rows, b->n_seqs), 32) * heads : 0;
+  int64_t s = 1;
   // 64 rows a wave where that leaves four workgroups for each that a CU holds (32 heads on 4, us with 32 and 64 rows:
   // 2048 tokens 53, 58; 4099 173, 167; 8192 599, 554); wider values leave no registers for them
   if (b->starts && c->v_dim <= 128 && rows / 64 * heads >= 2048) {
     p.r = 2;
     p.tiles = rows / 64 + b->n_seqs;
-    return p;
+  } else if (units > 0 && keys > 32) {
+    // Up to 1024 keys (eight rounds of the four waves) one launch: a round is 0.7 us, joining parts 3 of the host's and 2
+    // of the device's.  Then one workgroup per CU, from 4096 keys on two (32 heads on 4, one sequence, us by splits: 4000
+    // keys 1 28, 4 13.6, 16 9.4; eight sequences of 4000: 1 29, 4 14.7, 8 11.9, 16 12.4).
+    s = (keys <= 128 ? 256 : 512) / units;
+    s = s < keys / kWaves ? s : keys / kWaves;
   }
-  const int64_t units = p.tiles * heads, keys = (int64_t)b->max_pages * c->page_size / kKv8Tile;
-  // Up to 1024 keys (eight rounds of the four waves) one launch: a round is 0.7 us, joining parts 3 of the host's and 2
-  // of the device's.  Then one workgroup per CU, from 4096 keys on two (32 heads on 4, one sequence, us by splits: 4000
-  // keys 1 28, 4 13.6, 16 9.4; eight sequences of 4000: 1 29, 4 14.7, 8 11.9, 16 12.4).
-  if (units <= 0 || keys <= 32) return p;
-  int64_t s = (keys <= 128 ? 256 : 512) / units;
-  s = s < keys / kWaves ? s : keys / kWaves;
   // Sequences of one table may differ much: a part has about 4096 keys of the longest, from two workgroups per CU on
   // 8192, and a short sequence no more parts than above (32 heads on 4, us before and now: one of 65536 among 31 of 1000
-  // keys 153, 60, among 127 434, 104; but 128 of 500 in a table of 65536 16.7, 21.7, of 2000 46, 51).
-  const int64_t most = keys / (units >= 512 ? 256 : 128);
-  if (!b->starts && most > s) {
-    p.cut.least = (int)(units >= 512 ? 64 : (units + 31) / 32 * 4);
-    s = most;
+  // keys 153, 60, among 127 434, 104, 31 of 65536 beside a prompt of 1024 tokens 707, 438; but 128 of 500 in a table of 65536
+  // 16.7, 21.7, of 2000 46, 51).  Sequences whose rows fill the device stay whole (row_tile); the parts of all rows take
+  // 512 MiB at most.
+  int64_t most = keys / (units >= 512 ? 256 : 128);
+  if (b->n_seqs > 1 && most > s) {
+    const int64_t fit = ((int64_t)1 << 29) / (rows * heads * (c->v_dim + 2) * (int64_t)sizeof(float) + 1);
+    most = most < fit ? most : fit;
+    if (most > s) {
+      p.cut.least = (int)(units >= 512 ? 64 : (units + 31) / 32 * 4);
+      s = most;
+    }
   }
   p.cut.splits = (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
   return p;
@@ -500,6 +517,8 @@ AttArgs args_of(const tm_kv8_cache *c, const tm_kv8_batch *b, const void *q, int
   a.cut = p.cut;
   a.page_log2 = c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
   a.tiles1 = (int)tm_cdiv(a.groups, 32);
+  a.rows = 32 * p.r;
+  a.early = !b->starts && p.cut.least == 4;
   return a;
 }
 
@@ -584,8 +603,10 @@ extern "C" int tm_kv8_attention(const tm_kv8_cache *cache, const tm_kv8_batch *b
     }
     TM_LAUNCH_CHECK("tm_kv8_attention");
     if (p.cut.splits > 1) {
-      // (rows of a tile: one token's heads, or 32 of several tokens)
-      const dim3 grid((unsigned)p.tiles, (unsigned)cache->n_kv_heads, (unsigned)(!batch->starts && groups < 32 ? groups : 32));
+      // A workgroup per row: one token's heads, or 32 of several tokens.  Where prompts stay whole, two a tile (a
+      // workgroup that ends at once takes 1.2 ns: three pieces of 1024 tokens on 30000 keys 1682 us with 32, 1632 with 2).
+      const int z = !batch->starts ? (groups < 32 ? groups : 32) : p.cut.least > 4 ? 2 : 32;
+      const dim3 grid((unsigned)p.tiles, (unsigned)cache->n_kv_heads, (unsigned)z);
       constexpr int kSets = kThreads / (DV / 4);
       if (p.cut.splits <= 4 * kSets) hipLaunchKernelGGL((join_kernel<DT, DV, 4>), grid, dim3(kThreads), 0, s, a);
       else hipLaunchKernelGGL((join_kernel<DT, DV, (kMaxSplits + kSets - 1) / kSets>), grid, dim3(kThreads), 0, s, a);

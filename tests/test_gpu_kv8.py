@@ -611,6 +611,26 @@ def test_attend_lengths_that_differ(hip_device, h, kv, seqs, longest):
     assert bool(((z.double() - y[rest].double()).abs() <= 2 * half_step(BF16) * y[rest].double().abs() + 1e-5 * 448 * float(plain[3].max())).all())
 
 
+@pytest.mark.parametrize("h,kv,d,dv,lens,new", [
+    (8, 2, 64, 64, [17000, 30, 9000, 17000, 1100], [1, 1, 4, 2, 1100]),     # the prompt's rows fill the device
+    (8, 2, 192, 128, [17000, 700, 4500], [3, 300, 0]),                      # all are split
+    (64, 8, 64, 64, [33000, 2100, 5, 33000], [1, 2100, 5, 3]),              # 64 rows a wave
+])
+def test_attend_long_sequences_beside_a_prompt(hip_device, h, kv, d, dv, lens, new):
+    """Single and drafted tokens of long sequences in one call with a prompt: their keys are split, the prompt's may not be."""
+    g = torch.Generator().manual_seed(sum(lens))
+    dev, page = hip_device, 128
+    counts = [-(-x // page) for x in lens]
+    cache, plain = filled(g, sum(counts) + 1, kv, page, d, dv, dev)
+    table, lengths = table_of(g, counts, max(counts), sum(counts) + 1), torch.tensor(lens, dtype=torch.int32)
+    starts = torch.tensor([0, *torch.tensor(new).cumsum(0).tolist()], dtype=torch.int32)
+    n = sum(new)
+    q = (1.5 * torch.randn(n, h, d, generator=g)).to(BF16)
+    y, lse = cache.attend(q.to(dev), table.to(dev), lengths.to(dev), starts.to(dev), return_lse=True)
+    some = {0, 1, 2, 7, n // 2, n - 4, n - 2, n - 1}
+    check_attend(cache, plain, q, table, lengths, starts, y, lse, d ** -0.5, True, some)
+
+
 # ----------------------------------------------------------------- importance
 def check_importance(plain, q, table, lengths, scale, got):
     k = plain[0] * plain[1][:, :, None, None]
