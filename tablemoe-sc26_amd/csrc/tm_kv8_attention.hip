@@ -59,7 +59,7 @@ struct AttArgs {
   float *part;    // [row of the call][split][v_dim]
   float scale;
   Kv8Cut cut;
-  int32_t heads, groups, page_log2, causal, tiles1, rows, early;  // tiles1: row tiles of one token; rows: of a tile
+  int32_t heads, groups, page_log2, causal, tiles1, rows, early, turn;  // tiles1: row tiles of one token; rows: of a tile
 };
 
 // l 2^x, where 2^x alone may be too small for fp32.
@@ -84,27 +84,32 @@ __device__ __forceinline__ int64_t visible(const AttArgs &a, const Kv8Seq &s, ui
   e = e < cap ? e : cap;
   return e < 0 ? 0 : e;
 }
+// Row tile j of sequence t.b (false: it has no such rows).
+template <int ROWS = 32>
+__device__ __forceinline__ bool tile_at(const AttArgs &a, int64_t j, RowTile &t) {
+  t.s = tm_kv8_seq(a.b, t.b);
+  const int64_t all = t.s.n * a.groups;
+  if (j < 0 || j * ROWS >= all) return false;
+  t.r0 = (uint32_t)(j * ROWS);
+  t.rows = (int)(all - t.r0 < ROWS ? all - t.r0 : ROWS);
+  const uint32_t last = a.b.starts != nullptr ? (t.r0 + t.rows - 1) / (uint32_t)a.groups : 0;  // the tile's last token
+  t.end = visible(a, t.s, last);
+  t.tiles = (t.end + 31) >> 5;
+  const bool fills = a.cut.least > 4 && all * a.c.n_kv_heads >= 256 * 32;  // one workgroup per CU of its own
+  t.per = a.cut.splits == 1 || fills ? t.tiles + 3 : tm_kv8_per(t.tiles, a.cut);
+  return true;
+}
+// Row tile u of the call.
 template <int ROWS = 32>
 __device__ __forceinline__ bool row_tile(const AttArgs &a, int64_t u, RowTile &t) {
   int64_t j = 0;
-  uint32_t last = 0;  // the tile's last token
   if (a.b.starts == nullptr) {
     t.b = a.tiles1 == 1 ? (uint32_t)u : (uint32_t)u / (uint32_t)a.tiles1;
     j = u - t.b * a.tiles1;
   } else {
     t.b = tm_kv8_unit(a.b, u, a.groups, ROWS, 1, j);
   }
-  t.s = tm_kv8_seq(a.b, t.b);
-  const int64_t all = t.s.n * a.groups;
-  if (j < 0 || j * ROWS >= all) return false;
-  t.r0 = (uint32_t)(j * ROWS);
-  t.rows = (int)(all - t.r0 < ROWS ? all - t.r0 : ROWS);
-  if (a.b.starts != nullptr) last = (t.r0 + t.rows - 1) / (uint32_t)a.groups;
-  t.end = visible(a, t.s, last);
-  t.tiles = (t.end + 31) >> 5;
-  const bool fills = a.cut.least > 4 && all * a.c.n_kv_heads >= 256 * 32;  // one workgroup per CU of its own
-  t.per = a.cut.splits == 1 || fills ? t.tiles + 3 : tm_kv8_per(t.tiles, a.cut);
-  return true;
+  return tile_at<ROWS>(a, j, t);
 }
 // A row's token (of its sequence) and its head among the key head's.
 __device__ __forceinline__ uint32_t token_of(const AttArgs &a, uint32_t row) {
@@ -123,12 +128,30 @@ __global__ __launch_bounds__(kThreads, R == 2 || D + DV > 320 ? 2 : 3) void atte
   __shared__ float inv_s[32];
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
   const int c = lane & 31, g = lane >> 5;
-  const uint32_t heads = a.c.n_kv_heads, block = gridDim.x - 1 - blockIdx.x;  // the last tokens see most: they go first
+  // The last tokens see most: they go first.  (A call with starts counts up to twice the tiles that there are: with the
+  // tiles first, one sequence of 4 tokens of 131071 keys kept to half of the XCDs, 44 us, 36 so.)
+  const uint32_t heads = a.c.n_kv_heads, splits = a.cut.splits;
+  uint32_t block = gridDim.x - 1 - blockIdx.x, split = 0;
+  if (splits > 1) {
+    const uint32_t by = a.cut.least == 4 ? splits : gridDim.x / splits, quot = block / by;
+    if (a.cut.least == 4) {  // every tile is split: its parts one after the other, over all XCDs
+      split = block - quot * by;
+      block = quot;
+    } else {
+      block = block - quot * by;
+      split = splits - 1 - quot;
+    }
+  }
+  if (a.turn) {  // what has work may come at steps of 8, which is one XCD: these are turned against each other
+    const uint32_t units = gridDim.x / splits;
+    if (block < (units & ~7u)) block = (block & ~7u) | ((block + (block >> 3) + split) & 7);
+  }
+  block = __builtin_amdgcn_readfirstlane(block);
+  split = __builtin_amdgcn_readfirstlane(split);
   const int h = (int)(block % heads);
   RowTile t;
   if (!row_tile<32 * R>(a, block / heads, t)) return;
-  const int split = blockIdx.y;
-  const int t0 = (int)(split * t.per < t.tiles ? split * t.per : t.tiles), n = (int)(t0 + t.per < t.tiles ? t0 + t.per : t.tiles);
+  const int t0 = (int)((int64_t)split * t.per < t.tiles ? split * t.per : t.tiles), n = (int)(t0 + t.per < t.tiles ? t0 + t.per : t.tiles);
   if (t0 >= n && split > 0) return;
   const bool whole = t.per >= t.tiles;  // nothing to join with other workgroups
   auto head_of = [&](uint32_t row, uint32_t token) { return (int64_t)h * a.groups + (row - token * a.groups); };
@@ -442,13 +465,14 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttArgs a) {
   auto parts = [](const RowTile &t) { return (int)((t.tiles + t.per - 1) / t.per); };
   RowTile t = {};
   if (a.early) {
-    // one token each: a row is known without the lists, its parts are on their way before the length is read
-    const int64_t tok = a.tiles1 == 1 ? blockIdx.x : blockIdx.x / (uint32_t)a.tiles1;
-    const int64_t in = (blockIdx.x - tok * a.tiles1) * 32 + blockIdx.z;
-    if (in >= a.groups) return;
-    request(tok * a.heads + h * a.groups + in);
-    if (!row_tile(a, blockIdx.x, t) || t.per >= t.tiles) return;
-    join(tok, h * a.groups + in, parts(t));
+    // Most rows have parts: they are on their way before the lists are read.
+    const uint32_t tok = blockIdx.x / (uint32_t)a.groups, in = blockIdx.x - tok * a.groups;
+    const int64_t head = h * a.groups + in;
+    request((int64_t)tok * a.heads + head);
+    int64_t at = 0;
+    t.b = a.b.starts == nullptr ? tok : tm_kv8_unit(a.b, tok, 1, 1, 0, at);
+    if (!tile_at(a, (at * a.groups + in) / 32, t) || at < 0 || at >= t.s.n || t.per >= t.tiles) return;
+    join(tok, head, parts(t));
     return;
   }
   const bool any = a.rows == 64 ? row_tile<64>(a, blockIdx.x, t) : row_tile(a, blockIdx.x, t);
@@ -467,10 +491,11 @@ struct Plan {
   int r;
   Kv8Cut cut;
   int64_t tiles;
+  bool turn;  // workgroups with work are not evenly spread
 };
 Plan plan_of(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups) {
   const int64_t rows = b->n_tokens * groups, heads = c->n_kv_heads;
-  Plan p = {1, {1, 4}, b->starts ? rows / 32 + b->n_seqs : b->n_seqs * tm_cdiv(groups, 32)};
+  Plan p = {1, {1, 4}, b->starts ? rows / 32 + b->n_seqs : b->n_seqs * tm_cdiv(groups, 32), false};
   const int64_t keys = (int64_t)b->max_pages * c->page_size / kKv8Tile;
   // workgroups that have rows, if the sequences have as many each
   const int64_t units = b->n_seqs > 0 ? b->n_seqs * tm_cdiv(tm_cdiv(rows, b->n_seqs), 32) * heads : 0;
@@ -486,11 +511,12 @@ Plan plan_of(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups) {
     // keys 1 28, 4 13.6, 16 9.4; eight sequences of 4000: 1 29, 4 14.7, 8 11.9, 16 12.4).
     s = (keys <= 128 ? 256 : 512) / units;
     s = s < keys / kWaves ? s : keys / kWaves;
+    s = s < 1 ? 1 : s;
   }
   // Sequences of one table may differ much: a part has about 4096 keys of the longest, from two workgroups per CU on
   // 8192, and a short sequence no more parts than above (32 heads on 4, us before and now: one of 65536 among 31 of 1000
-  // keys 153, 60, among 127 434, 104, 31 of 65536 beside a prompt of 1024 tokens 707, 438; but 128 of 500 in a table of 65536
-  // 16.7, 21.7, of 2000 46, 51).  Sequences whose rows fill the device stay whole (row_tile); the parts of all rows take
+  // keys 153, 60, among 127 434, 98, 31 of 65536 beside a prompt of 1024 tokens 707, 438; but 128 of 500 in a table of 65536
+  // 16.7, 24, of 2000 46, 52).  Sequences whose rows fill the device stay whole (row_tile); the parts of all rows take
   // 512 MiB at most.
   int64_t most = keys / (units >= 512 ? 256 : 128);
   if (b->n_seqs > 1 && most > s) {
@@ -501,7 +527,9 @@ Plan plan_of(const tm_kv8_cache *c, const tm_kv8_batch *b, int groups) {
       s = most;
     }
   }
-  p.cut.splits = (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+  p.cut.splits = (int)(s > kMaxSplits ? kMaxSplits : s);
+  // (Prompts are not turned: a head's tiles share an XCD's L2; three pieces of 1024 tokens of 16 heads 216 us, 244 turned.)
+  p.turn = b->starts ? p.cut.splits == 1 && 2 * p.tiles * heads >= 3 * units : p.cut.least > 4;
   return p;
 }
 
@@ -518,13 +546,13 @@ AttArgs args_of(const tm_kv8_cache *c, const tm_kv8_batch *b, const void *q, int
   a.page_log2 = c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
   a.tiles1 = (int)tm_cdiv(a.groups, 32);
   a.rows = 32 * p.r;
-  a.early = !b->starts && p.cut.least == 4;
+  a.turn = p.turn;
   return a;
 }
 
 template <int DT, int D, int DV, int R>
 void launch(const AttArgs &a, const Plan &p, hipStream_t s) {
-  const dim3 grid((unsigned)(p.tiles * a.c.n_kv_heads), (unsigned)p.cut.splits);
+  const dim3 grid((unsigned)(p.tiles * a.c.n_kv_heads * p.cut.splits));
   hipLaunchKernelGGL((attend_kernel<DT, D, DV, R>), grid, dim3(kThreads), 0, s, a);
 }
 
@@ -580,7 +608,7 @@ extern "C" int tm_kv8_attention(const tm_kv8_cache *cache, const tm_kv8_batch *b
              TM_EINVAL_SHAPE, "tm_kv8_attention: rows of q and out must be 16-byte aligned, strides multiples of 8 elements");
   const int groups = n_heads / cache->n_kv_heads;
   const Plan p = plan_of(cache, batch, groups);
-  TM_REQUIRE(p.tiles * cache->n_kv_heads < kKv8MaxGrid && batch->n_tokens * groups < ((int64_t)1 << 31), TM_EINVAL_SHAPE,
+  TM_REQUIRE(p.tiles * cache->n_kv_heads * p.cut.splits < kKv8MaxGrid && batch->n_tokens * groups < ((int64_t)1 << 31), TM_EINVAL_SHAPE,
              "tm_kv8_attention: too many rows");
   const size_t need = tm_kv8_attention_workspace_size(cache, batch, n_heads);
   TM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && tm_aligned16(workspace)), TM_EWORKSPACE,
@@ -603,10 +631,12 @@ extern "C" int tm_kv8_attention(const tm_kv8_cache *cache, const tm_kv8_batch *b
     }
     TM_LAUNCH_CHECK("tm_kv8_attention");
     if (p.cut.splits > 1) {
-      // A workgroup per row: one token's heads, or 32 of several tokens.  Where prompts stay whole, two a tile (a
-      // workgroup that ends at once takes 1.2 ns: three pieces of 1024 tokens on 30000 keys 1682 us with 32, 1632 with 2).
-      const int z = !batch->starts ? (groups < 32 ? groups : 32) : p.cut.least > 4 ? 2 : 32;
-      const dim3 grid((unsigned)p.tiles, (unsigned)cache->n_kv_heads, (unsigned)z);
+      // A workgroup per row.  Where prompts may stay whole, two a tile (a workgroup that ends at once takes 1.2 ns: three
+      // pieces of 1024 tokens on 30000 keys 1682 us with 32, 1632 with 2).
+      const bool early = p.cut.least == 4;
+      a.early = early;
+      const dim3 grid((unsigned)(early ? batch->n_tokens * groups : p.tiles), (unsigned)cache->n_kv_heads,
+                      early ? 1u : batch->starts ? 2u : (unsigned)(groups < 32 ? groups : 32));
       constexpr int kSets = kThreads / (DV / 4);
       if (p.cut.splits <= 4 * kSets) hipLaunchKernelGGL((join_kernel<DT, DV, 4>), grid, dim3(kThreads), 0, s, a);
       else hipLaunchKernelGGL((join_kernel<DT, DV, (kMaxSplits + kSets - 1) / kSets>), grid, dim3(kThreads), 0, s, a);

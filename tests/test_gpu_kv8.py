@@ -611,6 +611,25 @@ def test_attend_lengths_that_differ(hip_device, h, kv, seqs, longest):
     assert bool(((z.double() - y[rest].double()).abs() <= 2 * half_step(BF16) * y[rest].double().abs() + 1e-5 * 448 * float(plain[3].max())).all())
 
 
+@pytest.mark.parametrize("h,kv,lens,new,page", [
+    (8, 2, [5000, 0, 3000, 40], [3, 0, 2, 1], 64), (12, 4, [6000], [33], 32), (40, 1, [4100, 2000], [2, 2], 128),
+    (4, 4, [2000] * 9, [4] * 9, 64), (8, 8, [300] * 40, [2] * 40, 64)])
+def test_attend_drafted_tokens(hip_device, h, kv, lens, new, page):
+    """A few new tokens for each of some sequences, keys split; rows behind the last sequence are left as they were."""
+    g = torch.Generator().manual_seed(len(lens) + h)
+    dev, d = hip_device, 128
+    counts = [-(-x // page) for x in lens]
+    cache, plain = filled(g, sum(counts) + 1, kv, page, d, d, dev)
+    table, lengths = table_of(g, counts, max(counts), sum(counts) + 1), torch.tensor(lens, dtype=torch.int32)
+    starts = torch.tensor([0, *torch.tensor(new).cumsum(0).tolist()], dtype=torch.int32)
+    n = sum(new)
+    q = (1.5 * torch.randn(n + 3, h, d, generator=g)).to(BF16)
+    out = torch.full((n + 3, h, d), 7.0, dtype=BF16, device=dev)
+    y, lse = cache.attend(q.to(dev), table.to(dev), lengths.to(dev), starts.to(dev), out=out, return_lse=True)
+    assert bool((y[n:] == 7).all())
+    check_attend(cache, plain, q, table, lengths, starts, y, lse, d ** -0.5, True, set(range(0, n, 5)) | {n - 1})
+
+
 @pytest.mark.parametrize("h,kv,d,dv,lens,new", [
     (8, 2, 64, 64, [17000, 30, 9000, 17000, 1100], [1, 1, 4, 2, 1100]),     # the prompt's rows fill the device
     (8, 2, 192, 128, [17000, 700, 4500], [3, 300, 0]),                      # all are split
