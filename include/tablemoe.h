@@ -632,7 +632,8 @@ int tm_fp8_expert_swiglu(const tm_fp8_experts *experts, int32_t dtype, const voi
  * fp32, rounded once.  inverse != 0 turns back (the gradient with respect to
  * the inputs).  Columns from rotary_dim on are copied.  Outputs have strides of
  * their own and may be the inputs themselves, but not overlap them otherwise.
- * Limits: head_dim <= 1024, rotary_dim even and <= head_dim, n_axes <= 4.
+ * Limits: head_dim <= 1024, rotary_dim even and <= head_dim, n_axes <= 4,
+ * n_tokens < 2^26 (2^25 where rotary_dim > 512).
  * ====================================================================== */
 int tm_rotate_positions(int32_t dtype, const void *q, int64_t n_tokens, int32_t n_heads, int64_t qs_t, int64_t qs_h,
                         const void *k, int32_t n_kv_heads, int64_t ks_t, int64_t ks_h, int32_t head_dim,
@@ -695,8 +696,8 @@ int tm_kv8_append(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t 
  * rounded to fp16 before it meets the values.  lse (nullable,
  * fp32 [n_tokens, n_heads] contiguous) = log sum exp of the scores, natural.  A
  * token that sees nothing gets zeros and -inf; rows of no sequence are left as
- * they were.  16-byte aligned rows of q and out; scale > 0; workspace
- * tm_kv8_attention_workspace_size (16-byte aligned, one call at a time). */
+ * they were.  16-byte aligned rows of q and out, which must not overlap; scale > 0; workspace
+ * tm_kv8_attention_workspace_size (16-byte aligned, one call at a time; it goes by the batch's sizes alone). */
 size_t tm_kv8_attention_workspace_size(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t n_heads);
 int tm_kv8_attention(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *q, int64_t qs_t,
                      int64_t qs_h, int32_t n_heads, float scale, int32_t causal, void *out, int64_t os_t, int64_t os_h,
