@@ -141,6 +141,41 @@ def test_rotate_gradients(hip_device):
         assert not rotate_positions(q, k, *args)[0].requires_grad
 
 
+def test_rotate_gradients_captured(hip_device):
+    """Forward and gradient in one captured graph, replayed over other inputs between eager work."""
+    from table_moe.ops import rotate_positions
+
+    dev = hip_device
+    g = torch.Generator().manual_seed(16)
+    n, h, kv, d = 13, 4, 2, 64
+    mk = lambda heads: torch.randn(n, heads, d, generator=g).to(BF16).to(dev)  # noqa: E731
+    inv = (1e4 ** (-torch.arange(32).double() / 32)).float().to(dev)
+    pos = torch.randint(0, 9000, (3, n), generator=g).to(dev)
+    q, k, wq, wk = mk(h), mk(kv), mk(h), mk(kv)
+
+    def step(q, k, wq, wk, pos):
+        a, b = q.detach().requires_grad_(), k.detach().requires_grad_()
+        y, z = rotate_positions(a, b, pos, inv, (12, 10, 10), interleaved=True)
+        return y.detach(), z.detach(), *torch.autograd.grad((y, z), (a, b), (wq, wk))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(q, k, wq, wk, pos)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(q, k, wq, wk, pos)
+    for _ in range(4):
+        q.copy_(mk(h)), k.copy_(mk(kv)), wq.copy_(mk(h)), wk.copy_(mk(kv))
+        pos.copy_(torch.randint(0, 9000, (3, n), generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(q.clone(), k.clone(), wq, wk, pos)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_rotate_refusals(hip_device):
     from table_moe.ops import rotate_positions
 
