@@ -715,6 +715,15 @@ int tm_kv8_importance(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int3
                       int64_t qs_h, int32_t n_heads, float scale, const float *lse, int64_t ld_lse, int64_t out_len,
                       float *out, int64_t ld_out, void *workspace, size_t workspace_bytes, tm_stream_t stream);
 
+/* The same of the batch's new tokens alone, by their row, as tm_expert_keep_mask
+ * takes it: out[starts[b] + i] (fp32 [n_tokens]) is the probability of position
+ * lengths[b] - n + i, n being the sequence's new tokens; 0 past the table's width.
+ * Rows of no sequence and of positions before 0 are left as they were.  starts
+ * NULL: one new token each.  Workspace as above. */
+int tm_kv8_importance_rows(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *q,
+                           int64_t qs_b, int64_t qs_h, int32_t n_heads, float scale, const float *lse, int64_t ld_lse,
+                           float *out, void *workspace, size_t workspace_bytes, tm_stream_t stream);
+
 /* ======================================================================
  * Mode G -- one MoE layer of the table path in ONE call.
  * Enqueues, back to back on `stream`: tm_topk_softmax (router) ->

@@ -8,6 +8,9 @@
 // waves of a workgroup take the key heads and tiles of its keys between them and
 // join through LDS in a fixed order.
 //
+// Written by position of each sequence, or by row of the call's new tokens (the
+// last positions of each sequence): then only these tokens' tiles are computed.
+//
 // Bound by HBM: 131071 keys of 4 heads of 128 (67 MB) with the log sum exp at hand 14.3 us,
 // 4.7 TB/s, as a large copy; 4099 keys without it 5.4 + 4.3 us, two launches of a few memory
 // round trips each.
@@ -35,7 +38,7 @@ struct ImpArgs {
   int64_t ld_out, out_len;
   float scale;
   Kv8Cut cut;
-  int32_t heads, groups, page_log2, per, head_waves, lanes_log2;
+  int32_t heads, groups, page_log2, per, head_waves, lanes_log2, by_row;
 };
 
 template <int DT, int D>
@@ -46,8 +49,19 @@ __global__ __launch_bounds__(kThreads) void importance_kernel(ImpArgs a) {
   __shared__ float acc[kWaves][kMaxPer][32];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int c = lane & 31, g = lane >> 5;
-  const int64_t b = blockIdx.y;
-  const int tile0 = (int)(blockIdx.x * a.per);
+  int64_t b = blockIdx.y;
+  int tile0 = (int)(blockIdx.x * a.per);
+  Kv8Seq s = {};
+  if (a.by_row) {
+    // a sequence of n new tokens touches at most (n - 2) / 32 + 2 tiles: at most n / (32 per) + 2 workgroups
+    int64_t j = 0;
+    b = blockIdx.x;
+    if (a.b.starts != nullptr) b = tm_kv8_unit(a.b, blockIdx.x, 1, 32 * a.per, 2, j);
+    s = tm_kv8_seq(a.b, b);
+    const int64_t old = s.len - s.n, at = ((old > 0 ? old : 0) >> 5) + j * a.per;
+    if (j < 0 || s.n == 0 || at * 32 >= s.len) return;
+    tile0 = (int)at;
+  }
   const int64_t cap = (int64_t)a.b.max_pages << a.page_log2;
   int64_t len = a.b.lengths[b];
   len = len < 0 ? 0 : len < cap ? len : cap;
@@ -138,12 +152,13 @@ __global__ __launch_bounds__(kThreads) void importance_kernel(ImpArgs a) {
       }
   __syncthreads();
   for (int i = tid; i < a.per * 32; i += kThreads) {
-    const int64_t t = (int64_t)tile0 * 32 + i;
-    if (t >= a.out_len) break;
+    const int64_t t = (int64_t)tile0 * 32 + i, row = t - (s.len - s.n);
+    if (a.by_row ? t >= s.len : t >= a.out_len) break;
+    if (a.by_row && row < 0) continue;
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) v += acc[w][i >> 5][i & 31];
-    a.out[b * a.ld_out + t] = t < len ? v / (float)a.heads : 0.f;
+    a.out[a.by_row ? s.first + row : b * a.ld_out + t] = t < len ? v / (float)a.heads : 0.f;
   }
 }
 
@@ -158,41 +173,43 @@ extern "C" size_t tm_kv8_importance_workspace_size(const tm_kv8_cache *cache, co
   return (size_t)batch->n_seqs * n_heads * tm_internal_kv8_cut(cache, &one, n_heads / cache->n_kv_heads).splits * sizeof(float2);
 }
 
-extern "C" int tm_kv8_importance(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *q,
-                                 int64_t qs_b, int64_t qs_h, int32_t n_heads, float scale, const float *lse,
-                                 int64_t ld_lse, int64_t out_len, float *out, int64_t ld_out, void *workspace,
-                                 size_t workspace_bytes, tm_stream_t stream) {
-  TM_REQUIRE(dtype == TM_DT_F16 || dtype == TM_DT_BF16, TM_EINVAL_DTYPE, "tm_kv8_importance: unsupported dtype tag %d",
-             (int)dtype);
-  TM_REQUIRE(cache && batch, TM_EINVAL_ARG, "tm_kv8_importance: null pointer");
-  tm_kv8_batch one = *batch;
-  one.starts = nullptr;
-  const int bad = tm_kv8_check("tm_kv8_importance", cache, &one);
+// What the entry points share: `batch` has starts only where out goes by row.
+static int importance(const char *what, const tm_kv8_cache *cache, const tm_kv8_batch *batch, bool by_row, int32_t dtype,
+                      const void *q, int64_t qs_b, int64_t qs_h, int32_t n_heads, float scale, const float *lse,
+                      int64_t ld_lse, int64_t out_len, float *out, int64_t ld_out, void *workspace,
+                      size_t workspace_bytes, tm_stream_t stream) {
+  TM_REQUIRE(dtype == TM_DT_F16 || dtype == TM_DT_BF16, TM_EINVAL_DTYPE, "%s: unsupported dtype tag %d", what, (int)dtype);
+  const int bad = tm_kv8_check(what, cache, batch);
   if (bad != TM_OK) return bad;
+  tm_kv8_batch one = *batch;  // one query per sequence
+  one.starts = nullptr;
+  one.n_tokens = one.n_seqs;
   TM_REQUIRE(n_heads >= 1 && n_heads <= kMaxHeads && n_heads % cache->n_kv_heads == 0, TM_EINVAL_SHAPE,
-             "tm_kv8_importance: %d query heads (at most %d) on %d key heads", n_heads, kMaxHeads, cache->n_kv_heads);
-  TM_REQUIRE(scale > 0.f && scale < __builtin_huge_valf(), TM_EINVAL_ARG, "tm_kv8_importance: scale must be positive and finite");
+             "%s: %d query heads (at most %d) on %d key heads", what, n_heads, kMaxHeads, cache->n_kv_heads);
+  TM_REQUIRE(scale > 0.f && scale < __builtin_huge_valf(), TM_EINVAL_ARG, "%s: scale must be positive and finite", what);
   TM_REQUIRE(out_len >= 0 && out_len < ((int64_t)1 << 31) && ld_out >= out_len && batch->n_seqs < 65536 &&
                  (lse == nullptr || ld_lse >= n_heads),
-             TM_EINVAL_SHAPE, "tm_kv8_importance: bad sizes (out_len %lld, %lld sequences)", (long long)out_len,
+             TM_EINVAL_SHAPE, "%s: bad sizes (out_len %lld, %lld sequences)", what, (long long)out_len,
              (long long)batch->n_seqs);
   if (batch->n_seqs == 0 || out_len == 0) return TM_OK;
-  TM_REQUIRE(q && out, TM_EINVAL_ARG, "tm_kv8_importance: null pointer");
+  TM_REQUIRE(q && out, TM_EINVAL_ARG, "%s: null pointer", what);
   if (batch->n_seqs == 1) qs_b = 0;  // (the stride of a single row means nothing)
   if (n_heads == 1) qs_h = 0;
   TM_REQUIRE(tm_aligned16(q) && qs_b % 8 == 0 && qs_h % 8 == 0, TM_EINVAL_SHAPE,
-             "tm_kv8_importance: rows of q must be 16-byte aligned, strides multiples of 8 elements");
+             "%s: rows of q must be 16-byte aligned, strides multiples of 8 elements", what);
   ImpArgs a = {};
   a.c = *cache;
   if (cache->n_pages == 0) one.max_pages = 0;
   a.b = one;
+  a.by_row = by_row;
+  if (by_row) a.b.starts = batch->starts, a.b.n_tokens = batch->n_tokens;
   a.groups = n_heads / cache->n_kv_heads;
   hipStream_t s = tm_hip_stream(stream);
   a.cut = tm_internal_kv8_cut(cache, &one, a.groups);
   if (lse == nullptr) {
     const size_t need = tm_kv8_importance_workspace_size(cache, batch, n_heads);
     TM_REQUIRE(workspace && workspace_bytes >= need && tm_aligned16(workspace), TM_EWORKSPACE,
-               "tm_kv8_importance: workspace %zu bytes < %zu", workspace_bytes, need);
+               "%s: workspace %zu bytes < %zu", what, workspace_bytes, need);
     a.stats = static_cast<const float2 *>(workspace);
     const int st = tm_internal_kv8_stats(cache, &one, dtype, q, qs_b, qs_h, n_heads, scale,
                                          static_cast<float2 *>(workspace), s);
@@ -207,11 +224,12 @@ extern "C" int tm_kv8_importance(const tm_kv8_cache *cache, const tm_kv8_batch *
   a.head_waves = cache->n_kv_heads >= 4 ? 4 : cache->n_kv_heads >= 2 ? 2 : 1;
   while (a.lanes_log2 < 6 && (kThreads >> (a.lanes_log2 + 1)) >= n_heads) ++a.lanes_log2;
   const int64_t tiles = tm_cdiv(out_len, 32);
-  int64_t per = tm_cdiv(tiles * one.n_seqs, 1024);
+  int64_t per = tm_cdiv(by_row ? tiles + one.n_seqs : tiles * one.n_seqs, 1024);
   const int tile_waves = kWaves / a.head_waves;
   per = tm_cdiv(per, tile_waves) * tile_waves;
   a.per = (int)(per > kMaxPer ? kMaxPer : per);
-  const dim3 grid((unsigned)tm_cdiv(tiles, a.per), (unsigned)one.n_seqs);
+  const dim3 grid = !by_row ? dim3((unsigned)tm_cdiv(tiles, a.per), (unsigned)one.n_seqs)
+                            : dim3((unsigned)(batch->starts ? out_len / (32 * a.per) + 2 * one.n_seqs : one.n_seqs));
   auto run = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     switch (cache->head_dim) {
@@ -223,6 +241,26 @@ extern "C" int tm_kv8_importance(const tm_kv8_cache *cache, const tm_kv8_batch *
   };
   if (dtype == TM_DT_F16) run(std::integral_constant<int, TM_DT_F16>{});
   else run(std::integral_constant<int, TM_DT_BF16>{});
-  TM_LAUNCH_CHECK("tm_kv8_importance");
+  TM_LAUNCH_CHECK(what);
   return TM_OK;
+}
+
+extern "C" int tm_kv8_importance(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *q,
+                                 int64_t qs_b, int64_t qs_h, int32_t n_heads, float scale, const float *lse,
+                                 int64_t ld_lse, int64_t out_len, float *out, int64_t ld_out, void *workspace,
+                                 size_t workspace_bytes, tm_stream_t stream) {
+  TM_REQUIRE(cache && batch, TM_EINVAL_ARG, "tm_kv8_importance: null pointer");
+  tm_kv8_batch one = *batch;
+  one.starts = nullptr;
+  return importance("tm_kv8_importance", cache, &one, false, dtype, q, qs_b, qs_h, n_heads, scale, lse, ld_lse, out_len,
+                    out, ld_out, workspace, workspace_bytes, stream);
+}
+
+extern "C" int tm_kv8_importance_rows(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *q,
+                                      int64_t qs_b, int64_t qs_h, int32_t n_heads, float scale, const float *lse,
+                                      int64_t ld_lse, float *out, void *workspace, size_t workspace_bytes,
+                                      tm_stream_t stream) {
+  TM_REQUIRE(cache && batch, TM_EINVAL_ARG, "tm_kv8_importance_rows: null pointer");
+  return importance("tm_kv8_importance_rows", cache, batch, true, dtype, q, qs_b, qs_h, n_heads, scale, lse, ld_lse,
+                    batch->n_tokens, out, batch->n_tokens, workspace, workspace_bytes, stream);
 }

@@ -99,6 +99,7 @@ PROTOTYPES = {
     "tm_kv8_attention": (C.c_int, [vp, vp, i32, vp, i64, i64, i32, f32, i32, vp, i64, i64, vp, vp, sz, vp]),
     "tm_kv8_importance_workspace_size": (sz, [vp, vp, i32]),
     "tm_kv8_importance": (C.c_int, [vp, vp, i32, vp, i64, i64, i32, f32, vp, i64, i64, vp, i64, vp, sz, vp]),
+    "tm_kv8_importance_rows": (C.c_int, [vp, vp, i32, vp, i64, i64, i32, f32, vp, i64, vp, vp, sz, vp]),
     "tm_project_workspace_size": (sz, [i64, i32, i32]),
     "tm_project_packed_size": (sz, [i32, i32, i32]),
     "tm_project_pack": (C.c_int, [i32, vp, i32, i32, i64, i64, vp, sz, vp]),

@@ -206,23 +206,32 @@ class Fp8KVCache:
         return (out, lse) if return_lse else out
 
     def importance(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *, scale: float | None = None,
-                   lse: torch.Tensor | None = None, out_len: int | None = None) -> torch.Tensor:
+                   lse: torch.Tensor | None = None, out_len: int | None = None,
+                   starts: torch.Tensor | None = None) -> torch.Tensor:
         """Head mean of the probabilities that one query per sequence, q [B,
         heads, head_dim], gives to each cached position: [B, out_len] float32
         (default: the table's width in tokens), 0 from a sequence's length on.
+        With ``starts`` (and out_len, the rows of the call) of the new tokens
+        alone: [out_len], row starts[b] + i being position lengths[b] - n + i of
+        a sequence with n of them; 0 where a row is no sequence's.
         lse [B, heads] float32: the queries' log sum exp where ``attend`` has
         given it (keys are read once then).  At most 256 heads.
         ``table_moe.utils.importance.cached_importance`` also stores the scores
         for the keep rule."""
         tag, scale = self._queries(q, scale)
         b, h, _ = q.shape
-        batch, kept = self._batch(table, lengths, None, b)
+        if starts is not None and out_len is None:
+            raise ValueError("Fp8KVCache.importance: starts needs out_len, the number of the call's rows")
+        if out_len is not None and int(out_len) < 0:
+            raise ValueError("Fp8KVCache.importance: out_len must not be negative")
+        batch, kept = self._batch(table, lengths, starts, b if starts is None else int(out_len))
+        if batch.n_seqs != b:
+            raise ValueError(f"Fp8KVCache.importance: {b} queries for {batch.n_seqs} sequences")
         dev = self.device
         q, qs_t, qs_h = _rows(q)
         out_len = batch.max_pages * self.page_size if out_len is None else int(out_len)
-        if out_len < 0:
-            raise ValueError("Fp8KVCache.importance: out_len must not be negative")
-        out = torch.empty((b, out_len), dtype=torch.float32, device=dev)
+        out = torch.empty((b, out_len), dtype=torch.float32, device=dev) if starts is None else \
+            torch.zeros(out_len, dtype=torch.float32, device=dev)
         ref, ld_lse, ws, nbytes = C.byref(batch), 0, None, 0
         if lse is not None:
             N.require_hip(q, lse)
@@ -235,6 +244,10 @@ class Fp8KVCache:
             nbytes = N.lib().tm_kv8_importance_workspace_size(self._ref, ref, h)
             ws = q.new_empty(nbytes // 2) if nbytes else None
         with N.on_device(dev):
-            N.call("tm_kv8_importance", self._ref, ref, tag, q.data_ptr(), qs_t, qs_h, h, scale, N.ptr(lse), ld_lse,
-                   out_len, out.data_ptr(), out_len, N.ptr(ws), nbytes, N.stream(dev))
+            if starts is None:
+                N.call("tm_kv8_importance", self._ref, ref, tag, q.data_ptr(), qs_t, qs_h, h, scale, N.ptr(lse), ld_lse,
+                       out_len, out.data_ptr(), out_len, N.ptr(ws), nbytes, N.stream(dev))
+            else:
+                N.call("tm_kv8_importance_rows", self._ref, ref, tag, q.data_ptr(), qs_t, qs_h, h, scale, N.ptr(lse),
+                       ld_lse, out.data_ptr(), N.ptr(ws), nbytes, N.stream(dev))
         return out

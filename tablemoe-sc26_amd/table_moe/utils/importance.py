@@ -91,14 +91,24 @@ def cache_last_token_attention(query_states: torch.Tensor, key_states: torch.Ten
 
 def cached_importance(cache, query_states: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
                       scaling: float | None = None, lse: torch.Tensor | None = None,
-                      query_length: int | None = None):
+                      query_length: int | None = None, starts: torch.Tensor | None = None):
     """cache_last_token_attention over keys that live in an 8-bit cache
     (table_moe.ops.Fp8KVCache): query_states [B, H, D], the last query of each
-    sequence after RoPE.  Stores and returns the scores of the first
-    query_length positions [B, query_length] (default: the table's width)."""
+    sequence after RoPE.  Stores and returns the scores of the layer's tokens:
+
+    with ``starts`` [B + 1], as in the cache's calls, [query_length]: one for each
+    row of the call, its new tokens, whatever each sequence holds before them
+    (query_length is the number of rows);
+    without it [B, query_length]: positions from each sequence's first on (default:
+    the table's width).  These are the layer's tokens only where one prompt of
+    query_length tokens has nothing before it; for a piece of a prompt, a shared
+    prefix or several sequences, give ``starts``."""
+    if starts is not None and query_length is None:
+        raise ValueError("cached_importance: starts needs query_length, the number of the call's rows")
     try:
         with torch.no_grad():
-            mean_score = cache.importance(query_states, table, lengths, scale=scaling, lse=lse, out_len=query_length)
+            mean_score = cache.importance(query_states, table, lengths, scale=scaling, lse=lse, out_len=query_length,
+                                          starts=starts)
             ModalityContext.set_attn_weights(mean_score.reshape(-1))
             return mean_score
     except N.NativeLibraryMissing:
