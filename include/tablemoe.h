@@ -681,10 +681,11 @@ typedef struct tm_kv8_batch {
 /* Writes the new tokens' k [n_tokens, n_kv_heads, head_dim] and v (v_dim) of
  * `dtype` (F32, F16, BF16; strides per token and head, unit along columns,
  * 16-byte aligned rows) into their pages.  A page's scale is the smallest power
- * of two s >= 2^-100 with max|x| / s <= 448 over the finite values written (1
- * where they are all 0), and no less than what it was where the page held
- * tokens before; where that rises, those tokens' values are rounded again under
- * the new scale.  Values are rounded to nearest even, a non-finite one becomes NaN.
+ * of two s >= 2^-100 with max|x| / s <= 448 over the finite values written, and
+ * no less than what it was where the page held tokens before; where that rises,
+ * those tokens' values are rounded again under the new scale.  Rows of zeros and
+ * non-finite values alone leave the scale as it is, 1 in a page of their own,
+ * which does not bind later rows.  Values are rounded to nearest even, a non-finite one becomes NaN.
  * Cells past a sequence's end keep their bytes.  A page that is written belongs to one sequence. */
 int tm_kv8_append(const tm_kv8_cache *cache, const tm_kv8_batch *batch, int32_t dtype, const void *k, int64_t ks_t,
                   int64_t ks_h, const void *v, int64_t vs_t, int64_t vs_h, tm_stream_t stream);

@@ -35,6 +35,26 @@ __device__ __forceinline__ uint4 rescale16(uint4 v, float f) {
   return make_uint4(rescale4(v.x, f), rescale4(v.y, f), rescale4(v.z, f), rescale4(v.w, f));
 }
 
+// Whether one of the page's tokens before `lo` holds a value other than 0 and NaN, which are the same bytes under any scale.
+template <int D, bool V>
+__device__ __forceinline__ bool holds_values(const uint8_t *page, int lo) {
+  uint32_t any = 0;
+  for (int i = threadIdx.x; i < ((lo + 31) >> 5) * (2 * D); i += kAppThreads) {
+    const uint4 w = reinterpret_cast<const uint4 *>(page)[i];
+    const uint32_t d[4] = {w.x, w.y, w.z, w.w};
+    const int lane = i & 63, t = i / (2 * D) * 32;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t x = d[q] & 0x7f7f7f7fu;
+      const uint32_t is = (x + 0x7f7f7f7fu) & ~(x + 0x01010101u) & 0x80808080u;  // 0x80: neither 0 nor 0x7f
+      // the dword's bytes before lo: a key's are all of one token, a value's of tokens one after the other
+      const int left = V ? lo - (t + 4 * (lane >> 5) + 8 * q) : (t + (lane & 31) < lo ? 4 : 0);
+      any |= left >= 4 ? is : left <= 0 ? 0u : is & (0xffffffffu >> (32 - 8 * left));
+    }
+  }
+  return __syncthreads_or(any != 0) != 0;
+}
+
 // The new rows [lo, hi) of a page from src (row 0: the page's first token).  A thread owns four consecutive tokens by
 // 8 columns, read once and kept in registers over the search for the maximum: as bytes they are whole dwords of
 // V's pieces and halves of K's.  These meet in an image of the page in LDS, and what changes goes out as 16-byte pieces.
@@ -77,7 +97,10 @@ __device__ __forceinline__ void write_page(const typename Elem<DT>::T *src, int6
   float s = fmaxf(tm_fp8_scale(m, inv), kKv8MinScale);
   float f = 1.f;  // what the page held is taken times this
   if (lo > 0) {
-    if (before > s) s = before;
+    // New rows of zeros and non-finite values alone ask for no scale; nor does the 1 that such rows left where they
+    // came first (an outlier's page may have 1, too: its bytes tell).
+    if (m == 0) s = before;
+    else if (before > s) s = before == 1.f && !holds_values<D, V>(page, lo) ? s : before;
     else f = before / s;  // powers of two
   }
   inv = 1.f / s;

@@ -139,8 +139,9 @@ class Fp8KVCache:
         """Writes the new tokens' k [T, heads, head_dim] and v [T, heads, v_dim]
         (float32, float16 or bfloat16) into their pages.  A page's scale is the
         smallest power of two that holds the largest value; where new tokens
-        raise it, the page's older values are rounded again.  A non-finite value is
-        stored as NaN.  A page that is written belongs to one sequence."""
+        raise it, the page's older values are rounded again; rows of zeros and
+        non-finite values alone never do.  A non-finite value is stored as NaN.
+        A page that is written belongs to one sequence."""
         n = k.shape[0]
         if k.shape != (n, self.n_kv_heads, self.head_dim) or v.shape != (n, self.n_kv_heads, self.v_dim) \
                 or k.dtype is not v.dtype:
