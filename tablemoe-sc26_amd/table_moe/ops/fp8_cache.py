@@ -21,7 +21,8 @@ _TAG16 = {torch.float16: N.TM_DT_F16, torch.bfloat16: N.TM_DT_BF16}
 def _int32(name: str, t: torch.Tensor, dims: int) -> torch.Tensor:
     if t.dim() != dims or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"Fp8KVCache: {name} must be {dims}-dimensional integers, got {tuple(t.shape)} {t.dtype}")
-    return t if t.dtype == torch.int32 else t.to(torch.int32)
+    # (what 32 bits do not hold stays out of range: as a page that is not there, a length past the table, rows past the call's)
+    return t if t.dtype == torch.int32 else t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
 
 
 def _rows(t: torch.Tensor):
