@@ -3,7 +3,8 @@
 the attention of this package take.
 
 One tm_rotate_positions call turns q and k: angles in 64 bits, the rotation in
-fp32, one rounding.  It is differentiable (the gradient is the rotation back).
+fp32, one rounding.  It is differentiable (the gradient is the rotation back, a
+tangent is turned as its tensor is).
 """
 
 from __future__ import annotations
@@ -12,6 +13,7 @@ import ctypes as C
 import functools
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .. import _native as N
 
@@ -112,12 +114,18 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, how):
         ctx.save_for_backward(positions, inv_freq)
+        ctx.save_for_forward(positions, inv_freq)
         ctx.how = how
         qq = _unit_rows(q)
         kk = None if k is None else _unit_rows(k)
         q_out, k_out = _new(qq), None if k is None else _new(kk)
         _run(qq, kk, positions, inv_freq, *how, q_out, k_out, q.device)
         return q_out, k_out
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        positions, inv_freq = ctx.saved_tensors
+        return _Rotate.apply(tq, tk, positions, inv_freq, ctx.how)
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -129,6 +137,11 @@ class _Rotate(torch.autograd.Function):
             return None, _Rotate.apply(dk, None, positions, inv_freq, how)[0], None, None, None
         dq, dk = _Rotate.apply(dq, dk if ctx.needs_input_grad[1] else None, positions, inv_freq, how)
         return dq, dk, None, None, None
+
+
+def _dual(t) -> bool:
+    """Whether it carries a tangent (which requires_grad does not say)."""
+    return t is not None and unpack_dual(t).tangent is not None
 
 
 def rotate_positions(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -146,7 +159,8 @@ def rotate_positions(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
     bits, the rest in fp32, rounded once.
 
     out: a pair (q_out, k_out) to write to, which may be (q, k) themselves; then
-    there are no gradients.  Otherwise gradients of any order flow to q and k."""
+    there are no gradients.  Otherwise gradients of any order flow to q and k, in
+    reverse and (torch.autograd.forward_ad) forward mode."""
     dev = N.require_hip(q, k, positions, inv_freq)
     if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]
                                            or k.dtype is not q.dtype)):
@@ -158,7 +172,8 @@ def rotate_positions(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
     if positions.dim() != 2 or positions.shape[1] != n or positions.dtype not in _INTEGERS:
         raise ValueError(f"rotate_positions: positions must be [A, {n}] or [{n}] integers, got {tuple(positions.shape)} "
                          f"{positions.dtype}")
-    if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float32 or inv_freq.requires_grad and torch.is_grad_enabled():
+    if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float32 or inv_freq.requires_grad and torch.is_grad_enabled() \
+            or _dual(inv_freq):
         raise ValueError("rotate_positions: inv_freq must be [R / 2] float32 and has no gradient")
     sections = (inv_freq.shape[0],) if sections is None else tuple(map(int, sections))
     if len(sections) != axes:
@@ -170,7 +185,7 @@ def rotate_positions(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
     if not inv_freq.is_contiguous():
         inv_freq = inv_freq.contiguous()
     how = (sections, 1 if interleaved else 0, 1 if adjacent else 0, 1 if inverse else 0)
-    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
+    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled() or _dual(q) or _dual(k):
         if out is not None:
             raise ValueError("rotate_positions: no gradients through out")
         return _Rotate.apply(q, k, positions, inv_freq, how)
@@ -182,6 +197,8 @@ def rotate_positions(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
         if (k is None) != (k_out is None):
             raise ValueError("rotate_positions: out holds a tensor for each of q and k")
         N.require_hip(q, q_out, k_out)
+        if _dual(q_out) or _dual(k_out):
+            raise ValueError("out has no gradient")
         _check_out("out[0]", q_out, q, () if k is None else (k, k_out))
         if k is not None:
             _check_out("out[1]", k_out, k, (q,))
