@@ -25,6 +25,12 @@ def _int32(name: str, t: torch.Tensor, dims: int) -> torch.Tensor:
     return t if t.dtype == torch.int32 else t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
 
 
+def _scales_hold(scales: torch.Tensor) -> bool:
+    """Whether they are powers of two in the range that append writes, or 0 (read on the host)."""
+    bits = scales.view(torch.int32)
+    return bool((((bits & 0x007fffff) == 0) & (bits >= 27 << 23) & (bits <= 247 << 23) | (bits == 0)).all())
+
+
 def _rows(t: torch.Tensor):
     """(t [T, H, D] or a copy of it with 16-byte aligned rows, its strides)."""
     if not t.is_contiguous() or t.data_ptr() % 16:
@@ -67,7 +73,10 @@ class Fp8KVCache:
 
     @classmethod
     def wrap(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> "Fp8KVCache":
-        """The cache on storage that is there already (k, v, k_scale, v_scale of another one, or kept elsewhere)."""
+        """The cache on storage that is there already (k, v, k_scale, v_scale of another one, or kept elsewhere).
+        Scales are powers of two from 2^-100 to 2^120, as ``append`` writes them (0 in pages that nobody has written to);
+        others are refused.  This reads them once and waits for it; in a stream that is being captured, which cannot
+        wait, they are taken as they are."""
         self = cls.__new__(cls)
         for name, t in (("k", k), ("v", v)):
             if t.dim() != 6 or t.dtype != torch.float8_e4m3fn or tuple(t.shape[4:]) != (64, 16) or not t.is_contiguous() \
@@ -81,6 +90,8 @@ class Fp8KVCache:
                 raise ValueError(f"Fp8KVCache: {name} must be {tuple(k.shape[:2])} float32, contiguous")
         self._check(k.shape[2] * TILE, k.shape[3] * TILE, v.shape[3] * TILE)
         self._init(k, v, k_scale, v_scale)
+        if not torch.cuda.is_current_stream_capturing() and not _scales_hold(torch.stack((k_scale, v_scale))):
+            raise ValueError("Fp8KVCache: scales must be powers of two from 2^-100 to 2^120 (or 0)")
         return self
 
     @staticmethod
