@@ -50,7 +50,8 @@ class Fp8KVCache:
 
     k and v are [pages, heads, page_size / 32, columns / 32, 64, 16]
     float8_e4m3fn in the order that the matrix instructions read (see
-    ``read_pages``), k_scale and v_scale [pages, heads] float32.
+    ``read_pages``), k_scale and v_scale [pages, heads] float32.  They are written
+    to in place, not assigned (``wrap`` makes a cache of other storage).
 
     A batch is given by ``table`` [B, M] (each sequence's pages in order),
     ``lengths`` [B] (its tokens, the new ones counted) and ``starts`` [B + 1]: the
@@ -104,13 +105,19 @@ class Fp8KVCache:
 
     def _init(self, k, v, k_scale, v_scale):
         self.device = N.require_hip(k, v, k_scale, v_scale)
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_kv_heads = k.shape[:2]
         self.page_size, self.head_dim, self.v_dim = k.shape[2] * TILE, k.shape[3] * TILE, v.shape[3] * TILE
         self._desc = N.Kv8Cache(self.n_pages, self.n_kv_heads, self.head_dim, self.v_dim, self.page_size, k.data_ptr(),
                                 v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
         self._ref = C.byref(self._desc)
         self._scale = self.head_dim ** -0.5
+
+    # The calls use these tensors' addresses, so the tensors live as long as the cache and are not exchanged.
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    k_scale = property(lambda self: self._k_scale)
+    v_scale = property(lambda self: self._v_scale)
 
     def read_pages(self, pages: torch.Tensor | None = None):
         """(K [n, heads, page_size, head_dim], V [n, heads, page_size, v_dim]) float32 of the given pages (all)."""
