@@ -20,6 +20,8 @@ native library raises instead (there is no silent fallback).
 
 from __future__ import annotations
 
+import warnings
+
 import torch
 
 from .. import _native as N
@@ -102,7 +104,10 @@ def cached_importance(cache, query_states: torch.Tensor, table: torch.Tensor, le
     without it [B, query_length]: positions from each sequence's first on (default:
     the table's width).  These are the layer's tokens only where one prompt of
     query_length tokens has nothing before it; for a piece of a prompt, a shared
-    prefix or several sequences, give ``starts``."""
+    prefix or several sequences, give ``starts``.
+
+    Queries are float16 or bfloat16.  A call that the cache refuses stores and
+    returns None, as the other functions do, and warns with the reason."""
     if starts is not None and query_length is None:
         raise ValueError("cached_importance: starts needs query_length, the number of the call's rows")
     try:
@@ -113,6 +118,7 @@ def cached_importance(cache, query_states: torch.Tensor, table: torch.Tensor, le
             return mean_score
     except N.NativeLibraryMissing:
         raise
-    except (ValueError, RuntimeError):
+    except (ValueError, RuntimeError) as e:
+        warnings.warn(f"cached_importance: no scores for the keep rule: {e}", RuntimeWarning, stacklevel=2)
         ModalityContext.set_attn_weights(None)
         return None
