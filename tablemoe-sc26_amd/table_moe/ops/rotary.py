@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 
 import torch
 from torch.autograd.forward_ad import unpack_dual
@@ -56,17 +57,22 @@ def written(*tensors) -> None:
 
 def overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
     """Whether the [T, H, D] views may share memory; views of one fused projection's rows that take different columns do
-    not."""
+    not, be they next to each other ([T, H + Hkv, D]) or by turns ([T, H, 2, D]); nor do heads of a buffer by heads."""
     if x.numel() == 0 or y.numel() == 0:
         return False
     (a, b), (c, d) = _span(x), _span(y)
     if a >= d or c >= b:
         return False
-    step = x.stride(0) * x.element_size()
-    if x.shape[0] == 1 or y.shape[0] == 1 or step != y.stride(0) * y.element_size() or step == 0:
-        return True
-    (a, b), (c, d) = _span(x[0]), _span(y[0])  # what a token takes of its row, modulo the rows' distance
-    return (c - a) % step < b - a or (a - c) % step < d - c
+    steps = [[t.stride(i) * t.element_size() for t in (x, y) if t.shape[i] > 1] for i in (0, 1)]
+    step = math.gcd(*steps[0], *steps[1])  # each view's rows start at one place modulo this
+    if step and x.shape[2] * x.element_size() <= (c - a) % step <= step - y.shape[2] * y.element_size():
+        return False
+    for i in (0, 1):  # what a token (or head) takes, modulo the distance between them
+        if len(set(steps[i])) == 1 and steps[i][0]:
+            step, (a, b), (c, d) = steps[i][0], _span(x.select(i, 0)), _span(y.select(i, 0))
+            if b - a <= (c - a) % step <= step - (d - c):
+                return False
+    return True
 
 
 def _check_out(name: str, out: torch.Tensor, x: torch.Tensor, others) -> None:
