@@ -75,12 +75,17 @@ def overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
     return True
 
 
+def _itself(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether views of one shape are the same elements (the stride of a single token or head means nothing)."""
+    return x.data_ptr() == y.data_ptr() and all(m == 1 or s == t for m, s, t in zip(x.shape, x.stride(), y.stride()))
+
+
 def _check_out(name: str, out: torch.Tensor, x: torch.Tensor, others) -> None:
     if not (out is x and x.is_contiguous()):
         if out.shape != x.shape or out.dtype != x.dtype or not rows_apart(out):
             raise ValueError(f"rotate_positions: {name} must be {tuple(x.shape)} {x.dtype} with unit stride along its last "
                              "dimension and rows that do not overlap")
-        if not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()) and overlap(out, x):
+        if not _itself(out, x) and overlap(out, x):
             raise ValueError(f"rotate_positions: {name} may be the input itself, not overlap it otherwise")
     if any(overlap(out, t) for t in others):
         raise ValueError(f"rotate_positions: {name} overlaps the other input or output")
