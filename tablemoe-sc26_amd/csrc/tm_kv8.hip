@@ -98,8 +98,8 @@ __device__ __forceinline__ void write_page(const typename Elem<DT>::T *src, int6
   float f = 1.f;  // what the page held is taken times this
   if (lo > 0) {
     // New rows of zeros and non-finite values alone ask for no scale; nor does the 1 that such rows left where they
-    // came first (an outlier's page may have 1, too: its bytes tell).
-    if (m == 0) s = before;
+    // came first (an outlier's page may have 1, too, so its bytes are read: 32 tokens, captured, 4.6 us instead of 4.0).
+    if (m == 0 && before > 0.f) s = before;  // (0: storage that nobody has written to)
     else if (before > s) s = before == 1.f && !holds_values<D, V>(page, lo) ? s : before;
     else f = before / s;  // powers of two
   }

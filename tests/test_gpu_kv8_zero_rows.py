@@ -129,3 +129,22 @@ def test_attention_over_a_page_with_a_zero_row(hip_device):
     # (under 2^-6 of the scale a step is 2^-9 of it)
     scale = float(cache.v_scale[0, 0])
     assert bool(((vd - v[:, 0]).abs() <= v[:, 0].abs() * 2.0 ** -4 + scale * 2.0 ** -10).all()) and scale < 2.0 ** -14
+
+
+@pytest.mark.parametrize("kind", [0.0, math.nan])
+def test_storage_of_zeros_that_a_length_counts_as_held(hip_device, kind):
+    """A wrapped pool of zeros, scales too, in a page of which a length says that it held tokens: zeros stay zeros."""
+    from table_moe.ops import Fp8KVCache
+
+    dev, d = hip_device, 64
+    c = Fp8KVCache(2, 1, d, page_size=32, device=dev)
+    z = lambda t: torch.zeros_like(t.view(torch.uint8)).view(t.dtype)  # noqa: E731
+    w = Fp8KVCache.wrap(z(c.k), z(c.v), torch.zeros_like(c.k_scale), torch.zeros_like(c.v_scale))
+    table, rows = torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.full((3, 1, d), kind, device=dev)
+    rows[1] = 0
+    w.append(rows, rows, table, torch.tensor([8], device=dev), torch.tensor([0, 3], device=dev))
+    for x in w.read_pages():
+        bad = torch.isnan(x[0, 0])
+        assert bool((x[0, 0][~bad] == 0).all())
+        assert bad.any(1).nonzero().flatten().tolist() == ([] if kind == 0 else [5, 7])
+    assert float(w.k_scale[0, 0]) == 1
