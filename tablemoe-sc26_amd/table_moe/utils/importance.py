@@ -119,6 +119,6 @@ def cached_importance(cache, query_states: torch.Tensor, table: torch.Tensor, le
     except N.NativeLibraryMissing:
         raise
     except (ValueError, RuntimeError) as e:
-        warnings.warn(f"cached_importance: no scores for the keep rule: {e}", RuntimeWarning, stacklevel=2)
         ModalityContext.set_attn_weights(None)
+        warnings.warn(f"cached_importance: no scores for the keep rule: {e}", RuntimeWarning, stacklevel=2)
         return None

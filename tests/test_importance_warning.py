@@ -32,3 +32,13 @@ def test_scores_do_not_warn():
         y = cached_importance(Cache(torch.ones(2, 3)), None, None, None)
     assert y.shape == (2, 3) and torch.equal(ModalityContext.get_attn_weights(), torch.ones(6))
     ModalityContext.set_attn_weights(None)
+
+
+def test_a_warning_that_is_an_error_leaves_no_scores():
+    """Where warnings are raised, the scores of the call before are gone all the same."""
+    cached_importance(Cache(torch.ones(2, 3)), None, None, None)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        with pytest.raises(RuntimeWarning):
+            cached_importance(Cache(ValueError("no")), None, None, None)
+    assert ModalityContext.get_attn_weights() is None
