@@ -6,9 +6,9 @@
 // (A scale per token would need no such rounding and a scale for every key in the
 // attention's inner loop.)
 //
-// Bound by HBM and latency: 9936 tokens of 4 heads of 128 in fp16 (30.5 MB) 10.7 us; one
-// token for each of 32 sequences 4.6 us, a chain of look-ups, rows, maximum and the
-// pieces to be merged.
+// Bound by HBM and latency: 9936 tokens of 4 heads of 128 in fp16 (30.5 MB) 10.9 us; one
+// token for each of 32 sequences 4.8 us, a chain of look-ups, rows, maximum and the
+// pieces to be merged (averages under the profiler).
 #include "tm_kv8.h"
 #include "tm_internal.h"
 

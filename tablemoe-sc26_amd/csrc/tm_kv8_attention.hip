@@ -16,11 +16,13 @@
 // probabilities of a lane's 16 keys sum to more than 2^15: no maximum is taken of
 // the other tiles, and O is seldom scaled again.  P is rounded to fp16 for the
 // second product whatever the queries' type, and V's bytes become fp16 (exact):
-// half a step is 2^-12 of a probability, where bf16 would leave 2^-9 (an output's
+// half a step is 2^-11 of a probability at most, where bf16 would leave 2^-8 (an output's
 // error against 64 bits 1.9e-3 of its size instead of 1.6e-3, which is its own
-// rounding); what lies under 2^-33 of a row's largest is lost.  All sums are fp32.
+// rounding); what lies under 2^-33 of a row's largest is lost.  All sums are fp32; l
+// takes the probabilities before that rounding (log sum exp has no other), so an
+// output's weights sum to 1 up to 2^-11.
 //
-// A prompt is bound by instructions: per 32 keys and 64 rows the products take 1024
+// A long prompt is bound by instructions: per 32 keys and 64 rows the products take 1024
 // cycles of the matrix units, of which about half keep the vector units from
 // issuing, and the conversions of K and V (64, 5 cycles each), exponentials (32, 8.5)
 // and the rest (about 110, 3 to 6) another 1000.  So a long prompt's waves own 64 rows,

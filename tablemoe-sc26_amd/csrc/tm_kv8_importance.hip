@@ -11,9 +11,9 @@
 // Written by position of each sequence, or by row of the call's new tokens (the
 // last positions of each sequence): then only these tokens' tiles are computed.
 //
-// Bound by HBM: 131071 keys of 4 heads of 128 (67 MB) with the log sum exp at hand 14.3 us,
-// 4.7 TB/s, as a large copy; 4099 keys without it 5.4 + 4.3 us, two launches of a few memory
-// round trips each.
+// Bound by HBM and the last cache: 131071 keys of 4 heads of 128 (67 MB) with the log sum exp at hand
+// 13.7 us, 4.9 TB/s, a large copy's rate; 4099 keys without it 5.5 + 5.3 us, two launches of a few memory
+// round trips each (averages under the profiler).
 #include "tm_internal.h"
 #include "tm_kv8_dev.h"
 

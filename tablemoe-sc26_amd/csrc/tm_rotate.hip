@@ -11,7 +11,7 @@
 // no multiples of 8 elements.
 //
 // Bound by HBM: 36 heads of 128, 30011 tokens in fp16 (554 MB) 117 us, 4.7 TB/s; 4099 in
-// bf16 (76 MB) 14.1 us, 5.4 TB/s; 8 tokens 5 us, of which the 64-bit angle and
+// bf16 (76 MB) 13.9 us, 5.4 TB/s; 8 tokens 5 us, of which the 64-bit angle and
 // sine and cosine about 2.
 #include "tm_internal.h"
 
